@@ -10,7 +10,7 @@ import array
 import ctypes
 import os
 import struct
-from ctypes import POINTER, c_char_p, c_double, c_int, c_int32, c_int64, c_uint64, c_void_p
+from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_uint64, c_void_p
 
 import torch
 
@@ -59,6 +59,16 @@ class DaricChunk(ctypes.Structure):
                 ("k", c_int64), ("tok_start", c_int64)]
 
 
+class DaricSequence(ctypes.Structure):
+    _fields_ = [("bt_offset", c_int64), ("row_start", c_int64), ("n_rows", c_int64), ("n_ctx", c_int64),
+                ("col_start", c_int64)]
+
+
+class DaricEviction(ctypes.Structure):
+    _fields_ = [("bt_offset", c_int64), ("col_start", c_int64), ("n_tokens", c_int64), ("keep", c_int64),
+                ("n_first", c_int64), ("n_recent", c_int64)]
+
+
 P = POINTER
 T = P(DaricTensor)
 I64P = c_void_p  # address of an I64 buffer
@@ -97,6 +107,12 @@ SIGNATURES = {
     "daric_merge_rows": (c_int, [T, c_int64, c_int, T, T, T, P(DaricChunk), c_int64, T, T, T, c_uint64]),
     "daric_select_merge": (c_int, [T, c_int64, c_int, T, T, T, P(DaricChunk), c_int64, T, T, T, T, c_int,
                                    c_uint64]),
+    # sequences and evictions: the address of an int64 [n, 5] or [n, 6] array
+    "daric_attend_workspace": (c_int, [T, c_int, T, I64P, c_int64, P(c_int64)]),
+    "daric_attend_pages": (c_int, [T, c_int, T, T, I64P, c_int64, T, c_float, T, T, T, T, c_void_p, c_int64,
+                                   c_uint64]),
+    "daric_weigh_tokens": (c_int, [T, c_int, T, T, T, I64P, c_int64, T, c_float, T, T, c_int, c_uint64]),
+    "daric_evict_tokens": (c_int, [T, c_int64, c_int, T, T, I64P, c_int64, T, T, c_uint64]),
 }
 
 _lib = None

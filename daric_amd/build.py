@@ -30,7 +30,8 @@ LIB = os.path.join(LIBDIR, "libdaric_cache_ops.so")
 HOSTTEST_LIB = os.path.join(LIBDIR, "libdaric_hosttest.so")
 
 SOURCES = ["capi.cpp", "runtime.cpp", "copy_kernels.hip", "rope_kernels.hip", "select_kernels.hip",
-           "token_kernels.hip", "noalloc.hip"]
+           "token_kernels.hip", "noalloc.hip", "attend_bf16.hip", "attend_f16.hip", "attend_e4m3_bf16.hip",
+           "attend_e4m3_f16.hip", "evict_kernels.hip"]
 
 ARCH = "gfx950"
 COMMON = ["-O3", "-std=c++17", "-fPIC", "-Wall", "-Wextra", "-Wshadow", "-Wno-unused-result",

@@ -11,7 +11,9 @@ Additions (no reference counterpart; the .pyi grows, nothing changes):
   allocation-free form scatter_pages_rerotate_noalloc),
   CacheCopier.gather_tokens / scatter_tokens (token-major staging for any
   cache layout), rerotate_pages, kv_deviation, topk_per_chunk, merge_rows,
-  select_merge (the three selection calls in one), kernel timing.
+  select_merge (the three selection calls in one), attend_pages (attention
+  over the paged cache), weigh_tokens and evict_tokens (eviction by
+  accumulated attention weight), kernel timing.
 
 Every call is asynchronous on `stream` (0 = the current torch stream of the
 first layer's device, as in reference copier.cpp:27-30). The wrapper keeps
@@ -36,7 +38,7 @@ from ._lib import I64, DaricChunk, DaricRope, check, desc, load, str_array
 __all__ = [
     "CacheCopier", "batched_memcpy_d2h", "batched_memcpy_h2d", "rerotate_pages",
     "kv_deviation", "topk_per_chunk", "merge_rows", "select_merge", "SELECT_KEYS_READY",
-    "SELECT_ONE_PASS", "timing_enable", "timing_read",
+    "SELECT_ONE_PASS", "attend_pages", "weigh_tokens", "evict_tokens", "timing_enable", "timing_read",
 ]
 
 
@@ -463,6 +465,126 @@ def select_merge(layers: Sequence[torch.Tensor], page_first: bool, block_table: 
                                     ctypes.c_uint64(st)))
     _record(st, dev, block_table, k_new, v_new, keys, sel_idx, k_scales, v_scales)
     return keys, sel_idx
+
+
+def _tuples(entries, widths, what):
+    """(address of int64 [n, widths[0]], n, keep-alive, list of columns) of a
+    sequence of integer tuples or an int64 array; entries shorter than
+    widths[0] (but of a width named) get zeros behind."""
+    full = widths[0]
+    a = np.asarray(entries if isinstance(entries, np.ndarray) else list(entries))
+    if a.size == 0:
+        a = np.zeros((0, full), np.int64)
+    if a.ndim != 2 or a.shape[1] not in widths or a.dtype.kind not in "iu":
+        raise ValueError(what)
+    if a.shape[1] < full:
+        a = np.concatenate([a, np.zeros((a.shape[0], full - a.shape[1]), np.int64)], axis=1)
+    a = np.ascontiguousarray(a, dtype=np.int64)
+    return a.ctypes.data, a.shape[0], a
+
+
+def _sequences(seqs):
+    return _tuples(seqs, (5, 4), "sequences must be (bt_offset, row_start, n_rows, n_ctx[, col_start]) entries of ints")
+
+
+def _ref(t: Optional[torch.Tensor]):
+    return ctypes.byref(desc(t)) if t is not None else None
+
+
+def _layer_desc(layer: torch.Tensor):
+    return _layer_array((layer,))
+
+
+def attend_pages(layer: torch.Tensor, page_first: bool, block_table: torch.Tensor, q: torch.Tensor, seqs,
+                 tree_mask: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                 k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None,
+                 out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
+                 stream: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
+    """Attention of q ([T, Hq, D]) over one layer's paged cache: (out [T, Hq, D]
+    of q's type, lse [T, Hq] fp32). seqs: (bt_offset, row_start, n_rows, n_ctx
+    [, col_start]); rows row_start .. + n_rows of q belong to tokens that stand in
+    the cache behind the sequence's n_ctx cached ones. Every row sees the n_ctx
+    tokens; of the others row i sees the first i + 1 (one token, a prompt's run
+    of rows), or those whose bits its row of tree_mask (int64 [T, words])
+    sets (drafted trees). Tokens in pages of id 0 are not there; rows that see
+    nothing get zeros and lse -inf; rows of no sequence are not written. scale:
+    D ** -0.5 if None. k_scale, v_scale: [H] fp32 scales of an fp8 cache. See
+    include/daric_cache_ops.h for what the arguments may be."""
+    dev = layer.device
+    st = _resolve_stream(stream, dev)
+    addr, n, _keep = _sequences(seqs)
+    lib, ld, qd = load(), _layer_desc(layer), desc(q)
+    pf = 1 if page_first else 0
+    need = ctypes.c_int64()
+    check(lib.daric_attend_workspace(ld, pf, ctypes.byref(qd), addr, n, ctypes.byref(need)))
+    work = None
+    if need.value or out is None or lse is None:
+        with _on_stream(st, dev):
+            if out is None:
+                out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+            if lse is None:
+                lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev)
+            if need.value:
+                work = torch.empty(need.value, dtype=torch.uint8, device=dev)
+    check(lib.daric_attend_pages(ld, pf, _ref(block_table), ctypes.byref(qd), addr, n, _ref(tree_mask),
+                                 float(q.shape[2] ** -0.5 if scale is None else scale), _ref(k_scale), _ref(v_scale),
+                                 _ref(out), _ref(lse), work.data_ptr() if work is not None else None, need.value,
+                                 ctypes.c_uint64(st)))
+    _record(st, dev, block_table, q, tree_mask, k_scale, v_scale, out, lse, work)
+    return out, lse
+
+
+def weigh_tokens(layer: torch.Tensor, page_first: bool, block_table: torch.Tensor, q: torch.Tensor,
+                 lse: torch.Tensor, seqs, weights: Optional[torch.Tensor] = None,
+                 tree_mask: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                 k_scale: Optional[torch.Tensor] = None, stream: int = 0) -> torch.Tensor:
+    """The attention weight that each token of the cache received in
+    attend_pages(layer, ..., q, seqs, ...), whose lse is passed, summed over the rows
+    and the query heads of each KV head: added to weights[:, col_start + j]
+    ([H, columns] fp32) for token j of a sequence (bt_offset, row_start, n_rows,
+    n_ctx, col_start), or without `weights` written to a new tensor, zeros where
+    no sequence is. Returns the weights."""
+    dev = layer.device
+    st = _resolve_stream(stream, dev)
+    addr, n, a = _sequences(seqs)
+    fresh = weights is None
+    ld, qd = _layer_desc(layer), desc(q)
+    if fresh:
+        end = int((a[:, 4] + a[:, 2] + a[:, 3]).max()) if n else 0
+        heads = layer.shape[1] if layer.dim() == 4 else layer.shape[3] if layer.dim() == 5 else 1
+        with _on_stream(st, dev):
+            weights = torch.zeros((heads, max(end, 0)), dtype=torch.float32, device=dev)
+    check(load().daric_weigh_tokens(ld, 1 if page_first else 0, _ref(block_table), ctypes.byref(qd), _ref(lse), addr, n,
+                                    _ref(tree_mask), float(q.shape[2] ** -0.5 if scale is None else scale),
+                                    _ref(k_scale), _ref(weights), 0 if fresh else 1, ctypes.c_uint64(st)))
+    _record(st, dev, block_table, q, lse, tree_mask, k_scale, weights)
+    return weights
+
+
+def evict_tokens(layers: Sequence[torch.Tensor], page_first: bool, block_table: torch.Tensor,
+                 weights: torch.Tensor, evictions, stream: int = 0) -> torch.Tensor:
+    """Keeps the heaviest tokens of each sequence, per layer and KV head, and
+    brings them to its first slots, in place. evictions: (bt_offset, col_start,
+    n_tokens, keep, n_first, n_recent); weights: [L, H, columns] fp32 ([L, 1,
+    columns]: one choice for all heads of a layer). Kept tokens among the first
+    `keep` slots stay, the i-th slot freed takes the i-th kept token from behind.
+    Returns kept [L, H or 1, n, kmax] int32: the token that each slot holds
+    now, -1 behind the last. The weights move with their tokens, those from
+    `keep` on become 0. Rows are bytes: any cache type, MLA caches too."""
+    layers = list(layers)
+    dev = layers[0].device
+    st = _resolve_stream(stream, dev)
+    addr, n, a = _tuples(evictions, (6,), "evictions must be (bt_offset, col_start, n_tokens, keep, n_first, n_recent) "
+                                          "entries of ints")
+    kmax = max(0, int(np.minimum(a[:, 2], a[:, 3]).max())) if n else 0
+    with _on_stream(st, dev):
+        both = torch.empty((2, len(layers), weights.shape[1] if weights.dim() == 3 else 1, n, kmax), dtype=torch.int32,
+                           device=dev)
+    kept, work = both[0], both[1]
+    check(load().daric_evict_tokens(_layer_array(layers), len(layers), 1 if page_first else 0, _ref(block_table),
+                                    _ref(weights), addr, n, _ref(kept), _ref(work), ctypes.c_uint64(st)))
+    _record(st, dev, block_table, weights, both)
+    return kept
 
 
 def timing_enable(enable: bool = True) -> None:

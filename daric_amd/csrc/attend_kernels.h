@@ -1,0 +1,656 @@
+// Attention over the paged KV cache, and the weight its tokens receive.
+//
+// Attention of a row r (one head of one query) over the tokens j it sees:
+//   t_j = c <q_r, K_j>,  c = scale * k_scale * log2(e)
+//   lse = (m + log2 l) ln 2,  l = sum_j 2^(t_j - m)
+//   out = v_scale / l * sum_j 2^(t_j - m) V_j
+// with the running maximum m, the sum l and the weighted rows kept in fp32
+// over one pass of the tokens. The products run on the matrix cores as
+// S^T = K Q^T and O^T = V^T P^T in tiles of 16 (rows of q in the columns) by
+// 32 tokens: S^T leaves a lane with 2 x 4 consecutive tokens of one row, which
+// is what the second product wants of P^T if V's tokens are taken in the same
+// order, so the weights never leave their lanes. A lane reads, of those 8
+// tokens, one slice of head_dim / 16 values of V and pairs the tokens' values
+// with byte permutes: K and V go from memory to the matrix cores without LDS.
+//
+// e4m3 codes become bf16 or fp16 (q's type) exactly; the scales of a head act
+// on c and on the result. The weights P are rounded to q's type for the second
+// product (half a step of it per weight, at random, where the output is
+// rounded to the same type); l sums them unrounded.
+#pragma once
+
+#include <cmath>
+
+#include "attend.h"
+#include "elem.h"
+#include "kernels.h"
+#include "launch.h"
+
+namespace daric {
+namespace attend {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+constexpr float kLn2 = 0.693147180559945309f;
+
+template <int QK>
+__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+#ifdef __HIP_DEVICE_COMPILE__
+    if constexpr (QK == kBF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                       0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c,
+                                                      0, 0, 0);
+#else
+    (void)a; (void)b;
+    return c;
+#endif
+}
+
+// Two e4m3 codes (the low or high half of w) as a word of q's type.
+template <int QK, bool HI>
+__device__ __forceinline__ uint32_t e4m3_pair(uint32_t w) {
+#ifdef __HIP_DEVICE_COMPILE__
+    if constexpr (QK == kBF16)
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
+    else
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HI));
+#else
+    return w;
+#endif
+}
+
+template <int QK>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    const float p[2] = {lo, hi};
+    return Elem<QK>::pack_word(p);
+}
+
+__device__ __forceinline__ uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) {
+#ifdef __HIP_DEVICE_COMPILE__
+    return __builtin_amdgcn_perm(hi, lo, sel);
+#else
+    (void)hi; (void)sel;
+    return lo;
+#endif
+}
+
+__device__ __forceinline__ float exp2_hw(float x) {
+#ifdef __HIP_DEVICE_COMPILE__
+    return __builtin_amdgcn_exp2f(x);
+#else
+    return x;
+#endif
+}
+
+// N words from p: one load of up to 16 bytes each, or (VALUES) value by value
+// of ES bytes, the values from `left` on zero.
+template <int N, int ES, bool VALUES>
+__device__ __forceinline__ void load_words(uint32_t* w, const uint8_t* p, int left) {
+    if constexpr (VALUES) {
+        constexpr int PW = 4 / ES;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            w[i] = 0;
+#pragma unroll
+            for (int b = 0; b < PW; ++b) {
+                if (i * PW + b < left) {
+                    const uint32_t v = ES == 2 ? *reinterpret_cast<const uint16_t*>(p + (i * PW + b) * ES)
+                                               : p[i * PW + b];
+                    w[i] |= v << (b * ES * 8);
+                }
+            }
+        }
+    } else if constexpr (N == 1) {
+        w[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else if constexpr (N == 2) {
+        const u32x2 v = *reinterpret_cast<const u32x2*>(p);
+        w[0] = v[0]; w[1] = v[1];
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const u32x4 v = *reinterpret_cast<const u32x4*>(p + i * 4);
+            w[i] = v[0]; w[i + 1] = v[1]; w[i + 2] = v[2]; w[i + 3] = v[3];
+        }
+    }
+}
+
+// Where a lane (n = lane % 16, g = lane / 16) stands:
+//   K, A operand of S^T, half h of the tile: token 16 h + n, values
+//     kdim(step, g) .. + 7 of each step of 32
+//   Q, B operand of S^T: row n, the same values
+//   S^T: row n, tokens 16 h + 4 g + i
+//   V, A operand of O^T: tokens 16 h + 4 g + i, values E n .. E n + E - 1
+//   O^T: row n, value E (4 g + i) + e of matrix e
+// A 16-byte unit of e4m3 K holds two steps' values.
+template <int CK>
+__device__ __forceinline__ int kdim(int step, int g) {
+    return CK == kE4M3 ? 64 * (step >> 1) + 16 * g + 8 * (step & 1) : 32 * step + 8 * g;
+}
+
+// Rows of K and V of one tile as they lie in memory.
+template <int CK, int DP>
+struct TileRows {
+    static constexpr int ES = CK == kE4M3 ? 1 : 2;
+    static constexpr int KU = DP * ES / 64;        // 16-byte units of K per lane and half
+    static constexpr int E = DP / 16;              // values of V per lane and token
+    static constexpr int VW = E * ES / 4;          // words of them
+    uint32_t k[2][KU][4];
+    uint32_t v[8][VW];
+    uint32_t ok;                                   // tokens that are there
+};
+
+// Reads the rows of one KV head.
+template <int CK, int DP, int MODE>
+struct RowReader {
+    using Rows = TileRows<CK, DP>;
+    static constexpr int ES = Rows::ES;
+    const uint8_t* head;       // K row of block 0, slot 0
+    const int32_t* bt;         // the sequence's block list
+    int64_t sb, ss, v_off;     // bytes
+    FastDiv page;
+    int PS, D, num_blocks, n_total, last_page;
+    int n, g;
+
+    __device__ __forceinline__ void init(const AttArgs& a, int64_t bt_offset, int total, int h, int lane) {
+        sb = a.g.sb * ES; ss = a.g.ss * ES; v_off = a.g.v_off * ES;
+        head = a.layer + a.g.sh * ES * h;
+        bt = a.block_table + bt_offset;
+        page = a.page;
+        PS = a.g.PS; D = a.g.D; num_blocks = a.g.num_blocks;
+        n_total = total;
+        last_page = static_cast<int>(page.div(static_cast<uint32_t>(total - 1)));
+        n = lane & 15; g = lane >> 4;
+    }
+    // Offset of a token's row, and whether the token is there: a page id of 0
+    // (the null block) or out of range has none. Tokens that are not there
+    // read a row of block 0 and count for nothing.
+    __device__ __forceinline__ int64_t row_of(int t, bool* there) const {
+        const int p = min(static_cast<int>(page.div(static_cast<uint32_t>(t))), last_page);
+        const int id = bt[p];
+        *there = t < n_total && id > 0 && id < num_blocks;
+        const int slot = *there ? t - p * PS : 0;
+        return static_cast<int64_t>(*there ? id : 0) * sb + static_cast<int64_t>(slot) * ss;
+    }
+    __device__ __forceinline__ void load_k(Rows& r, int64_t o0, int64_t o1) const {
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+            const uint8_t* p = head + (hh ? o1 : o0);
+#pragma unroll
+            for (int u = 0; u < Rows::KU; ++u) {
+                const int d = CK == kE4M3 ? 64 * u + 16 * g : 32 * u + 8 * g;
+                if constexpr (MODE == kAttWhole) {
+                    load_words<4, ES, false>(r.k[hh][u], p + d * ES, 0);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) r.k[hh][u][i] = 0;
+                    if (d < D) load_words<4, ES, MODE == kAttValues>(r.k[hh][u], p + d * ES, D - d);
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void load_v(uint32_t* w, int64_t o) const {
+        const uint8_t* p = head + v_off + o;
+        const int d = Rows::E * n;
+        if constexpr (MODE == kAttWhole) {
+            load_words<Rows::VW, ES, false>(w, p + d * ES, 0);
+        } else {
+#pragma unroll
+            for (int i = 0; i < Rows::VW; ++i) w[i] = 0;
+            constexpr int STEP = MODE == kAttValues || Rows::VW < 4 ? Rows::VW : (Rows::VW * 4 / ES > 8 ? 8 * ES / 4 : Rows::VW);
+            // slices of 8 values at most, each there or not as a whole
+#pragma unroll
+            for (int i = 0; i < Rows::VW; i += STEP) {
+                const int di = d + i * 4 / ES;
+                if (di < D) load_words<STEP, ES, MODE == kAttValues>(w + i, p + di * ES, D - di);
+            }
+        }
+    }
+    // The rows of tokens t0 .. t0 + 31. Lane L finds the row of token t0 +
+    // L % 32; the others get it from there.
+    template <bool WITH_V>
+    __device__ __forceinline__ void load(Rows& r, int t0) const {
+        bool there;
+        const int64_t mine = row_of(t0 + (16 * (g & 1) + n), &there);
+        r.ok = static_cast<uint32_t>(__ballot(there));
+        const int lo = static_cast<int>(mine), hi = static_cast<int>(mine >> 32);
+        const auto from = [&](int t) {
+            return static_cast<int64_t>((static_cast<uint64_t>(static_cast<uint32_t>(__shfl(hi, t, 64))) << 32) |
+                                        static_cast<uint32_t>(__shfl(lo, t, 64)));
+        };
+        load_k(r, from(n), from(16 + n));
+        if constexpr (WITH_V) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) load_v(r.v[j], from(16 * (j >> 2) + 4 * g + (j & 3)));
+        }
+    }
+};
+
+// One K operand of S^T.
+template <int CK, int QK, int DP>
+__device__ __forceinline__ u32x4 k_operand(const TileRows<CK, DP>& r, int half, int step) {
+    if constexpr (CK == kE4M3) {
+        const uint32_t* w = r.k[half][step >> 1] + 2 * (step & 1);
+        return u32x4{e4m3_pair<QK, false>(w[0]), e4m3_pair<QK, true>(w[0]), e4m3_pair<QK, false>(w[1]),
+                     e4m3_pair<QK, true>(w[1])};
+    } else {
+        const uint32_t* w = r.k[half][step];
+        return u32x4{w[0], w[1], w[2], w[3]};
+    }
+}
+
+// V operands of values e and e + 1 (e even): the lane's 8 tokens in order.
+template <int CK, int QK, int DP>
+__device__ __forceinline__ void v_operands(const TileRows<CK, DP>& r, int e, u32x4* lo, u32x4* hi) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (CK == kE4M3) {
+            const uint32_t x = perm(r.v[2 * i + 1][e >> 2], r.v[2 * i][e >> 2], e & 2 ? 0x07030602u : 0x05010400u);
+            (*lo)[i] = e4m3_pair<QK, false>(x);
+            (*hi)[i] = e4m3_pair<QK, true>(x);
+        } else {
+            (*lo)[i] = perm(r.v[2 * i + 1][e >> 1], r.v[2 * i][e >> 1], 0x05040100u);
+            (*hi)[i] = perm(r.v[2 * i + 1][e >> 1], r.v[2 * i][e >> 1], 0x07060302u);
+        }
+    }
+}
+
+// The row of q that matrix column `n` of row tile `rt` holds: query R / G,
+// head R % G of the KV head's group.
+struct QRow {
+    int i;        // query of the sequence, -1: none
+    int head;     // in all
+};
+__device__ __forceinline__ QRow q_row(const AttArgs& a, int n_rows, int h, int R) {
+    QRow r;
+    const int i = static_cast<int>(a.group.div(static_cast<uint32_t>(R)));
+    r.i = i < n_rows ? i : -1;
+    r.head = h * a.G + (R - i * a.G);
+    return r;
+}
+
+template <int CK, int DP, int MODE>
+__device__ __forceinline__ void load_q(const AttArgs& a, const AttSeq& s, const QRow& r, int g, u32x4 (&q)[DP / 32]) {
+#pragma unroll
+    for (int st = 0; st < DP / 32; ++st) {
+        uint32_t w[4] = {0, 0, 0, 0};
+        const int d = kdim<CK>(st, g);
+        if (r.i >= 0 && (MODE == kAttWhole || d < a.g.D)) {
+            const uint8_t* p = a.q + (static_cast<int64_t>(s.row0 + r.i) * a.q_row + r.head * a.q_head + d) * 2;
+            load_words<4, 2, MODE == kAttValues>(w, p, a.g.D - d);
+        }
+        q[st] = u32x4{w[0], w[1], w[2], w[3]};
+    }
+}
+
+// Bit b: the query sees token t0 + b, if it is there (32 tokens).
+__device__ __forceinline__ uint32_t row_sees(const AttArgs& a, const AttSeq& s, int i, int t0) {
+    if (i < 0) return 0;
+    const int d0 = t0 - s.n_ctx;                       // draft of the first token
+    if (d0 <= -32) return ~0u;
+    if (a.mask == nullptr) {
+        const int c = i - d0 + 1;
+        return c >= 32 ? ~0u : c <= 0 ? 0u : (1u << c) - 1u;
+    }
+    const uint64_t* w = a.mask + static_cast<int64_t>(s.row0 + i) * a.words;
+    if (d0 < 0) return ((1u << -d0) - 1u) | static_cast<uint32_t>(w[0] << -d0);
+    const int at = d0 >> 6, sh = d0 & 63;
+    uint64_t v = w[at] >> sh;
+    if (sh > 32 && at + 1 < a.words) v |= w[at + 1] << (64 - sh);
+    return static_cast<uint32_t>(v);
+}
+
+// ------------------------------------------------------------------ attend
+// One workgroup: one KV head, 16 rows of q and one part of a sequence's tokens,
+// whose tiles its wavefronts take in turn; they join in LDS at the end.
+template <int CK, int QK, int DP, int MODE>
+__global__ __launch_bounds__(256) void attend_kernel(DescArg d, AttArgs a) {
+    using Rows = TileRows<CK, DP>;
+    constexpr int E = Rows::E, STEPS = DP / 32, WAVES = 4;
+    constexpr int LD = DP + 4;                        // floats of a row in LDS: no two rows on one bank
+    __shared__ float s_o[WAVES][kAttRows][LD];
+    __shared__ float s_m[WAVES][kAttRows], s_l[WAVES][kAttRows];
+    const DescPtr<AttSeq> seqs = desc_at<AttSeq>(d, 0);
+    const int item = static_cast<int>(blockIdx.x);
+    const int si = __builtin_amdgcn_readfirstlane(find_by_tile(seqs, a.n_seqs, item));
+    const AttSeq s = desc_load(seqs + si);
+    const int tid = static_cast<int>(threadIdx.x), lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 15, g = lane >> 4;
+    // item of the sequence: (part, row tile, head), the head first
+    const int local = item - s.tile_begin;
+    const int pr = static_cast<int>(a.heads.div(static_cast<uint32_t>(local)));
+    const int h = local - pr * a.g.H;
+    const int row_tiles = (s.n_rows * a.G + kAttRows - 1) / kAttRows;
+    const int part = pr / row_tiles, rt = pr - part * row_tiles;
+    const int total = s.n_ctx + s.n_rows;
+    const QRow row = q_row(a, s.n_rows, h, rt * kAttRows + n);
+    // causal: nothing behind the last row's own token is seen
+    const int last_i = min(s.n_rows - 1, static_cast<int>(a.group.div(static_cast<uint32_t>(rt * kAttRows + kAttRows - 1))));
+    const int end = a.mask == nullptr ? s.n_ctx + last_i + 1 : total;
+    const int tile_end = min((part + 1) * a.part_tiles, (end + kAttTile - 1) / kAttTile);
+
+    RowReader<CK, DP, MODE> rd;
+    rd.init(a, s.bt_offset, total, h, lane);
+    u32x4 q[STEPS];
+    load_q<CK, DP, MODE>(a, s, row, g, q);
+    const float c = a.scale_log2 * (a.k_scale != nullptr ? a.k_scale[h] : 1.0f);
+    f32x4 acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = f32x4{0, 0, 0, 0};
+    float m = -3.402823466e38f, l = 0.0f;
+
+    const auto tile_of = [&](Rows& r, int tile) {
+        const int t0 = tile * kAttTile;
+        f32x4 sc[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+#pragma unroll
+        for (int st = 0; st < STEPS; ++st) {
+            sc[0] = mfma<QK>(k_operand<CK, QK, DP>(r, 0, st), q[st], sc[0]);
+            sc[1] = mfma<QK>(k_operand<CK, QK, DP>(r, 1, st), q[st], sc[1]);
+        }
+        float t[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t[j] = sc[j >> 2][j & 3] * c;
+        const bool drafts = t0 + kAttTile > s.n_ctx;
+        uint32_t vis = r.ok;
+        if (r.ok != ~0u || drafts) {
+            vis = r.ok & row_sees(a, s, row.i, t0);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int b = 16 * (j >> 2) + 4 * g + (j & 3);
+                if (!((vis >> b) & 1u)) t[j] = -__builtin_huge_valf();
+                if (!((r.ok >> b) & 1u)) {
+#pragma unroll
+                    for (int w = 0; w < Rows::VW; ++w) r.v[j][w] = 0;
+                }
+            }
+        }
+        // A new maximum only where a score passes the old one by 2^8: weights of
+        // up to 2^8 are as exact, and most tiles then skip the exchange.
+        float top = t[0];
+#pragma unroll
+        for (int j = 1; j < 8; ++j) top = fmaxf(top, t[j]);
+        if (__ballot(top - m > 8.0f) != 0) {
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float mn = fmaxf(m, top);
+            const float al = exp2_hw(m - mn);
+            m = mn;
+            l *= al;
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] *= al;
+        }
+        float p[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            p[j] = exp2_hw(t[j] - m);
+            l += p[j];
+        }
+        // V of a masked draft may be anything; a row that does not see it must
+        // not get 0 * inf. Such values are taken out of the product and added
+        // below to the rows that see them.
+        bool odd = false;
+        if (drafts) {
+            constexpr uint32_t EXP = CK == kBF16 ? 0x7f80u : CK == kF16 ? 0x7c00u : 0x7fu;
+            constexpr int ES = Rows::ES;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int w = 0; w < Rows::VW; ++w)
+#pragma unroll
+                    for (int b = 0; b < 4 / ES; ++b) {
+                        const uint32_t x = EXP << (b * ES * 8);
+                        if ((r.v[j][w] & x) == x) {
+                            odd = true;
+                            r.v[j][w] &= ~((ES == 2 ? 0xffffu : 0xffu) << (b * ES * 8));
+                        }
+                    }
+        }
+        const u32x4 pb = {pack2<QK>(p[0], p[1]), pack2<QK>(p[2], p[3]), pack2<QK>(p[4], p[5]), pack2<QK>(p[6], p[7])};
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+            u32x4 lo, hi;
+            v_operands<CK, QK, DP>(r, e, &lo, &hi);
+            acc[e] = mfma<QK>(lo, pb, acc[e]);
+            acc[e + 1] = mfma<QK>(hi, pb, acc[e + 1]);
+        }
+        if (__ballot(odd) != 0) {
+            // the wavefront's own LDS rows hold P meanwhile
+            float* sp = &s_o[wave][n][0];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sp[16 * (j >> 2) + 4 * g + (j & 3)] = p[j];
+            __builtin_amdgcn_wave_barrier();
+            for (int b = 0; b < kAttTile; ++b) {
+                if (!((vis >> b) & 1u)) continue;
+                const float pj = sp[b];
+                bool there;
+                const uint8_t* vr = rd.head + rd.v_off + rd.row_of(t0 + b, &there);
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int dd = E * (4 * g + i) + e;
+                        if (dd >= a.g.D) continue;
+                        float x;
+                        if constexpr (CK == kE4M3) x = e4m3_to_f32(vr[dd]);
+                        else if constexpr (CK == kBF16) x = bf16_to_f32(reinterpret_cast<const uint16_t*>(vr)[dd]);
+                        else x = f16_to_f32(reinterpret_cast<const uint16_t*>(vr)[dd]);
+                        if (!(fabsf(x) <= 3.402823466e38f)) acc[e][i] += pj * x;
+                    }
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+    };
+
+    for (int tile = part * a.part_tiles + wave; tile < tile_end; tile += WAVES) {
+        Rows r;
+        rd.template load<true>(r, tile * kAttTile);
+        tile_of(r, tile);
+    }
+
+    // Join the wavefronts.
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if (g == 0) {
+        s_m[wave][n] = m;
+        s_l[wave][n] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < E; ++e) s_o[wave][n][E * (4 * g + i) + e] = acc[e][i];
+    __syncthreads();
+    // lane: row tid / 16, values V8 * (tid % 16) ..
+    const int rn = tid >> 4, dc = (tid & 15) * E;
+    const QRow orow = q_row(a, s.n_rows, h, rt * kAttRows + rn);
+    float mm = s_m[0][rn];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) mm = fmaxf(mm, s_m[w][rn]);
+    float ll = 0.0f, o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        const float al = exp2_hw(s_m[w][rn] - mm);
+        ll += s_l[w][rn] * al;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] += s_o[w][rn][dc + e] * al;
+    }
+    if (orow.i < 0) return;
+    if (s.n_parts > 1) {
+        float* po = a.part + (static_cast<int64_t>(item) * kAttRows + rn) * a.g.D;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (dc + e < a.g.D) po[dc + e] = o[e];
+        if ((tid & 15) == 0) {
+            float* pm = a.part_ml + (static_cast<int64_t>(item) * kAttRows + rn) * 2;
+            pm[0] = mm;
+            pm[1] = ll;
+        }
+        return;
+    }
+    const int64_t at = static_cast<int64_t>(s.row0 + orow.i) * a.Hq + orow.head;
+    const float inv = ll == 0.0f ? 0.0f : (a.v_scale != nullptr ? a.v_scale[h] : 1.0f) / ll;
+    uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + at * a.g.D;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const float x = ll == 0.0f ? 0.0f : o[e] * inv;
+        if (dc + e < a.g.D) out[dc + e] = static_cast<uint16_t>(QK == kBF16 ? f32_to_bf16(x) : f32_to_f16(x));
+    }
+    if ((tid & 15) == 0) a.lse[at] = ll == 0.0f ? -__builtin_huge_valf() : (mm + log2f(ll)) * kLn2;
+}
+
+// Joins the parts of 16 rows of one KV head.
+template <int QK, int DP>
+__global__ __launch_bounds__(256) void attend_join_kernel(DescArg d, AttArgs a) {
+    constexpr int E = DP / 16;
+    const DescPtr<AttSeq> seqs = desc_at<AttSeq>(d, 0);
+    const int group = static_cast<int>(blockIdx.x);
+    int lo = 0, hi = a.n_seqs - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (seqs[mid].at <= group) lo = mid; else hi = mid - 1;
+    }
+    const AttSeq s = desc_load(seqs + __builtin_amdgcn_readfirstlane(lo));
+    if (s.n_parts <= 1) return;
+    const int local = group - s.at;
+    const int rt = static_cast<int>(a.heads.div(static_cast<uint32_t>(local)));
+    const int h = local - rt * a.g.H;
+    const int row_tiles = (s.n_rows * a.G + kAttRows - 1) / kAttRows;
+    const int tid = static_cast<int>(threadIdx.x);
+    const int rn = tid >> 4, dc = (tid & 15) * E;
+    const QRow row = q_row(a, s.n_rows, h, rt * kAttRows + rn);
+    if (row.i < 0) return;
+    const int64_t first = (static_cast<int64_t>(s.tile_begin) + local) * kAttRows + rn;
+    const int64_t step = static_cast<int64_t>(row_tiles) * a.g.H * kAttRows;
+    float mm = -3.402823466e38f;
+    for (int p = 0; p < s.n_parts; ++p) mm = fmaxf(mm, a.part_ml[(first + p * step) * 2]);
+    float ll = 0.0f, o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.0f;
+    for (int p = 0; p < s.n_parts; ++p) {
+        const int64_t at = first + p * step;
+        const float al = exp2_hw(a.part_ml[at * 2] - mm);
+        ll += a.part_ml[at * 2 + 1] * al;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (dc + e < a.g.D) o[e] += a.part[at * a.g.D + dc + e] * al;
+    }
+    const int64_t at = static_cast<int64_t>(s.row0 + row.i) * a.Hq + row.head;
+    const float inv = (a.v_scale != nullptr ? a.v_scale[h] : 1.0f) / ll;
+    uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + at * a.g.D;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const float x = ll == 0.0f ? 0.0f : o[e] * inv;
+        if (dc + e < a.g.D) out[dc + e] = static_cast<uint16_t>(QK == kBF16 ? f32_to_bf16(x) : f32_to_f16(x));
+    }
+    if ((tid & 15) == 0) a.lse[at] = ll == 0.0f ? -__builtin_huge_valf() : (mm + log2f(ll)) * kLn2;
+}
+
+// ------------------------------------------------------------------- weigh
+// One workgroup: one KV head, 128 tokens, 32 to a wavefront, whose K rows stay
+// in registers while all rows of the sequence pass. Each token's sum is one
+// lane's, then 16 lanes', in a fixed order.
+template <int CK, int QK, int DP, int MODE>
+__global__ __launch_bounds__(256) void weigh_kernel(DescArg d, AttArgs a) {
+    using Rows = TileRows<CK, DP>;
+    constexpr int STEPS = DP / 32;
+    const DescPtr<AttSeq> seqs = desc_at<AttSeq>(d, 0);
+    const int item = static_cast<int>(blockIdx.x);
+    const int si = __builtin_amdgcn_readfirstlane(find_by_tile(seqs, a.n_seqs, item));
+    const AttSeq s = desc_load(seqs + si);
+    const int tid = static_cast<int>(threadIdx.x), lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 15, g = lane >> 4;
+    const int local = item - s.tile_begin;
+    const int tg = static_cast<int>(a.heads.div(static_cast<uint32_t>(local)));
+    const int h = local - tg * a.g.H;
+    const int total = s.n_ctx + s.n_rows;
+    const int t0 = tg * kWeighTokens + wave * kAttTile;
+    if (t0 >= total) return;
+    RowReader<CK, DP, MODE> rd;
+    rd.init(a, s.bt_offset, total, h, lane);
+    Rows r;
+    rd.template load<false>(r, t0);
+    const float c = a.scale_log2 * (a.k_scale != nullptr ? a.k_scale[h] : 1.0f);
+    const bool edge = r.ok != ~0u || t0 + kAttTile > s.n_ctx;
+    float sum[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum[j] = 0.0f;
+    const int rows = s.n_rows * a.G;
+    for (int R0 = 0; R0 < rows; R0 += kAttRows) {
+        const QRow row = q_row(a, s.n_rows, h, R0 + n);
+        u32x4 q[STEPS];
+        load_q<CK, DP, MODE>(a, s, row, g, q);
+        const float lse = row.i >= 0 ? a.lse[static_cast<int64_t>(s.row0 + row.i) * a.Hq + row.head] * (1.0f / kLn2)
+                                     : -__builtin_huge_valf();
+        f32x4 sc[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+#pragma unroll
+        for (int st = 0; st < STEPS; ++st) {
+            sc[0] = mfma<QK>(k_operand<CK, QK, DP>(r, 0, st), q[st], sc[0]);
+            sc[1] = mfma<QK>(k_operand<CK, QK, DP>(r, 1, st), q[st], sc[1]);
+        }
+        // a row that saw nothing (lse -inf) gives no weight
+        uint32_t vis = lse == -__builtin_huge_valf() ? 0u : r.ok;
+        if (edge) vis &= row_sees(a, s, row.i, t0);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float x = exp2_hw(fmaf(sc[j >> 2][j & 3], c, -lse));
+            const int b = 16 * (j >> 2) + 4 * g + (j & 3);
+            sum[j] += (vis >> b) & 1u ? x : 0.0f;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+#pragma unroll
+        for (int x = 1; x < 16; x <<= 1) sum[j] += __shfl_xor(sum[j], x, 64);
+    }
+    // lane n of a group takes its token n (8 tokens)
+    float mine = sum[0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) mine = n == j ? sum[j] : mine;
+    const int t = t0 + 16 * (n >> 2) + 4 * g + (n & 3);
+    if (n < 8 && t < total) {
+        float* w = a.weights + h * a.columns + s.at + t;
+        *w = a.add ? *w + mine : mine;
+    }
+}
+
+// Instances of the kernels for one pair of cache and query types.
+template <typename F>
+void for_forms(int dp, int mode, F&& f) {
+    using std::integral_constant;
+    const auto with = [&](auto dpc) {
+        if (mode == kAttWhole) f(dpc, integral_constant<int, kAttWhole>());
+        else if (mode == kAttPadded) f(dpc, integral_constant<int, kAttPadded>());
+        else f(dpc, integral_constant<int, kAttValues>());
+    };
+    if (dp == 64) with(integral_constant<int, 64>());
+    else if (dp == 128) with(integral_constant<int, 128>());
+    else with(integral_constant<int, 256>());
+}
+
+template <int CK, int QK>
+void run_attend(const DescArg& d, const AttArgs& a, const AttPlan& p, hipStream_t stream) {
+    for_forms(p.dp, p.mode, [&](auto dp, auto mode) {
+        DARIC_LAUNCH((attend_kernel<CK, QK, decltype(dp)::value, decltype(mode)::value>),
+                     static_cast<unsigned>(p.items), 256, 0, stream, d, a);
+    });
+    check_launch("attend_pages");
+}
+
+template <int CK, int QK>
+void run_weigh(const DescArg& d, const AttArgs& a, int mode, int dp, int64_t items, hipStream_t stream) {
+    for_forms(dp, mode, [&](auto dpc, auto modec) {
+        DARIC_LAUNCH((weigh_kernel<CK, QK, decltype(dpc)::value, decltype(modec)::value>),
+                     static_cast<unsigned>(items), 256, 0, stream, d, a);
+    });
+    check_launch("weigh_tokens");
+}
+
+}  // namespace attend
+}  // namespace daric

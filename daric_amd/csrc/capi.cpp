@@ -12,6 +12,9 @@
 #include <tuple>
 #include <unordered_map>
 
+#include <cmath>
+
+#include "attend.h"
 #include "common.h"
 #include "elem.h"
 #include "kernels.h"
@@ -1507,6 +1510,363 @@ int daric_select_merge(const daric_tensor* layers, int64_t n_layers, int page_fi
             DescHandOver ho2(t.device, blob.data(), blob.size(), st);   // inline: copied by value
             merge(ho2.arg(), 0);
         }
+    });
+}
+
+}  // extern "C"
+
+// ====================================================== attention and eviction
+namespace {
+
+constexpr int64_t kMaxHeadDim = 256;
+constexpr int64_t kMaxTokens = kIntMax - 1024;     // of a sequence: tiles past its end are still 32-bit
+
+// Ranges [begin, begin + n) that share no element.
+void check_apart(std::vector<std::pair<int64_t, int64_t>>& r, const char* what) {
+    bool ordered = true;
+    for (size_t i = 1; i < r.size(); ++i) ordered = ordered && r[i - 1].first + r[i - 1].second <= r[i].first;
+    if (ordered) return;
+    std::sort(r.begin(), r.end());
+    for (size_t i = 1; i < r.size(); ++i)
+        DARIC_CHECK(r[i - 1].first + r[i - 1].second <= r[i].first, what, " ", r[i].first, " is in two sequences");
+}
+
+// One attention or weigh call after its checks, except the block table's.
+struct AttCall {
+    AttArgs a{};
+    AttPlan p{};
+    std::vector<AttSeq> seqs;
+    int ck = 0, qk = 0, device = -1;
+    int64_t T = 0;
+};
+
+AttCall attention_call(const daric_tensor* layer, int page_first, const daric_tensor* q,
+                       const daric_sequence* sequences, int64_t n, bool weigh) {
+    const char* what = weigh ? "weigh_tokens" : "attend_pages";
+    AttCall c;
+    check_tensor_struct(layer, "kv layer");
+    const daric_tensor& t = *layer;
+    DARIC_CHECK(t.device >= 0, "KV cache tensor must be on CUDA");
+    c.device = t.device;
+    c.ck = elem_kind(t);
+    DARIC_CHECK(c.ck >= 0, "unsupported KV cache dtype for ", what);
+    if (t.ndim == 3) throw Error(DARIC_ERR_VALUE, cat(what, " needs a cache of K and V rows, not a 3-D (MLA) cache"));
+    AttArgs& a = c.a;
+    a.g = kv_geom(t, page_first != 0);
+    const KVGeom& g = a.g;
+    DARIC_CHECK(g.H > 0 && g.PS > 0 && g.num_blocks > 0, "KV cache must not be empty");
+    DARIC_CHECK(g.D <= kMaxHeadDim, what, " takes head_dim up to ", kMaxHeadDim, ", got ", g.D);
+    a.layer = static_cast<const uint8_t*>(t.data);
+
+    check_tensor_struct(q, "q");
+    DARIC_CHECK(q->device == t.device, "q must be on the layer's device");
+    c.qk = q->dtype == DARIC_DTYPE_BFLOAT16 ? kBF16 : q->dtype == DARIC_DTYPE_FLOAT16 ? kF16 : -1;
+    DARIC_CHECK(c.qk >= 0 && (c.ck == kE4M3 || c.ck == c.qk),
+                "q must have the cache's element type, or be bfloat16 or float16 for an fp8 (e4m3) cache");
+    DARIC_CHECK(q->ndim == 3 && q->sizes[2] == g.D && q->sizes[1] > 0 && q->sizes[1] % g.H == 0 &&
+                q->strides[2] == 1,
+                "q must be [T, Hq, D] with Hq a multiple of the cache's ", g.H, " heads, D = ", g.D,
+                " and the values of a head contiguous");
+    DARIC_CHECK(q->strides[0] >= 0 && q->strides[1] >= 0, "q must not have negative strides");
+    DARIC_CHECK(q->sizes[1] <= kIntMax / 2, "too many query heads");
+    a.q = static_cast<const uint8_t*>(q->data);
+    a.q_row = q->strides[0];
+    a.q_head = q->strides[1];
+    a.Hq = static_cast<int32_t>(q->sizes[1]);
+    a.G = a.Hq / g.H;
+    c.T = q->sizes[0];
+
+    DARIC_CHECK(n >= 0 && (n == 0 || sequences != nullptr), "sequences must not be null");
+    std::vector<std::pair<int64_t, int64_t>> rows;
+    rows.reserve(n);
+    c.seqs.reserve(n);
+    for (int64_t i = 0; i < n; ++i) {
+        const daric_sequence& s = sequences[i];
+        DARIC_CHECK(s.bt_offset >= 0 && s.row_start >= 0 && s.n_rows >= 0 && s.n_ctx >= 0 && s.col_start >= 0,
+                    "negative field of sequence ", i);
+        DARIC_CHECK(s.n_ctx <= kMaxTokens && s.n_rows <= kMaxTokens && s.n_ctx + s.n_rows <= kMaxTokens &&
+                    s.n_rows <= (kIntMax - kAttRows) / a.G, "sequence ", i, " is too long");
+        DARIC_CHECK(s.row_start <= c.T && s.n_rows <= c.T - s.row_start, "sequence ", i, " rows exceed q");
+        DARIC_CHECK(s.row_start <= kIntMax, "sequence ", i, " starts too far into q");
+        if (s.n_rows == 0) continue;      // nothing to compute
+        rows.emplace_back(s.row_start, s.n_rows);
+        AttSeq x{};
+        x.bt_offset = s.bt_offset;
+        x.row0 = static_cast<int32_t>(s.row_start);
+        x.n_rows = static_cast<int32_t>(s.n_rows);
+        x.n_ctx = static_cast<int32_t>(s.n_ctx);
+        c.seqs.push_back(x);
+    }
+    check_apart(rows, "row");
+
+    const int64_t es = t.elem_size;
+    const bool whole_units = aligned(t.data, 16) && (g.sb * es) % 16 == 0 && (g.ss * es) % 16 == 0 &&
+                             (g.sh * es) % 16 == 0 && (g.v_off * es) % 16 == 0 && aligned(q->data, 16) &&
+                             a.q_row % 8 == 0 && a.q_head % 8 == 0 && (g.D * es) % 16 == 0;
+    c.p.dp = g.D <= 64 ? 64 : g.D <= 128 ? 128 : 256;
+    c.p.mode = !whole_units ? kAttValues : g.D == c.p.dp ? kAttWhole : kAttPadded;
+    a.group = FastDiv(static_cast<uint32_t>(a.G));
+    a.page = FastDiv(static_cast<uint32_t>(g.PS));
+    a.heads = FastDiv(static_cast<uint32_t>(g.H));
+    a.n_seqs = static_cast<int32_t>(c.seqs.size());
+    return c;
+}
+
+// Parts of the sequences' tokens: about kAttendGroups workgroups in all.
+constexpr int64_t kAttendGroups = 1024;
+void plan_attend(AttCall& c) {
+    int64_t work = 0;
+    for (const AttSeq& s : c.seqs) {
+        const int64_t row_tiles = (static_cast<int64_t>(s.n_rows) * c.a.G + kAttRows - 1) / kAttRows;
+        work += (static_cast<int64_t>(s.n_ctx) + s.n_rows + kAttTile - 1) / kAttTile * row_tiles * c.a.g.H;
+    }
+    const int64_t part = std::min<int64_t>(((work + kAttendGroups - 1) / kAttendGroups + 3) / 4 * 4, 1 << 26);
+    c.a.part_tiles = static_cast<int32_t>(std::max<int64_t>(part, 4));
+    for (AttSeq& s : c.seqs) {
+        const int64_t row_tiles = (static_cast<int64_t>(s.n_rows) * c.a.G + kAttRows - 1) / kAttRows;
+        const int64_t tiles = (static_cast<int64_t>(s.n_ctx) + s.n_rows + kAttTile - 1) / kAttTile;
+        const int64_t parts = (tiles + c.a.part_tiles - 1) / c.a.part_tiles;
+        s.tile_begin = static_cast<int32_t>(c.p.items);
+        s.at = static_cast<int32_t>(c.p.groups);
+        s.n_parts = static_cast<int32_t>(parts);
+        c.p.items += parts * row_tiles * c.a.g.H;
+        c.p.groups += row_tiles * c.a.g.H;
+        c.p.join = c.p.join || parts > 1;
+        DARIC_CHECK(c.p.items <= kMaxTiles, "too many rows in one attend_pages call");
+    }
+}
+int64_t attend_bytes(const AttCall& c) {
+    return c.p.join ? c.p.items * kAttRows * (c.a.g.D + 2) * static_cast<int64_t>(sizeof(float)) : 0;
+}
+
+void attention_inputs(AttCall& c, const daric_tensor* block_table, const daric_sequence* sequences, int64_t n,
+                      const daric_tensor* tree_mask, float scale, const daric_tensor* k_scale,
+                      const daric_tensor* v_scale) {
+    AttArgs& a = c.a;
+    check_block_table(block_table, c.device);
+    a.block_table = static_cast<const int32_t*>(block_table->data);
+    const int64_t bt_n = numel(*block_table);
+    int64_t longest = 0;
+    for (int64_t i = 0; i < n; ++i) {
+        const daric_sequence& s = sequences[i];
+        const int64_t pages = (s.n_ctx + s.n_rows + a.g.PS - 1) / a.g.PS;
+        DARIC_CHECK(s.bt_offset <= bt_n && pages <= bt_n - s.bt_offset, "sequence ", i,
+                    " reads past the end of block_table");
+        longest = std::max(longest, s.n_rows);
+    }
+    if (tree_mask != nullptr) {
+        check_tensor_struct(tree_mask, "tree_mask");
+        DARIC_CHECK(tree_mask->device == c.device && tree_mask->dtype == DARIC_DTYPE_INT64 && tree_mask->ndim == 2 &&
+                    tree_mask->sizes[0] == c.T && is_contiguous(*tree_mask),
+                    "tree_mask must be a contiguous int64 [T, words] tensor on the layer's device");
+        DARIC_CHECK(tree_mask->sizes[1] <= kIntMax / 64 && tree_mask->sizes[1] * 64 >= longest,
+                    "tree_mask has ", tree_mask->sizes[1], " words for ", longest, " rows");
+        a.mask = static_cast<const uint64_t*>(tree_mask->data);
+        a.words = static_cast<int32_t>(tree_mask->sizes[1]);
+    }
+    const auto scales = [&](const daric_tensor* s, const char* what) -> const float* {
+        if (s == nullptr || s->data == nullptr) return nullptr;
+        check_tensor_struct(s, what);
+        DARIC_CHECK(c.ck == kE4M3, what, " applies to fp8 (e4m3) caches only");
+        DARIC_CHECK(s->device == c.device && s->dtype == DARIC_DTYPE_FLOAT32 && is_contiguous(*s) &&
+                    numel(*s) == a.g.H, what, " must be a contiguous float32 [H] tensor on the layer's device");
+        return static_cast<const float*>(s->data);
+    };
+    a.k_scale = scales(k_scale, "k_scale");
+    a.v_scale = scales(v_scale, "v_scale");
+    DARIC_CHECK(std::isfinite(scale), "scale must be finite");
+    a.scale_log2 = scale * 1.44269504088896341f;
+}
+
+const float* check_lse(const AttCall& c, const daric_tensor* lse) {
+    check_tensor_struct(lse, "lse");
+    DARIC_CHECK(lse->device == c.device && lse->dtype == DARIC_DTYPE_FLOAT32 && lse->ndim == 2 &&
+                lse->sizes[0] == c.T && lse->sizes[1] == c.a.Hq && is_contiguous(*lse),
+                "lse must be a contiguous float32 [T, Hq] tensor on the layer's device");
+    return static_cast<const float*>(lse->data);
+}
+
+}  // namespace
+
+extern "C" {
+
+int daric_attend_workspace(const daric_tensor* layer, int page_first, const daric_tensor* q,
+                           const daric_sequence* sequences, int64_t n_sequences, int64_t* bytes) {
+    return guarded([&] {
+        DARIC_CHECK(bytes != nullptr, "bytes must not be null");
+        AttCall c = attention_call(layer, page_first, q, sequences, n_sequences, false);
+        plan_attend(c);
+        *bytes = attend_bytes(c);
+    });
+}
+
+int daric_attend_pages(const daric_tensor* layer, int page_first, const daric_tensor* block_table,
+                       const daric_tensor* q, const daric_sequence* sequences, int64_t n_sequences,
+                       const daric_tensor* tree_mask, float scale, const daric_tensor* k_scale,
+                       const daric_tensor* v_scale, daric_tensor* out, daric_tensor* lse,
+                       void* workspace, int64_t workspace_bytes, uint64_t stream) {
+    return guarded([&] {
+        AttCall c = attention_call(layer, page_first, q, sequences, n_sequences, false);
+        attention_inputs(c, block_table, sequences, n_sequences, tree_mask, scale, k_scale, v_scale);
+        check_tensor_struct(out, "out");
+        DARIC_CHECK(out->device == c.device && out->dtype == q->dtype && out->ndim == 3 && out->sizes[0] == c.T &&
+                    out->sizes[1] == c.a.Hq && out->sizes[2] == c.a.g.D && is_contiguous(*out),
+                    "out must be a contiguous [T, Hq, D] tensor of q's type on the layer's device");
+        c.a.lse = const_cast<float*>(check_lse(c, lse));
+        c.a.out = static_cast<uint8_t*>(out->data);
+        if (c.seqs.empty()) return;
+        plan_attend(c);
+        const int64_t need = attend_bytes(c);
+        DARIC_CHECK(need == 0 || (workspace != nullptr && workspace_bytes >= need && aligned(workspace, 16)),
+                    "workspace must be 16-byte aligned and hold ", need, " bytes, got ", workspace_bytes);
+        c.a.part = static_cast<float*>(workspace);
+        if (need > 0) c.a.part_ml = c.a.part + c.p.items * kAttRows * c.a.g.D;
+        DeviceGuard guard(c.device);
+        const hipStream_t st = as_stream(stream);
+        DescHandOver ho(c.device, c.seqs.data(), c.seqs.size() * sizeof(AttSeq), st);
+        if (c.ck == kBF16) attend_bf16(ho.arg(), c.a, c.p, st);
+        else if (c.ck == kF16) attend_f16(ho.arg(), c.a, c.p, st);
+        else if (c.qk == kBF16) attend_e4m3_bf16(ho.arg(), c.a, c.p, st);
+        else attend_e4m3_f16(ho.arg(), c.a, c.p, st);
+        if (!c.p.join) return;
+        if (c.qk == kBF16) join_bf16(ho.arg(), c.a, c.p, st);
+        else join_f16(ho.arg(), c.a, c.p, st);
+    });
+}
+
+int daric_weigh_tokens(const daric_tensor* layer, int page_first, const daric_tensor* block_table,
+                       const daric_tensor* q, const daric_tensor* lse, const daric_sequence* sequences,
+                       int64_t n_sequences, const daric_tensor* tree_mask, float scale,
+                       const daric_tensor* k_scale, daric_tensor* weights, int accumulate, uint64_t stream) {
+    return guarded([&] {
+        AttCall c = attention_call(layer, page_first, q, sequences, n_sequences, true);
+        attention_inputs(c, block_table, sequences, n_sequences, tree_mask, scale, k_scale, nullptr);
+        c.a.lse = const_cast<float*>(check_lse(c, lse));
+        check_tensor_struct(weights, "weights");
+        DARIC_CHECK(weights->device == c.device && weights->dtype == DARIC_DTYPE_FLOAT32 && weights->ndim == 2 &&
+                    weights->sizes[0] == c.a.g.H && (weights->strides[1] == 1 || weights->sizes[1] <= 1) &&
+                    (weights->strides[0] >= weights->sizes[1] || weights->sizes[0] == 1),
+                    "weights must be a float32 [H, columns] tensor with contiguous columns on the layer's device");
+        const int64_t columns = weights->sizes[1];
+        std::vector<std::pair<int64_t, int64_t>> cols;
+        size_t at = 0;
+        int64_t items = 0;
+        for (int64_t i = 0; i < n_sequences; ++i) {
+            const daric_sequence& s = sequences[i];
+            const int64_t total = s.n_ctx + s.n_rows;
+            DARIC_CHECK(s.col_start <= columns && total <= columns - s.col_start && s.col_start <= kIntMax,
+                        "sequence ", i, " columns exceed weights");
+            if (s.n_rows == 0) continue;
+            cols.emplace_back(s.col_start, total);
+            AttSeq& x = c.seqs[at++];
+            x.at = static_cast<int32_t>(s.col_start);
+            x.tile_begin = static_cast<int32_t>(items);
+            items += (total + kWeighTokens - 1) / kWeighTokens * c.a.g.H;
+            DARIC_CHECK(items <= kMaxTiles, "too many tokens in one weigh_tokens call");
+        }
+        check_apart(cols, "column");
+        c.a.weights = static_cast<float*>(weights->data);
+        c.a.columns = weights->sizes[0] == 1 ? columns : weights->strides[0];
+        c.a.add = accumulate ? 1 : 0;
+        if (c.seqs.empty()) return;
+        DeviceGuard guard(c.device);
+        const hipStream_t st = as_stream(stream);
+        DescHandOver ho(c.device, c.seqs.data(), c.seqs.size() * sizeof(AttSeq), st);
+        if (c.ck == kBF16) weigh_bf16(ho.arg(), c.a, c.p.mode, c.p.dp, items, st);
+        else if (c.ck == kF16) weigh_f16(ho.arg(), c.a, c.p.mode, c.p.dp, items, st);
+        else if (c.qk == kBF16) weigh_e4m3_bf16(ho.arg(), c.a, c.p.mode, c.p.dp, items, st);
+        else weigh_e4m3_f16(ho.arg(), c.a, c.p.mode, c.p.dp, items, st);
+    });
+}
+
+int daric_evict_tokens(const daric_tensor* layers, int64_t n_layers, int page_first,
+                       const daric_tensor* block_table, daric_tensor* weights,
+                       const daric_eviction* evictions, int64_t n, daric_tensor* kept,
+                       daric_tensor* workspace, uint64_t stream) {
+    return guarded([&] {
+        DARIC_CHECK(n_layers > 0 && layers != nullptr, "layers must not be empty");
+        for (int64_t i = 0; i < n_layers; ++i) check_tensor_struct(&layers[i], "kv layer");
+        check_same_layers(layers, n_layers);
+        const daric_tensor& t = layers[0];
+        DARIC_CHECK(t.device >= 0, "KV cache tensor must be on CUDA");
+        const KVGeom g = kv_geom(t, page_first != 0);
+        DARIC_CHECK(g.H > 0 && g.PS > 0 && g.num_blocks > 0, "KV cache must not be empty");
+        check_block_table(block_table, t.device);
+        check_tensor_struct(weights, "weights");
+        DARIC_CHECK(weights->device == t.device && weights->dtype == DARIC_DTYPE_FLOAT32 && weights->ndim == 3 &&
+                    weights->sizes[0] == n_layers && (weights->sizes[1] == g.H || weights->sizes[1] == 1) &&
+                    is_contiguous(*weights),
+                    "weights must be a contiguous float32 [n_layers, H or 1, columns] tensor on the layers' device");
+        const int64_t heads = weights->sizes[1], columns = weights->sizes[2];
+        DARIC_CHECK(n >= 0 && (n == 0 || evictions != nullptr), "evictions must not be null");
+        const int64_t bt_n = numel(*block_table);
+        std::vector<EvictSeq> seqs;
+        std::vector<std::pair<int64_t, int64_t>> cols;
+        seqs.reserve(n);
+        int64_t kmax = 0, most = 0, slots = 0;
+        for (int64_t i = 0; i < n; ++i) {
+            const daric_eviction& s = evictions[i];
+            DARIC_CHECK(s.bt_offset >= 0 && s.col_start >= 0 && s.n_tokens >= 0 && s.keep >= 0 && s.n_first >= 0 &&
+                        s.n_recent >= 0, "negative field of eviction ", i);
+            DARIC_CHECK(s.n_tokens <= kMaxTokens && s.keep <= kIntMax, "eviction ", i, " is too long");
+            DARIC_CHECK(s.n_first <= s.keep && s.n_recent <= s.keep - s.n_first, "eviction ", i,
+                        ": n_first + n_recent must not exceed keep");
+            DARIC_CHECK(s.col_start <= columns && s.n_tokens <= columns - s.col_start, "eviction ", i,
+                        " columns exceed weights");
+            const int64_t pages = (s.n_tokens + g.PS - 1) / g.PS;
+            DARIC_CHECK(s.bt_offset <= bt_n && pages <= bt_n - s.bt_offset, "eviction ", i,
+                        " reads past the end of block_table");
+            if (s.n_tokens > 0) cols.emplace_back(s.col_start, s.n_tokens);
+            EvictSeq x{};
+            x.bt_offset = s.bt_offset;
+            x.col0 = s.col_start;
+            x.n = static_cast<int32_t>(s.n_tokens);
+            x.keep = static_cast<int32_t>(s.keep);
+            x.first = static_cast<int32_t>(s.n_first);
+            x.recent = static_cast<int32_t>(s.n_recent);
+            seqs.push_back(x);
+            kmax = std::max(kmax, std::min(s.keep, s.n_tokens));
+            if (s.n_tokens > s.keep) {
+                most = std::max(most, s.n_tokens - s.n_first - s.n_recent);
+                slots = std::max(slots, s.keep);
+            }
+        }
+        check_apart(cols, "column");
+        const auto check_ids = [&](const daric_tensor* x, const char* what) {
+            check_tensor_struct(x, what);
+            DARIC_CHECK(x->device == t.device && x->dtype == DARIC_DTYPE_INT32 && x->ndim == 4 &&
+                        x->sizes[0] == n_layers && x->sizes[1] == heads && x->sizes[2] == n && is_contiguous(*x) &&
+                        x->sizes[3] >= kmax, what, " must be a contiguous int32 [n_layers, H or 1, n_evictions, kmax] "
+                        "tensor on the layers' device with kmax at least ", kmax);
+        };
+        check_ids(kept, "kept");
+        check_ids(workspace, "workspace");
+        DARIC_CHECK(workspace->sizes[3] == kept->sizes[3], "workspace must have kept's shape");
+        const int64_t width = kept->sizes[3];
+        DARIC_CHECK(n <= kMaxTiles && width <= kIntMax, "too many evictions in one call");
+        if (n == 0) return;
+        int64_t unit = 16;
+        const int64_t es = t.elem_size;
+        const auto allows = [&](int64_t u) {
+            bool ok = (g.D * es) % u == 0 && (g.sb * es) % u == 0 && (g.ss * es) % u == 0 && (g.sh * es) % u == 0 &&
+                      (g.v_off < 0 || (g.v_off * es) % u == 0);
+            for (int64_t i = 0; ok && i < n_layers; ++i) ok = aligned(layers[i].data, u);
+            return ok;
+        };
+        while (unit > 1 && !allows(unit)) unit /= 2;
+        DeviceGuard guard(t.device);
+        const hipStream_t st = as_stream(stream);
+        const size_t cb = seqs.size() * sizeof(EvictSeq);
+        std::vector<uint8_t> blob(cb + n_layers * sizeof(uint8_t*));
+        std::memcpy(blob.data(), seqs.data(), cb);
+        const auto ptrs = layer_ptrs(layers, n_layers);
+        std::memcpy(blob.data() + cb, ptrs.data(), n_layers * sizeof(uint8_t*));
+        DescHandOver ho(t.device, blob.data(), blob.size(), st);
+        launch_evict(ho.arg(), static_cast<int>(cb), static_cast<int>(n_layers), g, static_cast<int>(es),
+                     static_cast<int>(unit), static_cast<const int32_t*>(block_table->data),
+                     static_cast<float*>(weights->data), columns, static_cast<int>(heads), static_cast<int>(n),
+                     static_cast<int>(most), static_cast<int>(slots), static_cast<int32_t*>(workspace->data),
+                     static_cast<int32_t*>(kept->data), static_cast<int>(width), st);
     });
 }
 

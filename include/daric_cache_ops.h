@@ -384,6 +384,95 @@ int daric_select_merge(const daric_tensor* layers, int64_t n_layers, int page_fi
                        const daric_tensor* k_scales, const daric_tensor* v_scales,
                        daric_tensor* keys, daric_tensor* sel_idx, int flags, uint64_t stream);
 
+/* ---------------------------------------------------------------------- */
+/* Attention over the paged cache and eviction from it (new entry points;   */
+/* no counterpart in the reference, whose attention is vLLM's).             */
+/* ---------------------------------------------------------------------- */
+
+/* A sequence of an attention call. Its query rows are rows
+ * [row_start, row_start + n_rows) of q; the K and V of these rows stand in the
+ * cache behind its n_ctx cached tokens: token j < n_ctx + n_rows is in page
+ * block_table[bt_offset + j / PS] at slot j % PS. A token whose page id is 0 (the
+ * null block) or outside [1, num_blocks) is not there: no row sees it.
+ * col_start: the column of `weights` of token 0 (daric_weigh_tokens only). */
+typedef struct daric_sequence {
+    int64_t bt_offset;
+    int64_t row_start;
+    int64_t n_rows;
+    int64_t n_ctx;
+    int64_t col_start;
+} daric_sequence;
+
+/* out[r, h] = v_scale[g] * sum over visible j of P V[j, g], with
+ * P = exp(s - lse), s = scale * k_scale[g] * <q[r, h], K[j, g]>, g = h / (Hq / H) and
+ * lse[r, h] = log(sum of exp(s)). Every row sees all n_ctx cached tokens of its
+ * sequence that are there. Of the n_rows tokens behind them, row i sees tokens
+ * 0..i (tree_mask NULL), or those whose bits are set in its mask row: bit b of
+ * word w says that it sees token n_ctx + 64 w + b. A row that sees nothing
+ * (or only scores of -inf) gets zeros and lse -inf. What a row does not see has
+ * no effect on it, whatever its K and V hold.
+ * layer: one paged cache with K and V (not a 3-D MLA cache), bfloat16, float16
+ * or e4m3, head_dim 2..256. q: [T, Hq, D], values of a head contiguous, other
+ * strides free, in the cache's type; bfloat16 or float16 for an e4m3 cache.
+ * tree_mask: contiguous int64 [T, words], 64 * words >= the longest n_rows.
+ * k_scale, v_scale: NULL (1) or contiguous fp32 [H], for an e4m3 cache only.
+ * out: contiguous [T, Hq, D] of q's type; lse: contiguous fp32 [T, Hq]; rows of
+ * no sequence are not written, and no row may be in two. workspace: at least
+ * the bytes that daric_attend_workspace gives for the same arguments (NULL where
+ * that is 0), in use until the call's work on `stream` is done.
+ * Sums and softmax statistics are fp32; the weights P are rounded to q's type
+ * for the product with V. The same call gives the same bits. */
+int daric_attend_workspace(const daric_tensor* layer, int page_first, const daric_tensor* q,
+                           const daric_sequence* sequences, int64_t n_sequences, int64_t* bytes);
+int daric_attend_pages(const daric_tensor* layer, int page_first, const daric_tensor* block_table,
+                       const daric_tensor* q, const daric_sequence* sequences, int64_t n_sequences,
+                       const daric_tensor* tree_mask, float scale, const daric_tensor* k_scale,
+                       const daric_tensor* v_scale, daric_tensor* out, daric_tensor* lse,
+                       void* workspace, int64_t workspace_bytes, uint64_t stream);
+
+/* weights[g, col_start + j] (+)= sum over the sequence's rows r that see token j
+ * and the heads h of KV head g of exp(s - lse[r, h]): the attention weight the
+ * token received, of the attention that daric_attend_pages computes. lse:
+ * contiguous fp32 [T, Hq] (rows with -inf add nothing). weights: fp32 [H, columns],
+ * columns contiguous. accumulate 1 adds to it, 0 sets the columns of every sequence
+ * that has rows. Other columns are not written; no column may be in two sequences.
+ * Sums are fp32, in a fixed order. */
+int daric_weigh_tokens(const daric_tensor* layer, int page_first, const daric_tensor* block_table,
+                       const daric_tensor* q, const daric_tensor* lse, const daric_sequence* sequences,
+                       int64_t n_sequences, const daric_tensor* tree_mask, float scale,
+                       const daric_tensor* k_scale, daric_tensor* weights, int accumulate, uint64_t stream);
+
+/* A sequence of an eviction: token j < n_tokens is in page
+ * block_table[bt_offset + j / PS] at slot j % PS, its weight in column
+ * col_start + j. */
+typedef struct daric_eviction {
+    int64_t bt_offset;
+    int64_t col_start;
+    int64_t n_tokens;
+    int64_t keep;        /* tokens that stay (all, if it has no more) */
+    int64_t n_first;     /* first and last tokens that always stay; */
+    int64_t n_recent;    /* n_first + n_recent <= keep */
+} daric_eviction;
+
+/* Keeps, per layer and head, the first n_first and the last n_recent tokens of a
+ * sequence and the heaviest of the others (weights ordered as
+ * daric_topk_per_chunk orders keys, ties to the lower token), `keep` in all, and
+ * brings them to its first `keep` slots: kept tokens that stand there stay, and
+ * the i-th slot whose token goes takes the i-th kept token from behind. Slots
+ * from `keep` on keep their rows. kept[l, h, i, slot] is the token that slot
+ * holds now (-1 from min(keep, n_tokens) on); the sequence's weights move alike, and
+ * columns col_start + keep .. + n_tokens are set to 0.
+ * weights: contiguous fp32 [n_layers, H, columns], or [n_layers, 1, columns]: one
+ * selection for all heads of a layer. kept: contiguous int32
+ * [n_layers, H or 1, n_evictions, kmax], kmax >= each min(keep, n_tokens). workspace:
+ * int32 of as many elements as kept. Rows are moved as bytes: layers of any type;
+ * a row whose page id, or whose slot's, is 0 or outside [1, num_blocks) is not
+ * moved. A page may be in one sequence of a call only, and no column in two. */
+int daric_evict_tokens(const daric_tensor* layers, int64_t n_layers, int page_first,
+                       const daric_tensor* block_table, daric_tensor* weights,
+                       const daric_eviction* evictions, int64_t n_evictions, daric_tensor* kept,
+                       daric_tensor* workspace, uint64_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,202 @@
+"""Attention, weighing and eviction without a GPU: the oracle against torch and
+brute force, and every refusal of the C ABI and the Python layer (fake device
+pointers; each case fails before any device call)."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from daric_amd import _lib, cache_ops
+from oracle import attend as oatt
+from tests.gpu_util import make_layer
+from tests.test_capi_cpu import fake
+
+lib = pytest.fixture(scope="module")(lambda: _lib.load())
+
+
+# ------------------------------------------------------------------ the oracle
+@pytest.mark.parametrize("layout", ["nhd", "hnd", "pf", "packed"])
+def test_oracle_attention_is_softmax_attention(layout):
+    g = torch.Generator().manual_seed(3)
+    layer, pf = make_layer(layout, 9, 4, 2, 8, torch.float16, g)
+    bt = np.array([5, 3, 8, 1], np.int32)
+    q = torch.randn(5, 4, 8, generator=g).to(torch.float16)
+    out, lse, *_ = oatt.attend(layer, pf, bt, q, [(0, 0, 5, 9)], scale=0.3)
+    k = torch.from_numpy(oatt.gather(oatt.k_rows_view(layer, pf), bt, 0, 14)[0]).repeat_interleave(2, 1).transpose(0, 1)
+    v = torch.from_numpy(oatt.gather(oatt.v_view(layer, pf), bt, 0, 14)[0]).repeat_interleave(2, 1).transpose(0, 1)
+    see = torch.arange(14)[None, :] <= torch.arange(5)[:, None] + 9
+    s = (q.double().transpose(0, 1) @ k.transpose(1, 2) * 0.3).masked_fill(~see, -torch.inf)
+    want = (s.softmax(-1) @ v).transpose(0, 1)
+    assert torch.allclose(torch.from_numpy(out), want, atol=1e-12)
+    assert torch.allclose(torch.from_numpy(lse), s.logsumexp(-1).t(), atol=1e-12)
+    w, *_ = oatt.weigh(layer, pf, bt, q, torch.from_numpy(lse), [(0, 0, 5, 9, 2)], np.ones((2, 17)), scale=0.3)
+    p = s.softmax(-1).sum(1).view(2, 2, 14).sum(1).numpy()
+    assert np.allclose(w[:, 2:16], 1 + p, atol=1e-12) and (w[:, [0, 1, 16]] == 1).all()
+
+
+def test_oracle_tree_and_missing_pages():
+    # draft 2 sees drafts 0 and 2; the null page's tokens are not there
+    assert oatt.sees(2, 3, 3, [0b101]).tolist() == [True] * 3 + [True, False, True]
+    wide = [1 << 63, 1]
+    assert np.nonzero(oatt.sees(0, 0, 70, wide))[0].tolist() == [63, 64]
+    layer, pf = make_layer("nhd", 4, 2, 1, 2, torch.float16, torch.Generator().manual_seed(0))
+    assert oatt.gather(oatt.k_rows_view(layer, pf), [1, 0, 9, 3], 0, 8)[1].tolist() == [True] * 2 + [False] * 4 + [True] * 2
+
+
+def test_oracle_eviction_keeps_the_heaviest_and_moves_few():
+    layer, pf = make_layer("nhd", 8, 2, 1, 2, torch.float16, torch.Generator().manual_seed(1))
+    before = layer.clone()
+    bt = [4, 2, 7, 1, 5]
+    w = np.array([[[0, 5, 1, 7, 2, 9, 2, 0, 3, 8]]], np.float32)
+    kept = oatt.evict([layer], pf, bt, w, [(0, 0, 10, 5, 1, 1)], 5)
+    # stay: 0 (first), 9 (recent), 5 (9), 3 (7), 1 (5); slots 2 and 4 are free, taken by 5 and 9
+    assert kept[0, 0, 0].tolist() == [0, 1, 5, 3, 9]
+    assert w[0, 0].tolist() == [0, 5, 9, 7, 8, 0, 0, 0, 0, 0]
+    k, kb = layer[0], before[0]
+    assert torch.equal(k[2, 0], kb[7, 1]) and torch.equal(k[7, 0], kb[5, 1]) and torch.equal(k[5], kb[5])
+
+
+# ------------------------------------------------------------------ the C ABI
+def seqs(*s):
+    a = np.array(s, np.int64).reshape(-1, 5)
+    return a.ctypes.data, len(a), a
+
+
+def test_attention_refusals(lib):
+    layer = fake((2, 8, 16, 4, 64), torch.bfloat16)
+    f8 = fake((2, 8, 16, 4, 64), torch.uint8)
+    bt = fake((8,), torch.int32, ptr=0x20000000)
+    q = fake((10, 8, 64), torch.bfloat16, ptr=0x30000000)
+    out = fake((10, 8, 64), torch.bfloat16, ptr=0x40000000)
+    lse = fake((10, 8), torch.float32, ptr=0x50000000)
+    w = fake((4, 200), torch.float32, ptr=0x60000000)
+    ok = (0, 0, 10, 100, 0)
+
+    def run(lay=layer, s=(ok,), q_=q, bt_=bt, mask=None, scale=1.0, ks=None, vs=None, out_=out, lse_=lse, w_=w, pf=0,
+            weigh=False):
+        ref = lambda t: ctypes.byref(t) if t is not None else None
+        addr, n, _k = seqs(*s)
+        if weigh:
+            st = lib.daric_weigh_tokens(ref(lay), pf, ref(bt_), ref(q_), ref(lse_), addr, n, ref(mask), scale, ref(ks),
+                                        ref(w_), 1, ctypes.c_uint64(0))
+        else:
+            need = ctypes.c_int64()
+            if lib.daric_attend_workspace(ref(lay), pf, ref(q_), addr, n, ctypes.byref(need)) == 0:
+                st = lib.daric_attend_pages(ref(lay), pf, ref(bt_), ref(q_), addr, n, ref(mask), scale, ref(ks), ref(vs),
+                                            ref(out_), ref(lse_), 0x70000000, need.value, ctypes.c_uint64(0))
+            else:
+                st = 1
+        assert st != 0
+        return lib.daric_last_error().decode()
+
+    for weigh in (False, True):
+        r = lambda **k: run(weigh=weigh, **k)
+        assert "unsupported KV cache dtype" in r(lay=fake((2, 8, 16, 4, 64), torch.float32))
+        assert "3-D (MLA) cache" in r(lay=fake((8, 16, 64), torch.bfloat16), pf=1)
+        assert "head_dim up to 256" in r(lay=fake((2, 8, 16, 4, 288), torch.bfloat16))
+        assert "q must have the cache's element type" in r(q_=fake((10, 8, 64), torch.float16))
+        assert "q must have the cache's element type" in r(q_=fake((10, 8, 64), torch.float32))
+        assert "multiple of the cache's 4 heads" in r(q_=fake((10, 6, 64), torch.bfloat16))
+        assert "multiple of the cache's 4 heads" in r(q_=fake((10, 8, 32), torch.bfloat16))
+        assert "multiple of the cache's 4 heads" in r(q_=fake((10, 512), torch.bfloat16))
+        assert "q must be on the layer's device" in r(q_=fake((10, 8, 64), torch.bfloat16, device=-1))
+        assert "negative field of sequence 0" in r(s=((0, 0, -1, 4, 0),))
+        assert "negative field of sequence 1" in r(s=((0, 0, 1, 4, 0), (0, 1, 1, -4, 50)))
+        assert "rows exceed q" in r(s=((0, 5, 6, 4, 0),))
+        assert "is too long" in r(s=((0, 0, 1, 2 ** 31, 0),))
+        assert "is too long" in r(s=((0, 0, 1, 2 ** 62, 0),))
+        assert "row 4 is in two sequences" in r(s=((0, 4, 2, 4, 50), (0, 0, 5, 4, 0)))
+        assert "reads past the end of block_table" in r(s=((2, 0, 10, 100, 0),))
+        assert "reads past the end of block_table" in r(s=((2 ** 62, 0, 1, 0, 0),))
+        assert "block_table must be a 1-D contiguous int32" in r(bt_=fake((8,), torch.int64))
+        assert "scale must be finite" in r(scale=float("nan"))
+        assert "tree_mask must be" in r(mask=fake((9, 1), torch.int64))
+        assert "tree_mask must be" in r(mask=fake((10, 1), torch.int32))
+        assert "tree_mask has 0 words for 10 rows" in r(mask=fake((10, 0), torch.int64))
+        assert "k_scale applies to fp8" in r(ks=fake((4,), torch.float32))
+        assert "k_scale must be a contiguous float32 [H]" in r(lay=f8, ks=fake((5,), torch.float32))
+        assert "lse must be" in r(lse_=fake((10, 4), torch.float32))
+    assert "v_scale applies to fp8" in run(vs=fake((4,), torch.float32))
+    assert "out must be" in run(out_=fake((10, 8, 64), torch.float16))
+    assert "weights must be" in run(weigh=True, w_=fake((8, 200), torch.float32))
+    assert "columns exceed weights" in run(weigh=True, s=((0, 0, 10, 100, 91),))
+    assert "column 60 is in two sequences" in run(weigh=True, s=((0, 0, 4, 70, 0), (0, 4, 2, 10, 60)))
+
+
+def test_attention_needs_its_workspace(lib):
+    layer = fake((2, 4000, 16, 4, 64), torch.bfloat16)
+    q, out = fake((1, 8, 64), torch.bfloat16), fake((1, 8, 64), torch.bfloat16, ptr=0x40000000)
+    bt, lse = fake((4000,), torch.int32), fake((1, 8), torch.float32, ptr=0x50000000)
+    addr, n, _k = seqs((0, 0, 1, 60000, 0))
+    need = ctypes.c_int64()
+    r = ctypes.byref
+    assert lib.daric_attend_workspace(r(layer), 0, r(q), addr, n, r(need)) == 0 and need.value > 0
+    for ptr, size in ((None, 0), (0x70000000, need.value - 1), (0x70000004, need.value)):
+        assert lib.daric_attend_pages(r(layer), 0, r(bt), r(q), addr, n, None, 1.0, None, None, r(out), r(lse), ptr, size,
+                                      ctypes.c_uint64(0)) == 1
+        assert b"workspace must be 16-byte aligned" in lib.daric_last_error()
+
+
+def test_nothing_to_attend_makes_no_device_call(lib):
+    layer = fake((2, 8, 16, 4, 64), torch.bfloat16)
+    bt, q = fake((8,), torch.int32), fake((10, 8, 64), torch.bfloat16)
+    out, lse = fake((10, 8, 64), torch.bfloat16), fake((10, 8), torch.float32)
+    w = fake((4, 200), torch.float32)
+    r = ctypes.byref
+    for s in ((), ((0, 0, 0, 100, 0),)):
+        addr, n, _k = seqs(*s)
+        need = ctypes.c_int64(7)
+        assert lib.daric_attend_workspace(r(layer), 0, r(q), addr, n, r(need)) == 0 and need.value == 0
+        assert lib.daric_attend_pages(r(layer), 0, r(bt), r(q), addr, n, None, 1.0, None, None, r(out), r(lse), None, 0,
+                                      ctypes.c_uint64(0)) == 0
+        assert lib.daric_weigh_tokens(r(layer), 0, r(bt), r(q), r(lse), addr, n, None, 1.0, None, r(w), 1,
+                                      ctypes.c_uint64(0)) == 0
+
+
+def test_eviction_refusals(lib):
+    layers = (_lib.DaricTensor * 2)(*[fake((2, 8, 16, 4, 64), torch.bfloat16, ptr=0x10000000 * (i + 1)) for i in range(2)])
+    bt = fake((8,), torch.int32)
+    w = fake((2, 4, 200), torch.float32)
+    kept = fake((2, 4, 1, 50), torch.int32)
+
+    def run(s=((0, 0, 100, 50, 0, 0),), w_=w, kept_=kept, ws=None, lay=layers, bt_=bt):
+        a = np.array(s, np.int64).reshape(-1, 6)
+        r = ctypes.byref
+        st = lib.daric_evict_tokens(lay, 2, 0, r(bt_), r(w_), a.ctypes.data, len(a), r(kept_), r(ws or kept_),
+                                    ctypes.c_uint64(0))
+        assert st != 0
+        return lib.daric_last_error().decode()
+
+    two = fake((2, 4, 2, 50), torch.int32)
+    assert "weights must be" in run(w_=fake((2, 2, 200), torch.float32))
+    assert "weights must be" in run(w_=fake((1, 4, 200), torch.float32))
+    assert "weights must be" in run(w_=fake((2, 4, 200), torch.float16))
+    assert "negative field of eviction 0" in run(s=((0, 0, 100, 50, -1, 0),))
+    assert "n_first + n_recent must not exceed keep" in run(s=((0, 0, 100, 50, 26, 25),))
+    assert "n_first + n_recent must not exceed keep" in run(s=((0, 0, 100, 50, 1, 2 ** 62),))
+    assert "columns exceed weights" in run(s=((0, 101, 100, 50, 0, 0),))
+    assert "reads past the end of block_table" in run(s=((3, 0, 100, 50, 0, 0),))
+    assert "is too long" in run(s=((0, 0, 2 ** 31, 50, 0, 0),))
+    assert "column 60 is in two sequences" in run(s=((0, 0, 64, 50, 0, 0), (4, 60, 64, 50, 0, 0)), kept_=two)
+    assert "kmax at least 50" in run(kept_=fake((2, 4, 1, 49), torch.int32))
+    assert "workspace must have kept's shape" in run(ws=fake((2, 4, 1, 51), torch.int32))
+    assert "kept must be" in run(kept_=fake((2, 1, 1, 50), torch.int32))
+    other = (_lib.DaricTensor * 2)(layers[0], fake((2, 8, 16, 4, 32), torch.bfloat16))
+    assert "must share shape" in run(lay=other)
+    # evictions of nothing need no device
+    a = np.zeros((0, 6), np.int64)
+    none = fake((2, 4, 0, 0), torch.int32)
+    r = ctypes.byref
+    assert lib.daric_evict_tokens(layers, 2, 0, r(bt), r(w), a.ctypes.data, 0, r(none), r(none), ctypes.c_uint64(0)) == 0
+
+
+def test_python_lists_of_sequences():
+    good = [(0, 0, 1, 5), (1, 1, 2, 6)]
+    addr, n, a = cache_ops._sequences(good)
+    assert n == 2 and a.shape == (2, 5) and a.tolist() == [[0, 0, 1, 5, 0], [1, 1, 2, 6, 0]]
+    assert cache_ops._sequences([])[1] == 0
+    assert cache_ops._sequences(np.array(good, np.int32))[2].dtype == np.int64
+    for bad in ([(0, 0, 1)], [(0, 0, 1.5, 2)], [("a", 0, 1, 2)]):
+        with pytest.raises(ValueError):
+            cache_ops._sequences(bad)
