@@ -21,7 +21,7 @@ struct alignas(16) AttSeq {
     int32_t row0, n_rows, n_ctx;
     int32_t tile_begin;   // first workgroup of the sequence
     int32_t n_parts;      // parts its tokens are cut into
-    int32_t at;           // attend: first group of rows in the join; weigh: first column of weights
+    int32_t at;           // attend: first of its rows times heads in the join; weigh: first column of weights
 };
 static_assert(sizeof(AttSeq) == 32, "AttSeq layout");
 
@@ -36,15 +36,15 @@ struct AttArgs {
     const float* v_scale;
     uint8_t* out;              // [T, Hq, D]
     float* lse;                // [T, Hq]
-    float* part;               // partial sums, [items][rows][D]
-    float* part_ml;            // their maxima and sums, [items][rows][2]
+    float* part;               // partial sums, [items][tile_rows][head_dim rounded up]
+    float* part_ml;            // their maxima and sums, [items][tile_rows][2]
     float* weights;            // weigh: [H, columns]
     int64_t columns;
     float scale_log2;          // scale * log2(e)
     int32_t words;             // 64-bit words of a mask row
     int32_t G, Hq;             // query heads per KV head, in all
     int32_t n_seqs;
-    int32_t part_tiles;        // tiles of a part
+    int32_t tile_rows;         // rows of q of a workgroup
     int32_t add;               // weigh: add to weights instead of setting them
     FastDiv group, page, heads;
 };
@@ -55,16 +55,16 @@ enum AttMode : int { kAttWhole = 0, kAttPadded = 1, kAttValues = 2 };
 
 // How an attend call is cut: rows of a workgroup, tiles of a part.
 struct AttPlan {
-    int mode, dp, row_tiles;       // head_dim rounded up to 64, 128 or 256
-    int64_t items, groups;         // workgroups; groups of rows joined by the second kernel
-    int32_t part_tiles;
-    bool join;                     // some sequence has several parts
+    int mode, dp;                  // head_dim rounded up to 64, 128 or 256
+    bool paged;                    // pages hold whole halves of a tile
+    int64_t items, join_rows;      // workgroups; rows times heads of all sequences
+    int64_t max_parts;             // of a sequence: with more than one, a second kernel joins them
 };
 
 // Launchers by cache and query type. `d` holds the sequences.
 #define DARIC_ATTEND_TYPES(name)                                                                                \
     void attend_##name(const DescArg& d, const AttArgs& a, const AttPlan& p, hipStream_t stream);               \
-    void weigh_##name(const DescArg& d, const AttArgs& a, int mode, int dp, int64_t items, hipStream_t stream);
+    void weigh_##name(const DescArg& d, const AttArgs& a, const AttPlan& p, hipStream_t stream);
 DARIC_ATTEND_TYPES(bf16)
 DARIC_ATTEND_TYPES(f16)
 DARIC_ATTEND_TYPES(e4m3_bf16)

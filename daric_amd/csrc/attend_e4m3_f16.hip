@@ -6,8 +6,8 @@ namespace daric {
 void attend_e4m3_f16(const DescArg& d, const AttArgs& a, const AttPlan& p, hipStream_t stream) {
     attend::run_attend<kE4M3, kF16>(d, a, p, stream);
 }
-void weigh_e4m3_f16(const DescArg& d, const AttArgs& a, int mode, int dp, int64_t items, hipStream_t stream) {
-    attend::run_weigh<kE4M3, kF16>(d, a, mode, dp, items, stream);
+void weigh_e4m3_f16(const DescArg& d, const AttArgs& a, const AttPlan& p, hipStream_t stream) {
+    attend::run_weigh<kE4M3, kF16>(d, a, p, stream);
 }
 
 }  // namespace daric

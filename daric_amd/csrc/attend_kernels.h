@@ -87,9 +87,15 @@ __device__ __forceinline__ float exp2_hw(float x) {
 #endif
 }
 
+template <bool NT, typename W>
+__device__ __forceinline__ W load_word(const W* p) {
+    if constexpr (NT) return __builtin_nontemporal_load(p);
+    else return *p;
+}
+
 // N words from p: one load of up to 16 bytes each, or (VALUES) value by value
-// of ES bytes, the values from `left` on zero.
-template <int N, int ES, bool VALUES>
+// of ES bytes, the values from `left` on zero. NT: read once, not to be kept.
+template <int N, int ES, bool VALUES, bool NT = false>
 __device__ __forceinline__ void load_words(uint32_t* w, const uint8_t* p, int left) {
     if constexpr (VALUES) {
         constexpr int PW = 4 / ES;
@@ -106,14 +112,14 @@ __device__ __forceinline__ void load_words(uint32_t* w, const uint8_t* p, int le
             }
         }
     } else if constexpr (N == 1) {
-        w[0] = *reinterpret_cast<const uint32_t*>(p);
+        w[0] = load_word<NT>(reinterpret_cast<const uint32_t*>(p));
     } else if constexpr (N == 2) {
-        const u32x2 v = *reinterpret_cast<const u32x2*>(p);
+        const u32x2 v = load_word<NT>(reinterpret_cast<const u32x2*>(p));
         w[0] = v[0]; w[1] = v[1];
     } else {
 #pragma unroll
         for (int i = 0; i < N; i += 4) {
-            const u32x4 v = *reinterpret_cast<const u32x4*>(p + i * 4);
+            const u32x4 v = load_word<NT>(reinterpret_cast<const u32x4*>(p + i * 4));
             w[i] = v[0]; w[i + 1] = v[1]; w[i + 2] = v[2]; w[i + 3] = v[3];
         }
     }
@@ -144,10 +150,25 @@ struct TileRows {
     uint32_t ok;                                   // tokens that are there
 };
 
-// Reads the rows of one KV head.
-template <int CK, int DP, int MODE>
+// Where a tile's rows lie. PAGED: each half of 16 tokens lies in one page (pages
+// of a multiple of 16 tokens), whose id all lanes share. Otherwise a lane holds
+// the row of one token.
+template <bool PAGED> struct TileAt;
+template <> struct TileAt<true> {
+    int32_t id[2], slot[2];
+    int t0;
+};
+template <> struct TileAt<false> {
+    int64_t row;
+    bool there;
+};
+
+// Reads the rows of one KV head. A page id of 0 (the null block) or out of range
+// has no tokens: they read a row of block 0 and count for nothing.
+template <int CK, int DP, int MODE, bool PAGED>
 struct RowReader {
     using Rows = TileRows<CK, DP>;
+    using At = TileAt<PAGED>;
     static constexpr int ES = Rows::ES;
     const uint8_t* head;       // K row of block 0, slot 0
     const int32_t* bt;         // the sequence's block list
@@ -166,66 +187,93 @@ struct RowReader {
         last_page = static_cast<int>(page.div(static_cast<uint32_t>(total - 1)));
         n = lane & 15; g = lane >> 4;
     }
-    // Offset of a token's row, and whether the token is there: a page id of 0
-    // (the null block) or out of range has none. Tokens that are not there
-    // read a row of block 0 and count for nothing.
+    __device__ __forceinline__ bool is_page(int id) const { return id > 0 && id < num_blocks; }
+    // Offset of a token's row, and whether the token is there.
     __device__ __forceinline__ int64_t row_of(int t, bool* there) const {
         const int p = min(static_cast<int>(page.div(static_cast<uint32_t>(t))), last_page);
         const int id = bt[p];
-        *there = t < n_total && id > 0 && id < num_blocks;
+        *there = t < n_total && is_page(id);
         const int slot = *there ? t - p * PS : 0;
         return static_cast<int64_t>(*there ? id : 0) * sb + static_cast<int64_t>(slot) * ss;
     }
-    __device__ __forceinline__ void load_k(Rows& r, int64_t o0, int64_t o1) const {
+    // Tile of tokens t0 .. t0 + 31.
+    __device__ __forceinline__ At locate(int t0) const {
+        At a;
+        if constexpr (PAGED) {
+            a.t0 = t0;
 #pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-            const uint8_t* p = head + (hh ? o1 : o0);
+            for (int hh = 0; hh < 2; ++hh) {
+                const int t = t0 + 16 * hh;
+                const int p = min(static_cast<int>(page.div(static_cast<uint32_t>(t))), last_page);
+                a.id[hh] = uniform_load(bt + p);
+                a.slot[hh] = t < n_total ? t - p * PS : 0;
+            }
+        } else {
+            a.row = row_of(t0 + (16 * (g & 1) + n), &a.there);
+        }
+        return a;
+    }
+    __device__ __forceinline__ void load_k(uint32_t (*k)[4], const uint8_t* p) const {
 #pragma unroll
-            for (int u = 0; u < Rows::KU; ++u) {
-                const int d = CK == kE4M3 ? 64 * u + 16 * g : 32 * u + 8 * g;
-                if constexpr (MODE == kAttWhole) {
-                    load_words<4, ES, false>(r.k[hh][u], p + d * ES, 0);
-                } else {
+        for (int u = 0; u < Rows::KU; ++u) {
+            const int d = CK == kE4M3 ? 64 * u + 16 * g : 32 * u + 8 * g;
+            if constexpr (MODE == kAttWhole) {
+                load_words<4, ES, false>(k[u], p + d * ES, 0);
+            } else {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) r.k[hh][u][i] = 0;
-                    if (d < D) load_words<4, ES, MODE == kAttValues>(r.k[hh][u], p + d * ES, D - d);
-                }
+                for (int i = 0; i < 4; ++i) k[u][i] = 0;
+                if (d < D) load_words<4, ES, MODE == kAttValues>(k[u], p + d * ES, D - d);
             }
         }
     }
-    __device__ __forceinline__ void load_v(uint32_t* w, int64_t o) const {
-        const uint8_t* p = head + v_off + o;
+    __device__ __forceinline__ void load_v(uint32_t* w, const uint8_t* p) const {
         const int d = Rows::E * n;
         if constexpr (MODE == kAttWhole) {
-            load_words<Rows::VW, ES, false>(w, p + d * ES, 0);
+            load_words<Rows::VW, ES, false, true>(w, p + d * ES, 0);
         } else {
 #pragma unroll
             for (int i = 0; i < Rows::VW; ++i) w[i] = 0;
-            constexpr int STEP = MODE == kAttValues || Rows::VW < 4 ? Rows::VW : (Rows::VW * 4 / ES > 8 ? 8 * ES / 4 : Rows::VW);
             // slices of 8 values at most, each there or not as a whole
+            constexpr int STEP = MODE != kAttValues && Rows::E > 8 ? 8 * ES / 4 : Rows::VW;
 #pragma unroll
             for (int i = 0; i < Rows::VW; i += STEP) {
                 const int di = d + i * 4 / ES;
-                if (di < D) load_words<STEP, ES, MODE == kAttValues>(w + i, p + di * ES, D - di);
+                if (di < D) load_words<STEP, ES, MODE == kAttValues, true>(w + i, p + di * ES, D - di);
             }
         }
     }
-    // The rows of tokens t0 .. t0 + 31. Lane L finds the row of token t0 +
-    // L % 32; the others get it from there.
     template <bool WITH_V>
-    __device__ __forceinline__ void load(Rows& r, int t0) const {
-        bool there;
-        const int64_t mine = row_of(t0 + (16 * (g & 1) + n), &there);
-        r.ok = static_cast<uint32_t>(__ballot(there));
-        const int lo = static_cast<int>(mine), hi = static_cast<int>(mine >> 32);
-        const auto from = [&](int t) {
-            return static_cast<int64_t>((static_cast<uint64_t>(static_cast<uint32_t>(__shfl(hi, t, 64))) << 32) |
-                                        static_cast<uint32_t>(__shfl(lo, t, 64)));
-        };
-        load_k(r, from(n), from(16 + n));
-        if constexpr (WITH_V) {
+    __device__ __forceinline__ void load(Rows& r, const At& a) const {
+        if constexpr (PAGED) {
+            r.ok = 0;
+            const uint32_t k_lane = static_cast<uint32_t>(n * static_cast<int>(ss));
+            const uint32_t v_lane = static_cast<uint32_t>(4 * g * static_cast<int>(ss));
 #pragma unroll
-            for (int j = 0; j < 8; ++j) load_v(r.v[j], from(16 * (j >> 2) + 4 * g + (j & 3)));
+            for (int hh = 0; hh < 2; ++hh) {
+                const bool is = is_page(a.id[hh]);
+                const int left = n_total - a.t0 - 16 * hh;
+                if (is && left > 0) r.ok |= (left >= 16 ? 0xffffu : (1u << left) - 1u) << (16 * hh);
+                const uint8_t* p = head + static_cast<int64_t>(is ? a.id[hh] : 0) * sb + static_cast<int64_t>(a.slot[hh]) * ss;
+                load_k(r.k[hh], p + k_lane);
+                if constexpr (WITH_V) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) load_v(r.v[4 * hh + i], p + v_off + i * ss + v_lane);
+                }
+            }
+        } else {
+            // lane L has the row of token L % 32; the others get it from there
+            r.ok = static_cast<uint32_t>(__ballot(a.there));
+            const int lo = static_cast<int>(a.row), hi = static_cast<int>(a.row >> 32);
+            const auto from = [&](int t) {
+                return head + static_cast<int64_t>((static_cast<uint64_t>(static_cast<uint32_t>(__shfl(hi, t, 64))) << 32) |
+                                                   static_cast<uint32_t>(__shfl(lo, t, 64)));
+            };
+            load_k(r.k[0], from(n));
+            load_k(r.k[1], from(16 + n));
+            if constexpr (WITH_V) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) load_v(r.v[j], from(16 * (j >> 2) + 4 * g + (j & 3)) + v_off);
+            }
         }
     }
 };
@@ -304,18 +352,30 @@ __device__ __forceinline__ uint32_t row_sees(const AttArgs& a, const AttSeq& s, 
     return static_cast<uint32_t>(v);
 }
 
+// The work item of block b, of n items whose KV head is their lowest digit:
+// workgroups go to the 8 XCDs in turn, and the heads of one part of a sequence
+// read the same pages, so they go to one XCD, whose address translations then
+// cover an eighth of the pages.
+__device__ __forceinline__ int xcd_item(int b, int n, const FastDiv& heads) {
+    const int H = static_cast<int>(heads.d);
+    const int set = b / (8 * H), in = b - set * 8 * H;
+    const int left = min(8, n / H - set * 8);            // parts of this set
+    const int h = in / left, p = in - h * left;
+    return (set * 8 + p) * H + h;
+}
+
 // ------------------------------------------------------------------ attend
 // One workgroup: one KV head, 16 rows of q and one part of a sequence's tokens,
 // whose tiles its wavefronts take in turn; they join in LDS at the end.
-template <int CK, int QK, int DP, int MODE>
-__global__ __launch_bounds__(256) void attend_kernel(DescArg d, AttArgs a) {
+template <int CK, int QK, int DP, int MODE, bool PAGED>
+__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_kernel(DescArg d, AttArgs a) {
     using Rows = TileRows<CK, DP>;
     constexpr int E = Rows::E, STEPS = DP / 32, WAVES = 4;
     constexpr int LD = DP + 4;                        // floats of a row in LDS: no two rows on one bank
     __shared__ float s_o[WAVES][kAttRows][LD];
     __shared__ float s_m[WAVES][kAttRows], s_l[WAVES][kAttRows];
     const DescPtr<AttSeq> seqs = desc_at<AttSeq>(d, 0);
-    const int item = static_cast<int>(blockIdx.x);
+    const int item = xcd_item(static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x), a.heads);
     const int si = __builtin_amdgcn_readfirstlane(find_by_tile(seqs, a.n_seqs, item));
     const AttSeq s = desc_load(seqs + si);
     const int tid = static_cast<int>(threadIdx.x), lane = tid & 63;
@@ -332,9 +392,12 @@ __global__ __launch_bounds__(256) void attend_kernel(DescArg d, AttArgs a) {
     // causal: nothing behind the last row's own token is seen
     const int last_i = min(s.n_rows - 1, static_cast<int>(a.group.div(static_cast<uint32_t>(rt * kAttRows + kAttRows - 1))));
     const int end = a.mask == nullptr ? s.n_ctx + last_i + 1 : total;
-    const int tile_end = min((part + 1) * a.part_tiles, (end + kAttTile - 1) / kAttTile);
+    // the sequence's tiles in equal parts
+    const int tiles = (total + kAttTile - 1) / kAttTile;
+    const int part_tiles = (tiles + s.n_parts - 1) / s.n_parts;
+    const int tile_end = min((part + 1) * part_tiles, (end + kAttTile - 1) / kAttTile);
 
-    RowReader<CK, DP, MODE> rd;
+    RowReader<CK, DP, MODE, PAGED> rd;
     rd.init(a, s.bt_offset, total, h, lane);
     u32x4 q[STEPS];
     load_q<CK, DP, MODE>(a, s, row, g, q);
@@ -446,10 +509,32 @@ __global__ __launch_bounds__(256) void attend_kernel(DescArg d, AttArgs a) {
         }
     };
 
-    for (int tile = part * a.part_tiles + wave; tile < tile_end; tile += WAVES) {
-        Rows r;
-        rd.template load<true>(r, tile * kAttTile);
-        tile_of(r, tile);
+    // A wavefront's next tile is on its way while it works on one, and the pages
+    // of the one after that are known (rows of 256 values leave no registers for
+    // a second tile).
+    constexpr bool AHEAD = DP < 256;
+    int tile = part * part_tiles + wave;
+    if (tile < tile_end) {
+        Rows cur;
+        rd.template load<true>(cur, rd.locate(tile * kAttTile));
+        auto at = rd.locate(min(tile + WAVES, tile_end - 1) * kAttTile);
+        for (;;) {
+            const int next = tile + WAVES;
+            Rows coming;
+            if (AHEAD && next < tile_end) {
+                rd.template load<true>(coming, at);
+                at = rd.locate(min(next + WAVES, tile_end - 1) * kAttTile);
+            }
+            tile_of(cur, tile);
+            if (next >= tile_end) break;
+            if constexpr (AHEAD) {
+                cur = coming;
+            } else {
+                rd.template load<true>(cur, at);
+                at = rd.locate(min(next + WAVES, tile_end - 1) * kAttTile);
+            }
+            tile = next;
+        }
     }
 
     // Join the wavefronts.
@@ -482,10 +567,9 @@ __global__ __launch_bounds__(256) void attend_kernel(DescArg d, AttArgs a) {
     }
     if (orow.i < 0) return;
     if (s.n_parts > 1) {
-        float* po = a.part + (static_cast<int64_t>(item) * kAttRows + rn) * a.g.D;
+        float* po = a.part + (static_cast<int64_t>(item) * kAttRows + rn) * DP;
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (dc + e < a.g.D) po[dc + e] = o[e];
+        for (int e = 0; e < E; ++e) po[dc + e] = o[e];
         if ((tid & 15) == 0) {
             float* pm = a.part_ml + (static_cast<int64_t>(item) * kAttRows + rn) * 2;
             pm[0] = mm;
@@ -504,63 +588,87 @@ __global__ __launch_bounds__(256) void attend_kernel(DescArg d, AttArgs a) {
     if ((tid & 15) == 0) a.lse[at] = ll == 0.0f ? -__builtin_huge_valf() : (mm + log2f(ll)) * kLn2;
 }
 
-// Joins the parts of 16 rows of one KV head.
-template <int QK, int DP>
-__global__ __launch_bounds__(256) void attend_join_kernel(DescArg d, AttArgs a) {
-    constexpr int E = DP / 16;
+// Joins the parts of the rows of q (one head of one query each), 32 lanes to a
+// row and part in turn, PG parts of a row at once. The parts' maxima come first,
+// a lane each, so that no load waits for another: with one lane walking all 61
+// parts of a row the join of two long sequences took 94 us, as long as their
+// attention.
+template <int QK, int DP, int PG>
+__global__ __launch_bounds__(256) void attend_join_kernel(DescArg d, AttArgs a, int n_rows) {
+    constexpr int V = DP / 32, ROWS = 8 / PG;
+    __shared__ float s_o[8][DP];
+    __shared__ float s_l[8];
     const DescPtr<AttSeq> seqs = desc_at<AttSeq>(d, 0);
-    const int group = static_cast<int>(blockIdx.x);
+    const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, slot = tid >> 5;
+    const int pg = slot % PG;
+    const int r = static_cast<int>(blockIdx.x) * ROWS + slot / PG;
     int lo = 0, hi = a.n_seqs - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (seqs[mid].at <= group) lo = mid; else hi = mid - 1;
+        if (seqs[mid].at <= r) lo = mid; else hi = mid - 1;
     }
-    const AttSeq s = desc_load(seqs + __builtin_amdgcn_readfirstlane(lo));
-    if (s.n_parts <= 1) return;
-    const int local = group - s.at;
-    const int rt = static_cast<int>(a.heads.div(static_cast<uint32_t>(local)));
-    const int h = local - rt * a.g.H;
-    const int row_tiles = (s.n_rows * a.G + kAttRows - 1) / kAttRows;
-    const int tid = static_cast<int>(threadIdx.x);
-    const int rn = tid >> 4, dc = (tid & 15) * E;
-    const QRow row = q_row(a, s.n_rows, h, rt * kAttRows + rn);
-    if (row.i < 0) return;
-    const int64_t first = (static_cast<int64_t>(s.tile_begin) + local) * kAttRows + rn;
-    const int64_t step = static_cast<int64_t>(row_tiles) * a.g.H * kAttRows;
+    const int parts = r < n_rows ? seqs[lo].n_parts : 0;
+    if (PG == 1 && parts <= 1) return;
+    const int local = r - seqs[lo].at;
+    const int i = local / a.Hq, head = local - i * a.Hq;
+    const int h = static_cast<int>(a.group.div(static_cast<uint32_t>(head)));
+    const int R = i * a.G + head - h * a.G;
+    const int row_tiles = (seqs[lo].n_rows * a.G + a.tile_rows - 1) / a.tile_rows;
+    const int rt = R / a.tile_rows;
+    const int64_t first = (static_cast<int64_t>(seqs[lo].tile_begin) + rt * a.g.H + h) * a.tile_rows + (R - rt * a.tile_rows);
+    const int64_t step = static_cast<int64_t>(row_tiles) * a.g.H * a.tile_rows;
+    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + first;
     float mm = -3.402823466e38f;
-    for (int p = 0; p < s.n_parts; ++p) mm = fmaxf(mm, a.part_ml[(first + p * step) * 2]);
-    float ll = 0.0f, o[E];
+    for (int p = lane; p < parts; p += 32) mm = fmaxf(mm, ml[p * step].x);
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = 0.0f;
-    for (int p = 0; p < s.n_parts; ++p) {
-        const int64_t at = first + p * step;
-        const float al = exp2_hw(a.part_ml[at * 2] - mm);
-        ll += a.part_ml[at * 2 + 1] * al;
+    for (int x = 16; x > 0; x >>= 1) mm = fmaxf(mm, __shfl_xor(mm, x, 64));
+    float ll = 0.0f, o[V];
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (dc + e < a.g.D) o[e] += a.part[at * a.g.D + dc + e] * al;
+    for (int v = 0; v < V; ++v) o[v] = 0.0f;
+    const float* po = a.part + first * DP + lane * V;
+#pragma unroll 4
+    for (int p = pg; p < parts; p += PG) {
+        const float2 x = ml[p * step];
+        const float al = exp2_hw(x.x - mm);
+        ll += x.y * al;
+        const float* src = po + p * step * DP;
+#pragma unroll
+        for (int v = 0; v < V; ++v) o[v] += src[v] * al;
     }
-    const int64_t at = static_cast<int64_t>(s.row0 + row.i) * a.Hq + row.head;
+    if constexpr (PG > 1) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) s_o[slot][lane * V + v] = o[v];
+        if (lane == 0) s_l[slot] = ll;
+        __syncthreads();
+        if (pg != 0 || parts <= 1) return;
+#pragma unroll
+        for (int x = 1; x < PG; ++x) {
+            ll += s_l[slot + x];
+#pragma unroll
+            for (int v = 0; v < V; ++v) o[v] += s_o[slot + x][lane * V + v];
+        }
+    }
+    const int64_t at = static_cast<int64_t>(seqs[lo].row0 + i) * a.Hq + head;
     const float inv = (a.v_scale != nullptr ? a.v_scale[h] : 1.0f) / ll;
     uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + at * a.g.D;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const float x = ll == 0.0f ? 0.0f : o[e] * inv;
-        if (dc + e < a.g.D) out[dc + e] = static_cast<uint16_t>(QK == kBF16 ? f32_to_bf16(x) : f32_to_f16(x));
+    for (int v = 0; v < V; ++v) {
+        const float x = ll == 0.0f ? 0.0f : o[v] * inv;
+        if (lane * V + v < a.g.D) out[lane * V + v] = static_cast<uint16_t>(QK == kBF16 ? f32_to_bf16(x) : f32_to_f16(x));
     }
-    if ((tid & 15) == 0) a.lse[at] = ll == 0.0f ? -__builtin_huge_valf() : (mm + log2f(ll)) * kLn2;
+    if (lane == 0) a.lse[at] = ll == 0.0f ? -__builtin_huge_valf() : (mm + log2f(ll)) * kLn2;
 }
 
 // ------------------------------------------------------------------- weigh
 // One workgroup: one KV head, 128 tokens, 32 to a wavefront, whose K rows stay
 // in registers while all rows of the sequence pass. Each token's sum is one
 // lane's, then 16 lanes', in a fixed order.
-template <int CK, int QK, int DP, int MODE>
+template <int CK, int QK, int DP, int MODE, bool PAGED>
 __global__ __launch_bounds__(256) void weigh_kernel(DescArg d, AttArgs a) {
     using Rows = TileRows<CK, DP>;
     constexpr int STEPS = DP / 32;
     const DescPtr<AttSeq> seqs = desc_at<AttSeq>(d, 0);
-    const int item = static_cast<int>(blockIdx.x);
+    const int item = xcd_item(static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x), a.heads);
     const int si = __builtin_amdgcn_readfirstlane(find_by_tile(seqs, a.n_seqs, item));
     const AttSeq s = desc_load(seqs + si);
     const int tid = static_cast<int>(threadIdx.x), lane = tid & 63;
@@ -572,10 +680,10 @@ __global__ __launch_bounds__(256) void weigh_kernel(DescArg d, AttArgs a) {
     const int total = s.n_ctx + s.n_rows;
     const int t0 = tg * kWeighTokens + wave * kAttTile;
     if (t0 >= total) return;
-    RowReader<CK, DP, MODE> rd;
+    RowReader<CK, DP, MODE, PAGED> rd;
     rd.init(a, s.bt_offset, total, h, lane);
     Rows r;
-    rd.template load<false>(r, t0);
+    rd.template load<false>(r, rd.locate(t0));
     const float c = a.scale_log2 * (a.k_scale != nullptr ? a.k_scale[h] : 1.0f);
     const bool edge = r.ok != ~0u || t0 + kAttTile > s.n_ctx;
     float sum[8];
@@ -622,12 +730,14 @@ __global__ __launch_bounds__(256) void weigh_kernel(DescArg d, AttArgs a) {
 
 // Instances of the kernels for one pair of cache and query types.
 template <typename F>
-void for_forms(int dp, int mode, F&& f) {
+void for_forms(int dp, int mode, bool paged, F&& f) {
     using std::integral_constant;
     const auto with = [&](auto dpc) {
-        if (mode == kAttWhole) f(dpc, integral_constant<int, kAttWhole>());
-        else if (mode == kAttPadded) f(dpc, integral_constant<int, kAttPadded>());
-        else f(dpc, integral_constant<int, kAttValues>());
+        if (mode == kAttValues) f(dpc, integral_constant<int, kAttValues>(), std::false_type());
+        else if (mode == kAttPadded && paged) f(dpc, integral_constant<int, kAttPadded>(), std::true_type());
+        else if (mode == kAttPadded) f(dpc, integral_constant<int, kAttPadded>(), std::false_type());
+        else if (paged) f(dpc, integral_constant<int, kAttWhole>(), std::true_type());
+        else f(dpc, integral_constant<int, kAttWhole>(), std::false_type());
     };
     if (dp == 64) with(integral_constant<int, 64>());
     else if (dp == 128) with(integral_constant<int, 128>());
@@ -636,20 +746,31 @@ void for_forms(int dp, int mode, F&& f) {
 
 template <int CK, int QK>
 void run_attend(const DescArg& d, const AttArgs& a, const AttPlan& p, hipStream_t stream) {
-    for_forms(p.dp, p.mode, [&](auto dp, auto mode) {
-        DARIC_LAUNCH((attend_kernel<CK, QK, decltype(dp)::value, decltype(mode)::value>),
+    for_forms(p.dp, p.mode, p.paged, [&](auto dp, auto mode, auto paged) {
+        DARIC_LAUNCH((attend_kernel<CK, QK, decltype(dp)::value, decltype(mode)::value, decltype(paged)::value>),
                      static_cast<unsigned>(p.items), 256, 0, stream, d, a);
     });
     check_launch("attend_pages");
 }
 
 template <int CK, int QK>
-void run_weigh(const DescArg& d, const AttArgs& a, int mode, int dp, int64_t items, hipStream_t stream) {
-    for_forms(dp, mode, [&](auto dpc, auto modec) {
-        DARIC_LAUNCH((weigh_kernel<CK, QK, decltype(dpc)::value, decltype(modec)::value>),
-                     static_cast<unsigned>(items), 256, 0, stream, d, a);
+void run_weigh(const DescArg& d, const AttArgs& a, const AttPlan& p, hipStream_t stream) {
+    for_forms(p.dp, p.mode, p.paged, [&](auto dp, auto mode, auto paged) {
+        DARIC_LAUNCH((weigh_kernel<CK, QK, decltype(dp)::value, decltype(mode)::value, decltype(paged)::value>),
+                     static_cast<unsigned>(p.items), 256, 0, stream, d, a);
     });
     check_launch("weigh_tokens");
+}
+
+template <int QK>
+void run_join(const DescArg& d, const AttArgs& a, const AttPlan& p, hipStream_t stream) {
+    for_forms(p.dp, kAttWhole, true, [&](auto dp, auto, auto) {
+        constexpr int DP = decltype(dp)::value;
+        const int rows = static_cast<int>(p.join_rows);
+        if (p.max_parts <= 4) DARIC_LAUNCH((attend_join_kernel<QK, DP, 1>), (rows + 7) / 8, 256, 0, stream, d, a, rows);
+        else DARIC_LAUNCH((attend_join_kernel<QK, DP, 8>), rows, 256, 0, stream, d, a, rows);
+    });
+    check_launch("attend_pages join");
 }
 
 }  // namespace attend

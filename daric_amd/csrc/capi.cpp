@@ -1604,6 +1604,7 @@ AttCall attention_call(const daric_tensor* layer, int page_first, const daric_te
                              (g.sh * es) % 16 == 0 && (g.v_off * es) % 16 == 0 && aligned(q->data, 16) &&
                              a.q_row % 8 == 0 && a.q_head % 8 == 0 && (g.D * es) % 16 == 0;
     c.p.dp = g.D <= 64 ? 64 : g.D <= 128 ? 128 : 256;
+    c.p.paged = g.PS % 16 == 0 && g.ss >= 0 && g.ss * es <= kIntMax / 16;
     c.p.mode = !whole_units ? kAttValues : g.D == c.p.dp ? kAttWhole : kAttPadded;
     a.group = FastDiv(static_cast<uint32_t>(a.G));
     a.page = FastDiv(static_cast<uint32_t>(g.PS));
@@ -1615,28 +1616,31 @@ AttCall attention_call(const daric_tensor* layer, int page_first, const daric_te
 // Parts of the sequences' tokens: about kAttendGroups workgroups in all.
 constexpr int64_t kAttendGroups = 1024;
 void plan_attend(AttCall& c) {
+    c.a.tile_rows = kAttRows;
+    const auto row_tiles = [&](const AttSeq& s) {
+        return (static_cast<int64_t>(s.n_rows) * c.a.G + c.a.tile_rows - 1) / c.a.tile_rows;
+    };
+    const auto tiles = [](const AttSeq& s) {
+        return (static_cast<int64_t>(s.n_ctx) + s.n_rows + kAttTile - 1) / kAttTile;
+    };
     int64_t work = 0;
-    for (const AttSeq& s : c.seqs) {
-        const int64_t row_tiles = (static_cast<int64_t>(s.n_rows) * c.a.G + kAttRows - 1) / kAttRows;
-        work += (static_cast<int64_t>(s.n_ctx) + s.n_rows + kAttTile - 1) / kAttTile * row_tiles * c.a.g.H;
-    }
-    const int64_t part = std::min<int64_t>(((work + kAttendGroups - 1) / kAttendGroups + 3) / 4 * 4, 1 << 26);
-    c.a.part_tiles = static_cast<int32_t>(std::max<int64_t>(part, 4));
+    for (const AttSeq& s : c.seqs) work += tiles(s) * row_tiles(s) * c.a.g.H;
+    const int64_t G_ = getenv("DARIC_G") ? atoi(getenv("DARIC_G")) : kAttendGroups;
+    const int64_t part = std::max<int64_t>(4, (work + G_ - 1) / G_);
     for (AttSeq& s : c.seqs) {
-        const int64_t row_tiles = (static_cast<int64_t>(s.n_rows) * c.a.G + kAttRows - 1) / kAttRows;
-        const int64_t tiles = (static_cast<int64_t>(s.n_ctx) + s.n_rows + kAttTile - 1) / kAttTile;
-        const int64_t parts = (tiles + c.a.part_tiles - 1) / c.a.part_tiles;
+        const int64_t parts = (tiles(s) + part - 1) / part;
         s.tile_begin = static_cast<int32_t>(c.p.items);
-        s.at = static_cast<int32_t>(c.p.groups);
+        s.at = static_cast<int32_t>(c.p.join_rows);
         s.n_parts = static_cast<int32_t>(parts);
-        c.p.items += parts * row_tiles * c.a.g.H;
-        c.p.groups += row_tiles * c.a.g.H;
-        c.p.join = c.p.join || parts > 1;
-        DARIC_CHECK(c.p.items <= kMaxTiles, "too many rows in one attend_pages call");
+        c.p.items += parts * row_tiles(s) * c.a.g.H;
+        c.p.join_rows += static_cast<int64_t>(s.n_rows) * c.a.Hq;
+        c.p.max_parts = std::max(c.p.max_parts, parts);
+        DARIC_CHECK(c.p.items <= kMaxTiles && c.p.join_rows <= kIntMax, "too many rows in one attend_pages call");
     }
+    DARIC_CHECK(c.p.max_parts <= 1 || c.p.join_rows <= kMaxTiles, "too many rows in one attend_pages call");
 }
 int64_t attend_bytes(const AttCall& c) {
-    return c.p.join ? c.p.items * kAttRows * (c.a.g.D + 2) * static_cast<int64_t>(sizeof(float)) : 0;
+    return c.p.max_parts > 1 ? c.p.items * c.a.tile_rows * (c.p.dp + 2) * static_cast<int64_t>(sizeof(float)) : 0;
 }
 
 void attention_inputs(AttCall& c, const daric_tensor* block_table, const daric_sequence* sequences, int64_t n,
@@ -1720,7 +1724,7 @@ int daric_attend_pages(const daric_tensor* layer, int page_first, const daric_te
         DARIC_CHECK(need == 0 || (workspace != nullptr && workspace_bytes >= need && aligned(workspace, 16)),
                     "workspace must be 16-byte aligned and hold ", need, " bytes, got ", workspace_bytes);
         c.a.part = static_cast<float*>(workspace);
-        if (need > 0) c.a.part_ml = c.a.part + c.p.items * kAttRows * c.a.g.D;
+        if (need > 0) c.a.part_ml = c.a.part + c.p.items * c.a.tile_rows * c.p.dp;
         DeviceGuard guard(c.device);
         const hipStream_t st = as_stream(stream);
         DescHandOver ho(c.device, c.seqs.data(), c.seqs.size() * sizeof(AttSeq), st);
@@ -1728,7 +1732,7 @@ int daric_attend_pages(const daric_tensor* layer, int page_first, const daric_te
         else if (c.ck == kF16) attend_f16(ho.arg(), c.a, c.p, st);
         else if (c.qk == kBF16) attend_e4m3_bf16(ho.arg(), c.a, c.p, st);
         else attend_e4m3_f16(ho.arg(), c.a, c.p, st);
-        if (!c.p.join) return;
+        if (c.p.max_parts <= 1) return;
         if (c.qk == kBF16) join_bf16(ho.arg(), c.a, c.p, st);
         else join_f16(ho.arg(), c.a, c.p, st);
     });
@@ -1750,7 +1754,7 @@ int daric_weigh_tokens(const daric_tensor* layer, int page_first, const daric_te
         const int64_t columns = weights->sizes[1];
         std::vector<std::pair<int64_t, int64_t>> cols;
         size_t at = 0;
-        int64_t items = 0;
+        int64_t& items = c.p.items;
         for (int64_t i = 0; i < n_sequences; ++i) {
             const daric_sequence& s = sequences[i];
             const int64_t total = s.n_ctx + s.n_rows;
@@ -1772,10 +1776,10 @@ int daric_weigh_tokens(const daric_tensor* layer, int page_first, const daric_te
         DeviceGuard guard(c.device);
         const hipStream_t st = as_stream(stream);
         DescHandOver ho(c.device, c.seqs.data(), c.seqs.size() * sizeof(AttSeq), st);
-        if (c.ck == kBF16) weigh_bf16(ho.arg(), c.a, c.p.mode, c.p.dp, items, st);
-        else if (c.ck == kF16) weigh_f16(ho.arg(), c.a, c.p.mode, c.p.dp, items, st);
-        else if (c.qk == kBF16) weigh_e4m3_bf16(ho.arg(), c.a, c.p.mode, c.p.dp, items, st);
-        else weigh_e4m3_f16(ho.arg(), c.a, c.p.mode, c.p.dp, items, st);
+        if (c.ck == kBF16) weigh_bf16(ho.arg(), c.a, c.p, st);
+        else if (c.ck == kF16) weigh_f16(ho.arg(), c.a, c.p, st);
+        else if (c.qk == kBF16) weigh_e4m3_bf16(ho.arg(), c.a, c.p, st);
+        else weigh_e4m3_f16(ho.arg(), c.a, c.p, st);
     });
 }
 
