@@ -10,6 +10,8 @@ namespace daric {
 
 // Tokens of a tile: the inner dimension of one matrix instruction over V.
 constexpr int kAttTile = 32;
+// Tokens of a step of the kernel for many rows.
+constexpr int kRowsStep = 64;
 // Query rows (a row is one head of one query) of a matrix tile.
 constexpr int kAttRows = 16;
 
@@ -45,6 +47,7 @@ struct AttArgs {
     int32_t G, Hq;             // query heads per KV head, in all
     int32_t n_seqs;
     int32_t tile_rows;         // rows of q of a workgroup
+    int32_t by_head;           // many rows: head by head on the XCDs
     int32_t add;               // weigh: add to weights instead of setting them
     FastDiv group, page, heads;
 };
@@ -57,6 +60,7 @@ enum AttMode : int { kAttWhole = 0, kAttPadded = 1, kAttValues = 2 };
 struct AttPlan {
     int mode, dp;                  // head_dim rounded up to 64, 128 or 256
     bool paged;                    // pages hold whole halves of a tile
+    int row_tile;                  // rows of a wavefront in 16s (many rows), 0: attend_kernel
     int64_t items, join_rows;      // workgroups; rows times heads of all sequences
     int64_t max_parts;             // of a sequence: with more than one, a second kernel joins them
 };

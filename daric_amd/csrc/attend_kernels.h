@@ -364,6 +364,24 @@ __device__ __forceinline__ int xcd_item(int b, int n, const FastDiv& heads) {
     return (set * 8 + p) * H + h;
 }
 
+// Adds a token's weight times those values of its V row that are no numbers to
+// a lane's part of O^T.
+template <int CK, int E>
+__device__ __forceinline__ void add_odd(const uint8_t* v_row, int D, int g, float p, f32x4 (&acc)[E]) {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int d = E * (4 * g + i) + e;
+            if (d >= D) continue;
+            float x;
+            if constexpr (CK == kE4M3) x = e4m3_to_f32(v_row[d]);
+            else if constexpr (CK == kBF16) x = bf16_to_f32(reinterpret_cast<const uint16_t*>(v_row)[d]);
+            else x = f16_to_f32(reinterpret_cast<const uint16_t*>(v_row)[d]);
+            if (!(fabsf(x) <= 3.402823466e38f)) acc[e][i] += p * x;
+        }
+}
+
 // ------------------------------------------------------------------ attend
 // One workgroup: one KV head, 16 rows of q and one part of a sequence's tokens,
 // whose tiles its wavefronts take in turn; they join in LDS at the end.
@@ -492,18 +510,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_kernel(DescArg 
                 const float pj = sp[b];
                 bool there;
                 const uint8_t* vr = rd.head + rd.v_off + rd.row_of(t0 + b, &there);
-#pragma unroll
-                for (int e = 0; e < E; ++e)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int dd = E * (4 * g + i) + e;
-                        if (dd >= a.g.D) continue;
-                        float x;
-                        if constexpr (CK == kE4M3) x = e4m3_to_f32(vr[dd]);
-                        else if constexpr (CK == kBF16) x = bf16_to_f32(reinterpret_cast<const uint16_t*>(vr)[dd]);
-                        else x = f16_to_f32(reinterpret_cast<const uint16_t*>(vr)[dd]);
-                        if (!(fabsf(x) <= 3.402823466e38f)) acc[e][i] += pj * x;
-                    }
+                add_odd<CK, E>(vr, a.g.D, g, pj, acc);
             }
             __builtin_amdgcn_wave_barrier();
         }
@@ -586,6 +593,295 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_kernel(DescArg 
         if (dc + e < a.g.D) out[dc + e] = static_cast<uint16_t>(QK == kBF16 ? f32_to_bf16(x) : f32_to_f16(x));
     }
     if ((tid & 15) == 0) a.lse[at] = ll == 0.0f ? -__builtin_huge_valf() : (mm + log2f(ll)) * kLn2;
+}
+
+// -------------------------------------------------------- attend, many rows
+// One workgroup: one KV head, 64 NT rows of q (16 NT to a wavefront) and one part
+// of a sequence's tokens, in steps of 64. K and V are staged in LDS as the
+// operands of the matrix instructions lie in registers, a wavefront's operand in
+// 1 KiB, so that reads and writes of it touch every bank alike: e4m3 becomes q's
+// type and V's tokens are paired once per workgroup, and a read feeds NT
+// instructions. The next step's rows come from memory meanwhile, into the other
+// half of the LDS.
+template <int CK, int QK, int DP, int MODE, int NT>
+__global__ __launch_bounds__(256, DP * NT <= 256 ? 2 : 1) void attend_rows_kernel(DescArg d, AttArgs a) {
+    using Rows = TileRows<CK, DP>;
+    constexpr int E = Rows::E, STEPS = DP / 32, ES = Rows::ES, ROWS = 64 * NT;
+    constexpr int K_AT = 0, V_AT = 4 * STEPS * 64, UNITS = V_AT + 2 * E * 64;    // 16-byte units of a step
+    __shared__ u32x4 s_kv[2][UNITS];
+    __shared__ float s_p[4][kAttRows][kAttTile + 1];
+    __shared__ uint32_t s_ok[2][4], s_odd[2][4];
+    const DescPtr<AttSeq> seqs = desc_at<AttSeq>(d, 0);
+    const int item = a.by_head ? static_cast<int>(blockIdx.x)
+                               : xcd_item(static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x), a.heads);
+    const int si = __builtin_amdgcn_readfirstlane(find_by_tile(seqs, a.n_seqs, item));
+    const AttSeq s = desc_load(seqs + si);
+    const int tid = static_cast<int>(threadIdx.x), lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 15, g = lane >> 4;
+    const int local = item - s.tile_begin;
+    const int pr = static_cast<int>(a.heads.div(static_cast<uint32_t>(local)));
+    const int h = local - pr * a.g.H;
+    const int row_tiles = (s.n_rows * a.G + ROWS - 1) / ROWS;
+    const int part = pr / row_tiles, rt = pr - part * row_tiles;
+    const int total = s.n_ctx + s.n_rows;
+    const int R0 = rt * ROWS + wave * 16 * NT;         // the wavefront's first row
+    const auto query = [&](int R) { return min(s.n_rows - 1, static_cast<int>(a.group.div(static_cast<uint32_t>(R)))); };
+    // tokens that some row of the workgroup, of the wavefront sees, and that all
+    // rows of the wavefront see
+    const bool causal = a.mask == nullptr;
+    const int end = causal ? s.n_ctx + query(rt * ROWS + ROWS - 1) + 1 : total;
+    const int wave_end = R0 < s.n_rows * a.G ? (causal ? s.n_ctx + query(R0 + 16 * NT - 1) + 1 : total) : 0;
+    const int wave_all = causal ? s.n_ctx + query(R0) + 1 : s.n_ctx;
+    const int steps = (total + kRowsStep - 1) / kRowsStep;
+    const int part_steps = (steps + s.n_parts - 1) / s.n_parts;
+    const int step0 = part * part_steps;
+    const int step_end = min(step0 + part_steps, (end + kRowsStep - 1) / kRowsStep);
+
+    RowReader<CK, DP, MODE, false> rd;
+    rd.init(a, s.bt_offset, total, h, lane);
+    u32x4 q[NT][STEPS];
+    int qi[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const QRow row = q_row(a, s.n_rows, h, R0 + t * 16 + n);
+        qi[t] = row.i;
+        load_q<CK, DP, MODE>(a, s, row, g, q[t]);
+    }
+    // A masked score becomes an infinity that c turns to -inf; with c = 0 all
+    // scores are 0, of a zero q.
+    float c = a.scale_log2 * (a.k_scale != nullptr ? a.k_scale[h] : 1.0f);
+    if (c == 0.0f) {
+        c = 1.0f;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int st = 0; st < STEPS; ++st) q[t][st] = u32x4{0, 0, 0, 0};
+    }
+    const float masked = c > 0.0f ? -__builtin_huge_valf() : __builtin_huge_valf();
+    f32x4 acc[NT][E];
+    float m[NT], l[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        m[t] = -3.402823466e38f;
+        l[t] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[t][e] = f32x4{0, 0, 0, 0};
+    }
+
+    // A wavefront stages 16 of a step's tokens.
+    const int sub = wave >> 1, half = wave & 1;
+    uint32_t sk[Rows::KU][4], sv[4][Rows::VW];
+    uint32_t there_k = 0, there_v = 0;
+    const auto fetch = [&](int step) {
+        const int t = step * kRowsStep + 16 * wave;
+        bool there;
+        const int64_t ko = rd.row_of(t + n, &there);
+        there_k = static_cast<uint32_t>(__ballot(there)) & 0xffffu;
+        rd.load_k(sk, rd.head + ko);
+        there_v = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t vo = rd.row_of(t + 4 * g + i, &there);
+            if (there) there_v |= 1u << i;
+            rd.load_v(sv[i], rd.head + rd.v_off + vo);
+        }
+    };
+    const auto stage = [&](int step, int buf) {
+        const int t = step * kRowsStep + 16 * wave;
+        if (there_k != 0xffffu) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int w = 0; w < Rows::VW; ++w) sv[i][w] = (there_v >> i) & 1u ? sv[i][w] : 0u;
+        }
+        bool odd = false;
+        if (t + 16 > s.n_ctx) {
+            // as in attend_kernel: no row may get 0 * inf of a draft it does not see
+            constexpr uint32_t EXP = CK == kBF16 ? 0x7f80u : CK == kF16 ? 0x7c00u : 0x7fu;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int w = 0; w < Rows::VW; ++w)
+#pragma unroll
+                    for (int b = 0; b < 4 / ES; ++b) {
+                        const uint32_t x = EXP << (b * ES * 8);
+                        if ((sv[i][w] & x) == x) {
+                            odd = true;
+                            sv[i][w] &= ~((ES == 2 ? 0xffffu : 0xffu) << (b * ES * 8));
+                        }
+                    }
+        }
+        const bool any_odd = __ballot(odd) != 0;
+        if (lane == 0) {
+            s_ok[buf][wave] = there_k;
+            s_odd[buf][wave] = any_odd ? 1u : 0u;
+        }
+        u32x4* ks = &s_kv[buf][K_AT + (sub * 2 + half) * STEPS * 64 + lane];
+#pragma unroll
+        for (int st = 0; st < STEPS; ++st) {
+            if constexpr (CK == kE4M3) {
+                const uint32_t* w = sk[st >> 1] + 2 * (st & 1);
+                ks[st * 64] = u32x4{e4m3_pair<QK, false>(w[0]), e4m3_pair<QK, true>(w[0]), e4m3_pair<QK, false>(w[1]),
+                                    e4m3_pair<QK, true>(w[1])};
+            } else {
+                ks[st * 64] = u32x4{sk[st][0], sk[st][1], sk[st][2], sk[st][3]};
+            }
+        }
+        u32x2* vs = reinterpret_cast<u32x2*>(&s_kv[buf][V_AT + sub * E * 64 + lane]) + half;
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+            u32x2 lo, hi;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if constexpr (CK == kE4M3) {
+                    const uint32_t x = perm(sv[2 * i + 1][e >> 2], sv[2 * i][e >> 2], e & 2 ? 0x07030602u : 0x05010400u);
+                    lo[i] = e4m3_pair<QK, false>(x);
+                    hi[i] = e4m3_pair<QK, true>(x);
+                } else {
+                    lo[i] = perm(sv[2 * i + 1][e >> 1], sv[2 * i][e >> 1], 0x05040100u);
+                    hi[i] = perm(sv[2 * i + 1][e >> 1], sv[2 * i][e >> 1], 0x07060302u);
+                }
+            }
+            vs[e * 128] = lo;
+            vs[e * 128 + 128] = hi;
+        }
+    };
+    const auto attend_tile = [&](int t0, int buf, int sb) {
+        const u32x4* ks = &s_kv[buf][K_AT + sb * 2 * STEPS * 64 + lane];
+        const u32x4* vs = &s_kv[buf][V_AT + sb * E * 64 + lane];
+        f32x4 sc[NT][2];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) sc[t][0] = sc[t][1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+            for (int st = 0; st < STEPS; ++st) {
+                const u32x4 k = ks[(hh * STEPS + st) * 64];
+#pragma unroll
+                for (int t = 0; t < NT; ++t) sc[t][hh] = mfma<QK>(k, q[t][st], sc[t][hh]);
+            }
+        const uint32_t ok = __builtin_amdgcn_readfirstlane(s_ok[buf][2 * sb] | (s_ok[buf][2 * sb + 1] << 16));
+        const bool odd = __builtin_amdgcn_readfirstlane(s_odd[buf][2 * sb] | s_odd[buf][2 * sb + 1]) != 0;
+        const bool edge = ok != ~0u || t0 + kAttTile > wave_all || odd;
+        uint32_t vis[NT];
+        if (edge) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                vis[t] = ok & row_sees(a, s, qi[t], t0);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (!((vis[t] >> (16 * (j >> 2) + 4 * g + (j & 3))) & 1u)) sc[t][j >> 2][j & 3] = masked;
+            }
+        }
+        // a new maximum only where a score passes the old one by 2^8 (see attend_kernel)
+        float over = -__builtin_huge_valf();
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) over = fmaxf(over, fmaf(sc[t][j >> 2][j & 3], c, -m[t]));
+        if (__ballot(over > 8.0f) != 0) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                float top = sc[t][0][0] * c;
+#pragma unroll
+                for (int j = 1; j < 8; ++j) top = fmaxf(top, sc[t][j >> 2][j & 3] * c);
+                top = fmaxf(top, __shfl_xor(top, 16, 64));
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                const float mn = fmaxf(m[t], top);
+                const float al = exp2_hw(m[t] - mn);
+                m[t] = mn;
+                l[t] *= al;
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[t][e] *= al;
+            }
+        }
+        u32x4 pb[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            float p[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                p[j] = exp2_hw(fmaf(sc[t][j >> 2][j & 3], c, -m[t]));
+                l[t] += p[j];
+            }
+            pb[t] = u32x4{pack2<QK>(p[0], p[1]), pack2<QK>(p[2], p[3]), pack2<QK>(p[4], p[5]), pack2<QK>(p[6], p[7])};
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const u32x4 v = vs[e * 64];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) acc[t][e] = mfma<QK>(v, pb[t], acc[t][e]);
+        }
+        if (odd) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                float* sp = &s_p[wave][n][0];
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    sp[16 * (j >> 2) + 4 * g + (j & 3)] = exp2_hw(fmaf(sc[t][j >> 2][j & 3], c, -m[t]));
+                __builtin_amdgcn_wave_barrier();
+                for (int b = 0; b < kAttTile; ++b) {
+                    if (!((vis[t] >> b) & 1u)) continue;
+                    bool there;
+                    const uint8_t* vr = rd.head + rd.v_off + rd.row_of(t0 + b, &there);
+                    add_odd<CK, E>(vr, a.g.D, g, sp[b], acc[t]);
+                }
+                __builtin_amdgcn_wave_barrier();
+            }
+        }
+    };
+
+    if (step0 < step_end) {
+        fetch(step0);
+        stage(step0, 0);
+        __syncthreads();
+        for (int step = step0; step < step_end; ++step) {
+            const int buf = (step - step0) & 1;
+            if (step + 1 < step_end) fetch(step + 1);
+#pragma unroll 1
+            for (int sb = 0; sb < 2; ++sb) {
+                const int t0 = step * kRowsStep + sb * kAttTile;
+                if (t0 < wave_end) attend_tile(t0, buf, sb);
+            }
+            if (step + 1 < step_end) stage(step + 1, buf ^ 1);
+            __syncthreads();
+        }
+    }
+
+    const float vsc = a.v_scale != nullptr ? a.v_scale[h] : 1.0f;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        l[t] += __shfl_xor(l[t], 16, 64);
+        l[t] += __shfl_xor(l[t], 32, 64);
+        if (qi[t] < 0) continue;
+        const int R = R0 + t * 16 + n;
+        if (s.n_parts > 1) {
+            const int64_t at = static_cast<int64_t>(item) * ROWS + wave * 16 * NT + t * 16 + n;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < E; ++e) a.part[at * DP + E * (4 * g + i) + e] = acc[t][e][i];
+            if (g == 0) {
+                a.part_ml[at * 2] = m[t];
+                a.part_ml[at * 2 + 1] = l[t];
+            }
+            continue;
+        }
+        const int64_t at = static_cast<int64_t>(s.row0 + qi[t]) * a.Hq + h * a.G + (R - qi[t] * a.G);
+        const float inv = vsc / l[t];
+        uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + at * a.g.D;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < E; e += 2) {
+                const int dd = E * (4 * g + i) + e;
+                if (MODE != kAttWhole && dd >= a.g.D) continue;      // head_dim is even here
+                const float x0 = l[t] == 0.0f ? 0.0f : acc[t][e][i] * inv, x1 = l[t] == 0.0f ? 0.0f : acc[t][e + 1][i] * inv;
+                *reinterpret_cast<uint32_t*>(out + dd) = pack2<QK>(x0, x1);
+            }
+        if (g == 0) a.lse[at] = l[t] == 0.0f ? -__builtin_huge_valf() : (m[t] + log2f(l[t])) * kLn2;
+    }
 }
 
 // Joins the parts of the rows of q (one head of one query each), 32 lanes to a
@@ -746,6 +1042,21 @@ void for_forms(int dp, int mode, bool paged, F&& f) {
 
 template <int CK, int QK>
 void run_attend(const DescArg& d, const AttArgs& a, const AttPlan& p, hipStream_t stream) {
+    if (p.row_tile > 0) {
+        const auto with = [&](auto dp, auto mode, auto nt) {
+            DARIC_LAUNCH((attend_rows_kernel<CK, QK, decltype(dp)::value, decltype(mode)::value, decltype(nt)::value>),
+                         static_cast<unsigned>(p.items), 256, 0, stream, d, a);
+        };
+        for_forms(p.dp, p.mode, true, [&](auto dp, auto mode, auto) {
+            if constexpr (decltype(mode)::value != kAttValues) {
+                if (p.row_tile == 1) with(dp, mode, std::integral_constant<int, 1>());
+                else if (p.row_tile == 2) with(dp, mode, std::integral_constant<int, 2>());
+                else if constexpr (decltype(dp)::value < 256) with(dp, mode, std::integral_constant<int, 4>());
+            }
+        });
+        check_launch("attend_pages");
+        return;
+    }
     for_forms(p.dp, p.mode, p.paged, [&](auto dp, auto mode, auto paged) {
         DARIC_LAUNCH((attend_kernel<CK, QK, decltype(dp)::value, decltype(mode)::value, decltype(paged)::value>),
                      static_cast<unsigned>(p.items), 256, 0, stream, d, a);

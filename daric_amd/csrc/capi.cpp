@@ -1613,34 +1613,67 @@ AttCall attention_call(const daric_tensor* layer, int page_first, const daric_te
     return c;
 }
 
-// Parts of the sequences' tokens: about kAttendGroups workgroups in all.
-constexpr int64_t kAttendGroups = 1024;
-void plan_attend(AttCall& c) {
-    c.a.tile_rows = kAttRows;
-    const auto row_tiles = [&](const AttSeq& s) {
-        return (static_cast<int64_t>(s.n_rows) * c.a.G + c.a.tile_rows - 1) / c.a.tile_rows;
-    };
-    const auto tiles = [](const AttSeq& s) {
-        return (static_cast<int64_t>(s.n_ctx) + s.n_rows + kAttTile - 1) / kAttTile;
-    };
-    int64_t work = 0;
-    for (const AttSeq& s : c.seqs) work += tiles(s) * row_tiles(s) * c.a.g.H;
-    const int64_t G_ = getenv("DARIC_G") ? atoi(getenv("DARIC_G")) : kAttendGroups;
-    const int64_t part = std::max<int64_t>(4, (work + G_ - 1) / G_);
-    for (AttSeq& s : c.seqs) {
-        const int64_t parts = (tiles(s) + part - 1) / part;
-        s.tile_begin = static_cast<int32_t>(c.p.items);
-        s.at = static_cast<int32_t>(c.p.join_rows);
-        s.n_parts = static_cast<int32_t>(parts);
-        c.p.items += parts * row_tiles(s) * c.a.g.H;
-        c.p.join_rows += static_cast<int64_t>(s.n_rows) * c.a.Hq;
-        c.p.max_parts = std::max(c.p.max_parts, parts);
-        DARIC_CHECK(c.p.items <= kMaxTiles && c.p.join_rows <= kIntMax, "too many rows in one attend_pages call");
+// A launch of an attention call: sequences whose rows of a KV head fill one
+// matrix tile at most (attend_kernel), or those with more (attend_rows_kernel).
+struct AttGroup {
+    AttArgs a;
+    AttPlan p;
+    std::vector<AttSeq> seqs;
+    int64_t bytes() const {
+        return p.max_parts > 1 ? p.items * a.tile_rows * (p.dp + 2) * static_cast<int64_t>(sizeof(float)) : 0;
     }
-    DARIC_CHECK(c.p.max_parts <= 1 || c.p.join_rows <= kMaxTiles, "too many rows in one attend_pages call");
-}
-int64_t attend_bytes(const AttCall& c) {
-    return c.p.max_parts > 1 ? c.p.items * c.a.tile_rows * (c.p.dp + 2) * static_cast<int64_t>(sizeof(float)) : 0;
+};
+
+constexpr int64_t kAttendGroups = 1024;
+std::vector<AttGroup> plan_attend(const AttCall& c) {
+    std::vector<AttGroup> groups;
+    const auto rows = [&](const AttSeq& s) { return static_cast<int64_t>(s.n_rows) * c.a.G; };
+    for (const bool many : {false, true}) {
+        AttGroup gr{c.a, c.p, {}};
+        for (const AttSeq& s : c.seqs)
+            if ((c.p.mode != kAttValues && rows(s) > kAttRows) == many) gr.seqs.push_back(s);
+        if (gr.seqs.empty()) continue;
+        gr.a.n_seqs = static_cast<int32_t>(gr.seqs.size());
+        int64_t step = kAttTile, target = kAttendGroups, least = 4;
+        gr.a.tile_rows = kAttRows;
+        if (many) {
+            step = kRowsStep;
+            double best = 0;
+            for (const int nt : {1, 2, 4}) {
+                if (nt * c.p.dp > 512) continue;
+                double cost = 0;
+                for (const AttSeq& s : gr.seqs)
+                    cost += (static_cast<double>(s.n_ctx) + s.n_rows) * static_cast<double>((rows(s) + 64 * nt - 1) / (64 * nt)) * (nt + 0.75);
+                if (gr.p.row_tile == 0 || cost < best) {
+                    best = cost;
+                    gr.p.row_tile = nt;
+                }
+            }
+            if (getenv("DARIC_NT")) gr.p.row_tile = atoi(getenv("DARIC_NT"));
+            gr.a.tile_rows = 64 * gr.p.row_tile;
+            target = gr.p.row_tile * c.p.dp <= 256 ? 512 : 256;
+        }
+        if (getenv("DARIC_G")) target = atoi(getenv("DARIC_G"));
+        const auto row_tiles = [&](const AttSeq& s) { return (rows(s) + gr.a.tile_rows - 1) / gr.a.tile_rows; };
+        const auto steps = [&](const AttSeq& s) { return (static_cast<int64_t>(s.n_ctx) + s.n_rows + step - 1) / step; };
+        int64_t work = 0;
+        for (const AttSeq& s : gr.seqs) work += steps(s) * row_tiles(s) * c.a.g.H;
+        const int64_t part = std::max(least, (work + target - 1) / target);
+        for (AttSeq& s : gr.seqs) {
+            const int64_t parts = (steps(s) + part - 1) / part;
+            s.tile_begin = static_cast<int32_t>(gr.p.items);
+            s.at = static_cast<int32_t>(gr.p.join_rows);
+            s.n_parts = static_cast<int32_t>(parts);
+            if (many && row_tiles(s) > 1) gr.a.by_head = 1;
+            gr.p.items += parts * row_tiles(s) * c.a.g.H;
+            gr.p.join_rows += static_cast<int64_t>(s.n_rows) * c.a.Hq;
+            gr.p.max_parts = std::max(gr.p.max_parts, parts);
+            DARIC_CHECK(gr.p.items <= kMaxTiles && gr.p.join_rows <= kIntMax, "too many rows in one attend_pages call");
+        }
+        DARIC_CHECK(gr.p.max_parts <= 1 || gr.p.join_rows <= kMaxTiles, "too many rows in one attend_pages call");
+        groups.push_back(std::move(gr));
+    }
+    return groups;
 }
 
 void attention_inputs(AttCall& c, const daric_tensor* block_table, const daric_sequence* sequences, int64_t n,
@@ -1698,9 +1731,9 @@ int daric_attend_workspace(const daric_tensor* layer, int page_first, const dari
                            const daric_sequence* sequences, int64_t n_sequences, int64_t* bytes) {
     return guarded([&] {
         DARIC_CHECK(bytes != nullptr, "bytes must not be null");
-        AttCall c = attention_call(layer, page_first, q, sequences, n_sequences, false);
-        plan_attend(c);
-        *bytes = attend_bytes(c);
+        const AttCall c = attention_call(layer, page_first, q, sequences, n_sequences, false);
+        *bytes = 0;
+        for (const AttGroup& g : plan_attend(c)) *bytes += g.bytes();
     });
 }
 
@@ -1719,22 +1752,27 @@ int daric_attend_pages(const daric_tensor* layer, int page_first, const daric_te
         c.a.lse = const_cast<float*>(check_lse(c, lse));
         c.a.out = static_cast<uint8_t*>(out->data);
         if (c.seqs.empty()) return;
-        plan_attend(c);
-        const int64_t need = attend_bytes(c);
+        std::vector<AttGroup> groups = plan_attend(c);
+        int64_t need = 0;
+        for (const AttGroup& g : groups) need += g.bytes();
         DARIC_CHECK(need == 0 || (workspace != nullptr && workspace_bytes >= need && aligned(workspace, 16)),
                     "workspace must be 16-byte aligned and hold ", need, " bytes, got ", workspace_bytes);
-        c.a.part = static_cast<float*>(workspace);
-        if (need > 0) c.a.part_ml = c.a.part + c.p.items * c.a.tile_rows * c.p.dp;
         DeviceGuard guard(c.device);
         const hipStream_t st = as_stream(stream);
-        DescHandOver ho(c.device, c.seqs.data(), c.seqs.size() * sizeof(AttSeq), st);
-        if (c.ck == kBF16) attend_bf16(ho.arg(), c.a, c.p, st);
-        else if (c.ck == kF16) attend_f16(ho.arg(), c.a, c.p, st);
-        else if (c.qk == kBF16) attend_e4m3_bf16(ho.arg(), c.a, c.p, st);
-        else attend_e4m3_f16(ho.arg(), c.a, c.p, st);
-        if (c.p.max_parts <= 1) return;
-        if (c.qk == kBF16) join_bf16(ho.arg(), c.a, c.p, st);
-        else join_f16(ho.arg(), c.a, c.p, st);
+        auto* work = static_cast<uint8_t*>(workspace);
+        for (AttGroup& g : groups) {
+            g.a.part = reinterpret_cast<float*>(work);
+            if (g.bytes() > 0) g.a.part_ml = g.a.part + g.p.items * g.a.tile_rows * g.p.dp;
+            work += g.bytes();
+            DescHandOver ho(c.device, g.seqs.data(), g.seqs.size() * sizeof(AttSeq), st);
+            if (c.ck == kBF16) attend_bf16(ho.arg(), g.a, g.p, st);
+            else if (c.ck == kF16) attend_f16(ho.arg(), g.a, g.p, st);
+            else if (c.qk == kBF16) attend_e4m3_bf16(ho.arg(), g.a, g.p, st);
+            else attend_e4m3_f16(ho.arg(), g.a, g.p, st);
+            if (g.p.max_parts <= 1) continue;
+            if (c.qk == kBF16) join_bf16(ho.arg(), g.a, g.p, st);
+            else join_f16(ho.arg(), g.a, g.p, st);
+        }
     });
 }
 

@@ -253,6 +253,27 @@ def test_unseen_drafts_with_infinities(dev, dtype, bad):
     c.check(out2, lse, wclean)
 
 
+@pytest.mark.parametrize("rows", [3, 20, 150])
+def test_infinities_that_are_seen(dev, rows):
+    """Values of V that are no numbers, in cached tokens and among the run's own, reach
+    every row that sees them."""
+    c = Case(dev, [(rows, 45), (2, 3)], d=64, seed=29)
+    clean = c.layer.clone()
+    for j, bad in ((7, float("inf")), (45 + 1, float("-inf")), (45 + rows - 1, float("nan"))):
+        c.layer[1, int(c.bt[j // 16]), j % 16, :, 3::16] = bad
+    with np.errstate(all="ignore"):
+        want = c.want()
+    dirty, c.layer = c.layer, clean
+    wclean = c.want()
+    c.layer = dirty
+    out, lse = c.run()
+    got, finite = out.double().cpu().numpy(), np.isfinite(want[0])
+    np.testing.assert_array_equal(got[~finite], want[0][~finite])
+    assert np.isnan(want[0][1:rows, :, 3]).all() and np.isposinf(want[0][0, :, 3]).all()
+    out2 = torch.where(torch.from_numpy(finite).to(dev), out.double(), torch.from_numpy(wclean[0]).to(dev))
+    c.check(out2, lse, wclean)
+
+
 def test_rows_that_see_nothing(dev):
     c = Case(dev, [(4, 0), (3, 50)], tree=True, seed=10)
     c.mask[:] = 0
@@ -265,7 +286,7 @@ def test_rows_that_see_nothing(dev):
 def test_scores_of_all_sizes(dev):
     """Rising, falling and huge scores, a negative and a zero scale."""
     for scale, f in ((0.125, 30.0), (-0.125, 30.0), (0.0, 1.0), (4.0, 100.0)):
-        c = Case(dev, [(1, 700), (9, 64)], d=64, seed=11)
+        c = Case(dev, [(1, 700), (9, 64), (40, 20)], d=64, seed=11)
         ramp = torch.linspace(-f, f, 64 * 16).view(1, -1, 1, 1)
         for bo, _, n, ctx, _ in c.seqs:
             for j in range(n + ctx):
@@ -304,7 +325,8 @@ def test_given_outputs_and_rows_of_no_sequence(dev):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.uint8])
 def test_strides_and_alignment(dev, dtype):
     """q as a slice of a wider projection, heads transposed, and caches that start
-    at odd addresses: the same bits as the plain call."""
+    at odd addresses (other kernels): the same bits as the plain call where the
+    rows stay whole units, the same result within the tolerance elsewhere."""
     c = Case(dev, [(2, 100), (30, 20)], dtype=dtype, d=64, seed=13)
     want, wl = c.run()
     q = c.q.to(dev)
@@ -315,9 +337,11 @@ def test_strides_and_alignment(dev, dtype):
     a = c.on_gpu()
     flat = torch.zeros(a["layer"].numel() + 3, dtype=dtype, device=dev)
     shifted = flat[3:].view(a["layer"].shape).copy_(a["layer"])
-    for more in (dict(q=wide[:, 1]), dict(q=turned), dict(q=odd), dict(layer=shifted)):
+    for same, more in ((True, dict(q=wide[:, 1])), (True, dict(q=turned)), (False, dict(q=odd)),
+                       (False, dict(layer=shifted))):
         out, lse = c.run(**more)
-        assert torch.equal(out, want) and torch.equal(lse, wl)
+        c.check(out, lse)
+        assert not same or (torch.equal(out, want) and torch.equal(lse, wl))
     for qq, layer in ((wide[:, 1], a["layer"]), (odd, shifted)):
         w = [cache_ops.weigh_tokens(ly, c.pf, a["block_table"], x, wl, c.seqs, scale=c.scale, k_scale=a["k_scale"])
              for ly, x in ((a["layer"], q), (layer, qq))]
