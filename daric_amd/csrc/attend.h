@@ -10,8 +10,6 @@ namespace daric {
 
 // Tokens of a tile: the inner dimension of one matrix instruction over V.
 constexpr int kAttTile = 32;
-// Tokens of a step of the kernel for many rows.
-constexpr int kRowsStep = 64;
 // Query rows (a row is one head of one query) of a matrix tile.
 constexpr int kAttRows = 16;
 
@@ -60,7 +58,7 @@ enum AttMode : int { kAttWhole = 0, kAttPadded = 1, kAttValues = 2 };
 struct AttPlan {
     int mode, dp;                  // head_dim rounded up to 64, 128 or 256
     bool paged;                    // pages hold whole halves of a tile
-    int row_tile;                  // rows of a wavefront in 16s (many rows), 0: attend_kernel
+    int row_tile;                  // attend_rows_kernel: rows of a workgroup in 64s (1, 2, 4); 0: attend_kernel
     int64_t items, join_rows;      // workgroups; rows times heads of all sequences
     int64_t max_parts;             // of a sequence: with more than one, a second kernel joins them
 };

@@ -364,22 +364,63 @@ __device__ __forceinline__ int xcd_item(int b, int n, const FastDiv& heads) {
     return (set * 8 + p) * H + h;
 }
 
-// Adds a token's weight times those values of its V row that are no numbers to
-// a lane's part of O^T.
-template <int CK, int E>
-__device__ __forceinline__ void add_odd(const uint8_t* v_row, int D, int g, float p, f32x4 (&acc)[E]) {
+// V of a draft may hold infinities and NaN, and a row that does not see the draft
+// must not get 0 times them. Where a tile behind the cached tokens holds such
+// values, they are taken out of the product (drop_odd) and the rows that see them
+// marked, in two bits per row and value of the head: a sum with them is +inf (1),
+// -inf (2) or NaN (3), whatever else is in it (mark_odd; rare, so slow and small).
+template <int CK, int N>
+__device__ __forceinline__ bool drop_odd(uint32_t (&w)[N]) {
+    constexpr uint32_t EXP = CK == kBF16 ? 0x7f80u : CK == kF16 ? 0x7c00u : 0x7fu;
+    constexpr int BITS = CK == kE4M3 ? 8 : 16;
+    bool odd = false;
 #pragma unroll
-    for (int e = 0; e < E; ++e)
+    for (int i = 0; i < N; ++i)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int d = E * (4 * g + i) + e;
-            if (d >= D) continue;
+        for (int b = 0; b < 32; b += BITS)
+            if ((w[i] & (EXP << b)) == (EXP << b)) {
+                odd = true;
+                w[i] &= ~(((1u << BITS) - 1u) << b);
+            }
+    return odd;
+}
+// Marks the `rows` rows from R0 on (rows of the head) that see tokens t0 .. + n of
+// a sequence; a wavefront's work. marks: [rows][words] of LDS.
+template <int CK>
+__device__ __forceinline__ void mark_odd(const AttArgs& a, const uint8_t* v_head, const int32_t* bt, int n_ctx,
+                                                   int n_rows, int row0, int t0, int n, int R0, int rows,
+                                                   uint32_t* marks, int words) {
+    constexpr int ES = CK == kE4M3 ? 1 : 2;
+    const int lane = static_cast<int>(threadIdx.x) & 63;
+#pragma unroll 1
+    for (int t = t0; t < min(t0 + n, n_ctx + n_rows); ++t) {
+        const int p = t / a.g.PS, id = bt[p];
+        if (id <= 0 || id >= a.g.num_blocks) continue;
+        const uint8_t* v = v_head + (static_cast<int64_t>(id) * a.g.sb + static_cast<int64_t>(t - p * a.g.PS) * a.g.ss) * ES;
+#pragma unroll 1
+        for (int d = lane; d < a.g.D; d += 64) {
             float x;
-            if constexpr (CK == kE4M3) x = e4m3_to_f32(v_row[d]);
-            else if constexpr (CK == kBF16) x = bf16_to_f32(reinterpret_cast<const uint16_t*>(v_row)[d]);
-            else x = f16_to_f32(reinterpret_cast<const uint16_t*>(v_row)[d]);
-            if (!(fabsf(x) <= 3.402823466e38f)) acc[e][i] += p * x;
+            if constexpr (CK == kE4M3) x = e4m3_to_f32(v[d]);
+            else if constexpr (CK == kBF16) x = bf16_to_f32(reinterpret_cast<const uint16_t*>(v)[d]);
+            else x = f16_to_f32(reinterpret_cast<const uint16_t*>(v)[d]);
+            if (fabsf(x) <= 3.402823466e38f) continue;
+            const uint32_t mark = (x != x ? 3u : x > 0.0f ? 1u : 2u) << (2 * (d & 15));
+#pragma unroll 1
+            for (int R = 0; R < rows; ++R) {
+                const int i = (R0 + R) / a.G, b = t - n_ctx;
+                if (i >= n_rows) break;
+                const bool sees = b < 0 || (a.mask == nullptr ? b <= i
+                    : ((a.mask[static_cast<int64_t>(row0 + i) * a.words + (b >> 6)] >> (b & 63)) & 1u) != 0);
+                if (sees) atomicOr(&marks[R * words + (d >> 4)], mark);
+            }
         }
+    }
+}
+// A sum with its mark.
+__device__ __forceinline__ float with_mark(float x, uint32_t word, int d) {
+    const uint32_t mark = (word >> (2 * (d & 15))) & 3u;
+    const float inf = __builtin_huge_valf();
+    return mark == 0 ? x : mark == 1 ? x + inf : mark == 2 ? x - inf : __builtin_nanf("");
 }
 
 // ------------------------------------------------------------------ attend
@@ -392,6 +433,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_kernel(DescArg 
     constexpr int LD = DP + 4;                        // floats of a row in LDS: no two rows on one bank
     __shared__ float s_o[WAVES][kAttRows][LD];
     __shared__ float s_m[WAVES][kAttRows], s_l[WAVES][kAttRows];
+    __shared__ uint32_t s_mark[kAttRows][DP / 16], s_marked;
     const DescPtr<AttSeq> seqs = desc_at<AttSeq>(d, 0);
     const int item = xcd_item(static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x), a.heads);
     const int si = __builtin_amdgcn_readfirstlane(find_by_tile(seqs, a.n_seqs, item));
@@ -424,6 +466,9 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_kernel(DescArg 
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = f32x4{0, 0, 0, 0};
     float m = -3.402823466e38f, l = 0.0f;
+    if (tid < kAttRows * (DP / 16)) (&s_mark[0][0])[tid] = 0;
+    if (tid == 0) s_marked = 0;
+    __syncthreads();
 
     const auto tile_of = [&](Rows& r, int tile) {
         const int t0 = tile * kAttTile;
@@ -455,7 +500,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_kernel(DescArg 
         float top = t[0];
 #pragma unroll
         for (int j = 1; j < 8; ++j) top = fmaxf(top, t[j]);
-        if (__ballot(top - m > 8.0f) != 0) {
+        if (__builtin_expect(__ballot(top - m > 8.0f) != 0, 0)) {
             top = fmaxf(top, __shfl_xor(top, 16, 64));
             top = fmaxf(top, __shfl_xor(top, 32, 64));
             const float mn = fmaxf(m, top);
@@ -471,25 +516,15 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_kernel(DescArg 
             p[j] = exp2_hw(t[j] - m);
             l += p[j];
         }
-        // V of a masked draft may be anything; a row that does not see it must
-        // not get 0 * inf. Such values are taken out of the product and added
-        // below to the rows that see them.
-        bool odd = false;
         if (drafts) {
-            constexpr uint32_t EXP = CK == kBF16 ? 0x7f80u : CK == kF16 ? 0x7c00u : 0x7fu;
-            constexpr int ES = Rows::ES;
+            bool odd = false;
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-#pragma unroll
-                for (int w = 0; w < Rows::VW; ++w)
-#pragma unroll
-                    for (int b = 0; b < 4 / ES; ++b) {
-                        const uint32_t x = EXP << (b * ES * 8);
-                        if ((r.v[j][w] & x) == x) {
-                            odd = true;
-                            r.v[j][w] &= ~((ES == 2 ? 0xffffu : 0xffu) << (b * ES * 8));
-                        }
-                    }
+            for (int j = 0; j < 8; ++j) odd |= drop_odd<CK>(r.v[j]);
+            if (__builtin_expect(__ballot(odd) != 0, 0)) {
+                mark_odd<CK>(a, rd.head + rd.v_off, rd.bt, s.n_ctx, s.n_rows, s.row0, t0, kAttTile, rt * kAttRows, kAttRows,
+                             &s_mark[0][0], DP / 16);
+                if (lane == 0) s_marked = 1;
+            }
         }
         const u32x4 pb = {pack2<QK>(p[0], p[1]), pack2<QK>(p[2], p[3]), pack2<QK>(p[4], p[5]), pack2<QK>(p[6], p[7])};
 #pragma unroll
@@ -498,21 +533,6 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_kernel(DescArg 
             v_operands<CK, QK, DP>(r, e, &lo, &hi);
             acc[e] = mfma<QK>(lo, pb, acc[e]);
             acc[e + 1] = mfma<QK>(hi, pb, acc[e + 1]);
-        }
-        if (__ballot(odd) != 0) {
-            // the wavefront's own LDS rows hold P meanwhile
-            float* sp = &s_o[wave][n][0];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sp[16 * (j >> 2) + 4 * g + (j & 3)] = p[j];
-            __builtin_amdgcn_wave_barrier();
-            for (int b = 0; b < kAttTile; ++b) {
-                if (!((vis >> b) & 1u)) continue;
-                const float pj = sp[b];
-                bool there;
-                const uint8_t* vr = rd.head + rd.v_off + rd.row_of(t0 + b, &there);
-                add_odd<CK, E>(vr, a.g.D, g, pj, acc);
-            }
-            __builtin_amdgcn_wave_barrier();
         }
     };
 
@@ -573,6 +593,10 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_kernel(DescArg 
         for (int e = 0; e < E; ++e) o[e] += s_o[w][rn][dc + e] * al;
     }
     if (orow.i < 0) return;
+    if (s_marked) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = with_mark(o[e], s_mark[rn][(dc + e) >> 4], dc + e);
+    }
     if (s.n_parts > 1) {
         float* po = a.part + (static_cast<int64_t>(item) * kAttRows + rn) * DP;
 #pragma unroll
@@ -596,21 +620,21 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_kernel(DescArg 
 }
 
 // -------------------------------------------------------- attend, many rows
-// One workgroup: one KV head, 64 NT rows of q (16 NT to a wavefront) and one part
-// of a sequence's tokens, in steps of 64. K and V are staged in LDS as the
+// One workgroup: one KV head, 16 NT rows of q to each of WAVES wavefronts and one
+// part of a sequence's tokens, in steps of 16 to a wavefront. K and V are staged in LDS as the
 // operands of the matrix instructions lie in registers, a wavefront's operand in
 // 1 KiB, so that reads and writes of it touch every bank alike: e4m3 becomes q's
 // type and V's tokens are paired once per workgroup, and a read feeds NT
 // instructions. The next step's rows come from memory meanwhile, into the other
 // half of the LDS.
-template <int CK, int QK, int DP, int MODE, int NT>
-__global__ __launch_bounds__(256, DP * NT <= 256 ? 2 : 1) void attend_rows_kernel(DescArg d, AttArgs a) {
+template <int CK, int QK, int DP, int MODE, bool PAGED, int WAVES, int NT>
+__global__ __launch_bounds__(WAVES * 64, DP * NT <= 256 ? 2 : 1) void attend_rows_kernel(DescArg d, AttArgs a) {
     using Rows = TileRows<CK, DP>;
-    constexpr int E = Rows::E, STEPS = DP / 32, ES = Rows::ES, ROWS = 64 * NT;
-    constexpr int K_AT = 0, V_AT = 4 * STEPS * 64, UNITS = V_AT + 2 * E * 64;    // 16-byte units of a step
+    constexpr int E = Rows::E, STEPS = DP / 32, ROWS = WAVES * 16 * NT, STEP = WAVES * 16;
+    constexpr int K_AT = 0, V_AT = WAVES * STEPS * 64, UNITS = V_AT + WAVES / 2 * E * 64;    // 16-byte units of a step
     __shared__ u32x4 s_kv[2][UNITS];
-    __shared__ float s_p[4][kAttRows][kAttTile + 1];
-    __shared__ uint32_t s_ok[2][4], s_odd[2][4];
+    __shared__ uint32_t s_ok[2][WAVES];
+    __shared__ uint32_t s_mark[ROWS][DP / 16], s_marked;
     const DescPtr<AttSeq> seqs = desc_at<AttSeq>(d, 0);
     const int item = a.by_head ? static_cast<int>(blockIdx.x)
                                : xcd_item(static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x), a.heads);
@@ -633,13 +657,18 @@ __global__ __launch_bounds__(256, DP * NT <= 256 ? 2 : 1) void attend_rows_kerne
     const int end = causal ? s.n_ctx + query(rt * ROWS + ROWS - 1) + 1 : total;
     const int wave_end = R0 < s.n_rows * a.G ? (causal ? s.n_ctx + query(R0 + 16 * NT - 1) + 1 : total) : 0;
     const int wave_all = causal ? s.n_ctx + query(R0) + 1 : s.n_ctx;
-    const int steps = (total + kRowsStep - 1) / kRowsStep;
+    const int steps = (total + STEP - 1) / STEP;
     const int part_steps = (steps + s.n_parts - 1) / s.n_parts;
     const int step0 = part * part_steps;
-    const int step_end = min(step0 + part_steps, (end + kRowsStep - 1) / kRowsStep);
+    const int step_end = min(step0 + part_steps, (end + STEP - 1) / STEP);
 
     RowReader<CK, DP, MODE, false> rd;
     rd.init(a, s.bt_offset, total, h, lane);
+    // The scores' factor c is made positive by q's sign, so that a score of -inf
+    // is a masked one; with c = 0 all scores are 0, of a zero q.
+    float c = a.scale_log2 * (a.k_scale != nullptr ? a.k_scale[h] : 1.0f);
+    const uint32_t q_keep = c == 0.0f ? 0u : ~0u, q_flip = c < 0.0f ? 0x80008000u : 0u;
+    c = c == 0.0f ? 1.0f : fabsf(c);
     u32x4 q[NT][STEPS];
     int qi[NT];
 #pragma unroll
@@ -647,76 +676,76 @@ __global__ __launch_bounds__(256, DP * NT <= 256 ? 2 : 1) void attend_rows_kerne
         const QRow row = q_row(a, s.n_rows, h, R0 + t * 16 + n);
         qi[t] = row.i;
         load_q<CK, DP, MODE>(a, s, row, g, q[t]);
-    }
-    // A masked score becomes an infinity that c turns to -inf; with c = 0 all
-    // scores are 0, of a zero q.
-    float c = a.scale_log2 * (a.k_scale != nullptr ? a.k_scale[h] : 1.0f);
-    if (c == 0.0f) {
-        c = 1.0f;
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int st = 0; st < STEPS; ++st) q[t][st] = u32x4{0, 0, 0, 0};
+        for (int st = 0; st < STEPS; ++st) q[t][st] = (q[t][st] & q_keep) ^ q_flip;
     }
-    const float masked = c > 0.0f ? -__builtin_huge_valf() : __builtin_huge_valf();
     f32x4 acc[NT][E];
-    float m[NT], l[NT];
+    float m[NT], l[NT], limit[NT];                     // limit: scores beyond it need a new maximum
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        m[t] = -3.402823466e38f;
+        m[t] = limit[t] = -3.402823466e38f;
         l[t] = 0.0f;
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[t][e] = f32x4{0, 0, 0, 0};
     }
 
-    // A wavefront stages 16 of a step's tokens.
+    // A wavefront stages 16 of a step's tokens: all in one page (PAGED), or lane n
+    // with the page of token n. The page is known a step before its rows are asked for.
     const int sub = wave >> 1, half = wave & 1;
     uint32_t sk[Rows::KU][4], sv[4][Rows::VW];
-    uint32_t there_k = 0, there_v = 0;
+    uint32_t there_k = 0;
+    int page_id = 0;
+    const auto locate = [&](int step) {
+        const int t = step * STEP + 16 * wave + (PAGED ? 0 : n);
+        const int p = min(static_cast<int>(rd.page.div(static_cast<uint32_t>(t))), rd.last_page);
+        page_id = PAGED ? uniform_load(rd.bt + p) : rd.bt[p];
+    };
     const auto fetch = [&](int step) {
-        const int t = step * kRowsStep + 16 * wave;
-        bool there;
-        const int64_t ko = rd.row_of(t + n, &there);
-        there_k = static_cast<uint32_t>(__ballot(there)) & 0xffffu;
-        rd.load_k(sk, rd.head + ko);
-        there_v = 0;
+        const int t = step * STEP + 16 * wave + (PAGED ? 0 : n);
+        const bool there = t < total && rd.is_page(page_id);
+        const int p = static_cast<int>(rd.page.div(static_cast<uint32_t>(t)));
+        const uint32_t id = there ? static_cast<uint32_t>(page_id) : 0u;
+        const uint32_t slot = there ? static_cast<uint32_t>(t - p * rd.PS) : 0u;
+        const int64_t row = static_cast<int64_t>(id) * rd.sb + static_cast<int64_t>(slot) * rd.ss;
+        if constexpr (PAGED) {
+            there_k = !there ? 0u : total - t >= 16 ? 0xffffu : (1u << (total - t)) - 1u;
+            const uint8_t* base = rd.head + row;
+            rd.load_k(sk, base + static_cast<uint32_t>(n * static_cast<int>(rd.ss)));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int64_t vo = rd.row_of(t + 4 * g + i, &there);
-            if (there) there_v |= 1u << i;
-            rd.load_v(sv[i], rd.head + rd.v_off + vo);
+            for (int i = 0; i < 4; ++i)
+                rd.load_v(sv[i], base + rd.v_off + i * rd.ss + static_cast<uint32_t>(4 * g * static_cast<int>(rd.ss)));
+        } else {
+            there_k = static_cast<uint32_t>(__ballot(there)) & 0xffffu;
+            const int lo = static_cast<int>(row), hi = static_cast<int>(row >> 32);
+            rd.load_k(sk, rd.head + row);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int from = 4 * g + i;
+                const int64_t o = static_cast<int64_t>((static_cast<uint64_t>(static_cast<uint32_t>(__shfl(hi, from, 64))) << 32) |
+                                                       static_cast<uint32_t>(__shfl(lo, from, 64)));
+                rd.load_v(sv[i], rd.head + rd.v_off + o);
+            }
         }
     };
     const auto stage = [&](int step, int buf) {
-        const int t = step * kRowsStep + 16 * wave;
+        const int t = step * STEP + 16 * wave;
         if (there_k != 0xffffu) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int w = 0; w < Rows::VW; ++w) sv[i][w] = (there_v >> i) & 1u ? sv[i][w] : 0u;
+                for (int w = 0; w < Rows::VW; ++w) sv[i][w] = (there_k >> (4 * g + i)) & 1u ? sv[i][w] : 0u;
         }
-        bool odd = false;
         if (t + 16 > s.n_ctx) {
-            // as in attend_kernel: no row may get 0 * inf of a draft it does not see
-            constexpr uint32_t EXP = CK == kBF16 ? 0x7f80u : CK == kF16 ? 0x7c00u : 0x7fu;
+            bool odd = false;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int w = 0; w < Rows::VW; ++w)
-#pragma unroll
-                    for (int b = 0; b < 4 / ES; ++b) {
-                        const uint32_t x = EXP << (b * ES * 8);
-                        if ((sv[i][w] & x) == x) {
-                            odd = true;
-                            sv[i][w] &= ~((ES == 2 ? 0xffffu : 0xffu) << (b * ES * 8));
-                        }
-                    }
+            for (int i = 0; i < 4; ++i) odd |= drop_odd<CK>(sv[i]);
+            if (__builtin_expect(__ballot(odd) != 0, 0)) {
+                mark_odd<CK>(a, rd.head + rd.v_off, rd.bt, s.n_ctx, s.n_rows, s.row0, t, 16, rt * ROWS, ROWS,
+                             &s_mark[0][0], DP / 16);
+                if (lane == 0) s_marked = 1;
+            }
         }
-        const bool any_odd = __ballot(odd) != 0;
-        if (lane == 0) {
-            s_ok[buf][wave] = there_k;
-            s_odd[buf][wave] = any_odd ? 1u : 0u;
-        }
+        if (lane == 0) s_ok[buf][wave] = there_k;
         u32x4* ks = &s_kv[buf][K_AT + (sub * 2 + half) * STEPS * 64 + lane];
 #pragma unroll
         for (int st = 0; st < STEPS; ++st) {
@@ -747,105 +776,143 @@ __global__ __launch_bounds__(256, DP * NT <= 256 ? 2 : 1) void attend_rows_kerne
             vs[e * 128 + 128] = hi;
         }
     };
-    const auto attend_tile = [&](int t0, int buf, int sb) {
+
+    // The scores of tile sb of a step, -inf where masked. K's operands are all asked
+    // for at once.
+    const auto scores = [&](f32x4 (&sc)[NT][2], int t0, int buf, int sb) {
         const u32x4* ks = &s_kv[buf][K_AT + sb * 2 * STEPS * 64 + lane];
-        const u32x4* vs = &s_kv[buf][V_AT + sb * E * 64 + lane];
-        f32x4 sc[NT][2];
+        const uint32_t ok = __builtin_amdgcn_readfirstlane(s_ok[buf][2 * sb] | (s_ok[buf][2 * sb + 1] << 16));
+        u32x4 kf[2 * STEPS];
+#pragma unroll
+        for (int i = 0; i < 2 * STEPS; ++i) kf[i] = ks[i * 64];
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int t = 0; t < NT; ++t) sc[t][0] = sc[t][1] = f32x4{0, 0, 0, 0};
+        // 2 NT sums in turn: an instruction that waits for its own sum stalls
 #pragma unroll
-        for (int hh = 0; hh < 2; ++hh)
+        for (int st = 0; st < STEPS; ++st)
 #pragma unroll
-            for (int st = 0; st < STEPS; ++st) {
-                const u32x4 k = ks[(hh * STEPS + st) * 64];
+            for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
-                for (int t = 0; t < NT; ++t) sc[t][hh] = mfma<QK>(k, q[t][st], sc[t][hh]);
-            }
-        const uint32_t ok = __builtin_amdgcn_readfirstlane(s_ok[buf][2 * sb] | (s_ok[buf][2 * sb + 1] << 16));
-        const bool odd = __builtin_amdgcn_readfirstlane(s_odd[buf][2 * sb] | s_odd[buf][2 * sb + 1]) != 0;
-        const bool edge = ok != ~0u || t0 + kAttTile > wave_all || odd;
-        uint32_t vis[NT];
-        if (edge) {
+                for (int t = 0; t < NT; ++t) sc[t][hh] = mfma<QK>(kf[hh * STEPS + st], q[t][st], sc[t][hh]);
+        if (__builtin_expect(ok != ~0u || t0 + kAttTile > wave_all, 0)) {
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                vis[t] = ok & row_sees(a, s, qi[t], t0);
+                const uint32_t vis = ok & row_sees(a, s, qi[t], t0);
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    if (!((vis[t] >> (16 * (j >> 2) + 4 * g + (j & 3))) & 1u)) sc[t][j >> 2][j & 3] = masked;
+                    if (!((vis >> (16 * (j >> 2) + 4 * g + (j & 3))) & 1u)) sc[t][j >> 2][j & 3] = -__builtin_huge_valf();
             }
         }
-        // a new maximum only where a score passes the old one by 2^8 (see attend_kernel)
-        float over = -__builtin_huge_valf();
+    };
+    const auto top_of = [&](const f32x4 (&sc)[NT][2], int t) {
+        float top = sc[t][0][0];
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int j = 1; j < 8; ++j) top = fmaxf(top, sc[t][j >> 2][j & 3]);
+        return top;
+    };
+    // The sums are never scaled: a scaling on a side way through the loop moved them
+    // to other registers and back in every tile (38 of its 190 instructions). A row's
+    // maximum is that of the first tile in which it sees a token, and weights up to
+    // 2^14 of it are as exact. A wavefront whose scores pass that takes its rows'
+    // maxima in a second pass over the tokens and its sums in a third.
+    constexpr float LOWEST = -3.402823466e38f;
+    enum { kFirst, kMaxima, kLast, kDone };
+    int pass = wave_end > 0 ? kFirst : kDone;
+    bool failed = false;
+    const auto attend_tiles = [&](int step, int buf, int tiles) {
+#pragma unroll 1
+        for (int sb = 0; sb < tiles; ++sb) {
+            const int t0 = step * STEP + sb * kAttTile;
+            const u32x4* vs = &s_kv[buf][V_AT + sb * E * 64 + lane];
+            f32x4 sc[NT][2];
+            scores(sc, t0, buf, sb);
+            bool over = false;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) over = fmaxf(over, fmaf(sc[t][j >> 2][j & 3], c, -m[t]));
-        if (__ballot(over > 8.0f) != 0) {
+            for (int t = 0; t < NT; ++t) over |= top_of(sc, t) > limit[t];
+            if (__builtin_expect(__ballot(over) != 0, 0)) {
+                bool known = false;                    // a row with a maximum, and sums, already
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                float top = sc[t][0][0] * c;
-#pragma unroll
-                for (int j = 1; j < 8; ++j) top = fmaxf(top, sc[t][j >> 2][j & 3] * c);
-                top = fmaxf(top, __shfl_xor(top, 16, 64));
-                top = fmaxf(top, __shfl_xor(top, 32, 64));
-                const float mn = fmaxf(m[t], top);
-                const float al = exp2_hw(m[t] - mn);
-                m[t] = mn;
-                l[t] *= al;
-#pragma unroll
-                for (int e = 0; e < E; ++e) acc[t][e] *= al;
-            }
-        }
-        u32x4 pb[NT];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            float p[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                p[j] = exp2_hw(fmaf(sc[t][j >> 2][j & 3], c, -m[t]));
-                l[t] += p[j];
-            }
-            pb[t] = u32x4{pack2<QK>(p[0], p[1]), pack2<QK>(p[2], p[3]), pack2<QK>(p[4], p[5]), pack2<QK>(p[6], p[7])};
-        }
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const u32x4 v = vs[e * 64];
-#pragma unroll
-            for (int t = 0; t < NT; ++t) acc[t][e] = mfma<QK>(v, pb[t], acc[t][e]);
-        }
-        if (odd) {
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                float* sp = &s_p[wave][n][0];
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    sp[16 * (j >> 2) + 4 * g + (j & 3)] = exp2_hw(fmaf(sc[t][j >> 2][j & 3], c, -m[t]));
-                __builtin_amdgcn_wave_barrier();
-                for (int b = 0; b < kAttTile; ++b) {
-                    if (!((vis[t] >> b) & 1u)) continue;
-                    bool there;
-                    const uint8_t* vr = rd.head + rd.v_off + rd.row_of(t0 + b, &there);
-                    add_odd<CK, E>(vr, a.g.D, g, sp[b], acc[t]);
+                for (int t = 0; t < NT; ++t) {
+                    float top = top_of(sc, t);
+                    top = fmaxf(top, __shfl_xor(top, 16, 64));
+                    top = fmaxf(top, __shfl_xor(top, 32, 64));
+                    if (top > limit[t]) {
+                        known |= m[t] != LOWEST;
+                        m[t] = fmaxf(m[t], top * c);
+                        limit[t] = pass == kMaxima ? top : fmaxf((m[t] + 14.0f) / c, top);
+                    }
                 }
-                __builtin_amdgcn_wave_barrier();
+                if (pass == kFirst && __ballot(known) != 0) {
+                    failed = true;
+                    return;
+                }
+            }
+            if (pass == kMaxima) continue;
+            constexpr int VF = E < 8 ? E : 8;          // V operands read at once
+            u32x4 vf[VF];
+#pragma unroll
+            for (int e = 0; e < VF; ++e) vf[e] = vs[e * 64];
+            __builtin_amdgcn_sched_barrier(0);
+            u32x4 pb[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                float p[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    p[j] = exp2_hw(fmaf(sc[t][j >> 2][j & 3], c, -m[t]));
+                    l[t] += p[j];
+                }
+                pb[t] = u32x4{pack2<QK>(p[0], p[1]), pack2<QK>(p[2], p[3]), pack2<QK>(p[4], p[5]), pack2<QK>(p[6], p[7])};
+            }
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const u32x4 v = e < VF ? vf[e % VF] : vs[e * 64];
+#pragma unroll
+                for (int t = 0; t < NT; ++t) acc[t][e] = mfma<QK>(v, pb[t], acc[t][e]);
             }
         }
     };
 
+    for (int i = tid; i < ROWS * (DP / 16); i += WAVES * 64) (&s_mark[0][0])[i] = 0;
+    if (tid == 0) s_marked = 0;
+    __syncthreads();
     if (step0 < step_end) {
-        fetch(step0);
-        stage(step0, 0);
-        __syncthreads();
-        for (int step = step0; step < step_end; ++step) {
-            const int buf = (step - step0) & 1;
-            if (step + 1 < step_end) fetch(step + 1);
 #pragma unroll 1
-            for (int sb = 0; sb < 2; ++sb) {
-                const int t0 = step * kRowsStep + sb * kAttTile;
-                if (t0 < wave_end) attend_tile(t0, buf, sb);
+        for (;;) {
+            if (pass != kDone) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    l[t] = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) acc[t][e] = f32x4{0, 0, 0, 0};
+                }
             }
-            if (step + 1 < step_end) stage(step + 1, buf ^ 1);
+            locate(step0);
+            fetch(step0);
+            locate(min(step0 + 1, steps - 1));
+            stage(step0, 0);
             __syncthreads();
+#pragma unroll 1
+            for (int step = step0; step < step_end; ++step) {
+                const int buf = (step - step0) & 1;
+                const int tiles = pass == kDone || failed
+                                      ? 0 : min(WAVES / 2, (wave_end - step * STEP + kAttTile - 1) / kAttTile);
+                if (step + 1 < step_end) {
+                    fetch(step + 1);
+                    locate(min(step + 2, steps - 1));
+                }
+                attend_tiles(step, buf, tiles);
+                if (step + 1 < step_end) stage(step + 1, buf ^ 1);
+                __syncthreads();
+            }
+            pass = failed ? kMaxima : pass == kMaxima ? kLast : kDone;
+            failed = false;
+            if (__builtin_expect(__syncthreads_or(pass != kDone) == 0, 1)) break;
+            if (pass == kLast) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t) limit[t] = __builtin_huge_valf();
+            }
         }
     }
 
@@ -856,6 +923,15 @@ __global__ __launch_bounds__(256, DP * NT <= 256 ? 2 : 1) void attend_rows_kerne
         l[t] += __shfl_xor(l[t], 32, 64);
         if (qi[t] < 0) continue;
         const int R = R0 + t * 16 + n;
+        if (s_marked) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const int dd = E * (4 * g + i) + e;
+                    acc[t][e][i] = with_mark(acc[t][e][i], s_mark[wave * 16 * NT + t * 16 + n][dd >> 4], dd);
+                }
+        }
         if (s.n_parts > 1) {
             const int64_t at = static_cast<int64_t>(item) * ROWS + wave * 16 * NT + t * 16 + n;
 #pragma unroll
@@ -1043,15 +1119,20 @@ void for_forms(int dp, int mode, bool paged, F&& f) {
 template <int CK, int QK>
 void run_attend(const DescArg& d, const AttArgs& a, const AttPlan& p, hipStream_t stream) {
     if (p.row_tile > 0) {
-        const auto with = [&](auto dp, auto mode, auto nt) {
-            DARIC_LAUNCH((attend_rows_kernel<CK, QK, decltype(dp)::value, decltype(mode)::value, decltype(nt)::value>),
-                         static_cast<unsigned>(p.items), 256, 0, stream, d, a);
+        const auto with = [&](auto dp, auto mode, auto paged, auto waves, auto nt) {
+            DARIC_LAUNCH((attend_rows_kernel<CK, QK, decltype(dp)::value, decltype(mode)::value, decltype(paged)::value,
+                                             decltype(waves)::value, decltype(nt)::value>),
+                         static_cast<unsigned>(p.items), decltype(waves)::value * 64, 0, stream, d, a);
         };
-        for_forms(p.dp, p.mode, true, [&](auto dp, auto mode, auto) {
-            if constexpr (decltype(mode)::value != kAttValues) {
-                if (p.row_tile == 1) with(dp, mode, std::integral_constant<int, 1>());
-                else if (p.row_tile == 2) with(dp, mode, std::integral_constant<int, 2>());
-                else if constexpr (decltype(dp)::value < 256) with(dp, mode, std::integral_constant<int, 4>());
+        // pages of other sizes: the padded form for whole heads too
+        for_forms(p.dp, p.paged ? p.mode : static_cast<int>(kAttPadded), p.paged, [&](auto dp, auto mode, auto paged) {
+            using std::integral_constant;
+            if constexpr (decltype(mode)::value == kAttPadded || (decltype(mode)::value == kAttWhole && decltype(paged)::value)) {
+                if (p.row_tile == 1) with(dp, mode, paged, integral_constant<int, 4>(), integral_constant<int, 1>());
+                else if constexpr (decltype(dp)::value < 256) {
+                    if (p.row_tile == 2) with(dp, mode, paged, integral_constant<int, 4>(), integral_constant<int, 2>());
+                    else with(dp, mode, paged, integral_constant<int, 8>(), integral_constant<int, 2>());
+                }
             }
         });
         check_launch("attend_pages");
@@ -1078,7 +1159,8 @@ void run_join(const DescArg& d, const AttArgs& a, const AttPlan& p, hipStream_t 
     for_forms(p.dp, kAttWhole, true, [&](auto dp, auto, auto) {
         constexpr int DP = decltype(dp)::value;
         const int rows = static_cast<int>(p.join_rows);
-        if (p.max_parts <= 4) DARIC_LAUNCH((attend_join_kernel<QK, DP, 1>), (rows + 7) / 8, 256, 0, stream, d, a, rows);
+        // many rows fill the chip by themselves
+        if (p.max_parts <= 4 || rows >= 4096) DARIC_LAUNCH((attend_join_kernel<QK, DP, 1>), (rows + 7) / 8, 256, 0, stream, d, a, rows);
         else DARIC_LAUNCH((attend_join_kernel<QK, DP, 8>), rows, 256, 0, stream, d, a, rows);
     });
     check_launch("attend_pages join");

@@ -1637,10 +1637,9 @@ std::vector<AttGroup> plan_attend(const AttCall& c) {
         int64_t step = kAttTile, target = kAttendGroups, least = 4;
         gr.a.tile_rows = kAttRows;
         if (many) {
-            step = kRowsStep;
             double best = 0;
             for (const int nt : {1, 2, 4}) {
-                if (nt * c.p.dp > 512) continue;
+                if (nt > 1 && c.p.dp > 128) continue;
                 double cost = 0;
                 for (const AttSeq& s : gr.seqs)
                     cost += (static_cast<double>(s.n_ctx) + s.n_rows) * static_cast<double>((rows(s) + 64 * nt - 1) / (64 * nt)) * (nt + 0.75);
@@ -1651,7 +1650,8 @@ std::vector<AttGroup> plan_attend(const AttCall& c) {
             }
             if (getenv("DARIC_NT")) gr.p.row_tile = atoi(getenv("DARIC_NT"));
             gr.a.tile_rows = 64 * gr.p.row_tile;
-            target = gr.p.row_tile * c.p.dp <= 256 ? 512 : 256;
+            step = gr.p.row_tile == 4 ? 128 : 64;
+            target = gr.p.row_tile == 4 || c.p.dp > 128 ? 256 : 512;
         }
         if (getenv("DARIC_G")) target = atoi(getenv("DARIC_G"));
         const auto row_tiles = [&](const AttSeq& s) { return (rows(s) + gr.a.tile_rows - 1) / gr.a.tile_rows; };

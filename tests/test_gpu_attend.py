@@ -297,6 +297,24 @@ def test_scores_of_all_sizes(dev):
         c.check_weigh(lse)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,ctx", [(1, 2000), (70, 1500), (300, 700)])
+def test_rising_scores(dev, dtype, rows, ctx):
+    """Scores that rise by hundreds along the context, for some rows only, late and
+    more than once: maxima taken early do not hold."""
+    c = Case(dev, [(rows, ctx)], dtype=dtype, d=64, g=2, h=2, seed=28)
+    c.layer[0, ..., 0] = 0
+    for j in range(ctx):
+        b = int(c.bt[j // 16])
+        c.layer[0, b, j % 16, :, 0] = 8.0 * (j // 400) + (40.0 if j == ctx - 3 else 0.0)
+    c.q[..., 0] = 0
+    c.q[::3, :, 0] = 30.0
+    c.q[1::5, :, 0] = -20.0
+    out, lse = c.run()
+    c.check(out, lse)
+    c.check_weigh(lse)
+
+
 def test_given_outputs_and_rows_of_no_sequence(dev):
     c = Case(dev, [(3, 40), (2, 17)], seed=12)
     seqs = [(s[0], s[1] + 1 + i, *s[2:]) for i, s in enumerate(c.seqs)]     # a row free before each
