@@ -788,6 +788,7 @@ __global__ __launch_bounds__(WAVES * 64, DP * NT <= 256 ? 2 : 1) void attend_row
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int t = 0; t < NT; ++t) sc[t][0] = sc[t][1] = f32x4{0, 0, 0, 0};
+        __builtin_amdgcn_s_setprio(1);
         // 2 NT sums in turn: an instruction that waits for its own sum stalls
 #pragma unroll
         for (int st = 0; st < STEPS; ++st)
@@ -795,6 +796,7 @@ __global__ __launch_bounds__(WAVES * 64, DP * NT <= 256 ? 2 : 1) void attend_row
             for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
                 for (int t = 0; t < NT; ++t) sc[t][hh] = mfma<QK>(kf[hh * STEPS + st], q[t][st], sc[t][hh]);
+        __builtin_amdgcn_s_setprio(0);
         if (__builtin_expect(ok != ~0u || t0 + kAttTile > wave_all, 0)) {
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
@@ -820,9 +822,22 @@ __global__ __launch_bounds__(WAVES * 64, DP * NT <= 256 ? 2 : 1) void attend_row
     enum { kFirst, kMaxima, kLast, kDone };
     int pass = wave_end > 0 ? kFirst : kDone;
     bool failed = false;
+    // The rows in registers go to LDS, and the next ones are asked for, in the middle
+    // of a step's tiles, by the two wavefronts of a SIMD at different tiles, so that
+    // one of them feeds the matrix cores meanwhile.
+    const int stage_at = WAVES == 8 && wave < 4 ? 1 : WAVES / 2 - 1;
+    const auto stage_next = [&](int step, int buf) {
+        if (step + 1 >= step_end) return;
+        stage(step + 1, buf ^ 1);
+        if (step + 2 >= step_end) return;
+        fetch(step + 2);
+        locate(min(step + 3, steps - 1));
+    };
     const auto attend_tiles = [&](int step, int buf, int tiles) {
 #pragma unroll 1
-        for (int sb = 0; sb < tiles; ++sb) {
+        for (int sb = 0; sb < WAVES / 2; ++sb) {
+            if (sb == stage_at) stage_next(step, buf);
+            if (sb >= tiles || failed) continue;
             const int t0 = step * STEP + sb * kAttTile;
             const u32x4* vs = &s_kv[buf][V_AT + sb * E * 64 + lane];
             f32x4 sc[NT][2];
@@ -845,7 +860,7 @@ __global__ __launch_bounds__(WAVES * 64, DP * NT <= 256 ? 2 : 1) void attend_row
                 }
                 if (pass == kFirst && __ballot(known) != 0) {
                     failed = true;
-                    return;
+                    continue;
                 }
             }
             if (pass == kMaxima) continue;
@@ -855,8 +870,7 @@ __global__ __launch_bounds__(WAVES * 64, DP * NT <= 256 ? 2 : 1) void attend_row
             for (int e = 0; e < VF; ++e) vf[e] = vs[e * 64];
             __builtin_amdgcn_sched_barrier(0);
             u32x4 pb[NT];
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
+            const auto softmax = [&](int t) {
                 float p[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
@@ -864,12 +878,22 @@ __global__ __launch_bounds__(WAVES * 64, DP * NT <= 256 ? 2 : 1) void attend_row
                     l[t] += p[j];
                 }
                 pb[t] = u32x4{pack2<QK>(p[0], p[1]), pack2<QK>(p[2], p[3]), pack2<QK>(p[4], p[5]), pack2<QK>(p[6], p[7])};
-            }
+            };
+            softmax(0);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const u32x4 v = e < VF ? vf[e % VF] : vs[e * 64];
+            for (int t = 0; t < NT; ++t) {
+                if (t + 1 < NT) softmax(t + 1);
 #pragma unroll
-                for (int t = 0; t < NT; ++t) acc[t][e] = mfma<QK>(v, pb[t], acc[t][e]);
+                for (int e = 0; e < E; ++e) acc[t][e] = mfma<QK>(e < VF ? vf[e % VF] : vs[e * 64], pb[t], acc[t][e]);
+                if (t + 1 < NT) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x2, 5, 0);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
         }
     };
@@ -892,18 +916,16 @@ __global__ __launch_bounds__(WAVES * 64, DP * NT <= 256 ? 2 : 1) void attend_row
             fetch(step0);
             locate(min(step0 + 1, steps - 1));
             stage(step0, 0);
+            if (step0 + 1 < step_end) {
+                fetch(step0 + 1);
+                locate(min(step0 + 2, steps - 1));
+            }
             __syncthreads();
 #pragma unroll 1
             for (int step = step0; step < step_end; ++step) {
-                const int buf = (step - step0) & 1;
-                const int tiles = pass == kDone || failed
+                const int tiles = pass == kDone
                                       ? 0 : min(WAVES / 2, (wave_end - step * STEP + kAttTile - 1) / kAttTile);
-                if (step + 1 < step_end) {
-                    fetch(step + 1);
-                    locate(min(step + 2, steps - 1));
-                }
-                attend_tiles(step, buf, tiles);
-                if (step + 1 < step_end) stage(step + 1, buf ^ 1);
+                attend_tiles(step, (step - step0) & 1, tiles);
                 __syncthreads();
             }
             pass = failed ? kMaxima : pass == kMaxima ? kLast : kDone;
@@ -1033,7 +1055,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(DescArg d, AttArgs a, 
 
 // ------------------------------------------------------------------- weigh
 // One workgroup: one KV head, 128 tokens, 32 to a wavefront, whose K rows stay
-// in registers while all rows of the sequence pass. Each token's sum is one
+// in registers while all rows of the sequence pass (a few, or any of odd layouts). Each token's sum is one
 // lane's, then 16 lanes', in a fixed order.
 template <int CK, int QK, int DP, int MODE, bool PAGED>
 __global__ __launch_bounds__(256) void weigh_kernel(DescArg d, AttArgs a) {
@@ -1100,6 +1122,130 @@ __global__ __launch_bounds__(256) void weigh_kernel(DescArg d, AttArgs a) {
     }
 }
 
+// ------------------------------------------------------- weigh, many rows
+// One workgroup: one KV head, 256 tokens, 64 to a wavefront, whose K operands stay
+// in registers while the rows pass through LDS as operands, 64 at a time, one
+// matrix tile staged by each wavefront and read by all. Bound by the exponentials:
+// 16 of them (of a quarter of the vector rate) per lane to 16 matrix instructions.
+template <int CK, int QK, int DP, int MODE>
+__global__ __launch_bounds__(256) void weigh_rows_kernel(DescArg d, AttArgs a) {
+    using Rows = TileRows<CK, DP>;
+    constexpr int STEPS = DP / 32, WAVES = 4, STEP = WAVES * kAttRows;
+    __shared__ u32x4 s_q[2][WAVES][STEPS][64];
+    __shared__ float s_lse[2][WAVES][kAttRows];
+    const DescPtr<AttSeq> seqs = desc_at<AttSeq>(d, 0);
+    const int item = xcd_item(static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x), a.heads);
+    const int si = __builtin_amdgcn_readfirstlane(find_by_tile(seqs, a.n_seqs, item));
+    const AttSeq s = desc_load(seqs + si);
+    const int tid = static_cast<int>(threadIdx.x), lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 15, g = lane >> 4;
+    const int local = item - s.tile_begin;
+    const int tg = static_cast<int>(a.heads.div(static_cast<uint32_t>(local)));
+    const int h = local - tg * a.g.H;
+    const int total = s.n_ctx + s.n_rows;
+    const int first = tg * kWeighRowsTokens, t0 = first + wave * 2 * kAttTile;
+    RowReader<CK, DP, MODE, false> rd;
+    rd.init(a, s.bt_offset, total, h, lane);
+    u32x4 k[2][2][STEPS];
+    uint32_t ok[2];
+    bool edge = false;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+        Rows r;
+        rd.template load<false>(r, rd.locate(t0 + b * kAttTile));
+        ok[b] = __builtin_amdgcn_readfirstlane(r.ok);
+        edge = edge || ok[b] != ~0u;
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+            for (int st = 0; st < STEPS; ++st) k[b][hh][st] = k_operand<CK, QK, DP>(r, hh, st);
+    }
+    edge = edge || t0 + 2 * kAttTile > s.n_ctx;
+    const float c = a.scale_log2 * (a.k_scale != nullptr ? a.k_scale[h] : 1.0f);
+    f32x4 sum[2][2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) sum[b][0] = sum[b][1] = f32x4{0, 0, 0, 0};
+    const int rows = s.n_rows * a.G;
+    u32x4 sq[STEPS];
+    float sl = 0.0f;
+    const auto fetch = [&](int R) {
+        const QRow row = q_row(a, s.n_rows, h, R + wave * kAttRows + n);
+        load_q<CK, DP, MODE>(a, s, row, g, sq);
+        sl = row.i >= 0 ? a.lse[static_cast<int64_t>(s.row0 + row.i) * a.Hq + row.head] : -__builtin_huge_valf();
+    };
+    const auto stage = [&](int buf) {
+#pragma unroll
+        for (int st = 0; st < STEPS; ++st) s_q[buf][wave][st][lane] = sq[st];
+        if (g == 0) s_lse[buf][wave][n] = sl * (1.0f / kLn2);
+    };
+    // causal: the first tokens' rows come first
+    const int R_first = a.mask == nullptr ? max(0, first - s.n_ctx) * a.G / STEP * STEP : 0;
+    fetch(R_first);
+    stage(0);
+    __syncthreads();
+#pragma unroll 1
+    for (int R = R_first; R < rows; R += STEP) {
+        const int buf = (R - R_first) / STEP & 1;
+        if (R + STEP < rows) fetch(R + STEP);
+        const int tiles = min(WAVES, (rows - R + kAttRows - 1) / kAttRows);
+#pragma unroll 1
+        for (int t = 0; t < tiles; ++t) {
+            u32x4 q[STEPS];
+#pragma unroll
+            for (int st = 0; st < STEPS; ++st) q[st] = s_q[buf][t][st][lane];
+            const float lse = s_lse[buf][t][n];
+            f32x4 sc[2][2];
+#pragma unroll
+            for (int b = 0; b < 2; ++b) sc[b][0] = sc[b][1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int st = 0; st < STEPS; ++st)
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int hh = 0; hh < 2; ++hh) sc[b][hh] = mfma<QK>(k[b][hh][st], q[st], sc[b][hh]);
+            // a row that saw nothing, or is none, gives no weight
+            const bool dead = lse == -__builtin_huge_valf();
+            if (__builtin_expect(edge || __ballot(dead) != 0, 0)) {
+                const int i = static_cast<int>(a.group.div(static_cast<uint32_t>(R + t * kAttRows + n)));
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const uint32_t vis = dead || i >= s.n_rows ? 0u : ok[b] & row_sees(a, s, i, t0 + b * kAttTile);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float x = exp2_hw(fmaf(sc[b][j >> 2][j & 3], c, -lse));
+                        sum[b][j >> 2][j & 3] += (vis >> (16 * (j >> 2) + 4 * g + (j & 3))) & 1u ? x : 0.0f;
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        sum[b][j >> 2][j & 3] += exp2_hw(fmaf(sc[b][j >> 2][j & 3], c, -lse));
+            }
+        }
+        if (R + STEP < rows) stage(buf ^ 1);
+        __syncthreads();
+    }
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+        float mine = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float x = sum[b][j >> 2][j & 3];
+#pragma unroll
+            for (int o = 1; o < 16; o <<= 1) x += __shfl_xor(x, o, 64);
+            mine = n == j ? x : mine;
+        }
+        const int t = t0 + b * kAttTile + 16 * (n >> 2) + 4 * g + (n & 3);
+        if (n < 8 && t < total) {
+            float* w = a.weights + h * a.columns + s.at + t;
+            *w = a.add ? *w + mine : mine;
+        }
+    }
+}
+
 // Instances of the kernels for one pair of cache and query types.
 template <typename F>
 void for_forms(int dp, int mode, bool paged, F&& f) {
@@ -1147,6 +1293,15 @@ void run_attend(const DescArg& d, const AttArgs& a, const AttPlan& p, hipStream_
 
 template <int CK, int QK>
 void run_weigh(const DescArg& d, const AttArgs& a, const AttPlan& p, hipStream_t stream) {
+    if (p.row_tile > 0) {
+        for_forms(p.dp, p.mode, true, [&](auto dp, auto mode, auto) {
+            if constexpr (decltype(mode)::value != kAttValues)
+                DARIC_LAUNCH((weigh_rows_kernel<CK, QK, decltype(dp)::value, decltype(mode)::value>),
+                             static_cast<unsigned>(p.items), 256, 0, stream, d, a);
+        });
+        check_launch("weigh_tokens");
+        return;
+    }
     for_forms(p.dp, p.mode, p.paged, [&](auto dp, auto mode, auto paged) {
         DARIC_LAUNCH((weigh_kernel<CK, QK, decltype(dp)::value, decltype(mode)::value, decltype(paged)::value>),
                      static_cast<unsigned>(p.items), 256, 0, stream, d, a);

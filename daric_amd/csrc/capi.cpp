@@ -1624,6 +1624,9 @@ struct AttGroup {
     }
 };
 
+// Rows of a KV head up to which weigh_kernel takes a sequence.
+constexpr int64_t kWeighFewRows = 16;
+
 constexpr int64_t kAttendGroups = 1024;
 std::vector<AttGroup> plan_attend(const AttCall& c) {
     std::vector<AttGroup> groups;
@@ -1642,7 +1645,7 @@ std::vector<AttGroup> plan_attend(const AttCall& c) {
                 if (nt > 1 && c.p.dp > 128) continue;
                 double cost = 0;
                 for (const AttSeq& s : gr.seqs)
-                    cost += (static_cast<double>(s.n_ctx) + s.n_rows) * static_cast<double>((rows(s) + 64 * nt - 1) / (64 * nt)) * (nt + 0.75);
+                    cost += (static_cast<double>(s.n_ctx) + s.n_rows) * static_cast<double>((rows(s) + 64 * nt - 1) / (64 * nt)) * (0.5 * nt + 0.5);
                 if (gr.p.row_tile == 0 || cost < best) {
                     best = cost;
                     gr.p.row_tile = nt;
@@ -1651,14 +1654,16 @@ std::vector<AttGroup> plan_attend(const AttCall& c) {
             if (getenv("DARIC_NT")) gr.p.row_tile = atoi(getenv("DARIC_NT"));
             gr.a.tile_rows = 64 * gr.p.row_tile;
             step = gr.p.row_tile == 4 ? 128 : 64;
-            target = gr.p.row_tile == 4 || c.p.dp > 128 ? 256 : 512;
+            target = 512;
         }
         if (getenv("DARIC_G")) target = atoi(getenv("DARIC_G"));
         const auto row_tiles = [&](const AttSeq& s) { return (rows(s) + gr.a.tile_rows - 1) / gr.a.tile_rows; };
         const auto steps = [&](const AttSeq& s) { return (static_cast<int64_t>(s.n_ctx) + s.n_rows + step - 1) / step; };
         int64_t work = 0;
         for (const AttSeq& s : gr.seqs) work += steps(s) * row_tiles(s) * c.a.g.H;
-        const int64_t part = std::max(least, (work + target - 1) / target);
+        int64_t whole = 0;      // workgroups without a cut
+        for (const AttSeq& s : gr.seqs) whole += row_tiles(s) * c.a.g.H;
+        const int64_t part = many && whole >= 256 ? kIntMax : std::max(least, (work + target - 1) / target);
         for (AttSeq& s : gr.seqs) {
             const int64_t parts = (steps(s) + part - 1) / part;
             s.tile_begin = static_cast<int32_t>(gr.p.items);
@@ -1792,7 +1797,6 @@ int daric_weigh_tokens(const daric_tensor* layer, int page_first, const daric_te
         const int64_t columns = weights->sizes[1];
         std::vector<std::pair<int64_t, int64_t>> cols;
         size_t at = 0;
-        int64_t& items = c.p.items;
         for (int64_t i = 0; i < n_sequences; ++i) {
             const daric_sequence& s = sequences[i];
             const int64_t total = s.n_ctx + s.n_rows;
@@ -1800,24 +1804,37 @@ int daric_weigh_tokens(const daric_tensor* layer, int page_first, const daric_te
                         "sequence ", i, " columns exceed weights");
             if (s.n_rows == 0) continue;
             cols.emplace_back(s.col_start, total);
-            AttSeq& x = c.seqs[at++];
-            x.at = static_cast<int32_t>(s.col_start);
-            x.tile_begin = static_cast<int32_t>(items);
-            items += (total + kWeighTokens - 1) / kWeighTokens * c.a.g.H;
-            DARIC_CHECK(items <= kMaxTiles, "too many tokens in one weigh_tokens call");
+            c.seqs[at++].at = static_cast<int32_t>(s.col_start);
         }
         check_apart(cols, "column");
         c.a.weights = static_cast<float*>(weights->data);
         c.a.columns = weights->sizes[0] == 1 ? columns : weights->strides[0];
         c.a.add = accumulate ? 1 : 0;
-        if (c.seqs.empty()) return;
+        std::vector<AttGroup> groups;
+        for (const bool many : {false, true}) {
+            AttGroup gr{c.a, c.p, {}};
+            gr.p.row_tile = many ? 1 : 0;
+            const int64_t per = many ? kWeighRowsTokens : kWeighTokens;
+            for (const AttSeq& s : c.seqs) {
+                if ((c.p.mode != kAttValues && static_cast<int64_t>(s.n_rows) * c.a.G > kWeighFewRows) != many) continue;
+                gr.seqs.push_back(s);
+                gr.seqs.back().tile_begin = static_cast<int32_t>(gr.p.items);
+                gr.p.items += (static_cast<int64_t>(s.n_ctx) + s.n_rows + per - 1) / per * c.a.g.H;
+                DARIC_CHECK(gr.p.items <= kMaxTiles, "too many tokens in one weigh_tokens call");
+            }
+            gr.a.n_seqs = static_cast<int32_t>(gr.seqs.size());
+            if (!gr.seqs.empty()) groups.push_back(std::move(gr));
+        }
+        if (groups.empty()) return;
         DeviceGuard guard(c.device);
         const hipStream_t st = as_stream(stream);
-        DescHandOver ho(c.device, c.seqs.data(), c.seqs.size() * sizeof(AttSeq), st);
-        if (c.ck == kBF16) weigh_bf16(ho.arg(), c.a, c.p, st);
-        else if (c.ck == kF16) weigh_f16(ho.arg(), c.a, c.p, st);
-        else if (c.qk == kBF16) weigh_e4m3_bf16(ho.arg(), c.a, c.p, st);
-        else weigh_e4m3_f16(ho.arg(), c.a, c.p, st);
+        for (const AttGroup& g : groups) {
+            DescHandOver ho(c.device, g.seqs.data(), g.seqs.size() * sizeof(AttSeq), st);
+            if (c.ck == kBF16) weigh_bf16(ho.arg(), g.a, g.p, st);
+            else if (c.ck == kF16) weigh_f16(ho.arg(), g.a, g.p, st);
+            else if (c.qk == kBF16) weigh_e4m3_bf16(ho.arg(), g.a, g.p, st);
+            else weigh_e4m3_f16(ho.arg(), g.a, g.p, st);
+        }
     });
 }
 
