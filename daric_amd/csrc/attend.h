@@ -87,10 +87,11 @@ struct alignas(16) EvictSeq {
 static_assert(sizeof(EvictSeq) == 32, "EvictSeq layout");
 // d: the sequences, then (at layer_off) the layers' addresses. heads: H, or 1 where
 // one selection serves all heads of a layer; unit: bytes of an access that all
-// rows allow; max_tokens: the most tokens a selection chooses from, max_keep the
-// most slots of a sequence that loses tokens (0: none does).
+// rows allow; max_tokens: the most tokens a selection chooses from, max_chosen the
+// most it takes, max_keep the most slots of a sequence that loses tokens (0: none
+// does).
 void launch_evict(const DescArg& d, int layer_off, int n_layers, const KVGeom& g, int es, int unit,
                   const int32_t* block_table, float* weights, int64_t columns, int heads, int n_seqs,
-                  int max_tokens, int max_keep, int32_t* sel, int32_t* kept, int kmax, hipStream_t stream);
+                  int max_tokens, int max_keep, int max_chosen, int32_t* sel, int32_t* kept, int kmax, hipStream_t stream);
 
 }  // namespace daric

@@ -1053,6 +1053,26 @@ __global__ __launch_bounds__(256) void attend_join_kernel(DescArg d, AttArgs a, 
     if (lane == 0) a.lse[at] = ll == 0.0f ? -__builtin_huge_valf() : (mm + log2f(ll)) * kLn2;
 }
 
+// Sums 8 values over the 16 lanes of a group: a lane of n < 8 gets the sum of
+// value sum_of(n). Each step exchanges half of what is left, 8 exchanges in all
+// (32 where every value goes through every step).
+__device__ __forceinline__ int sum_of(int n) { return 4 * (n & 1) + (n & 2) + ((n >> 2) & 1); }
+template <int W>
+__device__ __forceinline__ void sum_halves(float (&v)[8], int n) {
+    const bool up = (n & (4 / W)) != 0;
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+        const float lo = v[k], hi = v[k + W];
+        v[k] = (up ? hi : lo) + __shfl_xor(up ? lo : hi, 4 / W, 64);
+    }
+}
+__device__ __forceinline__ float sum_group(float (&v)[8], int n) {
+    sum_halves<4>(v, n);
+    sum_halves<2>(v, n);
+    sum_halves<1>(v, n);
+    return v[0] + __shfl_xor(v[0], 8, 64);
+}
+
 // ------------------------------------------------------------------- weigh
 // One workgroup: one KV head, 128 tokens, 32 to a wavefront, whose K rows stay
 // in registers while all rows of the sequence pass (a few, or any of odd layouts). Each token's sum is one
@@ -1106,16 +1126,8 @@ __global__ __launch_bounds__(256) void weigh_kernel(DescArg d, AttArgs a) {
             sum[j] += (vis >> b) & 1u ? x : 0.0f;
         }
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-#pragma unroll
-        for (int x = 1; x < 16; x <<= 1) sum[j] += __shfl_xor(sum[j], x, 64);
-    }
-    // lane n of a group takes its token n (8 tokens)
-    float mine = sum[0];
-#pragma unroll
-    for (int j = 1; j < 8; ++j) mine = n == j ? sum[j] : mine;
-    const int t = t0 + 16 * (n >> 2) + 4 * g + (n & 3);
+    const float mine = sum_group(sum, n);
+    const int j = sum_of(n), t = t0 + 16 * (j >> 2) + 4 * g + (j & 3);
     if (n < 8 && t < total) {
         float* w = a.weights + h * a.columns + s.at + t;
         *w = a.add ? *w + mine : mine;
@@ -1128,7 +1140,7 @@ __global__ __launch_bounds__(256) void weigh_kernel(DescArg d, AttArgs a) {
 // matrix tile staged by each wavefront and read by all. Bound by the exponentials:
 // 16 of them (of a quarter of the vector rate) per lane to 16 matrix instructions.
 template <int CK, int QK, int DP, int MODE>
-__global__ __launch_bounds__(256) void weigh_rows_kernel(DescArg d, AttArgs a) {
+__global__ __launch_bounds__(256, DP == 256 ? 1 : 3) void weigh_rows_kernel(DescArg d, AttArgs a) {
     using Rows = TileRows<CK, DP>;
     constexpr int STEPS = DP / 32, WAVES = 4, STEP = WAVES * kAttRows;
     __shared__ u32x4 s_q[2][WAVES][STEPS][64];
@@ -1163,9 +1175,11 @@ __global__ __launch_bounds__(256) void weigh_rows_kernel(DescArg d, AttArgs a) {
     }
     edge = edge || t0 + 2 * kAttTile > s.n_ctx;
     const float c = a.scale_log2 * (a.k_scale != nullptr ? a.k_scale[h] : 1.0f);
-    f32x4 sum[2][2];
+    float sum[2][8];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) sum[b][0] = sum[b][1] = f32x4{0, 0, 0, 0};
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum[b][j] = 0.0f;
     const int rows = s.n_rows * a.G;
     u32x4 sq[STEPS];
     float sl = 0.0f;
@@ -1214,7 +1228,7 @@ __global__ __launch_bounds__(256) void weigh_rows_kernel(DescArg d, AttArgs a) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const float x = exp2_hw(fmaf(sc[b][j >> 2][j & 3], c, -lse));
-                        sum[b][j >> 2][j & 3] += (vis >> (16 * (j >> 2) + 4 * g + (j & 3))) & 1u ? x : 0.0f;
+                        sum[b][j] += (vis >> (16 * (j >> 2) + 4 * g + (j & 3))) & 1u ? x : 0.0f;
                     }
                 }
             } else {
@@ -1222,7 +1236,7 @@ __global__ __launch_bounds__(256) void weigh_rows_kernel(DescArg d, AttArgs a) {
                 for (int b = 0; b < 2; ++b)
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
-                        sum[b][j >> 2][j & 3] += exp2_hw(fmaf(sc[b][j >> 2][j & 3], c, -lse));
+                        sum[b][j] += exp2_hw(fmaf(sc[b][j >> 2][j & 3], c, -lse));
             }
         }
         if (R + STEP < rows) stage(buf ^ 1);
@@ -1230,15 +1244,8 @@ __global__ __launch_bounds__(256) void weigh_rows_kernel(DescArg d, AttArgs a) {
     }
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-        float mine = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            float x = sum[b][j >> 2][j & 3];
-#pragma unroll
-            for (int o = 1; o < 16; o <<= 1) x += __shfl_xor(x, o, 64);
-            mine = n == j ? x : mine;
-        }
-        const int t = t0 + b * kAttTile + 16 * (n >> 2) + 4 * g + (n & 3);
+        const float mine = sum_group(sum[b], n);
+        const int j = sum_of(n), t = t0 + b * kAttTile + 16 * (j >> 2) + 4 * g + (j & 3);
         if (n < 8 && t < total) {
             float* w = a.weights + h * a.columns + s.at + t;
             *w = a.add ? *w + mine : mine;

@@ -1862,7 +1862,7 @@ int daric_evict_tokens(const daric_tensor* layers, int64_t n_layers, int page_fi
         std::vector<EvictSeq> seqs;
         std::vector<std::pair<int64_t, int64_t>> cols;
         seqs.reserve(n);
-        int64_t kmax = 0, most = 0, slots = 0;
+        int64_t kmax = 0, most = 0, slots = 0, chosen = 0;
         for (int64_t i = 0; i < n; ++i) {
             const daric_eviction& s = evictions[i];
             DARIC_CHECK(s.bt_offset >= 0 && s.col_start >= 0 && s.n_tokens >= 0 && s.keep >= 0 && s.n_first >= 0 &&
@@ -1888,6 +1888,7 @@ int daric_evict_tokens(const daric_tensor* layers, int64_t n_layers, int page_fi
             if (s.n_tokens > s.keep) {
                 most = std::max(most, s.n_tokens - s.n_first - s.n_recent);
                 slots = std::max(slots, s.keep);
+                chosen = std::max(chosen, s.keep - s.n_first - s.n_recent);
             }
         }
         check_apart(cols, "column");
@@ -1924,7 +1925,8 @@ int daric_evict_tokens(const daric_tensor* layers, int64_t n_layers, int page_fi
         launch_evict(ho.arg(), static_cast<int>(cb), static_cast<int>(n_layers), g, static_cast<int>(es),
                      static_cast<int>(unit), static_cast<const int32_t*>(block_table->data),
                      static_cast<float*>(weights->data), columns, static_cast<int>(heads), static_cast<int>(n),
-                     static_cast<int>(most), static_cast<int>(slots), static_cast<int32_t*>(workspace->data),
+                     static_cast<int>(most), static_cast<int>(slots), static_cast<int>(chosen),
+                     static_cast<int32_t*>(workspace->data),
                      static_cast<int32_t*>(kept->data), static_cast<int>(width), st);
     });
 }

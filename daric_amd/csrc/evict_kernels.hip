@@ -10,9 +10,7 @@
 // over a row that another still has to be read from.
 //
 // evict_plan_kernel, a workgroup per (layer, head, sequence): the top-k of the
-// weights (topk.h), then the slots from its ascending indices alone. Index b of
-// the selection leaves the slots between its predecessor and itself empty, and
-// before the slot y there are y - b empty ones: each lane takes one index.
+// weights (topk.h), then the slots from its ascending indices alone.
 // evict_move_kernel: tiles of slots, whose moving rows are gathered in LDS
 // first, so that all lanes copy.
 #include "attend.h"
@@ -25,21 +23,26 @@ namespace {
 
 constexpr int kMoveSlots = 256;
 constexpr int kMoveThreads = 256;
+// Selected indices of a plan workgroup in LDS, beside the top-k's 8 KiB.
+constexpr size_t kPlanLds = 48 * 1024;
 
-template <int T, int KPT>
+// The selected indices stand in LDS (IN_LDS: as many as the call selects at most),
+// or in the workspace `sel` where they do not fit.
+template <int T, int KPT, bool IN_LDS>
 __global__ __launch_bounds__(T) void evict_plan_kernel(DescArg d, float* __restrict__ weights, int64_t columns,
                                                        int n_seqs, int32_t* sel, int32_t* __restrict__ kept,
                                                        int kmax, int64_t rows0) {
     static_assert(T <= 256 || sizeof(TopkLds<T>) >= sizeof(TopkLds<256>), "the short forms' LDS fits");
     __shared__ __align__(16) uint8_t s_mem[sizeof(TopkLds<T>)];
     __shared__ int s_early;
+    extern __shared__ int32_t s_ids[];
     const int64_t row = rows0 + blockIdx.y;                // (layer, head)
     const int si = static_cast<int>(blockIdx.x);
     const EvictSeq s = desc_load(desc_at<EvictSeq>(d, 0) + si);
     const int tid = static_cast<int>(threadIdx.x);
     float* w = weights + row * columns + s.col0;
     int32_t* o = kept + (row * n_seqs + si) * kmax;
-    int32_t* ids = sel + (row * n_seqs + si) * kmax;
+    int32_t* const ids = IN_LDS ? s_ids : sel + (row * n_seqs + si) * kmax;
     const int n = s.n, keep = min(s.keep, n);
     for (int i = keep + tid; i < kmax; i += T) o[i] = -1;
     if (n <= s.keep) {
@@ -54,7 +57,8 @@ __global__ __launch_bounds__(T) void evict_plan_kernel(DescArg d, float* __restr
         if (tid == 0) s_early = 0;
         const auto key_at = [&](int i) -> uint32_t { return order_key(w[s.first + i]); };
         if (k > 0)
-            chunk_topk<N, decltype(slots)::value>(key_at, mid, k, ids, nullptr, *reinterpret_cast<TopkLds<N>*>(s_mem));
+            chunk_topk<N, decltype(slots)::value>(key_at, mid, k, IN_LDS ? nullptr : ids, IN_LDS ? ids : nullptr,
+                                                  *reinterpret_cast<TopkLds<N>*>(s_mem));
         __syncthreads();
         // early: indices whose token stands in one of the `keep` slots
         const int edge = min(keep - s.first, mid);
@@ -64,31 +68,20 @@ __global__ __launch_bounds__(T) void evict_plan_kernel(DescArg d, float* __restr
         const int early = s_early;
         const int late = k - early;
         const int behind = max(keep, n - s.recent);        // first of the recent tokens that move
-        // slot y of the chosen range takes moving token i
-        const auto fill = [&](int y, int i) {
+        for (int x = tid; x < early; x += N) o[s.first + ids[x]] = s.first + ids[x];
+        // Free slot i is y = i + (selected indices before it): index x has ids[x] - x
+        // free slots before it. A lane searches for its slot; the gap of each index
+        // filled by the index's lane took 112 us instead of 58 where one token in
+        // nine stays (640 rows of 16384 tokens).
+        for (int i = tid; i < edge - early; i += N) {
+            int lo = 0, hi = early;
+            while (lo < hi) {
+                const int at = (lo + hi) >> 1;
+                if (ids[at] - at <= i) lo = at + 1; else hi = at;
+            }
             const int src = i < late ? s.first + ids[early + i] : behind + (i - late);
-            o[s.first + y] = src;
-            w[s.first + y] = w[src];
-        };
-        for (int b0 = 0; b0 <= early; b0 += N) {
-            const int b = b0 + tid;
-            int lo = 0, hi = 0;
-            if (b <= early) {
-                lo = b > 0 ? ids[b - 1] + 1 : 0;
-                hi = b < early ? ids[b] : edge;
-                if (b < early) o[s.first + hi] = s.first + hi;
-            }
-            // long gaps by the whole wavefront
-            unsigned long long wide = __ballot(hi - lo > 8);
-            while (wide != 0) {
-                const int from = __ffsll(static_cast<long long>(wide)) - 1;
-                wide &= wide - 1;
-                const int flo = __builtin_amdgcn_readlane(lo, from), fhi = __builtin_amdgcn_readlane(hi, from);
-                const int fb = __builtin_amdgcn_readlane(b, from);
-                for (int y = flo + (tid & 63); y < fhi; y += 64) fill(y, y - fb);
-            }
-            if (hi - lo <= 8)
-                for (int y = lo; y < hi; ++y) fill(y, y - b);
+            o[s.first + i + lo] = src;
+            w[s.first + i + lo] = w[src];
         }
         for (int i = tid; i < s.first; i += N) o[i] = i;
         for (int i = n - s.recent + tid; i < keep; i += N) o[i] = i;
@@ -169,7 +162,7 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(DescArg d, int
 #pragma unroll
         for (int x = 0; x < UNROLL; ++x) offset(i + x * kMoveThreads, &from[x], &to[x]);
 #pragma unroll
-        for (int x = 0; x < UNROLL; ++x) v[x] = *reinterpret_cast<const U*>(base + from[x]);
+        for (int x = 0; x < UNROLL; ++x) v[x] = __builtin_nontemporal_load(reinterpret_cast<const U*>(base + from[x]));
 #pragma unroll
         for (int x = 0; x < UNROLL; ++x) *reinterpret_cast<U*>(base + to[x]) = v[x];
     }
@@ -184,13 +177,21 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(DescArg d, int
 
 void launch_evict(const DescArg& d, int layer_off, int n_layers, const KVGeom& g, int es, int unit,
                   const int32_t* block_table, float* weights, int64_t columns, int heads, int n_seqs,
-                  int max_tokens, int max_keep, int32_t* sel, int32_t* kept, int kmax, hipStream_t stream) {
+                  int max_tokens, int max_keep, int max_chosen, int32_t* sel, int32_t* kept, int kmax, hipStream_t stream) {
     constexpr int kMaxGridY = 65535;
     const int64_t rows = static_cast<int64_t>(n_layers) * heads;
     const int64_t groups = rows * n_seqs;
     for (int64_t r0 = 0; r0 < rows; r0 += kMaxGridY) {
         const dim3 grid(static_cast<unsigned>(n_seqs), static_cast<unsigned>(std::min<int64_t>(kMaxGridY, rows - r0)));
-#define DARIC_EP(TH, KPT) DARIC_LAUNCH((evict_plan_kernel<TH, KPT>), grid, TH, 0, stream, d, weights, columns, n_seqs, sel, kept, kmax, r0)
+        const size_t lds = static_cast<size_t>(max_chosen) * sizeof(int32_t);
+        const bool in_lds = lds <= kPlanLds;
+#define DARIC_EP(TH, KPT)                                                                                          \
+    do {                                                                                                           \
+        if (in_lds) DARIC_LAUNCH((evict_plan_kernel<TH, KPT, true>), grid, TH, lds, stream, d, weights, columns,   \
+                                 n_seqs, sel, kept, kmax, r0);                                                     \
+        else DARIC_LAUNCH((evict_plan_kernel<TH, KPT, false>), grid, TH, 0, stream, d, weights, columns, n_seqs,   \
+                          sel, kept, kmax, r0);                                                                    \
+    } while (0)
         // as many lanes as the top-k takes (launch_topk)
         if (max_tokens <= kTopkWave) DARIC_EP(64, kTopkWave / 64);
         else if (max_tokens <= kTopkGroup) DARIC_EP(256, kTopkGroup / 256);
