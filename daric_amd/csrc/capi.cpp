@@ -1654,16 +1654,32 @@ std::vector<AttGroup> plan_attend(const AttCall& c) {
             if (getenv("DARIC_NT")) gr.p.row_tile = atoi(getenv("DARIC_NT"));
             gr.a.tile_rows = 64 * gr.p.row_tile;
             step = gr.p.row_tile == 4 ? 128 : 64;
-            target = 512;
+            target = gr.p.row_tile == 4 || c.p.dp > 128 ? 256 : 512;     // that run at once
         }
         if (getenv("DARIC_G")) target = atoi(getenv("DARIC_G"));
         const auto row_tiles = [&](const AttSeq& s) { return (rows(s) + gr.a.tile_rows - 1) / gr.a.tile_rows; };
         const auto steps = [&](const AttSeq& s) { return (static_cast<int64_t>(s.n_ctx) + s.n_rows + step - 1) / step; };
-        int64_t work = 0;
-        for (const AttSeq& s : gr.seqs) work += steps(s) * row_tiles(s) * c.a.g.H;
-        int64_t whole = 0;      // workgroups without a cut
-        for (const AttSeq& s : gr.seqs) whole += row_tiles(s) * c.a.g.H;
-        const int64_t part = many && whole >= 256 ? kIntMax : std::max(least, (work + target - 1) / target);
+        int64_t work = 0, whole = 0;      // steps in all, workgroups without a cut
+        for (const AttSeq& s : gr.seqs) {
+            work += steps(s) * row_tiles(s) * c.a.g.H;
+            whole += row_tiles(s) * c.a.g.H;
+        }
+        int64_t part = std::max(least, (work + target - 1) / target);
+        if (many) {
+            // the shortest parts that make no more workgroups than run at once: one more
+            // would take as long as all of them
+            const auto items = [&](int64_t p) {
+                int64_t n = 0;
+                for (const AttSeq& s : gr.seqs) n += (steps(s) + p - 1) / p * row_tiles(s) * c.a.g.H;
+                return n;
+            };
+            int64_t hi = kIntMax;
+            if (whole > target) part = hi;
+            while (part < hi) {
+                const int64_t mid = part + (hi - part) / 2;
+                if (items(mid) <= target) hi = mid; else part = mid + 1;
+            }
+        }
         for (AttSeq& s : gr.seqs) {
             const int64_t parts = (steps(s) + part - 1) / part;
             s.tile_begin = static_cast<int32_t>(gr.p.items);
