@@ -1651,12 +1651,10 @@ std::vector<AttGroup> plan_attend(const AttCall& c) {
                     gr.p.row_tile = nt;
                 }
             }
-            if (getenv("DARIC_NT")) gr.p.row_tile = atoi(getenv("DARIC_NT"));
             gr.a.tile_rows = 64 * gr.p.row_tile;
             step = gr.p.row_tile == 4 ? 128 : 64;
             target = gr.p.row_tile == 4 || c.p.dp > 128 ? 256 : 512;     // that run at once
         }
-        if (getenv("DARIC_G")) target = atoi(getenv("DARIC_G"));
         const auto row_tiles = [&](const AttSeq& s) { return (rows(s) + gr.a.tile_rows - 1) / gr.a.tile_rows; };
         const auto steps = [&](const AttSeq& s) { return (static_cast<int64_t>(s.n_ctx) + s.n_rows + step - 1) / step; };
         int64_t work = 0, whole = 0;      // steps in all, workgroups without a cut
