@@ -59,7 +59,8 @@ struct AttPlan {
     int mode, dp;                  // head_dim rounded up to 64, 128 or 256
     bool paged;                    // pages hold whole halves of a tile
     int row_tile;                  // attend_rows_kernel: rows of a workgroup in 64s (1, 2, 4);
-                                   // weigh_rows_kernel: 1; 0: attend_kernel, weigh_kernel
+                                   // weigh_rows_kernel: 1, weigh_split_kernel: 2;
+                                   // 0: attend_kernel, weigh_kernel
     int64_t items, join_rows;      // workgroups; rows times heads of all sequences
     int64_t max_parts;             // of a sequence: with more than one, a second kernel joins them
 };
@@ -76,8 +77,8 @@ DARIC_ATTEND_TYPES(e4m3_f16)
 // The join of the parts, by query type.
 void join_bf16(const DescArg& d, const AttArgs& a, const AttPlan& p, hipStream_t stream);
 void join_f16(const DescArg& d, const AttArgs& a, const AttPlan& p, hipStream_t stream);
-// Tokens of a weigh workgroup: of a few rows, of many.
-constexpr int kWeighTokens = 128, kWeighRowsTokens = 256;
+// Tokens of a weigh workgroup: of few rows, of many, of many rows and few tokens.
+constexpr int kWeighTokens = 128, kWeighRowsTokens = 256, kWeighSplitTokens = 64;
 
 // An eviction: the tokens [0, n) of a sequence, of which `keep` stay.
 struct alignas(16) EvictSeq {

@@ -1135,13 +1135,85 @@ __global__ __launch_bounds__(256) void weigh_kernel(DescArg d, AttArgs a) {
 }
 
 // ------------------------------------------------------- weigh, many rows
+// A wavefront's 64 tokens: K as operands, and the tokens' sums.
+template <int CK, int QK, int DP, int MODE>
+struct WeighTokens {
+    using Rows = TileRows<CK, DP>;
+    static constexpr int STEPS = DP / 32;
+    u32x4 k[2][2][STEPS];
+    uint32_t ok[2];
+    float sum[2][8];
+    float c;
+    int t0, n, g;
+    bool edge;
+
+    __device__ __forceinline__ void init(const AttArgs& a, const AttSeq& s, int h, int first, int lane) {
+        const int total = s.n_ctx + s.n_rows;
+        RowReader<CK, DP, MODE, false> rd;
+        rd.init(a, s.bt_offset, total, h, lane);
+        t0 = first;
+        n = lane & 15; g = lane >> 4;
+        c = a.scale_log2 * (a.k_scale != nullptr ? a.k_scale[h] : 1.0f);
+        edge = t0 + 2 * kAttTile > s.n_ctx;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            Rows r;
+            rd.template load<false>(r, rd.locate(t0 + b * kAttTile));
+            ok[b] = __builtin_amdgcn_readfirstlane(r.ok);
+            edge = edge || ok[b] != ~0u;
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+                for (int st = 0; st < STEPS; ++st) k[b][hh][st] = k_operand<CK, QK, DP>(r, hh, st);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum[b][j] = 0.0f;
+        }
+    }
+    // Adds the weights of the 16 rows from R on; lse: of row n, in powers of 2.
+    __device__ __forceinline__ void add(const AttArgs& a, const AttSeq& s, const u32x4 (&q)[STEPS], float lse, int R) {
+        f32x4 sc[2][2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) sc[b][0] = sc[b][1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int st = 0; st < STEPS; ++st)
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh) sc[b][hh] = mfma<QK>(k[b][hh][st], q[st], sc[b][hh]);
+        // a row that saw nothing, or is none, gives no weight
+        const bool dead = lse == -__builtin_huge_valf();
+        if (__builtin_expect(edge || __ballot(dead) != 0, 0)) {
+            const int i = static_cast<int>(a.group.div(static_cast<uint32_t>(R + n)));
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const uint32_t vis = dead || i >= s.n_rows ? 0u : ok[b] & row_sees(a, s, i, t0 + b * kAttTile);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float x = exp2_hw(fmaf(sc[b][j >> 2][j & 3], c, -lse));
+                    sum[b][j] += (vis >> (16 * (j >> 2) + 4 * g + (j & 3))) & 1u ? x : 0.0f;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum[b][j] += exp2_hw(fmaf(sc[b][j >> 2][j & 3], c, -lse));
+        }
+    }
+};
+template <int CK, int DP, int MODE>
+__device__ __forceinline__ float load_row(const AttArgs& a, const AttSeq& s, int h, int R, int g, u32x4 (&q)[DP / 32]) {
+    const QRow row = q_row(a, s.n_rows, h, R);
+    load_q<CK, DP, MODE>(a, s, row, g, q);
+    return row.i >= 0 ? a.lse[static_cast<int64_t>(s.row0 + row.i) * a.Hq + row.head] * (1.0f / kLn2) : -__builtin_huge_valf();
+}
+
 // One workgroup: one KV head, 256 tokens, 64 to a wavefront, whose K operands stay
 // in registers while the rows pass through LDS as operands, 64 at a time, one
 // matrix tile staged by each wavefront and read by all. Bound by the exponentials:
 // 16 of them (of a quarter of the vector rate) per lane to 16 matrix instructions.
 template <int CK, int QK, int DP, int MODE>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 3) void weigh_rows_kernel(DescArg d, AttArgs a) {
-    using Rows = TileRows<CK, DP>;
     constexpr int STEPS = DP / 32, WAVES = 4, STEP = WAVES * kAttRows;
     __shared__ u32x4 s_q[2][WAVES][STEPS][64];
     __shared__ float s_lse[2][WAVES][kAttRows];
@@ -1155,101 +1227,99 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 3) void weigh_rows_kernel(Desc
     const int local = item - s.tile_begin;
     const int tg = static_cast<int>(a.heads.div(static_cast<uint32_t>(local)));
     const int h = local - tg * a.g.H;
-    const int total = s.n_ctx + s.n_rows;
-    const int first = tg * kWeighRowsTokens, t0 = first + wave * 2 * kAttTile;
-    RowReader<CK, DP, MODE, false> rd;
-    rd.init(a, s.bt_offset, total, h, lane);
-    u32x4 k[2][2][STEPS];
-    uint32_t ok[2];
-    bool edge = false;
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-        Rows r;
-        rd.template load<false>(r, rd.locate(t0 + b * kAttTile));
-        ok[b] = __builtin_amdgcn_readfirstlane(r.ok);
-        edge = edge || ok[b] != ~0u;
-#pragma unroll
-        for (int hh = 0; hh < 2; ++hh)
-#pragma unroll
-            for (int st = 0; st < STEPS; ++st) k[b][hh][st] = k_operand<CK, QK, DP>(r, hh, st);
-    }
-    edge = edge || t0 + 2 * kAttTile > s.n_ctx;
-    const float c = a.scale_log2 * (a.k_scale != nullptr ? a.k_scale[h] : 1.0f);
-    float sum[2][8];
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sum[b][j] = 0.0f;
+    const int first = tg * kWeighRowsTokens;
+    WeighTokens<CK, QK, DP, MODE> w;
+    w.init(a, s, h, first + wave * 2 * kAttTile, lane);
     const int rows = s.n_rows * a.G;
     u32x4 sq[STEPS];
     float sl = 0.0f;
-    const auto fetch = [&](int R) {
-        const QRow row = q_row(a, s.n_rows, h, R + wave * kAttRows + n);
-        load_q<CK, DP, MODE>(a, s, row, g, sq);
-        sl = row.i >= 0 ? a.lse[static_cast<int64_t>(s.row0 + row.i) * a.Hq + row.head] : -__builtin_huge_valf();
-    };
     const auto stage = [&](int buf) {
 #pragma unroll
         for (int st = 0; st < STEPS; ++st) s_q[buf][wave][st][lane] = sq[st];
-        if (g == 0) s_lse[buf][wave][n] = sl * (1.0f / kLn2);
+        if (g == 0) s_lse[buf][wave][n] = sl;
     };
     // causal: the first tokens' rows come first
     const int R_first = a.mask == nullptr ? max(0, first - s.n_ctx) * a.G / STEP * STEP : 0;
-    fetch(R_first);
+    sl = load_row<CK, DP, MODE>(a, s, h, R_first + wave * kAttRows + n, g, sq);
     stage(0);
     __syncthreads();
 #pragma unroll 1
     for (int R = R_first; R < rows; R += STEP) {
         const int buf = (R - R_first) / STEP & 1;
-        if (R + STEP < rows) fetch(R + STEP);
+        if (R + STEP < rows) sl = load_row<CK, DP, MODE>(a, s, h, R + STEP + wave * kAttRows + n, g, sq);
         const int tiles = min(WAVES, (rows - R + kAttRows - 1) / kAttRows);
 #pragma unroll 1
         for (int t = 0; t < tiles; ++t) {
             u32x4 q[STEPS];
 #pragma unroll
             for (int st = 0; st < STEPS; ++st) q[st] = s_q[buf][t][st][lane];
-            const float lse = s_lse[buf][t][n];
-            f32x4 sc[2][2];
-#pragma unroll
-            for (int b = 0; b < 2; ++b) sc[b][0] = sc[b][1] = f32x4{0, 0, 0, 0};
-#pragma unroll
-            for (int st = 0; st < STEPS; ++st)
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
-#pragma unroll
-                    for (int hh = 0; hh < 2; ++hh) sc[b][hh] = mfma<QK>(k[b][hh][st], q[st], sc[b][hh]);
-            // a row that saw nothing, or is none, gives no weight
-            const bool dead = lse == -__builtin_huge_valf();
-            if (__builtin_expect(edge || __ballot(dead) != 0, 0)) {
-                const int i = static_cast<int>(a.group.div(static_cast<uint32_t>(R + t * kAttRows + n)));
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    const uint32_t vis = dead || i >= s.n_rows ? 0u : ok[b] & row_sees(a, s, i, t0 + b * kAttTile);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float x = exp2_hw(fmaf(sc[b][j >> 2][j & 3], c, -lse));
-                        sum[b][j] += (vis >> (16 * (j >> 2) + 4 * g + (j & 3))) & 1u ? x : 0.0f;
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        sum[b][j] += exp2_hw(fmaf(sc[b][j >> 2][j & 3], c, -lse));
-            }
+            w.add(a, s, q, s_lse[buf][t][n], R + t * kAttRows);
         }
         if (R + STEP < rows) stage(buf ^ 1);
         __syncthreads();
     }
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-        const float mine = sum_group(sum[b], n);
-        const int j = sum_of(n), t = t0 + b * kAttTile + 16 * (j >> 2) + 4 * g + (j & 3);
-        if (n < 8 && t < total) {
-            float* w = a.weights + h * a.columns + s.at + t;
-            *w = a.add ? *w + mine : mine;
+        const float mine = sum_group(w.sum[b], n);
+        const int j = sum_of(n), t = w.t0 + b * kAttTile + 16 * (j >> 2) + 4 * g + (j & 3);
+        if (n < 8 && t < s.n_ctx + s.n_rows) {
+            float* o = a.weights + h * a.columns + s.at + t;
+            *o = a.add ? *o + mine : mine;
         }
+    }
+}
+
+// The same where the tokens are few: 64 to a workgroup, whose 8 wavefronts take the
+// rows' tiles in turn from memory and join in LDS.
+template <int CK, int QK, int DP, int MODE>
+__global__ __launch_bounds__(512, 2) void weigh_split_kernel(DescArg d, AttArgs a) {
+    constexpr int STEPS = DP / 32, WAVES = 8;
+    __shared__ float s_sum[WAVES][2 * kAttTile];
+    const DescPtr<AttSeq> seqs = desc_at<AttSeq>(d, 0);
+    const int item = xcd_item(static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x), a.heads);
+    const int si = __builtin_amdgcn_readfirstlane(find_by_tile(seqs, a.n_seqs, item));
+    const AttSeq s = desc_load(seqs + si);
+    const int tid = static_cast<int>(threadIdx.x), lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 15, g = lane >> 4;
+    const int local = item - s.tile_begin;
+    const int tg = static_cast<int>(a.heads.div(static_cast<uint32_t>(local)));
+    const int h = local - tg * a.g.H;
+    const int first = tg * kWeighSplitTokens;
+    WeighTokens<CK, QK, DP, MODE> w;
+    w.init(a, s, h, first, lane);
+    const int rows = s.n_rows * a.G;
+    constexpr int STEP = WAVES * kAttRows;
+    int R = (a.mask == nullptr ? max(0, first - s.n_ctx) * a.G / STEP * STEP : 0) + wave * kAttRows;
+    if (R < rows) {
+        u32x4 q[STEPS];
+        float l = load_row<CK, DP, MODE>(a, s, h, R + n, g, q);
+#pragma unroll 1
+        for (;;) {
+            u32x4 next[STEPS];
+            float nl = 0.0f;
+            if (R + STEP < rows) nl = load_row<CK, DP, MODE>(a, s, h, R + STEP + n, g, next);
+            w.add(a, s, q, l, R);
+            R += STEP;
+            if (R >= rows) break;
+#pragma unroll
+            for (int st = 0; st < STEPS; ++st) q[st] = next[st];
+            l = nl;
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+        const float mine = sum_group(w.sum[b], n);
+        const int j = sum_of(n);
+        if (n < 8) s_sum[wave][b * kAttTile + 16 * (j >> 2) + 4 * g + (j & 3)] = mine;
+    }
+    __syncthreads();
+    if (tid < 2 * kAttTile && first + tid < s.n_ctx + s.n_rows) {
+        float x = 0.0f;
+#pragma unroll
+        for (int v = 0; v < WAVES; ++v) x += s_sum[v][tid];
+        float* o = a.weights + h * a.columns + s.at + first + tid;
+        *o = a.add ? *o + x : x;
     }
 }
 
@@ -1302,9 +1372,14 @@ template <int CK, int QK>
 void run_weigh(const DescArg& d, const AttArgs& a, const AttPlan& p, hipStream_t stream) {
     if (p.row_tile > 0) {
         for_forms(p.dp, p.mode, true, [&](auto dp, auto mode, auto) {
-            if constexpr (decltype(mode)::value != kAttValues)
-                DARIC_LAUNCH((weigh_rows_kernel<CK, QK, decltype(dp)::value, decltype(mode)::value>),
-                             static_cast<unsigned>(p.items), 256, 0, stream, d, a);
+            if constexpr (decltype(mode)::value != kAttValues) {
+                if (p.row_tile == 1)
+                    DARIC_LAUNCH((weigh_rows_kernel<CK, QK, decltype(dp)::value, decltype(mode)::value>),
+                                 static_cast<unsigned>(p.items), 256, 0, stream, d, a);
+                else
+                    DARIC_LAUNCH((weigh_split_kernel<CK, QK, decltype(dp)::value, decltype(mode)::value>),
+                                 static_cast<unsigned>(p.items), 512, 0, stream, d, a);
+            }
         });
         check_launch("weigh_tokens");
         return;

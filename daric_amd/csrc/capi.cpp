@@ -1626,6 +1626,8 @@ struct AttGroup {
 
 // Rows of a KV head up to which weigh_kernel takes a sequence.
 constexpr int64_t kWeighFewRows = 16;
+// Workgroups of 256 tokens from which weigh_rows_kernel takes the others.
+constexpr int64_t kWeighWhole = 512;
 
 constexpr int64_t kAttendGroups = 1024;
 std::vector<AttGroup> plan_attend(const AttCall& c) {
@@ -1827,10 +1829,19 @@ int daric_weigh_tokens(const daric_tensor* layer, int page_first, const daric_te
         std::vector<AttGroup> groups;
         for (const bool many : {false, true}) {
             AttGroup gr{c.a, c.p, {}};
-            gr.p.row_tile = many ? 1 : 0;
-            const int64_t per = many ? kWeighRowsTokens : kWeighTokens;
+            const auto mine = [&](const AttSeq& s) {
+                return (c.p.mode != kAttValues && static_cast<int64_t>(s.n_rows) * c.a.G > kWeighFewRows) == many;
+            };
+            int64_t per = kWeighTokens;
+            if (many) {
+                int64_t whole = 0;
+                for (const AttSeq& s : c.seqs)
+                    if (mine(s)) whole += (static_cast<int64_t>(s.n_ctx) + s.n_rows + kWeighRowsTokens - 1) / kWeighRowsTokens * c.a.g.H;
+                gr.p.row_tile = whole >= kWeighWhole ? 1 : 2;
+                per = gr.p.row_tile == 1 ? kWeighRowsTokens : kWeighSplitTokens;
+            }
             for (const AttSeq& s : c.seqs) {
-                if ((c.p.mode != kAttValues && static_cast<int64_t>(s.n_rows) * c.a.G > kWeighFewRows) != many) continue;
+                if (!mine(s)) continue;
                 gr.seqs.push_back(s);
                 gr.seqs.back().tile_begin = static_cast<int32_t>(gr.p.items);
                 gr.p.items += (static_cast<int64_t>(s.n_ctx) + s.n_rows + per - 1) / per * c.a.g.H;

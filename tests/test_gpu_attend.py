@@ -93,14 +93,16 @@ class Case:
         torch.cuda.synchronize()
         return r
 
-    def check_weigh(self, lse, weights=None):
+    def check_weigh(self, lse, weights=None, **more):
         a = self.on_gpu()
+        a.update(more)
         start = np.zeros((self.h, self.columns)) if weights is None else weights.double().numpy()
         w = weights.to(self.dev) if weights is not None else None
         got = cache_ops.weigh_tokens(a["layer"], self.pf, a["block_table"], a["q"], lse, self.seqs, weights=w,
                                      tree_mask=a["tree_mask"], scale=self.scale, k_scale=a["k_scale"])
         torch.cuda.synchronize()
         assert w is None or got is w
+        self.weights = got
         ref, size, amax, rows = oatt.weigh(self.layer, self.pf, self.bt, self.q, lse.cpu(), self.seqs, start, self.mask,
                                            self.scale, self.ks)
         D = self.q.shape[2]
@@ -360,10 +362,11 @@ def test_strides_and_alignment(dev, dtype):
         out, lse = c.run(**more)
         c.check(out, lse)
         assert not same or (torch.equal(out, want) and torch.equal(lse, wl))
-    for qq, layer in ((wide[:, 1], a["layer"]), (odd, shifted)):
-        w = [cache_ops.weigh_tokens(ly, c.pf, a["block_table"], x, wl, c.seqs, scale=c.scale, k_scale=a["k_scale"])
-             for ly, x in ((a["layer"], q), (layer, qq))]
-        assert torch.equal(*w)
+    c.check_weigh(wl)
+    w = c.weights
+    c.check_weigh(wl, q=wide[:, 1])
+    assert torch.equal(w, c.weights)
+    c.check_weigh(wl, q=odd, layer=shifted)
 
 
 def test_many_sequences(dev):
