@@ -1626,8 +1626,12 @@ struct AttGroup {
 
 // Rows of a KV head up to which weigh_kernel takes a sequence.
 constexpr int64_t kWeighFewRows = 16;
-// Workgroups of 256 tokens from which weigh_rows_kernel takes the others.
-constexpr int64_t kWeighWhole = 512;
+// weigh_rows_kernel takes the others where they make two workgroups of 256 tokens per
+// CU, or one for every second CU and few rows; weigh_split_kernel the rest. MI355X,
+// 8 KV heads of 128, bf16, rows and split: 30000 tokens and 256 rows 41 and 94 us,
+// 14000 26 and 59, 8000 21 and 35; 8000 tokens and 8192 rows 412 and 297, 3000 and
+// 8192 424 and 113.
+constexpr int64_t kWeighWhole = 512, kWeighHalf = 128, kWeighHalfRows = 1024;
 
 constexpr int64_t kAttendGroups = 1024;
 std::vector<AttGroup> plan_attend(const AttCall& c) {
@@ -1834,10 +1838,13 @@ int daric_weigh_tokens(const daric_tensor* layer, int page_first, const daric_te
             };
             int64_t per = kWeighTokens;
             if (many) {
-                int64_t whole = 0;
-                for (const AttSeq& s : c.seqs)
-                    if (mine(s)) whole += (static_cast<int64_t>(s.n_ctx) + s.n_rows + kWeighRowsTokens - 1) / kWeighRowsTokens * c.a.g.H;
-                gr.p.row_tile = whole >= kWeighWhole ? 1 : 2;
+                int64_t whole = 0, rows = 0;
+                for (const AttSeq& s : c.seqs) {
+                    if (!mine(s)) continue;
+                    whole += (static_cast<int64_t>(s.n_ctx) + s.n_rows + kWeighRowsTokens - 1) / kWeighRowsTokens * c.a.g.H;
+                    rows = std::max(rows, static_cast<int64_t>(s.n_rows) * c.a.G);
+                }
+                gr.p.row_tile = whole >= kWeighWhole || (whole >= kWeighHalf && rows <= kWeighHalfRows) ? 1 : 2;
                 per = gr.p.row_tile == 1 ? kWeighRowsTokens : kWeighSplitTokens;
             }
             for (const AttSeq& s : c.seqs) {
