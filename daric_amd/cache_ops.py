@@ -491,6 +491,12 @@ def _ref(t: Optional[torch.Tensor]):
     return ctypes.byref(desc(t)) if t is not None else None
 
 
+def _scale(scale: Optional[float], q: torch.Tensor) -> float:
+    """The scores' factor; without one, that of q's head size (the library refuses
+    a q that has none)."""
+    return float(scale) if scale is not None else q.shape[-1] ** -0.5 if q.dim() and q.shape[-1] else 1.0
+
+
 def _layer_desc(layer: torch.Tensor):
     return _layer_array((layer,))
 
@@ -527,7 +533,7 @@ def attend_pages(layer: torch.Tensor, page_first: bool, block_table: torch.Tenso
             if need.value:
                 work = torch.empty(need.value, dtype=torch.uint8, device=dev)
     check(lib.daric_attend_pages(ld, pf, _ref(block_table), ctypes.byref(qd), addr, n, _ref(tree_mask),
-                                 float(q.shape[2] ** -0.5 if scale is None else scale), _ref(k_scale), _ref(v_scale),
+                                 _scale(scale, q), _ref(k_scale), _ref(v_scale),
                                  _ref(out), _ref(lse), work.data_ptr() if work is not None else None, need.value,
                                  ctypes.c_uint64(st)))
     _record(st, dev, block_table, q, tree_mask, k_scale, v_scale, out, lse, work)
@@ -555,7 +561,7 @@ def weigh_tokens(layer: torch.Tensor, page_first: bool, block_table: torch.Tenso
         with _on_stream(st, dev):
             weights = torch.zeros((heads, max(end, 0)), dtype=torch.float32, device=dev)
     check(load().daric_weigh_tokens(ld, 1 if page_first else 0, _ref(block_table), ctypes.byref(qd), _ref(lse), addr, n,
-                                    _ref(tree_mask), float(q.shape[2] ** -0.5 if scale is None else scale),
+                                    _ref(tree_mask), _scale(scale, q),
                                     _ref(k_scale), _ref(weights), 0 if fresh else 1, ctypes.c_uint64(st)))
     _record(st, dev, block_table, q, lse, tree_mask, k_scale, weights)
     return weights

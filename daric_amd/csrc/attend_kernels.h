@@ -340,6 +340,7 @@ __device__ __forceinline__ uint32_t row_sees(const AttArgs& a, const AttSeq& s, 
     if (i < 0) return 0;
     const int d0 = t0 - s.n_ctx;                       // draft of the first token
     if (d0 <= -32) return ~0u;
+    if (d0 >= s.n_rows) return 0;                      // no such drafts: no mask word of them either
     if (a.mask == nullptr) {
         const int c = i - d0 + 1;
         return c >= 32 ? ~0u : c <= 0 ? 0u : (1u << c) - 1u;
@@ -628,7 +629,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_kernel(DescArg 
 // instructions. The next step's rows come from memory meanwhile, into the other
 // half of the LDS.
 template <int CK, int QK, int DP, int MODE, bool PAGED, int WAVES, int NT>
-__global__ __launch_bounds__(WAVES * 64, DP * NT <= 256 ? 2 : 1) void attend_rows_kernel(DescArg d, AttArgs a) {
+__global__ __launch_bounds__(WAVES * 64, DP == 256 ? 1 : 2) void attend_rows_kernel(DescArg d, AttArgs a) {
     using Rows = TileRows<CK, DP>;
     constexpr int E = Rows::E, STEPS = DP / 32, ROWS = WAVES * 16 * NT, STEP = WAVES * 16;
     constexpr int K_AT = 0, V_AT = WAVES * STEPS * 64, UNITS = V_AT + WAVES / 2 * E * 64;    // 16-byte units of a step
@@ -1302,7 +1303,6 @@ __global__ __launch_bounds__(512, 2) void weigh_split_kernel(DescArg d, AttArgs 
             w.add(a, s, q, l, R);
             R += STEP;
             if (R >= rows) break;
-#pragma unroll
             for (int st = 0; st < STEPS; ++st) q[st] = next[st];
             l = nl;
         }

@@ -1585,7 +1585,7 @@ AttCall attention_call(const daric_tensor* layer, int page_first, const daric_te
         DARIC_CHECK(s.bt_offset >= 0 && s.row_start >= 0 && s.n_rows >= 0 && s.n_ctx >= 0 && s.col_start >= 0,
                     "negative field of sequence ", i);
         DARIC_CHECK(s.n_ctx <= kMaxTokens && s.n_rows <= kMaxTokens && s.n_ctx + s.n_rows <= kMaxTokens &&
-                    s.n_rows <= (kIntMax - kAttRows) / a.G, "sequence ", i, " is too long");
+                    s.n_rows <= (kIntMax - 1024) / a.G, "sequence ", i, " is too long");
         DARIC_CHECK(s.row_start <= c.T && s.n_rows <= c.T - s.row_start, "sequence ", i, " rows exceed q");
         DARIC_CHECK(s.row_start <= kIntMax, "sequence ", i, " starts too far into q");
         if (s.n_rows == 0) continue;      // nothing to compute
@@ -1623,6 +1623,11 @@ struct AttGroup {
         return p.max_parts > 1 ? p.items * a.tile_rows * (p.dp + 2) * static_cast<int64_t>(sizeof(float)) : 0;
     }
 };
+
+// A call of several groups refuses capture before any of them is enqueued.
+void check_capture(const std::vector<AttGroup>& groups, hipStream_t stream) {
+    for (const AttGroup& g : groups) DescHandOver::check_capture(g.seqs.size() * sizeof(AttSeq), stream);
+}
 
 // Rows of a KV head up to which weigh_kernel takes a sequence.
 constexpr int64_t kWeighFewRows = 16;
@@ -1693,7 +1698,7 @@ std::vector<AttGroup> plan_attend(const AttCall& c) {
             gr.p.items += parts * row_tiles(s) * c.a.g.H;
             gr.p.join_rows += static_cast<int64_t>(s.n_rows) * c.a.Hq;
             gr.p.max_parts = std::max(gr.p.max_parts, parts);
-            DARIC_CHECK(gr.p.items <= kMaxTiles && gr.p.join_rows <= kIntMax, "too many rows in one attend_pages call");
+            DARIC_CHECK(gr.p.items <= kMaxTiles / 2 && gr.p.join_rows <= kIntMax, "too many rows in one attend_pages call");
         }
         DARIC_CHECK(gr.p.max_parts <= 1 || gr.p.join_rows <= kMaxTiles, "too many rows in one attend_pages call");
         groups.push_back(std::move(gr));
@@ -1784,6 +1789,7 @@ int daric_attend_pages(const daric_tensor* layer, int page_first, const daric_te
                     "workspace must be 16-byte aligned and hold ", need, " bytes, got ", workspace_bytes);
         DeviceGuard guard(c.device);
         const hipStream_t st = as_stream(stream);
+        check_capture(groups, st);
         auto* work = static_cast<uint8_t*>(workspace);
         for (AttGroup& g : groups) {
             g.a.part = reinterpret_cast<float*>(work);
@@ -1852,7 +1858,7 @@ int daric_weigh_tokens(const daric_tensor* layer, int page_first, const daric_te
                 gr.seqs.push_back(s);
                 gr.seqs.back().tile_begin = static_cast<int32_t>(gr.p.items);
                 gr.p.items += (static_cast<int64_t>(s.n_ctx) + s.n_rows + per - 1) / per * c.a.g.H;
-                DARIC_CHECK(gr.p.items <= kMaxTiles, "too many tokens in one weigh_tokens call");
+                DARIC_CHECK(gr.p.items <= kMaxTiles / 2, "too many tokens in one weigh_tokens call");
             }
             gr.a.n_seqs = static_cast<int32_t>(gr.seqs.size());
             if (!gr.seqs.empty()) groups.push_back(std::move(gr));
@@ -1860,6 +1866,7 @@ int daric_weigh_tokens(const daric_tensor* layer, int page_first, const daric_te
         if (groups.empty()) return;
         DeviceGuard guard(c.device);
         const hipStream_t st = as_stream(stream);
+        check_capture(groups, st);
         for (const AttGroup& g : groups) {
             DescHandOver ho(c.device, g.seqs.data(), g.seqs.size() * sizeof(AttSeq), st);
             if (c.ck == kBF16) weigh_bf16(ho.arg(), g.a, g.p, st);
@@ -1935,7 +1942,7 @@ int daric_evict_tokens(const daric_tensor* layers, int64_t n_layers, int page_fi
         check_ids(workspace, "workspace");
         DARIC_CHECK(workspace->sizes[3] == kept->sizes[3], "workspace must have kept's shape");
         const int64_t width = kept->sizes[3];
-        DARIC_CHECK(n <= kMaxTiles && width <= kIntMax, "too many evictions in one call");
+        DARIC_CHECK(n <= kMaxTiles / 4 && width <= kIntMax, "too many evictions in one call");
         if (n == 0) return;
         int64_t unit = 16;
         const int64_t es = t.elem_size;

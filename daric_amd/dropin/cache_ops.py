@@ -7,8 +7,10 @@ signatures; the rest are additions.
 """
 from daric_amd.cache_ops import (  # noqa: F401
     CacheCopier,
+    attend_pages,
     batched_memcpy_d2h,
     batched_memcpy_h2d,
+    evict_tokens,
     kv_deviation,
     merge_rows,
     rerotate_pages,
@@ -16,4 +18,5 @@ from daric_amd.cache_ops import (  # noqa: F401
     timing_enable,
     timing_read,
     topk_per_chunk,
+    weigh_tokens,
 )

@@ -624,6 +624,40 @@ def test_serving_loop(dev, dtype):
             gpu[:, int(bt[starts[i] + j // ps]), j % ps] = row[:, 0, 0].to(dev)
 
 
+def test_nothing_to_do(dev):
+    """No rows, no kept tokens, no sequences, a q without rows."""
+    c = Case(dev, [(2, 30)], seed=51)
+    a = c.on_gpu()
+    out, lse = cache_ops.attend_pages(a["layer"], False, a["block_table"], a["q"][:0], [])
+    assert out.shape == (0, 8, 64) and lse.shape == (0, 8)
+    w = cache_ops.weigh_tokens(a["layer"], False, a["block_table"], a["q"], torch.zeros(2, 8, device=dev), [(0, 0, 0, 30, 4)])
+    assert w.shape == (2, 34) and (w == 0).all()
+    assert cache_ops.weigh_tokens(a["layer"], False, a["block_table"], a["q"], torch.zeros(2, 8, device=dev), []).shape == (2, 0)
+    before = a["layer"].clone()
+    w = torch.rand(1, 2, 32, device=dev)
+    kept = cache_ops.evict_tokens([a["layer"]], False, a["block_table"], w, [(0, 1, 30, 0, 0, 0)])
+    assert kept.shape == (1, 2, 1, 0) and (w[:, :, 1:31] == 0).all() and (w[:, :, [0, 31]] > 0).all()
+    assert torch.equal(before, a["layer"])
+    assert cache_ops.evict_tokens([a["layer"]], False, a["block_table"], w, []).shape == (1, 2, 0, 0)
+
+
+@pytest.mark.filterwarnings("ignore:The CUDA Graph is empty")
+def test_mixed_large_call_refuses_capture_whole(dev):
+    """Few sequences of many rows beside more of one row than a capture allows: no
+    part of the call is enqueued."""
+    c = Case(dev, [(20, 4)] + [(1, 4)] * 100, h=1, g=1, d=64, seed=52)
+    out, lse = c.run()
+    c.check(out, lse)
+    a = c.on_gpu()
+    out.fill_(3.0)
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="cannot be captured in a graph"):
+        with torch.cuda.graph(g):
+            cache_ops.attend_pages(a["layer"], c.pf, a["block_table"], a["q"], c.seqs, out=out, lse=lse)
+    torch.cuda.synchronize()
+    assert (out == 3.0).all()
+
+
 def test_refusals_on_the_gpu(dev):
     c = Case(dev, [(2, 30)], seed=50)
     a = c.on_gpu()
@@ -636,6 +670,8 @@ def test_refusals_on_the_gpu(dev):
         call(seqs=[(0, 0, 3, 10)])
     with pytest.raises(RuntimeError, match="reads past the end of block_table"):
         call(seqs=[(0, 0, 2, 47)])
+    with pytest.raises(RuntimeError, match="multiple of the cache's 2 heads"):
+        cache_ops.weigh_tokens(a["layer"], False, a["block_table"], a["q"][:, 0], a["q"][:, 0].float(), c.seqs)
     with pytest.raises(ValueError, match="MLA"):
         cache_ops.attend_pages(torch.zeros(4, 16, 64, dtype=torch.bfloat16, device=dev), True, a["block_table"], a["q"],
                                c.seqs)
