@@ -427,6 +427,13 @@ __device__ __forceinline__ float with_mark(float x, uint32_t word, int d) {
 // ------------------------------------------------------------------ attend
 // One workgroup: one KV head, 16 rows of q and one part of a sequence's tokens,
 // whose tiles its wavefronts take in turn; they join in LDS at the end.
+// Bound by memory: K and V are read once, by whole rows of a head. V is read past the
+// caches; K, of which an instruction takes half a line of each row, must find the
+// other half there. MI355X, one row to a sequence: 32 sequences of 310 to 8191 tokens
+// (bf16, 8 KV heads of 128, 412 MB) 68 us, 6.0 TB/s, where a plain read of as much
+// takes 62; with K past the caches too 81, V through them 86, without the next tile's
+// rows on their way the same 86 (the memory is busy either way). Two sequences of
+// 131072 and 100001 tokens, e4m3, 473 MB: 88 us, 5.4 TB/s; head-major pages 79.
 template <int CK, int QK, int DP, int MODE, bool PAGED>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_kernel(DescArg d, AttArgs a) {
     using Rows = TileRows<CK, DP>;
@@ -628,6 +635,12 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_kernel(DescArg 
 // type and V's tokens are paired once per workgroup, and a read feeds NT
 // instructions. The next step's rows come from memory meanwhile, into the other
 // half of the LDS.
+// Bound by the matrix cores and the exponentials together, which the two wavefronts of
+// a SIMD overlap only in part. MI355X, 2048 rows of 32 heads behind 6144 tokens (bf16,
+// 8 KV heads of 128, 240 GFLOP): 263 us by the clock, 914 TFLOP/s, where a library
+// product of 8192 x 8192 x 8192 reaches 1208; 311 under the tracer, of which the
+// scores, products and LDS reads alone take 254, and staging none that shows. 128
+// rows to a workgroup 365, 64 rows 505 (each traced).
 template <int CK, int QK, int DP, int MODE, bool PAGED, int WAVES, int NT>
 __global__ __launch_bounds__(WAVES * 64, DP == 256 ? 1 : 2) void attend_rows_kernel(DescArg d, AttArgs a) {
     using Rows = TileRows<CK, DP>;
@@ -1076,7 +1089,9 @@ __device__ __forceinline__ float sum_group(float (&v)[8], int n) {
 
 // ------------------------------------------------------------------- weigh
 // One workgroup: one KV head, 128 tokens, 32 to a wavefront, whose K rows stay
-// in registers while all rows of the sequence pass (a few, or any of odd layouts). Each token's sum is one
+// in registers while all rows of the sequence pass (a few, or any of odd layouts).
+// Bound by memory: the batch above, 212 MB of K, 43 us, 4.9 TB/s (64 tokens to a
+// wavefront 45, K past the caches 53). Each token's sum is one
 // lane's, then 16 lanes', in a fixed order.
 template <int CK, int QK, int DP, int MODE, bool PAGED>
 __global__ __launch_bounds__(256) void weigh_kernel(DescArg d, AttArgs a) {
@@ -1213,6 +1228,8 @@ __device__ __forceinline__ float load_row(const AttArgs& a, const AttSeq& s, int
 // in registers while the rows pass through LDS as operands, 64 at a time, one
 // matrix tile staged by each wavefront and read by all. Bound by the exponentials:
 // 16 of them (of a quarter of the vector rate) per lane to 16 matrix instructions.
+// MI355X, the last 64 rows of 64 heads against 32768 and 20064 tokens, e4m3, 55
+// GFLOP: 83 us, 667 TFLOP/s (205 us by weigh_kernel).
 template <int CK, int QK, int DP, int MODE>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 3) void weigh_rows_kernel(DescArg d, AttArgs a) {
     constexpr int STEPS = DP / 32, WAVES = 4, STEP = WAVES * kAttRows;

@@ -19,6 +19,11 @@
 #include "launch.h"
 #include "topk.h"
 
+//
+// Bound by memory, the plan by the latency of its passes. MI355X, 8 sequences of 1100
+// to 2500 tokens cut to 1024 in 32 layers of 8 x 128 bf16: plan 41 us, rows 180 us for
+// 970 MB read and written, 5.4 TB/s (a copy of 1 GiB by torch: 4.8); one sequence of
+// 16384 cut to 2048 in 80 e4m3 layers: 61 and 115 us.
 namespace daric {
 namespace {
 

@@ -12,6 +12,8 @@ function on the path, each citing the reference file:line it follows:
   fp8.py     OCP e4m3 encode/decode used by the fp8 path
   select.py  deviation keys, per-chunk top-k and merge (spec of the selection
              kernels; the reference has no such kernel)
+  attend.py  attention over the paged cache, token weights and eviction, in 64
+             bits (spec of the attention kernels; no reference kernel)
   kvio.py    store/load record format and copy plan of the daric-store GPU I/O
              (daric/management/service/gpu_kv_io.py)
   c/oracle_copy.c + native.py
