@@ -431,9 +431,8 @@ __device__ __forceinline__ float with_mark(float x, uint32_t word, int d) {
 // caches; K, of which an instruction takes half a line of each row, must find the
 // other half there. MI355X, one row to a sequence: 32 sequences of 310 to 8191 tokens
 // (bf16, 8 KV heads of 128, 412 MB) 68 us, 6.0 TB/s, where a plain read of as much
-// takes 62; with K past the caches too 81, V through them 86, without the next tile's
-// rows on their way the same 86 (the memory is busy either way). Two sequences of
-// 131072 and 100001 tokens, e4m3, 473 MB: 88 us, 5.4 TB/s; head-major pages 79.
+// takes 62; with K past the caches too 81, with V through them 86. Two sequences of
+// 131072 and 100001 tokens, e4m3, 473 MB: 90 us, 5.2 TB/s; head-major pages 79.
 template <int CK, int QK, int DP, int MODE, bool PAGED>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_kernel(DescArg d, AttArgs a) {
     using Rows = TileRows<CK, DP>;
@@ -635,12 +634,14 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_kernel(DescArg 
 // type and V's tokens are paired once per workgroup, and a read feeds NT
 // instructions. The next step's rows come from memory meanwhile, into the other
 // half of the LDS.
-// Bound by the matrix cores and the exponentials together, which the two wavefronts of
-// a SIMD overlap only in part. MI355X, 2048 rows of 32 heads behind 6144 tokens (bf16,
-// 8 KV heads of 128, 240 GFLOP): 263 us by the clock, 914 TFLOP/s, where a library
-// product of 8192 x 8192 x 8192 reaches 1208; 311 under the tracer, of which the
-// scores, products and LDS reads alone take 254, and staging none that shows. 128
-// rows to a workgroup 365, 64 rows 505 (each traced).
+// Bound by products, softmax and staging, of which the two wavefronts of a SIMD overlap
+// only a part: the matrix cores are busy 35% of the time, the vector unit issues 41%.
+// MI355X, 2048 rows of 32 heads behind 6144 tokens (bf16, 8 KV heads of 128, 240
+// GFLOP): 264 us by the clock, 911 TFLOP/s, where a library product of 8192 x 8192 x
+// 8192 reaches 1208; 310 in a kernel trace. Of 328 traced us of an earlier form 254
+// were left without the staging, 270 without the softmax, 185 without both. Traced:
+// 256 rows to a workgroup 312 us, 128 rows 365, 64 rows 505 (the last before the
+// staging was spread over the step).
 template <int CK, int QK, int DP, int MODE, bool PAGED, int WAVES, int NT>
 __global__ __launch_bounds__(WAVES * 64, DP == 256 ? 1 : 2) void attend_rows_kernel(DescArg d, AttArgs a) {
     using Rows = TileRows<CK, DP>;
@@ -1090,8 +1091,8 @@ __device__ __forceinline__ float sum_group(float (&v)[8], int n) {
 // ------------------------------------------------------------------- weigh
 // One workgroup: one KV head, 128 tokens, 32 to a wavefront, whose K rows stay
 // in registers while all rows of the sequence pass (a few, or any of odd layouts).
-// Bound by memory: the batch above, 212 MB of K, 43 us, 4.9 TB/s (64 tokens to a
-// wavefront 45, K past the caches 53). Each token's sum is one
+// Bound by memory: the batch of attend_kernel, 212 MB of K, 43 us, 4.9 TB/s (45 by
+// weigh_rows_kernel, 53 with K past the caches). Each token's sum is one
 // lane's, then 16 lanes', in a fixed order.
 template <int CK, int QK, int DP, int MODE, bool PAGED>
 __global__ __launch_bounds__(256) void weigh_kernel(DescArg d, AttArgs a) {
@@ -1229,7 +1230,7 @@ __device__ __forceinline__ float load_row(const AttArgs& a, const AttSeq& s, int
 // matrix tile staged by each wavefront and read by all. Bound by the exponentials:
 // 16 of them (of a quarter of the vector rate) per lane to 16 matrix instructions.
 // MI355X, the last 64 rows of 64 heads against 32768 and 20064 tokens, e4m3, 55
-// GFLOP: 83 us, 667 TFLOP/s (205 us by weigh_kernel).
+// GFLOP: 83 us by the clock, 667 TFLOP/s (204 us by weigh_kernel).
 template <int CK, int QK, int DP, int MODE>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 3) void weigh_rows_kernel(DescArg d, AttArgs a) {
     constexpr int STEPS = DP / 32, WAVES = 4, STEP = WAVES * kAttRows;
@@ -1413,7 +1414,8 @@ void run_join(const DescArg& d, const AttArgs& a, const AttPlan& p, hipStream_t 
     for_forms(p.dp, kAttWhole, true, [&](auto dp, auto, auto) {
         constexpr int DP = decltype(dp)::value;
         const int rows = static_cast<int>(p.join_rows);
-        // many rows fill the chip by themselves
+        // many rows fill the chip by themselves (MI355X, 12000 rows in few parts: eight
+        // parts of a row at once 27 us, one 10)
         if (p.max_parts <= 4 || rows >= 4096) DARIC_LAUNCH((attend_join_kernel<QK, DP, 1>), (rows + 7) / 8, 256, 0, stream, d, a, rows);
         else DARIC_LAUNCH((attend_join_kernel<QK, DP, 8>), rows, 256, 0, stream, d, a, rows);
     });

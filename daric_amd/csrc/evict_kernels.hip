@@ -13,17 +13,17 @@
 // weights (topk.h), then the slots from its ascending indices alone.
 // evict_move_kernel: tiles of slots, whose moving rows are gathered in LDS
 // first, so that all lanes copy. Read and written past the caches (202 -> 180 us for
-// the 970 MB that an eviction of 8 sequences from 32 layers moves; MI355X).
+// the 992 MB that an eviction of 8 sequences from 32 layers moves; MI355X).
 #include "attend.h"
 #include "kernels.h"
 #include "launch.h"
 #include "topk.h"
 
 //
-// Bound by memory, the plan by the latency of its passes. MI355X, 8 sequences of 1100
-// to 2500 tokens cut to 1024 in 32 layers of 8 x 128 bf16: plan 41 us, rows 180 us for
-// 970 MB read and written, 5.4 TB/s (a copy of 1 GiB by torch: 4.8); one sequence of
-// 16384 cut to 2048 in 80 e4m3 layers: 61 and 115 us.
+// The move is bound by memory. MI355X, 8 sequences of 1100 to 2500 tokens cut to 1024 in
+// 32 layers of 8 x 128 bf16: plan 42 us, rows 180 us for 992 MB read and written, 5.5
+// TB/s (a copy of 1 GiB by torch: 4.8); one sequence of 16384 cut to 2048 in 80 e4m3
+// layers, 681 MB: 63 and 113 us.
 namespace daric {
 namespace {
 
@@ -77,8 +77,8 @@ __global__ __launch_bounds__(T) void evict_plan_kernel(DescArg d, float* __restr
         for (int x = tid; x < early; x += N) o[s.first + ids[x]] = s.first + ids[x];
         // Free slot i is y = i + (selected indices before it): index x has ids[x] - x
         // free slots before it. A lane searches for its slot; the gap of each index
-        // filled by the index's lane took 112 us instead of 58 where one token in
-        // nine stays (640 rows of 16384 tokens).
+        // filled by the index's lane took 112 us instead of 88 (with 1024 lanes) where
+        // one token in nine stays (640 rows of 16384 tokens).
         for (int i = tid; i < edge - early; i += N) {
             int lo = 0, hi = early;
             while (lo < hi) {
