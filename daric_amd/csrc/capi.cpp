@@ -1522,6 +1522,22 @@ constexpr int64_t kMaxHeadDim = 256;
 constexpr int64_t kMaxTokens = kIntMax - 1024;     // of a sequence: tiles past its end are still 32-bit
 
 // Ranges [begin, begin + n) that share no element.
+// Whether the memory from the first to the last element of two tensors overlaps.
+bool overlap(const daric_tensor& a, const daric_tensor& b) {
+    const auto span = [](const daric_tensor& t) {
+        int64_t lo = 0, hi = 0;
+        for (int d = 0; d < t.ndim; ++d) {
+            const int64_t end = (t.sizes[d] - 1) * t.strides[d];
+            (end < 0 ? lo : hi) += end;
+        }
+        const auto at = reinterpret_cast<uintptr_t>(t.data);
+        return std::pair(at + lo * t.elem_size, at + (hi + 1) * t.elem_size);
+    };
+    if (numel(a) == 0 || numel(b) == 0) return false;
+    const auto x = span(a), y = span(b);
+    return x.first < y.second && y.first < x.second;
+}
+
 void check_apart(std::vector<std::pair<int64_t, int64_t>>& r, const char* what) {
     bool ordered = true;
     for (size_t i = 1; i < r.size(); ++i) ordered = ordered && r[i - 1].first + r[i - 1].second <= r[i].first;
@@ -1790,6 +1806,8 @@ int daric_attend_pages(const daric_tensor* layer, int page_first, const daric_te
         c.a.lse = const_cast<float*>(check_lse(c, lse));
         c.a.out = static_cast<uint8_t*>(out->data);
         if (c.seqs.empty()) return;
+        // another workgroup may still read a row of q when its out is written
+        DARIC_CHECK(!overlap(*out, *q), "out must not overlap q");
         std::vector<AttGroup> groups = plan_attend(c);
         int64_t need = 0;
         for (const AttGroup& g : groups) need += g.bytes();
@@ -1952,6 +1970,11 @@ int daric_evict_tokens(const daric_tensor* layers, int64_t n_layers, int page_fi
         const int64_t width = kept->sizes[3];
         DARIC_CHECK(n <= kMaxTiles / 4 && width <= kIntMax, "too many evictions in one call");
         if (n == 0) return;
+        DARIC_CHECK(!overlap(*kept, *workspace), "workspace must not overlap kept");
+        std::vector<const void*> data;
+        for (int64_t i = 0; i < n_layers; ++i) data.push_back(layers[i].data);
+        std::sort(data.begin(), data.end());
+        DARIC_CHECK(std::adjacent_find(data.begin(), data.end()) == data.end(), "a layer is given twice");
         int64_t unit = 16;
         const int64_t es = t.elem_size;
         const auto allows = [&](int64_t u) {

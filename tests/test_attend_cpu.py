@@ -191,6 +191,32 @@ def test_eviction_refusals(lib):
     assert lib.daric_evict_tokens(layers, 2, 0, r(bt), r(w), a.ctypes.data, 0, r(none), r(none), ctypes.c_uint64(0)) == 0
 
 
+def test_memory_that_is_read_and_written(lib):
+    """Written memory that other workgroups of the call read or write is refused
+    before any device call."""
+    r = ctypes.byref
+    layer, bt = fake((2, 8, 16, 4, 64), torch.bfloat16, ptr=0x10000000), fake((8,), torch.int32, ptr=0x20000000)
+    lse = fake((10, 8), torch.float32, ptr=0x50000000)
+    q = fake((10, 8, 64), torch.bfloat16, ptr=0x40000000)
+    addr, n, _k = seqs((0, 0, 10, 50, 0))
+    for ptr in (0x40000000, 0x40000000 + 10 * 8 * 64 * 2 - 2, 0x40000000 - 10 * 8 * 64 * 2 + 2):
+        out = fake((10, 8, 64), torch.bfloat16, ptr=ptr)
+        assert lib.daric_attend_pages(r(layer), 0, r(bt), r(q), addr, n, None, 1.0, None, None, r(out), r(lse), None, 0,
+                                      ctypes.c_uint64(0)) == 1
+        assert b"out must not overlap q" in lib.daric_last_error()
+
+    def evict(ptrs, ws):
+        layers = (_lib.DaricTensor * 2)(*[fake((2, 8, 16, 4, 64), torch.bfloat16, ptr=p) for p in ptrs])
+        w = fake((2, 4, 200), torch.float32, ptr=0x50000000)
+        kept, work = fake((2, 4, 1, 50), torch.int32, ptr=0x60000000), fake((2, 4, 1, 50), torch.int32, ptr=ws)
+        a = np.array([(0, 0, 100, 50, 0, 0)], np.int64)
+        assert lib.daric_evict_tokens(layers, 2, 0, r(bt), r(w), a.ctypes.data, 1, r(kept), r(work), ctypes.c_uint64(0)) == 1
+        return lib.daric_last_error().decode()
+
+    assert "a layer is given twice" in evict((0x10000000, 0x10000000), 0x70000000)
+    assert "workspace must not overlap kept" in evict((0x10000000, 0x18000000), 0x60000000 + 2 * 4 * 50 * 4 - 4)
+
+
 def test_python_lists_of_sequences():
     good = [(0, 0, 1, 5), (1, 1, 2, 6)]
     addr, n, a = cache_ops._sequences(good)
