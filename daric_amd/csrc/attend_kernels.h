@@ -15,8 +15,9 @@
 //
 // e4m3 codes become bf16 or fp16 (q's type) exactly; the scales of a head act
 // on c and on the result. The weights P are rounded to q's type for the second
-// product (half a step of it per weight, at random, where the output is
-// rounded to the same type); l sums them unrounded.
+// product, by at most half a step of it each, where the output is rounded to the
+// same type; l sums them unrounded. fp16 has that step above 2^-14 only, and
+// nothing below 2^-25: its weights are scaled (WeightRange).
 #pragma once
 
 #include <cmath>
@@ -50,6 +51,24 @@ __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     return c;
 #endif
 }
+
+// The running maximum m of a row is kept so that weights 2^(t - m) use what q's type
+// holds: a score t that passes it by more than OVER makes m = t - START, so the
+// heaviest token met so far weighs 2^START to 2^OVER. bf16 has fp32's range: a new
+// maximum weighs 1, and weights up to 2^8 save most tiles the exchange. fp16 holds half
+// steps from 2^-14 to 2^16: the heaviest weighs 2^14 to 2^15, so weights down to 2^-28
+// of it (19 in powers of e) keep their half step and lighter ones lose at most 2^-39 of
+// it. (With a heaviest weight of 1 a token 17 below it in powers of e weighed 2^-24 for
+// 2^-24.5, and one 18 below nothing.) Scores past 2^20 are so coarse in fp32 that START
+// could be lost in their rounding: their maxima weigh 1.
+template <int QK>
+struct WeightRange {
+    static constexpr bool FP16 = QK == kF16;
+    static constexpr float OVER = FP16 ? 15.0f : 8.0f;
+    static __device__ __forceinline__ float below(float t) {
+        return FP16 && fabsf(t) < 1048576.0f ? t - 14.0f : t;
+    }
+};
 
 // Two e4m3 codes (the low or high half of w) as a word of q's type.
 template <int QK, bool HI>
@@ -502,15 +521,15 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_kernel(DescArg 
                 }
             }
         }
-        // A new maximum only where a score passes the old one by 2^8: weights of
-        // up to 2^8 are as exact, and most tiles then skip the exchange.
+        // A new maximum only where a score passes the old one by so much: most tiles
+        // then skip the exchange.
         float top = t[0];
 #pragma unroll
         for (int j = 1; j < 8; ++j) top = fmaxf(top, t[j]);
-        if (__builtin_expect(__ballot(top - m > 8.0f) != 0, 0)) {
+        if (__builtin_expect(__ballot(top - m > WeightRange<QK>::OVER) != 0, 0)) {
             top = fmaxf(top, __shfl_xor(top, 16, 64));
             top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const float mn = fmaxf(m, top);
+            const float mn = fmaxf(m, WeightRange<QK>::below(top));
             const float al = exp2_hw(m - mn);
             m = mn;
             l *= al;
@@ -694,6 +713,7 @@ __global__ __launch_bounds__(WAVES * 64, DP == 256 ? 1 : 2) void attend_rows_ker
 #pragma unroll
         for (int st = 0; st < STEPS; ++st) q[t][st] = (q[t][st] & q_keep) ^ q_flip;
     }
+    constexpr bool SCALED = WeightRange<QK>::FP16;     // scores are scaled before they are compared
     f32x4 acc[NT][E];
     float m[NT], l[NT], limit[NT];                     // limit: scores beyond it need a new maximum
 #pragma unroll
@@ -821,6 +841,10 @@ __global__ __launch_bounds__(WAVES * 64, DP == 256 ? 1 : 2) void attend_rows_ker
                     if (!((vis >> (16 * (j >> 2) + 4 * g + (j & 3))) & 1u)) sc[t][j >> 2][j & 3] = -__builtin_huge_valf();
             }
         }
+        if constexpr (SCALED) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) sc[t][0] *= c, sc[t][1] *= c;
+        }
     };
     const auto top_of = [&](const f32x4 (&sc)[NT][2], int t) {
         float top = sc[t][0][0];
@@ -828,11 +852,13 @@ __global__ __launch_bounds__(WAVES * 64, DP == 256 ? 1 : 2) void attend_rows_ker
         for (int j = 1; j < 8; ++j) top = fmaxf(top, sc[t][j >> 2][j & 3]);
         return top;
     };
-    // The sums are never scaled: a scaling on a side way through the loop moved them
-    // to other registers and back in every tile (38 of its 190 instructions). A row's
-    // maximum is that of the first tile in which it sees a token, and weights up to
-    // 2^14 of it are as exact. A wavefront whose scores pass that takes its rows'
-    // maxima in a second pass over the tokens and its sums in a third.
+    // With bf16 weights the sums are never scaled: a scaling on a side way through the
+    // loop moved them to other registers and back in every tile (38 of its 190
+    // instructions). A row's maximum is that of the first tile in which it sees a token,
+    // and weights up to 2^14 of it are as exact. A wavefront whose scores pass that takes
+    // its rows' maxima in a second pass over the tokens and its sums in a third.
+    // fp16 weights have no such range to spare (WeightRange): sums are scaled where a
+    // score passes the maximum by 2^OVER, in one pass.
     constexpr float LOWEST = -3.402823466e38f;
     enum { kFirst, kMaxima, kLast, kDone };
     int pass = wave_end > 0 ? kFirst : kDone;
@@ -859,8 +885,22 @@ __global__ __launch_bounds__(WAVES * 64, DP == 256 ? 1 : 2) void attend_rows_ker
             scores(sc, t0, buf, sb);
             bool over = false;
 #pragma unroll
-            for (int t = 0; t < NT; ++t) over |= top_of(sc, t) > limit[t];
-            if (__builtin_expect(__ballot(over) != 0, 0)) {
+            for (int t = 0; t < NT; ++t)
+                over |= SCALED ? top_of(sc, t) - m[t] > WeightRange<QK>::OVER : top_of(sc, t) > limit[t];
+            if (SCALED && __builtin_expect(__ballot(over) != 0, 0)) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    float top = top_of(sc, t);
+                    top = fmaxf(top, __shfl_xor(top, 16, 64));
+                    top = fmaxf(top, __shfl_xor(top, 32, 64));
+                    const float mn = fmaxf(m[t], WeightRange<QK>::below(top));
+                    const float al = exp2_hw(m[t] - mn);
+                    m[t] = mn;
+                    l[t] *= al;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) acc[t][e] *= al;
+                }
+            } else if (!SCALED && __builtin_expect(__ballot(over) != 0, 0)) {
                 bool known = false;                    // a row with a maximum, and sums, already
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
@@ -889,7 +929,8 @@ __global__ __launch_bounds__(WAVES * 64, DP == 256 ? 1 : 2) void attend_rows_ker
                 float p[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    p[j] = exp2_hw(fmaf(sc[t][j >> 2][j & 3], c, -m[t]));
+                    const float x = sc[t][j >> 2][j & 3];
+                    p[j] = exp2_hw(SCALED ? x - m[t] : fmaf(x, c, -m[t]));
                     l[t] += p[j];
                 }
                 pb[t] = u32x4{pack2<QK>(p[0], p[1]), pack2<QK>(p[2], p[3]), pack2<QK>(p[4], p[5]), pack2<QK>(p[6], p[7])};

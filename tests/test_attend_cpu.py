@@ -226,3 +226,42 @@ def test_python_lists_of_sequences():
     for bad in ([(0, 0, 1)], [(0, 0, 1.5, 2)], [("a", 0, 1, 2)]):
         with pytest.raises(ValueError):
             cache_ops._sequences(bad)
+
+
+# ------------------------------------------------------ the oracle over matrices
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.uint8])
+def test_oracle_matrices_are_its_rows(tree, dtype):
+    from tests.test_gpu_attend import Case
+    c = Case(None, [(5, 40), (0, 3), (70, 9)], dtype=dtype, qtype=torch.float16, h=2, g=2, d=16, tree=tree, seed=60)
+    c.bt[c.seqs[2][0] + 1] = 0
+    if tree:
+        c.mask[3] = 0
+        c.bt[:c.seqs[1][0]] = 0                          # rows that see nothing
+    args = (c.layer, c.pf, c.bt, c.q, c.seqs, c.mask, c.scale, c.ks)
+    want, got = oatt.attend(*args, c.vs), oatt.attend_matrix(*args, c.vs)
+    for x, y in zip(want, got):
+        np.testing.assert_allclose(y, x, rtol=1e-11, atol=1e-13)
+    lse = torch.from_numpy(want[1]).float()
+    w0 = np.random.default_rng(0).random((2, c.columns))
+    wargs = (c.layer, c.pf, c.bt, c.q, lse, c.seqs, w0, c.mask, c.scale, c.ks)
+    for x, y in zip(oatt.weigh(*wargs), oatt.weigh_matrix(*wargs)):
+        np.testing.assert_allclose(y, x, rtol=1e-11, atol=1e-13)
+
+
+@pytest.mark.parametrize("layout,shared", [("nhd", False), ("hnd", True), ("packed", False), ("mla", True)])
+def test_oracle_eviction_over_matrices(layout, shared):
+    g = torch.Generator().manual_seed(61)
+    h = 1 if layout == "mla" else 3
+    layers = [make_layer(layout, 40, 4, h, 8, torch.uint8, g, kind="bytes") for _ in range(2)]
+    pf, a = layers[0][1], [t for t, _ in layers]
+    b = [t.clone() for t in a]
+    bt = np.random.default_rng(1).permutation(np.arange(1, 40)).astype(np.int32)
+    bt[[2, 20]] = 0, 99
+    ev = [(0, 1, 50, 20, 2, 3), (13, 60, 30, 30, 0, 0), (21, 100, 60, 11, 0, 5)]
+    w = torch.randn(2, 1 if shared else h, 170, generator=g).round(decimals=1).numpy()
+    w[0, 0, 5:9] = np.nan
+    v = w.copy()
+    np.testing.assert_array_equal(oatt.evict(a, pf, bt, w, ev, 30), oatt.evict_matrix(b, pf, bt, v, ev, 30))
+    np.testing.assert_array_equal(w, v)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
