@@ -863,6 +863,10 @@ __global__ __launch_bounds__(WAVES * 64, DP == 256 ? 1 : 2) void attend_rows_ker
     enum { kFirst, kMaxima, kLast, kDone };
     int pass = wave_end > 0 ? kFirst : kDone;
     bool failed = false;
+    // Past 2^20 the product c times a score may be rounded by more than the weights'
+    // range: there it is rounded for the score as it was for the maximum (c_in is 1).
+    bool far = false;
+    float c_in = c;
     // The rows in registers go to LDS, and the next ones are asked for, in the middle
     // of a step's tiles, by the two wavefronts of a SIMD at different tiles, so that
     // one of them feeds the matrix cores meanwhile.
@@ -911,14 +915,21 @@ __global__ __launch_bounds__(WAVES * 64, DP == 256 ? 1 : 2) void attend_rows_ker
                         known |= m[t] != LOWEST;
                         m[t] = fmaxf(m[t], top * c);
                         limit[t] = pass == kMaxima ? top : fmaxf((m[t] + 14.0f) / c, top);
+                        far |= fabsf(m[t]) > 1048576.0f;
                     }
                 }
+                far = __ballot(far) != 0;
+                c_in = far ? 1.0f : c;
                 if (pass == kFirst && __ballot(known) != 0) {
                     failed = true;
                     continue;
                 }
             }
             if (pass == kMaxima) continue;
+            if (__builtin_expect(far, 0)) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t) sc[t][0] *= c, sc[t][1] *= c;
+            }
             constexpr int VF = E < 8 ? E : 8;          // V operands read at once
             u32x4 vf[VF];
 #pragma unroll
@@ -930,7 +941,7 @@ __global__ __launch_bounds__(WAVES * 64, DP == 256 ? 1 : 2) void attend_rows_ker
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const float x = sc[t][j >> 2][j & 3];
-                    p[j] = exp2_hw(SCALED ? x - m[t] : fmaf(x, c, -m[t]));
+                    p[j] = exp2_hw(SCALED ? x - m[t] : fmaf(x, c_in, -m[t]));
                     l[t] += p[j];
                 }
                 pb[t] = u32x4{pack2<QK>(p[0], p[1]), pack2<QK>(p[2], p[3]), pack2<QK>(p[4], p[5]), pack2<QK>(p[6], p[7])};

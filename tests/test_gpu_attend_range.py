@@ -87,3 +87,31 @@ def test_scores_that_rise_by_little(dev, rows):
         out, lse = c.run()
         check(c, out)
         c.check(out, lse, want(c))
+
+
+@pytest.mark.parametrize("dtype,top", [(torch.float16, 6e4), (torch.bfloat16, 6e4), (torch.bfloat16, 1e7)])
+@pytest.mark.parametrize("rows,d", [(1, 64), (40, 64), (40, 128), (300, 128), (40, 256)])
+@pytest.mark.parametrize("late", [False, True])
+def test_huge_scores_choose_one_token(dev, dtype, top, rows, d, late):
+    """Scores up to 10^14, further apart than 100 each: a row's output is V of the
+    heaviest token that it sees, whatever fp32 makes of the others."""
+    c = Case(dev, [(rows, 700)], dtype=dtype, g=2, h=1, d=d, seed=98)
+    c.layer[0] = 0
+    c.q[:] = 0
+    c.q[..., 0] = top
+    c.q[1::3, :, 0] = -top
+    c.scale = 0.3
+    n = rows + 700
+    heavy, light = (690, 3) if late else (3, 690)        # of positive, of negative q
+    gen = torch.Generator().manual_seed(1)
+    k = top * (0.1 + 0.3 * torch.rand(n, generator=gen)) * torch.sign(torch.randn(n, generator=gen))
+    k[heavy], k[light] = top * 0.9, -top * 0.9
+    j = torch.arange(n)
+    c.layer[0, torch.from_numpy(c.bt[(j // 16).numpy()]).long(), j % 16, :, 0] = k.to(dtype)[:, None]
+    out, lse = c.run()
+    for sign, at in ((1, heavy), (-1, light)):
+        mine = [i for i in range(rows) if (sign < 0) == (i % 3 == 1)]
+        v = c.layer[1, int(c.bt[at // 16]), at % 16, 0]
+        if mine:
+            assert torch.equal(out[mine].cpu(), v.expand(len(mine), 2, d))
+    assert torch.isfinite(lse).all()
