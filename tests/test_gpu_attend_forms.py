@@ -1,0 +1,74 @@
+"""GPU parity of the forms that attention, weights and eviction take for large
+calls: many rows under wide heads, windows of rows over long contexts, and
+selections of many long sequences. Against oracle/attend.py's definitions over
+whole matrices; tolerances as in tests/test_gpu_attend.py."""
+import numpy as np
+import pytest
+import torch
+
+from daric_amd import cache_ops
+from oracle import attend as oatt
+from tests.gpu_util import make_layer, same_bytes, to_dev
+from tests.test_gpu_attend import E, Case
+
+pytestmark = pytest.mark.gpu
+BF, FP, F8 = torch.bfloat16, torch.float16, torch.uint8
+
+
+def want(c):
+    return oatt.attend_matrix(c.layer, c.pf, c.bt, c.q, c.seqs, c.mask, c.scale, c.ks, c.vs)
+
+
+def check_weigh(c, lse, weights=None):
+    """weigh_tokens against its definition, and a second call against the first."""
+    a = c.on_gpu()
+    start = np.zeros((c.h, c.columns)) if weights is None else weights.double().numpy()
+    got = []
+    for _ in range(2):
+        w = weights.to(c.dev) if weights is not None else None
+        got.append(cache_ops.weigh_tokens(a["layer"], c.pf, a["block_table"], a["q"], lse, c.seqs, weights=w,
+                                          tree_mask=a["tree_mask"], scale=c.scale, k_scale=a["k_scale"]))
+    assert torch.equal(*got)
+    ref, size, amax, rows = oatt.weigh_matrix(c.layer, c.pf, c.bt, c.q, lse.cpu(), c.seqs, start, c.mask, c.scale, c.ks)
+    tol = (ref - start) * ((c.q.shape[2] + 10) * E * amax + 24 * E + 4 * E * size + rows * E) + 2 * E * np.abs(ref) + 1e-37
+    err = np.abs(got[0].double().cpu().numpy() - ref)
+    assert (err <= tol).all(), f"weights off by {(err / tol).max():.2f} of their tolerance"
+
+
+# --------------------------------------------------------------- weights
+# 128 workgroups of 256 tokens and more, of up to 1024 rows of a KV head, or 512 of any
+# (weigh_rows_kernel).
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("dtype,qtype,layout,d,ps", [
+    (BF, None, "nhd", 128, 16), (FP, None, "hnd", 128, 32), (F8, BF, "nhd", 128, 16), (F8, FP, "packed", 64, 16),
+    (BF, None, "pf", 96, 16), (FP, None, "nhd", 72, 5), (F8, BF, "hnd", 80, 24), (BF, None, "nhd", 128, 5),
+    (BF, None, "nhd", 256, 16), (F8, FP, "nhd", 200 - 8, 5), (FP, None, "nhd_pad", 136, 16)])
+def test_windows_of_rows(dev, tree, dtype, qtype, layout, d, ps):
+    c = Case(dev, [(40, 6000), (1, 70), (20, 3001)], layout, dtype, qtype, ps=ps, h=8, g=2, d=d, tree=tree, seed=70)
+    c.bt[c.seqs[0][0] + 7] = 0
+    c.bt[c.seqs[2][0] + 3] = -5
+    if tree:
+        c.mask[5::9] = 0
+    out, lse = c.run()
+    c.check(out, lse, want(c))
+    check_weigh(c, lse)
+    check_weigh(c, lse, torch.rand(8, c.columns))
+
+
+@pytest.mark.parametrize("dtype", [BF, F8])
+@pytest.mark.parametrize("rows,ctx,h", [(700, 4000, 8), (1100, 15300, 8), (1030, 100, 128)])
+def test_windows_whose_own_rows_span_workgroups(dev, dtype, rows, ctx, h):
+    """The rows that see the last tokens only are passed over for the others."""
+    c = Case(dev, [(rows, ctx)], dtype=dtype, h=h, g=1, d=64, seed=71)
+    _, lse = c.run()
+    check_weigh(c, lse)
+
+
+def test_window_of_rows_that_see_nothing(dev):
+    c = Case(dev, [(40, 6000), (30, 500)], h=8, g=2, d=64, tree=True, seed=72)
+    c.bt[:c.seqs[1][0]] = 0
+    c.mask[:] = 0
+    out, lse = c.run()
+    c.check(out, lse, want(c))
+    assert (lse[:40] == -torch.inf).all()
+    check_weigh(c, lse)
