@@ -72,3 +72,54 @@ def test_window_of_rows_that_see_nothing(dev):
     c.check(out, lse, want(c))
     assert (lse[:40] == -torch.inf).all()
     check_weigh(c, lse)
+
+
+# ------------------------------------------------- many rows of wide heads
+WIDE = [(BF, None, 136, "packed"), (BF, None, 200, "nhd"), (BF, None, 256, "nhd"), (FP, None, 192, "hnd"),
+        (FP, None, 256, "pf"), (F8, BF, 192, "nhd"), (F8, FP, 256, "hnd"), (F8, BF, 256, "packed"), (BF, None, 150, "nhd")]
+
+
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("ps", [5, 16])
+@pytest.mark.parametrize("dtype,qtype,d,layout", WIDE)
+def test_many_rows_of_wide_heads(dev, dtype, qtype, d, layout, ps, tree):
+    c = Case(dev, [(20, 300), (70, 900), (1, 65), (33, 0)], layout, dtype, qtype, ps=ps, h=2, g=2, d=d, tree=tree, seed=73)
+    c.bt[c.seqs[1][0] + 2] = 0
+    out, lse = c.run()
+    c.check(out, lse, want(c))
+    check_weigh(c, lse)
+
+
+@pytest.mark.parametrize("dtype,qtype", [(BF, None), (FP, None), (F8, BF)])
+def test_wide_heads_in_parts(dev, dtype, qtype):
+    c = Case(dev, [(17, 9000), (300, 2000)], dtype=dtype, qtype=qtype, h=2, g=1, d=256, seed=74)
+    out, lse = c.run()
+    c.check(out, lse, want(c))
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("d", [136, 256])
+def test_rising_scores_of_wide_heads(dev, dtype, d):
+    """Maxima of the first tiles that do not hold, for some rows only."""
+    c = Case(dev, [(70, 1500)], dtype=dtype, d=d, g=2, h=2, seed=75)
+    c.layer[0, ..., 0] = 0
+    for j in range(1500):
+        c.layer[0, int(c.bt[j // 16]), j % 16, :, 0] = 8.0 * (j // 400) + (40.0 if j == 1497 else 0.0)
+    c.q[..., 0] = 0
+    c.q[::3, :, 0] = 30.0
+    c.q[1::5, :, 0] = -20.0
+    out, lse = c.run()
+    c.check(out, lse, want(c))
+    check_weigh(c, lse)
+
+
+def test_values_that_are_no_numbers_of_wide_heads(dev):
+    c = Case(dev, [(60, 45)], d=256, g=1, h=2, seed=76)
+    clean = want(c)
+    c.layer[1, int(c.bt[50 // 16]), 50 % 16, :, 3::16] = float("inf")       # draft 5: rows from 5 on see it
+    out, lse = c.run()
+    bad = np.zeros(clean[0].shape, bool)
+    bad[5:, :, 3::16] = True
+    got = out.double().cpu()
+    assert torch.isposinf(got[torch.from_numpy(bad)]).all()
+    c.check(torch.where(torch.from_numpy(bad), torch.from_numpy(clean[0]), got), lse, clean)
