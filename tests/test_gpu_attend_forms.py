@@ -123,3 +123,64 @@ def test_values_that_are_no_numbers_of_wide_heads(dev):
     got = out.double().cpu()
     assert torch.isposinf(got[torch.from_numpy(bad)]).all()
     c.check(torch.where(torch.from_numpy(bad), torch.from_numpy(clean[0]), got), lse, clean)
+
+
+# ------------------------------------------------------------- evictions
+def evict(dev, L, h, tokens, keep, seed, shared=False, first=1, recent=2, decimals=2):
+    """Sequences of these lengths over layers of small rows; many equal weights."""
+    g = torch.Generator().manual_seed(seed)
+    nb = sum(-(-n // 16) for n in tokens) + 1
+    layers = [make_layer("nhd", nb, 16, h, 2, torch.float16, g, kind="bytes")[0] for _ in range(L)]
+    bt = np.random.default_rng(seed).permutation(np.arange(1, nb)).astype(np.int32)
+    ev, at, col = [], 0, 0
+    for n, k in zip(tokens, keep):
+        k = max(min(n, first + recent), k)
+        ev.append((at, col, n, k, min(first, k), min(recent, k - min(first, k))))
+        at, col = at + -(-n // 16), col + n
+    w = torch.randn(L, 1 if shared else h, col, generator=g).round(decimals=decimals)
+    gl, gw = [to_dev(t, dev) for t in layers], w.to(dev)
+    kept = cache_ops.evict_tokens(gl, False, torch.from_numpy(bt).to(dev), gw, ev)
+    torch.cuda.synchronize()
+    wn = w.numpy().copy()
+    ref = oatt.evict_matrix(layers, False, bt, wn, ev, kept.shape[3])
+    np.testing.assert_array_equal(kept.cpu().numpy(), ref)
+    np.testing.assert_array_equal(gw.cpu().numpy().view(np.uint32), wn.view(np.uint32))
+    assert all(same_bytes(a, b) for a, b in zip(gl, layers))
+
+
+# More than 256 selections of a call, the longest from 2049 to 16384 tokens, shorter ones
+# beside it, and more than 1024 with a longer one.
+@pytest.mark.parametrize("longest", [2052, 8192, 8195, 8196, 16384, 16387])
+@pytest.mark.parametrize("frac", [0.1, 0.8])
+def test_many_selections_of_long_sequences(dev, longest, frac):
+    tokens = [longest, 20, 255, 2049, 300, 1, 2051, 64, 1500, 259, 17, 33, 700, 128, 31, 5, 2050]
+    evict(dev, 2, 8, tokens, [int(n * frac) for n in tokens], 80 + longest)
+
+
+@pytest.mark.parametrize("keep", [12291, 12292, 16000])
+def test_many_selections_beside_the_lds(dev, keep):
+    """As many chosen as a workgroup's LDS holds, and more."""
+    tokens = [16384] + [40] * 16
+    evict(dev, 2, 8, tokens, [keep] + [9] * 16, keep)
+
+
+@pytest.mark.parametrize("n,keep", [(9000, 8500), (20000, 12291), (20000, 12292), (32771, 30000), (32772, 13000)])
+def test_few_selections_beside_the_lds(dev, n, keep):
+    evict(dev, 1, 2, [n, 300], [keep, 100], n)
+
+
+@pytest.mark.parametrize("keep", [2000, 20000])
+def test_very_many_selections_with_a_long_one(dev, keep):
+    tokens = [32772] + [24 + i % 50 for i in range(31)] + [2500]
+    evict(dev, 2, 16, tokens, [keep] + [11] * 31 + [1200], 90, decimals=1)
+
+
+def test_many_selections_for_all_heads(dev):
+    tokens = [9000, 2500] + [100] * 15
+    evict(dev, 16, 2, tokens, [4000, 100] + [30] * 15, 91, shared=True)
+
+
+def test_longest_sequences_need_no_selection(dev):
+    """All but the recent tokens are chosen, or none is, of more than 256 sequences' heads."""
+    tokens = [3000] * 17
+    evict(dev, 2, 8, tokens, [2999, 3, 3000] + [4] * 14, 92)
