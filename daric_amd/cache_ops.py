@@ -513,9 +513,8 @@ def attend_pages(layer: torch.Tensor, page_first: bool, block_table: torch.Tenso
     tokens; of the others row i sees the first i + 1 (one token, a prompt's run
     of rows), or those whose bits its row of tree_mask (int64 [T, words])
     sets (drafted trees). Tokens in pages of id 0 are not there; rows that see
-    nothing get zeros and lse -inf; rows of no sequence are not written. out must
-    not overlap q. scale:
-    D ** -0.5 if None. k_scale, v_scale: [H] fp32 scales of an fp8 cache. See
+    nothing get zeros and lse -inf; rows of no sequence are not written. out and
+    lse must overlap neither each other nor an input. scale: D ** -0.5 if None. k_scale, v_scale: [H] fp32 scales of an fp8 cache. See
     include/daric_cache_ops.h for what the arguments may be."""
     dev = layer.device
     st = _resolve_stream(stream, dev)

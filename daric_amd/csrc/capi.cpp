@@ -1521,23 +1521,41 @@ namespace {
 constexpr int64_t kMaxHeadDim = 256;
 constexpr int64_t kMaxTokens = kIntMax - 1024;     // of a sequence: tiles past its end are still 32-bit
 
-// Ranges [begin, begin + n) that share no element.
-// Whether the memory from the first to the last element of two tensors overlaps.
-bool overlap(const daric_tensor& a, const daric_tensor& b) {
-    const auto span = [](const daric_tensor& t) {
+// The memory of an argument, from its first to its last byte.
+struct Span {
+    uintptr_t begin = 0, end = 0;
+    const char* name = "";
+    Span(const daric_tensor* t, const char* what) : name(what) {
+        if (t == nullptr || t->data == nullptr || numel(*t) == 0) return;
         int64_t lo = 0, hi = 0;
-        for (int d = 0; d < t.ndim; ++d) {
-            const int64_t end = (t.sizes[d] - 1) * t.strides[d];
-            (end < 0 ? lo : hi) += end;
+        for (int d = 0; d < t->ndim; ++d) {
+            const int64_t last = (t->sizes[d] - 1) * t->strides[d];
+            (last < 0 ? lo : hi) += last;
         }
-        const auto at = reinterpret_cast<uintptr_t>(t.data);
-        return std::pair(at + lo * t.elem_size, at + (hi + 1) * t.elem_size);
-    };
-    if (numel(a) == 0 || numel(b) == 0) return false;
-    const auto x = span(a), y = span(b);
-    return x.first < y.second && y.first < x.second;
+        begin = reinterpret_cast<uintptr_t>(t->data) + lo * t->elem_size;
+        end = reinterpret_cast<uintptr_t>(t->data) + (hi + 1) * t->elem_size;
+    }
+    Span(const void* p, int64_t bytes, const char* what) : name(what) {
+        if (p == nullptr || bytes <= 0) return;
+        begin = reinterpret_cast<uintptr_t>(p);
+        end = begin + bytes;
+    }
+};
+
+// What a call writes must be apart from all that it reads and from what else it
+// writes: its workgroups run in no order, and one may still read what another writes.
+void check_written(std::initializer_list<Span> written, std::initializer_list<Span> read) {
+    for (auto w = written.begin(); w != written.end(); ++w) {
+        const auto apart = [&](const Span& x) {
+            DARIC_CHECK(w->end <= x.begin || x.end <= w->begin || w->begin == w->end || x.begin == x.end, w->name,
+                        " must not overlap ", x.name);
+        };
+        for (const Span& x : read) apart(x);
+        for (auto x = w + 1; x != written.end(); ++x) apart(*x);
+    }
 }
 
+// Ranges [begin, begin + n) that share no element.
 void check_apart(std::vector<std::pair<int64_t, int64_t>>& r, const char* what) {
     bool ordered = true;
     for (size_t i = 1; i < r.size(); ++i) ordered = ordered && r[i - 1].first + r[i - 1].second <= r[i].first;
@@ -1806,13 +1824,14 @@ int daric_attend_pages(const daric_tensor* layer, int page_first, const daric_te
         c.a.lse = const_cast<float*>(check_lse(c, lse));
         c.a.out = static_cast<uint8_t*>(out->data);
         if (c.seqs.empty()) return;
-        // another workgroup may still read a row of q when its out is written
-        DARIC_CHECK(!overlap(*out, *q), "out must not overlap q");
         std::vector<AttGroup> groups = plan_attend(c);
         int64_t need = 0;
         for (const AttGroup& g : groups) need += g.bytes();
         DARIC_CHECK(need == 0 || (workspace != nullptr && workspace_bytes >= need && aligned(workspace, 16)),
                     "workspace must be 16-byte aligned and hold ", need, " bytes, got ", workspace_bytes);
+        check_written({{out, "out"}, {lse, "lse"}, {workspace, need, "workspace"}},
+                      {{q, "q"}, {layer, "the layer"}, {block_table, "block_table"}, {tree_mask, "tree_mask"},
+                       {k_scale, "k_scale"}, {v_scale, "v_scale"}});
         DeviceGuard guard(c.device);
         const hipStream_t st = as_stream(stream);
         check_capture(groups, st);
@@ -1890,6 +1909,8 @@ int daric_weigh_tokens(const daric_tensor* layer, int page_first, const daric_te
             if (!gr.seqs.empty()) groups.push_back(std::move(gr));
         }
         if (groups.empty()) return;
+        check_written({{weights, "weights"}}, {{q, "q"}, {lse, "lse"}, {layer, "the layer"}, {block_table, "block_table"},
+                                               {tree_mask, "tree_mask"}, {k_scale, "k_scale"}});
         DeviceGuard guard(c.device);
         const hipStream_t st = as_stream(stream);
         check_capture(groups, st);
@@ -1970,11 +1991,14 @@ int daric_evict_tokens(const daric_tensor* layers, int64_t n_layers, int page_fi
         const int64_t width = kept->sizes[3];
         DARIC_CHECK(n <= kMaxTiles / 4 && width <= kIntMax, "too many evictions in one call");
         if (n == 0) return;
-        DARIC_CHECK(!overlap(*kept, *workspace), "workspace must not overlap kept");
+        check_written({{workspace, "workspace"}, {kept, "kept"}, {weights, "weights"}}, {{block_table, "block_table"}});
         std::vector<const void*> data;
         for (int64_t i = 0; i < n_layers; ++i) data.push_back(layers[i].data);
         std::sort(data.begin(), data.end());
         DARIC_CHECK(std::adjacent_find(data.begin(), data.end()) == data.end(), "a layer is given twice");
+        for (int64_t i = 0; i < n_layers; ++i)
+            check_written({{&layers[i], "a layer"}}, {{block_table, "block_table"}, {weights, "weights"}, {kept, "kept"},
+                                                      {workspace, "workspace"}});
         int64_t unit = 16;
         const int64_t es = t.elem_size;
         const auto allows = [&](int64_t u) {

@@ -417,10 +417,12 @@ typedef struct daric_sequence {
  * tree_mask: contiguous int64 [T, words], 64 * words >= the longest n_rows.
  * k_scale, v_scale: NULL (1) or contiguous fp32 [H], for an e4m3 cache only.
  * out: contiguous [T, Hq, D] of q's type; lse: contiguous fp32 [T, Hq]; rows of
- * no sequence are not written, and no row may be in two; out does not overlap q.
+ * no sequence are not written, and no row may be in two.
  * workspace: at least
  * the bytes that daric_attend_workspace gives for the same arguments (NULL where
  * that is 0), in use until the call's work on `stream` is done.
+ * out, lse and workspace overlap neither each other nor what the call reads (their
+ * memory from the first to the last element).
  * Sums and softmax statistics are fp32; the weights P are rounded to q's type
  * for the product with V. The same call gives the same bits. */
 int daric_attend_workspace(const daric_tensor* layer, int page_first, const daric_tensor* q,
@@ -436,7 +438,8 @@ int daric_attend_pages(const daric_tensor* layer, int page_first, const daric_te
  * token received, of the attention that daric_attend_pages computes. lse:
  * contiguous fp32 [T, Hq] (rows with -inf add nothing). weights: fp32 [H, columns],
  * columns contiguous. accumulate 1 adds to it, 0 sets the columns of every sequence
- * that has rows. Other columns are not written; no column may be in two sequences.
+ * that has rows. Other columns are not written; no column may be in two sequences,
+ * and weights overlap nothing that the call reads.
  * Sums are fp32, in a fixed order. */
 int daric_weigh_tokens(const daric_tensor* layer, int page_first, const daric_tensor* block_table,
                        const daric_tensor* q, const daric_tensor* lse, const daric_sequence* sequences,
@@ -466,7 +469,8 @@ typedef struct daric_eviction {
  * weights: contiguous fp32 [n_layers, H, columns], or [n_layers, 1, columns]: one
  * selection for all heads of a layer. kept: contiguous int32
  * [n_layers, H or 1, n_evictions, kmax], kmax >= each min(keep, n_tokens). workspace:
- * int32 of kept's shape, apart from it. No layer may be given twice. Rows are moved as bytes: layers of any type;
+ * int32 of kept's shape. weights, kept, workspace, block_table and the layers
+ * overlap nowhere, and no layer may be given twice. Rows are moved as bytes: layers of any type;
  * a row whose page id, or whose slot's, is 0 or outside [1, num_blocks) is not
  * moved. A page may be in one sequence of a call only, and no column in two. */
 int daric_evict_tokens(const daric_tensor* layers, int64_t n_layers, int page_first,

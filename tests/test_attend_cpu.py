@@ -265,3 +265,64 @@ def test_oracle_eviction_over_matrices(layout, shared):
     np.testing.assert_array_equal(oatt.evict(a, pf, bt, w, ev, 30), oatt.evict_matrix(b, pf, bt, v, ev, 30))
     np.testing.assert_array_equal(w, v)
     assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+# --------------------------------------------- memory that a call writes, and sizes
+def test_written_memory_overlaps_nothing(lib):
+    """Each pair of an argument that is written and another one, by its last or first
+    bytes; refused before any device call."""
+    r = ctypes.byref
+    at = dict(layer=0x10000000, bt=0x20000000, q=0x30000000, out=0x40000000, lse=0x50000000, mask=0x60000000,
+              ks=0x70000000, vs=0x80000000, work=0x90000000, w=0xa0000000)
+    shape = dict(layer=((2, 40, 16, 4, 64), torch.uint8), bt=((40,), torch.int32), q=((1, 64, 64), torch.bfloat16),
+                 out=((1, 64, 64), torch.bfloat16), lse=((1, 64), torch.float32), mask=((1, 1), torch.int64),
+                 ks=((4,), torch.float32), vs=((4,), torch.float32), w=((4, 640), torch.float32))
+    size = {k: int(np.prod(s)) * torch.empty(0, dtype=t).element_size() for k, (s, t) in shape.items()}
+    names = dict(layer="the layer", bt="block_table", mask="tree_mask", ks="k_scale", vs="v_scale", work="workspace", w="weights")
+    addr, n, _k = seqs((0, 0, 1, 639, 0))
+    need = ctypes.c_int64()
+    t = {k: fake(*shape[k], ptr=at[k]) for k in shape}
+    assert lib.daric_attend_workspace(r(t["layer"]), 0, r(t["q"]), addr, n, r(need)) == 0
+    size["work"] = need.value
+    assert need.value > 0
+
+    def call(weigh, moved):
+        p = dict(at, **moved)
+        t = {k: fake(*shape[k], ptr=p[k]) for k in shape}
+        if weigh:
+            st = lib.daric_weigh_tokens(r(t["layer"]), 0, r(t["bt"]), r(t["q"]), r(t["lse"]), addr, n, r(t["mask"]), 1.0,
+                                        r(t["ks"]), r(t["w"]), 1, ctypes.c_uint64(0))
+        else:
+            st = lib.daric_attend_pages(r(t["layer"]), 0, r(t["bt"]), r(t["q"]), addr, n, r(t["mask"]), 1.0, r(t["ks"]),
+                                        r(t["vs"]), r(t["out"]), r(t["lse"]), p["work"], need.value, ctypes.c_uint64(0))
+        assert st == 1
+        return lib.daric_last_error().decode()
+
+    reads = ["q", "layer", "bt", "mask", "ks"]
+    for weigh, pairs in ((True, [("w", x) for x in reads + ["lse"]]),
+                         (False, [(w, x) for w in ("out", "lse", "work") for x in reads + ["vs"]] +
+                                 [("out", "lse"), ("out", "work"), ("lse", "work")])):
+        for w, x in pairs:
+            unit = 16 if w == "work" else 2 if w == "out" else 4
+            ends = [at[x] + size[x] - unit, at[x] - size[w] + unit]
+            for ptr in ends if w != "work" else [(p // 16) * 16 for p in (at[x] + size[x] - 1, at[x])]:
+                assert f"{names.get(w, w)} must not overlap {names.get(x, x)}" in call(weigh, {w: ptr}), (w, x)
+
+
+def test_evictions_write_apart(lib):
+    r = ctypes.byref
+    at = dict(l0=0x10000000, l1=0x18000000, bt=0x20000000, w=0x50000000, kept=0x60000000, work=0x70000000)
+    shape = dict(l0=((2, 8, 16, 4, 64), torch.bfloat16), l1=((2, 8, 16, 4, 64), torch.bfloat16), bt=((8,), torch.int32),
+                 w=((2, 4, 200), torch.float32), kept=((2, 4, 1, 50), torch.int32), work=((2, 4, 1, 50), torch.int32))
+    size = {k: int(np.prod(s)) * torch.empty(0, dtype=t).element_size() for k, (s, t) in shape.items()}
+    a = np.array([(0, 0, 100, 50, 0, 0)], np.int64)
+    names = dict(l0="a layer", l1="a layer", bt="block_table", w="weights", work="workspace")
+    for x, y in [("work", "kept"), ("work", "w"), ("work", "bt"), ("kept", "w"), ("kept", "bt"), ("w", "bt"), ("l0", "bt"),
+                 ("l1", "w"), ("l0", "kept"), ("l1", "work")]:
+        for ptr in (at[y] + size[y] - 4, at[y] - size[x] + 4):
+            p = dict(at, **{x: ptr})
+            t = {k: fake(*shape[k], ptr=p[k]) for k in shape}
+            layers = (_lib.DaricTensor * 2)(t["l0"], t["l1"])
+            assert lib.daric_evict_tokens(layers, 2, 0, r(t["bt"]), r(t["w"]), a.ctypes.data, 1, r(t["kept"]), r(t["work"]),
+                                          ctypes.c_uint64(0)) == 1, (x, y)
+            assert f"{names.get(x, x)} must not overlap {names.get(y, y)}" in lib.daric_last_error().decode(), (x, y)
