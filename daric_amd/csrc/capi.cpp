@@ -1621,7 +1621,7 @@ AttCall attention_call(const daric_tensor* layer, int page_first, const daric_te
         DARIC_CHECK(s.n_ctx <= kMaxTokens && s.n_rows <= kMaxTokens && s.n_ctx + s.n_rows <= kMaxTokens &&
                     s.n_rows <= (kIntMax - 1024) / a.G, "sequence ", i, " is too long");
         DARIC_CHECK(s.row_start <= c.T && s.n_rows <= c.T - s.row_start, "sequence ", i, " rows exceed q");
-        DARIC_CHECK(s.row_start <= kIntMax, "sequence ", i, " starts too far into q");
+        DARIC_CHECK(s.row_start + s.n_rows <= kIntMax, "sequence ", i, " reaches too far into q");
         if (s.n_rows == 0) continue;      // nothing to compute
         rows.emplace_back(s.row_start, s.n_rows);
         AttSeq x{};

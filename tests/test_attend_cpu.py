@@ -326,3 +326,25 @@ def test_evictions_write_apart(lib):
             assert lib.daric_evict_tokens(layers, 2, 0, r(t["bt"]), r(t["w"]), a.ctypes.data, 1, r(t["kept"]), r(t["work"]),
                                           ctypes.c_uint64(0)) == 1, (x, y)
             assert f"{names.get(x, x)} must not overlap {names.get(y, y)}" in lib.daric_last_error().decode(), (x, y)
+
+
+def test_rows_past_32_bits_are_refused(lib):
+    """The kernels count rows of q in 32 bits."""
+    layer, bt = fake((2, 8, 16, 1, 2), torch.bfloat16), fake((8,), torch.int32)
+    T = 2 ** 31 + 50
+    q, lse = fake((T, 1, 2), torch.bfloat16, ptr=2 ** 40), fake((T, 1), torch.float32, ptr=2 ** 41)
+    out, w = fake((T, 1, 2), torch.bfloat16, ptr=2 ** 42), fake((1, 100), torch.float32, ptr=2 ** 43)
+    need = ctypes.c_int64()
+    r = ctypes.byref
+    for start in (2 ** 31 - 8, 2 ** 31 - 1, 2 ** 31, 2 ** 31 + 40):
+        addr, n, _k = seqs((0, start, 9, 20, 0))
+        assert lib.daric_attend_workspace(r(layer), 0, r(q), addr, n, r(need)) == 1
+        assert b"reaches too far into q" in lib.daric_last_error()
+        assert lib.daric_attend_pages(r(layer), 0, r(bt), r(q), addr, n, None, 1.0, None, None, r(out), r(lse), None, 0,
+                                      ctypes.c_uint64(0)) == 1
+        assert b"reaches too far into q" in lib.daric_last_error()
+        assert lib.daric_weigh_tokens(r(layer), 0, r(bt), r(q), r(lse), addr, n, None, 1.0, None, r(w), 1,
+                                      ctypes.c_uint64(0)) == 1
+        assert b"reaches too far into q" in lib.daric_last_error()
+    addr, n, _k = seqs((0, 2 ** 31 - 10, 9, 20, 0))
+    assert lib.daric_attend_workspace(r(layer), 0, r(q), addr, n, r(need)) == 0
