@@ -1783,8 +1783,8 @@ void attention_inputs(AttCall& c, const daric_tensor* block_table, const daric_s
     };
     a.k_scale = scales(k_scale, "k_scale");
     a.v_scale = scales(v_scale, "v_scale");
-    DARIC_CHECK(std::isfinite(scale), "scale must be finite");
     a.scale_log2 = scale * 1.44269504088896341f;
+    DARIC_CHECK(std::isfinite(a.scale_log2), "scale must be finite, in powers of 2 too (times log2(e))");
 }
 
 const float* check_lse(const AttCall& c, const daric_tensor* lse) {

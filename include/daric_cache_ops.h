@@ -416,6 +416,7 @@ typedef struct daric_sequence {
  * strides free, in the cache's type; bfloat16 or float16 for an e4m3 cache.
  * tree_mask: contiguous int64 [T, words], 64 * words >= the longest n_rows.
  * k_scale, v_scale: NULL (1) or contiguous fp32 [H], for an e4m3 cache only.
+ * scale: finite, and times log2(e) too.
  * out: contiguous [T, Hq, D] of q's type; lse: contiguous fp32 [T, Hq]; rows of
  * no sequence are not written, and no row may be in two.
  * workspace: at least

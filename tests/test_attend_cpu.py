@@ -348,3 +348,18 @@ def test_rows_past_32_bits_are_refused(lib):
         assert b"reaches too far into q" in lib.daric_last_error()
     addr, n, _k = seqs((0, 2 ** 31 - 10, 9, 20, 0))
     assert lib.daric_attend_workspace(r(layer), 0, r(q), addr, n, r(need)) == 0
+
+
+def test_scales_whose_power_of_2_is_infinite_are_refused(lib):
+    layer, bt = fake((2, 8, 16, 4, 64), torch.bfloat16), fake((8,), torch.int32, ptr=0x20000000)
+    q, lse = fake((10, 8, 64), torch.bfloat16, ptr=0x30000000), fake((10, 8), torch.float32, ptr=0x50000000)
+    out, w = fake((10, 8, 64), torch.bfloat16, ptr=0x40000000), fake((4, 200), torch.float32, ptr=0x60000000)
+    addr, n, _k = seqs((0, 0, 10, 50, 0))
+    r = ctypes.byref
+    for scale in (2.5e38, -3.4e38, float("inf"), float("nan")):
+        assert lib.daric_attend_pages(r(layer), 0, r(bt), r(q), addr, n, None, scale, None, None, r(out), r(lse), None, 0,
+                                      ctypes.c_uint64(0)) == 1
+        assert b"scale must be finite" in lib.daric_last_error()
+        assert lib.daric_weigh_tokens(r(layer), 0, r(bt), r(q), r(lse), addr, n, None, scale, None, r(w), 1,
+                                      ctypes.c_uint64(0)) == 1
+        assert b"scale must be finite" in lib.daric_last_error()
