@@ -497,6 +497,13 @@ def _scale(scale: Optional[float], q: torch.Tensor) -> float:
     return float(scale) if scale is not None else q.shape[-1] ** -0.5 if q.dim() and q.shape[-1] else 1.0
 
 
+def _no_backward(what: str, *tensors) -> None:
+    """These calls have no backward pass: an input that asks for a gradient is
+    refused, not answered by an output that silently has none."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad(), or detach what requires a gradient")
+
+
 def _layer_desc(layer: torch.Tensor):
     return _layer_array((layer,))
 
@@ -515,7 +522,9 @@ def attend_pages(layer: torch.Tensor, page_first: bool, block_table: torch.Tenso
     sets (drafted trees). Tokens in pages of id 0 are not there; rows that see
     nothing get zeros and lse -inf; rows of no sequence are not written. out and
     lse must overlap neither each other nor an input. scale: D ** -0.5 if None. k_scale, v_scale: [H] fp32 scales of an fp8 cache. See
-    include/daric_cache_ops.h for what the arguments may be."""
+    include/daric_cache_ops.h for what the arguments may be. No backward pass:
+    inputs that require a gradient are refused while gradients are enabled."""
+    _no_backward("attend_pages", layer, q, k_scale, v_scale, out, lse)
     dev = layer.device
     st = _resolve_stream(stream, dev)
     addr, n, _keep = _sequences(seqs)
@@ -549,7 +558,8 @@ def weigh_tokens(layer: torch.Tensor, page_first: bool, block_table: torch.Tenso
     and the query heads of each KV head: added to weights[:, col_start + j]
     ([H, columns] fp32) for token j of a sequence (bt_offset, row_start, n_rows,
     n_ctx, col_start), or without `weights` written to a new tensor, zeros where
-    no sequence is. Returns the weights."""
+    no sequence is. Returns the weights. No backward pass, as attend_pages."""
+    _no_backward("weigh_tokens", layer, q, lse, weights, k_scale)
     dev = layer.device
     st = _resolve_stream(stream, dev)
     addr, n, a = _sequences(seqs)
@@ -576,8 +586,10 @@ def evict_tokens(layers: Sequence[torch.Tensor], page_first: bool, block_table: 
     `keep` slots stay, the i-th slot freed takes the i-th kept token from behind.
     Returns kept [L, H or 1, n, kmax] int32: the token that each slot holds
     now, -1 behind the last. The weights move with their tokens, those from
-    `keep` on become 0. Rows are bytes: any cache type, MLA caches too."""
+    `keep` on become 0. Rows are bytes: any cache type, MLA caches too. No
+    backward pass, as attend_pages."""
     layers = list(layers)
+    _no_backward("evict_tokens", weights, *layers)
     dev = layers[0].device
     st = _resolve_stream(stream, dev)
     addr, n, a = _tuples(evictions, (6,), "evictions must be (bt_offset, col_start, n_tokens, keep, n_first, n_recent) "

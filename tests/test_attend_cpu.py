@@ -363,3 +363,24 @@ def test_scales_whose_power_of_2_is_infinite_are_refused(lib):
         assert lib.daric_weigh_tokens(r(layer), 0, r(bt), r(q), r(lse), addr, n, None, scale, None, r(w), 1,
                                       ctypes.c_uint64(0)) == 1
         assert b"scale must be finite" in lib.daric_last_error()
+
+
+def test_inputs_that_require_a_gradient_are_refused():
+    """No output silently without a gradient; under no_grad, and for detached inputs, the
+    calls go on (here to the refusal of tensors that are not on a GPU)."""
+    layer, bt = torch.zeros(2, 4, 16, 2, 64), torch.ones(4, dtype=torch.int32)
+    q, lse, w, s = torch.zeros(1, 4, 64), torch.zeros(1, 4), torch.zeros(2, 40), torch.ones(2)
+    want = lambda t: t.clone().requires_grad_()
+    attend = lambda l=layer, q=q, **k: cache_ops.attend_pages(l, False, bt, q, [(0, 0, 1, 20)], **k)
+    weigh = lambda l=layer, q=q, lse=lse, w=w, **k: cache_ops.weigh_tokens(l, False, bt, q, lse, [(0, 0, 1, 20, 0)], weights=w, **k)
+    evict = lambda l=layer, w=w: cache_ops.evict_tokens([l], False, bt, w[None], [(0, 0, 20, 10, 0, 0)])
+    for call in (lambda: attend(q=want(q)), lambda: attend(want(layer)), lambda: attend(k_scale=want(s)),
+                 lambda: attend(v_scale=want(s)), lambda: weigh(q=want(q)), lambda: weigh(lse=want(lse)),
+                 lambda: weigh(w=want(w)), lambda: weigh(k_scale=want(s)), lambda: evict(w=want(w)), lambda: evict(want(layer))):
+        with pytest.raises(RuntimeError, match="has no backward pass"):
+            call()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="must be on CUDA"):
+            call()
+    for call in (attend, weigh, evict):
+        with pytest.raises(RuntimeError, match="must be on CUDA"):
+            call()
