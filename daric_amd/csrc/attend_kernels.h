@@ -35,6 +35,9 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
+// A word at any element of a 16-bit type: `out` may begin at an odd one.
+typedef uint32_t word_any __attribute__((aligned(2)));
+
 constexpr float kLn2 = 0.693147180559945309f;
 
 template <int QK>
@@ -1043,7 +1046,7 @@ __global__ __launch_bounds__(WAVES * 64, DP == 256 ? 1 : 2) void attend_rows_ker
                 const int dd = E * (4 * g + i) + e;
                 if (MODE != kAttWhole && dd >= a.g.D) continue;      // head_dim is even here
                 const float x0 = l[t] == 0.0f ? 0.0f : acc[t][e][i] * inv, x1 = l[t] == 0.0f ? 0.0f : acc[t][e + 1][i] * inv;
-                *reinterpret_cast<uint32_t*>(out + dd) = pack2<QK>(x0, x1);
+                *reinterpret_cast<word_any*>(out + dd) = pack2<QK>(x0, x1);
             }
         if (g == 0) a.lse[at] = l[t] == 0.0f ? -__builtin_huge_valf() : (m[t] + log2f(l[t])) * kLn2;
     }

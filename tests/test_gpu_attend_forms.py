@@ -184,3 +184,18 @@ def test_longest_sequences_need_no_selection(dev):
     """All but the recent tokens are chosen, or none is, of more than 256 sequences' heads."""
     tokens = [3000] * 17
     evict(dev, 2, 8, tokens, [2999, 3, 3000] + [4] * 14, 92)
+
+
+# ------------------------------------------------------------- alignment
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("sizes,d", [([(2, 100)], 64), ([(30, 20), (1, 300)], 64), ([(300, 50)], 128), ([(40, 2000)], 256)])
+def test_out_at_an_odd_element(dev, dtype, sizes, d):
+    """Any element of a larger buffer may be out's first; what lies beside stays."""
+    c = Case(dev, sizes, dtype=dtype, g=2, h=2, d=d, seed=77)
+    plain, pl = c.run()
+    for at in (1, 2, 3):
+        flat = torch.full((plain.numel() + 8,), 7.0, dtype=dtype, device=dev)
+        out = flat[at:at + plain.numel()].view(plain.shape)
+        got, lse = c.run(out=out)
+        assert got is out and torch.equal(out, plain) and torch.equal(lse, pl)
+        assert (flat[:at] == 7).all() and (flat[at + plain.numel():] == 7).all()
