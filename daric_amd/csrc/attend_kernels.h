@@ -71,6 +71,10 @@ struct WeightRange {
     static __device__ __forceinline__ float below(float t) {
         return FP16 && fabsf(t) < 1048576.0f ? t - 14.0f : t;
     }
+    // log(l 2^m), without the factor 2^START that m and l both hold in fp16.
+    static __device__ __forceinline__ float log_sum(float m, float l) {
+        return (FP16 ? m + 14.0f + log2f(l * 0x1p-14f) : m + log2f(l)) * kLn2;
+    }
 };
 
 // Two e4m3 codes (the low or high half of w) as a word of q's type.
@@ -645,7 +649,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_kernel(DescArg 
         const float x = ll == 0.0f ? 0.0f : o[e] * inv;
         if (dc + e < a.g.D) out[dc + e] = static_cast<uint16_t>(QK == kBF16 ? f32_to_bf16(x) : f32_to_f16(x));
     }
-    if ((tid & 15) == 0) a.lse[at] = ll == 0.0f ? -__builtin_huge_valf() : (mm + log2f(ll)) * kLn2;
+    if ((tid & 15) == 0) a.lse[at] = ll == 0.0f ? -__builtin_huge_valf() : WeightRange<QK>::log_sum(mm, ll);
 }
 
 // -------------------------------------------------------- attend, many rows
@@ -1048,7 +1052,7 @@ __global__ __launch_bounds__(WAVES * 64, DP == 256 ? 1 : 2) void attend_rows_ker
                 const float x0 = l[t] == 0.0f ? 0.0f : acc[t][e][i] * inv, x1 = l[t] == 0.0f ? 0.0f : acc[t][e + 1][i] * inv;
                 *reinterpret_cast<word_any*>(out + dd) = pack2<QK>(x0, x1);
             }
-        if (g == 0) a.lse[at] = l[t] == 0.0f ? -__builtin_huge_valf() : (m[t] + log2f(l[t])) * kLn2;
+        if (g == 0) a.lse[at] = l[t] == 0.0f ? -__builtin_huge_valf() : WeightRange<QK>::log_sum(m[t], l[t]);
     }
 }
 
@@ -1120,7 +1124,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(DescArg d, AttArgs a, 
         const float x = ll == 0.0f ? 0.0f : o[v] * inv;
         if (lane * V + v < a.g.D) out[lane * V + v] = static_cast<uint16_t>(QK == kBF16 ? f32_to_bf16(x) : f32_to_f16(x));
     }
-    if (lane == 0) a.lse[at] = ll == 0.0f ? -__builtin_huge_valf() : (mm + log2f(ll)) * kLn2;
+    if (lane == 0) a.lse[at] = ll == 0.0f ? -__builtin_huge_valf() : WeightRange<QK>::log_sum(mm, ll);
 }
 
 // Sums 8 values over the 16 lanes of a group: a lane of n < 8 gets the sum of

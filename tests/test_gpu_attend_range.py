@@ -115,3 +115,16 @@ def test_huge_scores_choose_one_token(dev, dtype, top, rows, d, late):
         if mine:
             assert torch.equal(out[mine].cpu(), v.expand(len(mine), 2, d))
     assert torch.isfinite(lse).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,ctx", [(1, 0), (1, 6), (7, 0), (60, 0), (1, 900), (30, 900)])
+def test_lse_of_equal_scores(dev, dtype, rows, ctx):
+    """Scores of 0 over n tokens: log n. The logarithm in powers of 2 is good to an ulp,
+    2 e of a value of up to 10 (e = 2^-24), and the parts' sums (of ones) are exact; with the
+    product by log 2 and its constant, 4 e of the larger of 1 and log n."""
+    c = Case(dev, [(rows, ctx)], dtype=dtype, g=2, h=1, d=64, seed=99)
+    c.q[:] = 0
+    _, lse = c.run()
+    ref = np.log(ctx + 1.0 + np.arange(rows))[:, None]
+    assert (np.abs(lse.double().cpu().numpy() - ref) <= 4 * E * np.maximum(1.0, ref)).all()
