@@ -586,7 +586,9 @@ def evict_tokens(layers: Sequence[torch.Tensor], page_first: bool, block_table: 
     `keep` slots stay, the i-th slot freed takes the i-th kept token from behind.
     Returns kept [L, H or 1, n, kmax] int32: the token that each slot holds
     now, -1 behind the last. The weights move with their tokens, those from
-    `keep` on become 0. Rows are bytes: any cache type, MLA caches too. No
+    `keep` on become 0. Rows are bytes: any cache type, MLA caches too. A slot is
+    then no longer its position's: not for the calls that pair slots with tokens
+    (kv_deviation, merge_rows, select_merge, records of reusable chunks). No
     backward pass, as attend_pages."""
     layers = list(layers)
     _no_backward("evict_tokens", weights, *layers)

@@ -67,13 +67,13 @@ __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
 template <int QK>
 struct WeightRange {
     static constexpr bool FP16 = QK == kF16;
-    static constexpr float OVER = FP16 ? 15.0f : 8.0f;
+    static constexpr float START = FP16 ? 14.0f : 0.0f, OVER = FP16 ? 15.0f : 8.0f;
     static __device__ __forceinline__ float below(float t) {
-        return FP16 && fabsf(t) < 1048576.0f ? t - 14.0f : t;
+        return FP16 && fabsf(t) < 1048576.0f ? t - START : t;
     }
     // log(l 2^m), without the factor 2^START that m and l both hold in fp16.
     static __device__ __forceinline__ float log_sum(float m, float l) {
-        return (FP16 ? m + 14.0f + log2f(l * 0x1p-14f) : m + log2f(l)) * kLn2;
+        return (FP16 ? m + START + log2f(l * 0x1p-14f) : m + log2f(l)) * kLn2;
     }
 };
 
@@ -456,9 +456,10 @@ __device__ __forceinline__ float with_mark(float x, uint32_t word, int d) {
 // Bound by memory: K and V are read once, by whole rows of a head. V is read past the
 // caches; K, of which an instruction takes half a line of each row, must find the
 // other half there. MI355X, one row to a sequence: 32 sequences of 310 to 8191 tokens
-// (bf16, 8 KV heads of 128, 412 MB) 68 us, 6.0 TB/s, where a plain read of as much
-// takes 62; with K past the caches too 81, with V through them 86. Two sequences of
-// 131072 and 100001 tokens, e4m3, 473 MB: 90 us, 5.2 TB/s; head-major pages 79.
+// (bf16, 8 KV heads of 128, 414 MB read from HBM) 67 us, 6.2 TB/s, where a plain read of
+// as much takes 62; with K past the caches too 81, with V through them 86. Two sequences
+// of 131072 and 100001 tokens, e4m3, 474 MB from HBM: 88 us, 5.4 TB/s; head-major pages
+// 76.
 template <int CK, int QK, int DP, int MODE, bool PAGED>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_kernel(DescArg d, AttArgs a) {
     using Rows = TileRows<CK, DP>;
@@ -661,13 +662,14 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_kernel(DescArg 
 // instructions. The next step's rows come from memory meanwhile, into the other
 // half of the LDS.
 // Bound by products, softmax and staging, of which the two wavefronts of a SIMD overlap
-// only a part: the matrix cores are busy 35% of the time, the vector unit issues 41%.
+// only a part: the matrix cores are busy 36% of the time, the vector unit issues 40%.
 // MI355X, 2048 rows of 32 heads behind 6144 tokens (bf16, 8 KV heads of 128, 240
-// GFLOP): 264 us by the clock, 911 TFLOP/s, where a library product of 8192 x 8192 x
-// 8192 reaches 1208; 310 in a kernel trace. Of 328 traced us of an earlier form 254
-// were left without the staging, 270 without the softmax, 185 without both. Traced:
-// 256 rows to a workgroup 312 us, 128 rows 365, 64 rows 505 (the last before the
-// staging was spread over the step).
+// GFLOP): 262 us, 918 TFLOP/s, where a library product of 8192 x 8192 x 8192 reaches
+// 1208 (the first launches after a pause take 303 to 310, at lower clocks). Of 328 us of
+// an earlier form, in first launches, 254 were left without the staging, 270 without the
+// softmax, 185 without both; 256 rows to a workgroup 312, 128 rows 365, 64 rows 505 (the
+// last before the staging was spread over the step). e4m3 263, fp16 282; heads of 64
+// 193 (625 TFLOP/s), of 256 1481 (325).
 template <int CK, int QK, int DP, int MODE, bool PAGED, int WAVES, int NT>
 __global__ __launch_bounds__(WAVES * 64, DP == 256 ? 1 : 2) void attend_rows_kernel(DescArg d, AttArgs a) {
     using Rows = TileRows<CK, DP>;
@@ -863,9 +865,12 @@ __global__ __launch_bounds__(WAVES * 64, DP == 256 ? 1 : 2) void attend_rows_ker
     // loop moved them to other registers and back in every tile (38 of its 190
     // instructions). A row's maximum is that of the first tile in which it sees a token,
     // and weights up to 2^14 of it are as exact. A wavefront whose scores pass that takes
-    // its rows' maxima in a second pass over the tokens and its sums in a third.
+    // its rows' maxima in a second pass over the tokens and its sums in a third: 2048 rows
+    // whose heaviest token, 16 powers of 2 above the rest, comes late take 623 us, 264
+    // where it is the first or none is; eight trees of up to 61 drafts 137 and 72.
     // fp16 weights have no such range to spare (WeightRange): sums are scaled where a
-    // score passes the maximum by 2^OVER, in one pass.
+    // score passes the maximum by 2^OVER, in one pass: 288 to 298 us wherever the heaviest
+    // stands (276 without the scaling).
     constexpr float LOWEST = -3.402823466e38f;
     enum { kFirst, kMaxima, kLast, kDone };
     int pass = wave_end > 0 ? kFirst : kDone;
@@ -1150,8 +1155,9 @@ __device__ __forceinline__ float sum_group(float (&v)[8], int n) {
 // ------------------------------------------------------------------- weigh
 // One workgroup: one KV head, 128 tokens, 32 to a wavefront, whose K rows stay
 // in registers while all rows of the sequence pass (a few, or any of odd layouts).
-// Bound by memory: the batch of attend_kernel, 212 MB of K, 43 us, 4.9 TB/s (45 by
-// weigh_rows_kernel, 53 with K past the caches). Each token's sum is one
+// Bound by memory, and by the wait for it (57% of the wavefronts' time): the batch of
+// attend_kernel, 213 MB of K from HBM, 42 us, 5.1 TB/s (45 by weigh_rows_kernel, 53 with
+// K past the caches). Each token's sum is one
 // lane's, then 16 lanes', in a fixed order.
 template <int CK, int QK, int DP, int MODE, bool PAGED>
 __global__ __launch_bounds__(256) void weigh_kernel(DescArg d, AttArgs a) {
@@ -1286,10 +1292,12 @@ __device__ __forceinline__ float load_row(const AttArgs& a, const AttSeq& s, int
 
 // One workgroup: one KV head, 256 tokens, 64 to a wavefront, whose K operands stay
 // in registers while the rows pass through LDS as operands, 64 at a time, one
-// matrix tile staged by each wavefront and read by all. Bound by the exponentials:
-// 16 of them (of a quarter of the vector rate) per lane to 16 matrix instructions.
-// MI355X, the last 64 rows of 64 heads against 32768 and 20064 tokens, e4m3, 55
-// GFLOP: 83 us by the clock, 667 TFLOP/s (204 us by weigh_kernel).
+// matrix tile staged by each wavefront and read by all. Bound by neither unit alone: the
+// vector unit issues 44% of the time (16 exponentials of a quarter of its rate per lane to
+// 16 matrix instructions), the matrix cores are busy 25%, and the wavefronts wait 42% of
+// theirs: each tile's exponentials follow its products. MI355X, the last 64 rows of 64
+// heads against 32768 and 20064 tokens, e4m3, 55 GFLOP: 83 us, 667 TFLOP/s (204 us by
+// weigh_kernel).
 template <int CK, int QK, int DP, int MODE>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 3) void weigh_rows_kernel(DescArg d, AttArgs a) {
     constexpr int STEPS = DP / 32, WAVES = 4, STEP = WAVES * kAttRows;

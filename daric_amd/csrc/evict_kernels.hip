@@ -13,17 +13,18 @@
 // weights (topk.h), then the slots from its ascending indices alone.
 // evict_move_kernel: tiles of slots, whose moving rows are gathered in LDS
 // first, so that all lanes copy. Read and written past the caches (202 -> 180 us for
-// the 992 MB that an eviction of 8 sequences from 32 layers moves; MI355X).
+// an eviction of 8 sequences from 32 layers).
+//
+// The plan is bound by the latency of its passes (its wavefronts wait 59% of their time,
+// vector issue 30%), the move by memory. MI355X, 8 sequences of 1100 to 2500 tokens cut to
+// 1024 in 32 layers of 8 x 128 bf16: plan 41 us, rows 179 us for 962 MB of HBM read and
+// written, 5.4 TB/s (a copy of 1 GiB by torch: 4.8); one sequence of 16384 cut to 2048 in
+// 80 e4m3 layers: 61 us, and 112 for 598 MB, 5.3 TB/s.
 #include "attend.h"
 #include "kernels.h"
 #include "launch.h"
 #include "topk.h"
 
-//
-// The move is bound by memory. MI355X, 8 sequences of 1100 to 2500 tokens cut to 1024 in
-// 32 layers of 8 x 128 bf16: plan 42 us, rows 180 us for 992 MB read and written, 5.5
-// TB/s (a copy of 1 GiB by torch: 4.8); one sequence of 16384 cut to 2048 in 80 e4m3
-// layers, 681 MB: 63 and 113 us.
 namespace daric {
 namespace {
 

@@ -473,7 +473,10 @@ typedef struct daric_eviction {
  * int32 of kept's shape. weights, kept, workspace, block_table and the layers
  * overlap nowhere, and no layer may be given twice. Rows are moved as bytes: layers of any type;
  * a row whose page id, or whose slot's, is 0 or outside [1, num_blocks) is not
- * moved. A page may be in one sequence of a call only, and no column in two. */
+ * moved. A page may be in one sequence of a call only, and no column in two.
+ * Afterwards a slot is no longer its position's, and differs from head to head: such
+ * pages are for attention and further evictions, not for the calls that pair slots
+ * with tokens (gathers into records, deviation, merge and selection). */
 int daric_evict_tokens(const daric_tensor* layers, int64_t n_layers, int page_first,
                        const daric_tensor* block_table, daric_tensor* weights,
                        const daric_eviction* evictions, int64_t n_evictions, daric_tensor* kept,
