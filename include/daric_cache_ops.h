@@ -425,7 +425,8 @@ typedef struct daric_sequence {
  * out, lse and workspace overlap neither each other nor what the call reads (their
  * memory from the first to the last element).
  * Sums and softmax statistics are fp32; the weights P are rounded to q's type
- * for the product with V. The same call gives the same bits. */
+ * for the product with V: by half a step each, but in float16 weights below 2^-28 of
+ * a row's heaviest by 2^-39 of that. The same call gives the same bits. */
 int daric_attend_workspace(const daric_tensor* layer, int page_first, const daric_tensor* q,
                            const daric_sequence* sequences, int64_t n_sequences, int64_t* bytes);
 int daric_attend_pages(const daric_tensor* layer, int page_first, const daric_tensor* block_table,

@@ -128,3 +128,42 @@ def test_lse_of_equal_scores(dev, dtype, rows, ctx):
     _, lse = c.run()
     ref = np.log(ctx + 1.0 + np.arange(rows))[:, None]
     assert (np.abs(lse.double().cpu().numpy() - ref) <= 4 * E * np.maximum(1.0, ref)).all()
+
+
+@pytest.mark.parametrize("dtype,top", [(torch.float16, 2.0 ** 15), (torch.bfloat16, 2.0 ** 17)])
+@pytest.mark.parametrize("rows,d", [(1, 64), (40, 64), (40, 128), (300, 128), (40, 256)])
+def test_huge_scores_an_ulp_apart(dev, dtype, top, rows, d):
+    """Scores of 2^30 and 2^34 that rise token by token by the least that fp32 holds
+    there, far more than a weight's range: whichever of them fp32 tells apart, the output
+    lies between V's smallest and largest value (half a step of it each, for the weights
+    and the result)."""
+    c = Case(dev, [(rows, 700)], dtype=dtype, g=2, h=1, d=d, seed=100)
+    n = rows + 700
+    c.layer[0] = 0
+    c.layer[1] = (1 + torch.rand(c.layer[1].shape, generator=torch.Generator().manual_seed(2))).to(dtype)
+    c.q[:] = 0
+    c.q[..., 0] = top
+    c.q[..., 1] = top * top * 2.0 ** -23 / 8               # times 8 steps: an ulp of top * top
+    c.q[1::3] *= 0.5
+    c.scale = 0.3
+    j = torch.arange(n)
+    page, slot = torch.from_numpy(c.bt[(j // 16).numpy()]).long(), j % 16
+    c.layer[0, page, slot, :, 0] = top
+    c.layer[0, page, slot, :, 1] = ((j // 20) * 8.0).to(dtype)[:, None]
+    out, lse = c.run()
+    assert torch.isfinite(lse).all()
+    u = U[dtype]
+    assert (out >= 1 - 2 * u).all() and (out <= 2 * (1 + 2 * u)).all()
+
+
+@pytest.mark.parametrize("dtype,qtype", [(torch.float16, None), (torch.uint8, torch.float16)])
+@pytest.mark.parametrize("rows,ctx", [(1, 3000), (40, 1000), (300, 700)])
+@pytest.mark.parametrize("nats", [20.5, 21.5, 22.5])
+def test_weights_below_the_normal_range(dev, dtype, qtype, rows, ctx, nats):
+    """Light tokens whose weights are subnormal in fp16, 2^-15.6 to 2^-18.5: they lose
+    bits, not all."""
+    c = Case(dev, [(rows, ctx)], dtype=dtype, qtype=qtype, g=2, h=1, d=64, seed=101)
+    spread(c, nats, 500)
+    out, lse = c.run()
+    check(c, out)
+    assert (out[..., 0] > 0).float().mean() > 0.9
