@@ -69,6 +69,10 @@ class DaricEviction(ctypes.Structure):
                 ("n_first", c_int64), ("n_recent", c_int64)]
 
 
+class DaricBeams(ctypes.Structure):
+    _fields_ = [("bt_offset", c_int64), ("stride", c_int64), ("n_beams", c_int64), ("n_tokens", c_int64)]
+
+
 P = POINTER
 T = P(DaricTensor)
 I64P = c_void_p  # address of an I64 buffer
@@ -113,6 +117,13 @@ SIGNATURES = {
                                    c_uint64]),
     "daric_weigh_tokens": (c_int, [T, c_int, T, T, T, I64P, c_int64, T, c_float, T, T, c_int, c_uint64]),
     "daric_evict_tokens": (c_int, [T, c_int64, c_int, T, T, I64P, c_int64, T, T, c_uint64]),
+    "daric_rotate_rows": (c_int, [T, T, P(DaricRope), c_float, T, c_uint64]),
+    "daric_append_tokens": (c_int, [T, c_int, T, T, T, I64P, c_int64, T, P(DaricRope), c_float, T, T, T, T,
+                                    c_uint64]),
+    "daric_select_workspace": (c_int, [T, c_int64, P(c_int64)]),
+    "daric_select_beams": (c_int, [T, T, T, c_int64, T, T, T, c_void_p, c_int64, c_uint64]),
+    # beams: the address of an int64 [n, 4] array
+    "daric_reorder_beams": (c_int, [T, c_int64, c_int, T, T, I64P, c_int64, c_uint64]),
 }
 
 _lib = None

@@ -31,7 +31,7 @@ HOSTTEST_LIB = os.path.join(LIBDIR, "libdaric_hosttest.so")
 
 SOURCES = ["capi.cpp", "runtime.cpp", "copy_kernels.hip", "rope_kernels.hip", "select_kernels.hip",
            "token_kernels.hip", "noalloc.hip", "attend_bf16.hip", "attend_f16.hip", "attend_e4m3_bf16.hip",
-           "attend_e4m3_f16.hip", "evict_kernels.hip"]
+           "attend_e4m3_f16.hip", "evict_kernels.hip", "append_kernels.hip", "beam_kernels.hip"]
 
 ARCH = "gfx950"
 COMMON = ["-O3", "-std=c++17", "-fPIC", "-Wall", "-Wextra", "-Wshadow", "-Wno-unused-result",

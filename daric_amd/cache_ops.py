@@ -13,7 +13,9 @@ Additions (no reference counterpart; the .pyi grows, nothing changes):
   cache layout), rerotate_pages, kv_deviation, topk_per_chunk, merge_rows,
   select_merge (the three selection calls in one), attend_pages (attention
   over the paged cache), weigh_tokens and evict_tokens (eviction by
-  accumulated attention weight), kernel timing.
+  accumulated attention weight), rotate_rows and append_tokens (new rows, rotated
+  into the cache), select_beams and reorder_beams (beam search over it), kernel
+  timing.
 
 Every call is asynchronous on `stream` (0 = the current torch stream of the
 first layer's device, as in reference copier.cpp:27-30). The wrapper keeps
@@ -38,7 +40,8 @@ from ._lib import I64, DaricChunk, DaricRope, check, desc, load, str_array
 __all__ = [
     "CacheCopier", "batched_memcpy_d2h", "batched_memcpy_h2d", "rerotate_pages",
     "kv_deviation", "topk_per_chunk", "merge_rows", "select_merge", "SELECT_KEYS_READY",
-    "SELECT_ONE_PASS", "attend_pages", "weigh_tokens", "evict_tokens", "timing_enable", "timing_read",
+    "SELECT_ONE_PASS", "attend_pages", "weigh_tokens", "evict_tokens", "rotate_rows", "append_tokens",
+    "select_beams", "reorder_beams", "timing_enable", "timing_read",
 ]
 
 
@@ -605,6 +608,114 @@ def evict_tokens(layers: Sequence[torch.Tensor], page_first: bool, block_table: 
                                     _ref(weights), addr, n, _ref(kept), _ref(work), ctypes.c_uint64(st)))
     _record(st, dev, block_table, weights, both)
     return kept
+
+
+def rotate_rows(rows: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, rotary_dim: int,
+                is_neox_style: bool = True, attention_scale: float = 1.0, out: Optional[torch.Tensor] = None,
+                stream: int = 0) -> torch.Tensor:
+    """Rotary positions of new rows ([T, H, D] bf16, fp16 or fp32: queries, keys, or
+    both heads after heads of a joint projection): pair i of the first rotary_dim values
+    turns by positions[t] * inv_freq[i] (int64 [T]; angles in fp64), cosine and sine
+    times attention_scale; the other values are copied. Pairs are (i, i +
+    rotary_dim / 2), or (2i, 2i + 1) with is_neox_style False. out: `rows` itself, or a
+    contiguous tensor (made if None). Frequencies of scaled models:
+    daric_amd.rotary.rotary_frequencies. Cached rows move by rerotate_pages. No
+    backward pass; the gradient of rows is rotate_rows of out's at -positions."""
+    _no_backward("rotate_rows", rows, inv_freq, out)
+    dev = rows.device
+    st = _resolve_stream(stream, dev)
+    rope = _rope(inv_freq, rotary_dim, is_neox_style, dev)
+    if out is None:
+        with _on_stream(st, dev):
+            out = torch.empty(rows.shape, dtype=rows.dtype, device=dev)
+    check(load().daric_rotate_rows(_ref(rows), _ref(positions), ctypes.byref(rope), float(attention_scale), _ref(out),
+                                   ctypes.c_uint64(st)))
+    _record(st, dev, rows, positions, inv_freq, out)
+    return out
+
+
+def append_tokens(layer: torch.Tensor, page_first: bool, block_table: torch.Tensor, k: torch.Tensor,
+                  v: Optional[torch.Tensor], seqs, inv_freq: Optional[torch.Tensor] = None, rotary_dim: int = 0,
+                  is_neox_style: bool = True, positions: Optional[torch.Tensor] = None, attention_scale: float = 1.0,
+                  q: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None,
+                  k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None,
+                  stream: int = 0) -> Optional[torch.Tensor]:
+    """Writes the rows of k and v ([T, H, D], strides free) into one layer's paged
+    cache, K rotated to its position on the way, and rotates the step's q with it: the
+    call before attend_pages, with the same seqs (bt_offset, row_start, n_rows, n_ctx
+    [, col_start]): row row_start + i becomes token n_ctx + i of the sequence.
+    positions: int64 [T] (None: the token's place, n_ctx + i; after an eviction they
+    differ); inv_freq None: nothing is rotated. rotary_dim, is_neox_style,
+    attention_scale as in rotate_rows. An fp8 (e4m3) cache takes bf16 or fp16 rows as
+    sat_rtne(x / scale) with its [H] fp32 k_scale / v_scale (None: 1). Tokens in pages
+    of id 0 are not written, nor is anything of rows of no sequence. Returns
+    q_out (q itself, or a contiguous tensor, made if None), or None without q. No
+    backward pass, as attend_pages."""
+    _no_backward("append_tokens", layer, k, v, q, q_out, inv_freq, k_scale, v_scale)
+    dev = layer.device
+    st = _resolve_stream(stream, dev)
+    addr, n, _keep = _sequences(seqs)
+    rope = _rope(inv_freq, rotary_dim, is_neox_style, dev) if inv_freq is not None else None
+    if q is not None and q_out is None:
+        with _on_stream(st, dev):
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    check(load().daric_append_tokens(_layer_desc(layer), 1 if page_first else 0, _ref(block_table), _ref(k), _ref(v),
+                                     addr, n, _ref(positions), ctypes.byref(rope) if rope is not None else None,
+                                     float(attention_scale), _ref(q), _ref(q_out) if q is not None else None,
+                                     _ref(k_scale), _ref(v_scale), ctypes.c_uint64(st)))
+    _record(st, dev, block_table, k, v, positions, inv_freq, q, q_out, k_scale, v_scale)
+    return q_out if q is not None else None
+
+
+def select_beams(logits: torch.Tensor, scores: torch.Tensor, k: Optional[int] = None,
+                 ended: Optional[torch.Tensor] = None, end_token: int = -1,
+                 stream: int = 0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The k best continuations (W if None, at most 64) of each request's W beams:
+    (scores [B, k] fp32, parents [B, k] int32, tokens [B, k] int32), best first. A
+    candidate's score is scores[b, w] + log_softmax(logits[b, w])[v] (logits: [B, W, V]
+    bf16, fp16 or fp32; scores: fp32), compared in 64 bits, ties to the lower beam,
+    then the lower token. Beams that `ended` (bool [B, W]) offer end_token alone, at
+    their own score. Candidates of score -inf or NaN are not there: score -inf, parent
+    and token -1 fill the places left. No backward pass, as attend_pages."""
+    _no_backward("select_beams", logits, scores)
+    dev = logits.device
+    st = _resolve_stream(stream, dev)
+    if k is None:
+        k = logits.shape[1] if logits.dim() == 3 else 1
+    k = int(k)
+    ld = desc(logits)
+    lib, need = load(), ctypes.c_int64()
+    check(lib.daric_select_workspace(ctypes.byref(ld), k, ctypes.byref(need)))
+    B = logits.shape[0]
+    with _on_stream(st, dev):
+        out = torch.empty((B, k), dtype=torch.float32, device=dev)
+        ids = torch.empty((2, B, k), dtype=torch.int32, device=dev)
+        work = torch.empty(need.value, dtype=torch.uint8, device=dev)
+    end = ended.view(torch.uint8) if ended is not None and ended.dtype == torch.bool else ended
+    parents, tokens = ids[0], ids[1]
+    check(lib.daric_select_beams(ctypes.byref(ld), _ref(scores), _ref(end), int(end_token), _ref(out),
+                                 _ref(parents), _ref(tokens), work.data_ptr(), need.value, ctypes.c_uint64(st)))
+    _record(st, dev, logits, scores, end, out, ids, work)
+    return out, parents, tokens
+
+
+def reorder_beams(layers: Sequence[torch.Tensor], page_first: bool, block_table: torch.Tensor,
+                  parents: torch.Tensor, beams, stream: int = 0) -> None:
+    """Beam w of request i goes on from beam parents[i, w] (int32 [n, columns], -1: it
+    stays), in place and without the host: beams holds (bt_offset, stride, n_beams,
+    n_tokens) per request, beam w's block list beginning at block_table[bt_offset +
+    w * stride]. The ids of its full pages become its parent's, and its last, partly
+    filled page, which no other list may hold there, takes the rows of the parent's, in
+    every layer at once. Up to 32 beams of a request; caches of any type and
+    layout."""
+    layers = list(layers)
+    _no_backward("reorder_beams", *layers)
+    dev = layers[0].device
+    st = _resolve_stream(stream, dev)
+    addr, n, _keep = _tuples(beams, (4,), "beams must be (bt_offset, stride, n_beams, n_tokens) entries of ints")
+    check(load().daric_reorder_beams(_layer_array(layers), len(layers), 1 if page_first else 0, _ref(block_table),
+                                     _ref(parents), addr, n, ctypes.c_uint64(st)))
+    _record(st, dev, block_table, parents)
 
 
 def timing_enable(enable: bool = True) -> None:

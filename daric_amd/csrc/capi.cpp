@@ -14,7 +14,9 @@
 
 #include <cmath>
 
+#include "append.h"
 #include "attend.h"
+#include "beams.h"
 #include "common.h"
 #include "elem.h"
 #include "kernels.h"
@@ -2022,6 +2024,499 @@ int daric_evict_tokens(const daric_tensor* layers, int64_t n_layers, int page_fi
                      static_cast<int>(most), static_cast<int>(slots), static_cast<int>(chosen),
                      static_cast<int32_t*>(workspace->data),
                      static_cast<int32_t*>(kept->data), static_cast<int>(width), st);
+    });
+}
+
+}  // extern "C"
+
+// ================================================== new rows and beam search
+namespace {
+
+constexpr int64_t kMaxRowValues = 1ll << 24;       // of a token's heads of one tensor
+
+int row_kind(const daric_tensor& t) {
+    return t.dtype == DARIC_DTYPE_FLOAT32 ? kF32 : t.dtype == DARIC_DTYPE_BFLOAT16 ? kBF16
+         : t.dtype == DARIC_DTYPE_FLOAT16 ? kF16 : -1;
+}
+
+// A [T, H, D] tensor of rows whose heads' values are contiguous.
+HeadRows check_head_rows(const daric_tensor* x, const char* what) {
+    check_tensor_struct(x, what);
+    DARIC_CHECK(x->device >= 0, what, " must be on CUDA");
+    DARIC_CHECK(x->ndim == 3 && x->sizes[1] > 0 && x->sizes[2] > 0 && (x->strides[2] == 1 || x->sizes[2] == 1), what,
+                " must be [T, H, D] with the values of a head contiguous");
+    DARIC_CHECK(x->strides[0] >= 0 && x->strides[1] >= 0, what, " must not have negative strides");
+    DARIC_CHECK(x->sizes[0] <= kMaxTokens && x->sizes[1] <= kMaxRowValues && x->sizes[2] <= kMaxRowValues &&
+                x->sizes[1] * x->sizes[2] <= kMaxRowValues, what, " is too large");
+    return {static_cast<const uint8_t*>(x->data), x->strides[0], x->strides[1]};
+}
+
+// Heads of one value have no pairs: the cache's geometry is not defined for them.
+void check_head_dim(const daric_tensor& t, const char* what) {
+    const int64_t D = t.ndim >= 3 ? t.sizes[t.ndim - 1] / (t.ndim == 4 ? 2 : 1) : 2;
+    DARIC_CHECK(D >= 2, what, " takes head_dim from 2 on, got ", D);
+}
+
+// No two elements of x share memory.
+bool elements_apart(const daric_tensor& x) {
+    std::vector<std::pair<int64_t, int64_t>> d;      // (stride, size)
+    for (int i = 0; i < x.ndim; ++i)
+        if (x.sizes[i] > 1) d.emplace_back(x.strides[i], x.sizes[i]);
+    std::sort(d.begin(), d.end());
+    int64_t extent = 1;
+    for (const auto& [stride, size] : d) {
+        if (stride < extent) return false;
+        extent += (size - 1) * stride;
+    }
+    return true;
+}
+
+// a's and b's rows lie beside each other in the same larger rows (parts of a joint
+// projection), so that their spans overlap and their elements do not.
+bool beside(const daric_tensor& a, const daric_tensor& b) {
+    const int64_t s = a.strides[0];
+    if (s <= 0 || b.strides[0] != s || a.elem_size != b.elem_size) return false;
+    const auto extent = [](const daric_tensor& t) {
+        int64_t e = 1;
+        for (int i = 1; i < t.ndim; ++i) e += (t.sizes[i] - 1) * t.strides[i];
+        return e;
+    };
+    const int64_t bytes = static_cast<const uint8_t*>(b.data) - static_cast<const uint8_t*>(a.data);
+    if (bytes % a.elem_size != 0) return false;
+    int64_t off = bytes / a.elem_size % s;
+    if (off < 0) off += s;
+    return extent(a) <= off && off + extent(b) <= s;
+}
+
+bool same_view(const daric_tensor& a, const daric_tensor& b) {
+    bool same = a.data == b.data && a.ndim == b.ndim && a.dtype == b.dtype;
+    for (int i = 0; same && i < a.ndim; ++i) same = a.sizes[i] == b.sizes[i] && (a.strides[i] == b.strides[i] || a.sizes[i] <= 1);
+    return same;
+}
+
+// `out` of rows x: x itself, or a contiguous tensor of its shape and type.
+bool check_rows_out(const daric_tensor& x, const daric_tensor* out, const char* what, const char* of) {
+    check_tensor_struct(out, what);
+    if (same_view(x, *out)) {
+        DARIC_CHECK(elements_apart(x), what, " must not be ", of, " where its elements share memory");
+        return true;
+    }
+    bool same = out->device == x.device && out->dtype == x.dtype && out->ndim == 3 && is_contiguous(*out);
+    for (int i = 0; same && i < 3; ++i) same = out->sizes[i] == x.sizes[i];
+    DARIC_CHECK(same, what, " must be ", of, " itself or a contiguous tensor of its shape and type on its device");
+    return false;
+}
+
+const int64_t* check_positions(const daric_tensor* p, int device, int64_t T) {
+    check_tensor_struct(p, "positions");
+    DARIC_CHECK(p->device == device && p->dtype == DARIC_DTYPE_INT64 && p->ndim == 1 && p->sizes[0] == T &&
+                is_contiguous(*p), "positions must be a contiguous int64 [T] tensor on the rows' device");
+    return static_cast<const int64_t*>(p->data);
+}
+
+// The rotation of an AppendArgs.
+void set_rotation(AppendArgs& a, const daric_rope* rope, float m) {
+    if (rope != nullptr) {
+        check_rope(rope);
+        DARIC_CHECK(rope->rotary_dim <= a.D, "rotary_dim must be positive, even and no greater than head_dim (", a.D,
+                    "), got ", rope->rotary_dim);
+        DARIC_CHECK(std::isfinite(m), "attention_scale must be finite");
+        a.inv_freq = rope->inv_freq;
+        a.R = rope->rotary_dim;
+        a.is_neox = rope->is_neox != 0 ? 1 : 0;
+    }
+    a.m = m;
+}
+
+// Rows of a workgroup: as many as have their angles computed in one round of its
+// lanes and the rest of a few, but no more than leave the chip full.
+constexpr int64_t kAppendGroups = 1024;
+int64_t append_tile(int64_t rows, int R) {
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(8, 512 / std::max(R, 64)));
+    int64_t tile = 1;
+    while (tile < most && rows / (2 * tile) >= kAppendGroups) tile *= 2;
+    return tile;
+}
+
+// Finishes the arguments and launches over the sequences.
+void append(AppendArgs& a, std::vector<AppendSeq>& seqs, int from, int to, int device, int64_t rows, hipStream_t stream) {
+    const int es = from == kF32 ? 4 : 2, ces = to == kE4M3 ? 1 : es;
+    int vec = append_vec(a.R / 2, a.D - a.R, 16 / es);
+    const auto whole = [&](const void* p, int64_t row, int64_t head, int size) {
+        return aligned(p, vec * size) && row % vec == 0 && head % vec == 0;
+    };
+    const auto fits = [&] {
+        bool ok = true;
+        if (a.Hq > 0) ok = ok && whole(a.q.data, a.q.row, a.q.head, es) && whole(a.q_out, a.out_row, a.out_head, es);
+        if (a.g.H > 0) {
+            ok = ok && whole(a.k.data, a.k.row, a.k.head, es) && whole(a.layer, a.g.ss, a.g.sh, ces) && a.g.sb % vec == 0;
+            if (a.g.v_off >= 0) ok = ok && whole(a.v.data, a.v.row, a.v.head, es) && a.g.v_off % vec == 0;
+        }
+        return ok;
+    };
+    while (vec > 1 && !fits()) vec /= 2;
+    const int rest = (a.D - a.R) / vec;
+    a.rot_items = a.R / 2 / vec + (rest + 1) / 2;
+    a.copy_items = (a.D / vec + 1) / 2;
+    a.q_end = a.Hq * a.rot_items;
+    a.k_end = a.q_end + a.g.H * a.rot_items;
+    const int64_t per = a.k_end + (a.g.v_off >= 0 ? static_cast<int64_t>(a.g.H) * a.copy_items : 0);
+    a.d_token = FastDiv(static_cast<uint32_t>(per));
+    a.d_rot = FastDiv(static_cast<uint32_t>(a.rot_items));
+    a.d_copy = FastDiv(static_cast<uint32_t>(a.copy_items));
+    a.d_half = FastDiv(static_cast<uint32_t>(std::max(1, a.R / 2)));
+    const int64_t tile = append_tile(rows, a.R);
+    int64_t tiles = 0;
+    a.one_tile = 1;
+    for (AppendSeq& s : seqs) {
+        s.tile_begin = static_cast<int32_t>(tiles);
+        tiles += (s.n_rows + tile - 1) / tile;
+        if (s.n_rows > tile) a.one_tile = 0;
+        DARIC_CHECK(tiles <= kMaxTiles, "too many rows in one call");
+    }
+    a.tile = static_cast<int32_t>(tile);
+    a.n_seqs = static_cast<int32_t>(seqs.size());
+    DeviceGuard guard(device);
+    const size_t bytes = seqs.size() * sizeof(AppendSeq);
+    DescHandOver ho(device, seqs.data(), bytes, stream, a.one_tile != 0 && bytes <= 16 * 1024);
+    launch_append(ho.arg(), a, from, to, vec, tiles, stream);
+}
+
+}  // namespace
+
+extern "C" {
+
+int daric_rotate_rows(const daric_tensor* rows, const daric_tensor* positions, const daric_rope* rope,
+                      float attention_scale, daric_tensor* out, uint64_t stream) {
+    return guarded([&] {
+        AppendArgs a{};
+        a.q = check_head_rows(rows, "rows");
+        const int kind = row_kind(*rows);
+        DARIC_CHECK(kind >= 0, "rows must be bfloat16, float16 or float32");
+        a.Hq = static_cast<int32_t>(rows->sizes[1]);
+        a.D = static_cast<int32_t>(rows->sizes[2]);
+        const int64_t T = rows->sizes[0];
+        a.positions = check_positions(positions, rows->device, T);
+        DARIC_CHECK(rope != nullptr, "rope parameters must not be null");
+        set_rotation(a, rope, attention_scale);
+        a.in_place = check_rows_out(*rows, out, "out", "rows") ? 1 : 0;
+        a.q_out = static_cast<uint8_t*>(out->data);
+        a.out_row = out->strides[0];
+        a.out_head = out->strides[1];
+        a.g.v_off = -1;
+        if (T == 0) return;
+        const Span freq(rope->inv_freq, rope->rotary_dim / 2 * 4, "inv_freq");
+        if (a.in_place) check_written({{out, "out"}}, {{positions, "positions"}, freq});
+        else check_written({{out, "out"}}, {{rows, "rows"}, {positions, "positions"}, freq});
+        AppendSeq s{};
+        s.n_rows = static_cast<int32_t>(T);
+        std::vector<AppendSeq> seqs{s};
+        append(a, seqs, kind, kind, rows->device, T, as_stream(stream));
+    });
+}
+
+int daric_append_tokens(const daric_tensor* layer, int page_first, const daric_tensor* block_table,
+                        const daric_tensor* k, const daric_tensor* v, const daric_sequence* sequences,
+                        int64_t n, const daric_tensor* positions, const daric_rope* rope, float attention_scale,
+                        const daric_tensor* q, daric_tensor* q_out, const daric_tensor* k_scale,
+                        const daric_tensor* v_scale, uint64_t stream) {
+    return guarded([&] {
+        check_tensor_struct(layer, "kv layer");
+        const daric_tensor& t = *layer;
+        DARIC_CHECK(t.device >= 0, "KV cache tensor must be on CUDA");
+        const int ck = elem_kind(t);
+        DARIC_CHECK(ck >= 0, "unsupported KV cache dtype for append_tokens");
+        AppendArgs a{};
+        check_head_dim(t, "append_tokens");
+        a.g = kv_geom(t, page_first != 0);
+        const KVGeom& g = a.g;
+        DARIC_CHECK(g.H > 0 && g.PS > 0 && g.num_blocks > 0, "KV cache must not be empty");
+        a.layer = static_cast<uint8_t*>(t.data);
+        a.D = g.D;
+        check_block_table(block_table, t.device);
+        a.block_table = static_cast<const int32_t*>(block_table->data);
+        const int64_t bt_n = numel(*block_table);
+
+        a.k = check_head_rows(k, "k");
+        const int from = k->dtype == DARIC_DTYPE_FLOAT32 ? -1 : row_kind(*k);
+        DARIC_CHECK(from >= 0 && (ck == kE4M3 || ck == from),
+                    "k must have the cache's element type, or be bfloat16 or float16 for an fp8 (e4m3) cache");
+        const int64_t T = k->sizes[0];
+        const auto like_cache = [&](const daric_tensor* x, const char* what) {
+            DARIC_CHECK(x->device == t.device && x->dtype == k->dtype && x->sizes[0] == T && x->sizes[1] == g.H &&
+                        x->sizes[2] == g.D, what, " must be [T, ", g.H, ", ", g.D,
+                        "] rows of k's type on the layer's device");
+        };
+        like_cache(k, "k");
+        if (g.v_off >= 0) {
+            a.v = check_head_rows(v, "v");
+            like_cache(v, "v");
+        } else {
+            DARIC_CHECK(v == nullptr || v->data == nullptr, "a 3-D (MLA) cache has no V rows: v must be None");
+        }
+        const bool has_q = q != nullptr && q->ndim > 0;
+        if (has_q) {
+            DARIC_CHECK(rope != nullptr, "q needs inv_freq: it is rotated only");
+            a.q = check_head_rows(q, "q");
+            DARIC_CHECK(q->device == t.device && q->dtype == k->dtype && q->sizes[0] == T && q->sizes[2] == g.D,
+                        "q must be [T, Hq, ", g.D, "] rows of k's type on the layer's device");
+            a.Hq = static_cast<int32_t>(q->sizes[1]);
+            a.in_place = check_rows_out(*q, q_out, "q_out", "q") ? 1 : 0;
+            a.q_out = static_cast<uint8_t*>(q_out->data);
+            a.out_row = q_out->strides[0];
+            a.out_head = q_out->strides[1];
+        }
+        set_rotation(a, rope, attention_scale);
+        if (positions != nullptr) a.positions = check_positions(positions, t.device, T);
+        const auto scales = [&](const daric_tensor* s, const char* what) -> const float* {
+            if (s == nullptr || s->data == nullptr) return nullptr;
+            check_tensor_struct(s, what);
+            DARIC_CHECK(ck == kE4M3, what, " applies to fp8 (e4m3) caches only");
+            DARIC_CHECK(s->device == t.device && s->dtype == DARIC_DTYPE_FLOAT32 && is_contiguous(*s) &&
+                        numel(*s) == g.H, what, " must be a contiguous float32 [H] tensor on the layer's device");
+            return static_cast<const float*>(s->data);
+        };
+        a.k_scale = scales(k_scale, "k_scale");
+        a.v_scale = scales(v_scale, "v_scale");
+
+        DARIC_CHECK(n >= 0 && (n == 0 || sequences != nullptr), "sequences must not be null");
+        std::vector<AppendSeq> seqs;
+        std::vector<std::pair<int64_t, int64_t>> rows;
+        seqs.reserve(n);
+        rows.reserve(n);
+        int64_t total = 0;
+        for (int64_t i = 0; i < n; ++i) {
+            const daric_sequence& s = sequences[i];
+            DARIC_CHECK(s.bt_offset >= 0 && s.row_start >= 0 && s.n_rows >= 0 && s.n_ctx >= 0 && s.col_start >= 0,
+                        "negative field of sequence ", i);
+            DARIC_CHECK(s.n_ctx <= kMaxTokens && s.n_rows <= kMaxTokens && s.n_ctx + s.n_rows <= kMaxTokens,
+                        "sequence ", i, " is too long");
+            DARIC_CHECK(s.row_start <= T && s.n_rows <= T - s.row_start, "sequence ", i, " rows exceed k");
+            const int64_t pages = (s.n_ctx + s.n_rows + g.PS - 1) / g.PS;
+            DARIC_CHECK(s.bt_offset <= bt_n && pages <= bt_n - s.bt_offset, "sequence ", i,
+                        " reaches past the end of block_table");
+            if (s.n_rows == 0) continue;      // nothing to append
+            rows.emplace_back(s.row_start, s.n_rows);
+            AppendSeq x{};
+            x.bt_offset = s.bt_offset;
+            x.row0 = static_cast<int32_t>(s.row_start);
+            x.n_rows = static_cast<int32_t>(s.n_rows);
+            x.n_ctx = static_cast<int32_t>(s.n_ctx);
+            seqs.push_back(x);
+            total += s.n_rows;
+        }
+        check_apart(rows, "row");
+        if (seqs.empty()) return;
+        const Span freq(rope != nullptr ? rope->inv_freq : nullptr, a.R / 2 * 4, "inv_freq");
+        const Span table(block_table, "block_table"), at(positions, "positions"), ks(k_scale, "k_scale"),
+            vs(v_scale, "v_scale"), kr(k, "k"), vr(g.v_off >= 0 ? v : nullptr, "v");
+        const Span out(has_q ? q_out : nullptr, "q_out");
+        check_written({{layer, "the layer"}, out}, {table, at, ks, vs, freq});
+        check_written({{layer, "the layer"}}, {kr, vr, {has_q ? q : nullptr, "q"}});
+        if (has_q) {
+            if (!a.in_place) check_written({out}, {{q, "q"}});
+            if (!beside(*q_out, *k)) check_written({out}, {kr});
+            if (g.v_off >= 0 && !beside(*q_out, *v)) check_written({out}, {vr});
+        }
+        append(a, seqs, from, ck == kE4M3 ? kE4M3 : from, t.device, total, as_stream(stream));
+    });
+}
+
+}  // extern "C"
+
+namespace {
+
+// Registers of a split's lane: 16 where splits of 64 would leave half the chip's wavefronts
+// idle.
+int select_regs(int64_t B, int64_t W, int64_t V, int es) {
+    const int64_t big = split_values(64, es), small = split_values(16, es);
+    const bool few = B * W * ((V + big - 1) / big) < 512;
+    return few && W * ((V + small - 1) / small) <= 4096 ? 16 : 64;
+}
+
+struct SelectCall {
+    SelectArgs a{};
+    int kind = -1, regs = 64, device = -1;
+    int64_t units() const { return static_cast<int64_t>(a.B) * a.W * a.splits; }
+    int64_t list_bytes() const { return units() * a.k * static_cast<int64_t>(sizeof(BeamCandidate)); }
+    int64_t bytes() const { return list_bytes() + units() * 2 * static_cast<int64_t>(sizeof(float)); }
+};
+
+SelectCall select_call(const daric_tensor* logits, int64_t k) {
+    SelectCall c;
+    check_tensor_struct(logits, "logits");
+    DARIC_CHECK(logits->device >= 0, "logits must be on CUDA");
+    c.device = logits->device;
+    c.kind = row_kind(*logits);
+    DARIC_CHECK(c.kind >= 0, "logits must be bfloat16, float16 or float32");
+    DARIC_CHECK(logits->ndim == 3 && logits->sizes[1] > 0 && logits->sizes[2] > 0 &&
+                (logits->strides[2] == 1 || logits->sizes[2] == 1) && logits->strides[0] >= 0 && logits->strides[1] >= 0,
+                "logits must be [requests, beams, vocabulary] with contiguous rows");
+    const int64_t B = logits->sizes[0], W = logits->sizes[1], V = logits->sizes[2];
+    DARIC_CHECK(W <= kMaxBeams, "select_beams takes up to ", kMaxBeams, " beams of a request, got ", W);
+    DARIC_CHECK(k >= 1 && k <= kMaxCandidates, "select_beams chooses 1 to ", kMaxCandidates, " candidates, got ", k);
+    DARIC_CHECK(V <= kMaxTokens, "the vocabulary is too large");
+    c.regs = select_regs(B, W, V, logits->elem_size);
+    const int64_t per = split_values(c.regs, logits->elem_size);
+    const int64_t splits = (V + per - 1) / per;
+    DARIC_CHECK(W * splits <= 32768, "the vocabulary is too large for ", W, " beams");
+    DARIC_CHECK(B * W * splits <= kMaxTiles && B <= kMaxTiles, "too many rows in one select_beams call");
+    SelectArgs& a = c.a;
+    a.logits = static_cast<const uint8_t*>(logits->data);
+    a.batch = logits->strides[0];
+    a.row = logits->strides[1];
+    a.B = static_cast<int32_t>(B);
+    a.W = static_cast<int32_t>(W);
+    a.V = V;
+    a.k = static_cast<int32_t>(k);
+    a.splits = static_cast<int32_t>(splits);
+    return c;
+}
+
+}  // namespace
+
+extern "C" {
+
+int daric_select_workspace(const daric_tensor* logits, int64_t k, int64_t* bytes) {
+    return guarded([&] {
+        DARIC_CHECK(bytes != nullptr, "bytes must not be null");
+        *bytes = select_call(logits, k).bytes();
+    });
+}
+
+int daric_select_beams(const daric_tensor* logits, const daric_tensor* scores, const daric_tensor* ended,
+                       int64_t end_token, daric_tensor* out_scores, daric_tensor* parents, daric_tensor* tokens,
+                       void* workspace, int64_t workspace_bytes, uint64_t stream) {
+    return guarded([&] {
+        check_tensor_struct(parents, "parents");
+        DARIC_CHECK(parents->ndim == 2, "parents must be [requests, k]");
+        SelectCall c = select_call(logits, parents->sizes[1]);
+        SelectArgs& a = c.a;
+        const auto check_out = [&](const daric_tensor* x, int dtype, const char* what) {
+            check_tensor_struct(x, what);
+            DARIC_CHECK(x->device == c.device && x->dtype == dtype && x->ndim == 2 && x->sizes[0] == a.B &&
+                        x->sizes[1] == a.k && is_contiguous(*x), what, " must be a contiguous ",
+                        dtype == DARIC_DTYPE_INT32 ? "int32" : "float32", " [requests, k] tensor on the logits' device");
+        };
+        check_out(out_scores, DARIC_DTYPE_FLOAT32, "out_scores");
+        check_out(parents, DARIC_DTYPE_INT32, "parents");
+        check_out(tokens, DARIC_DTYPE_INT32, "tokens");
+        check_tensor_struct(scores, "scores");
+        DARIC_CHECK(scores->device == c.device && scores->dtype == DARIC_DTYPE_FLOAT32 && scores->ndim == 2 &&
+                    scores->sizes[0] == a.B && scores->sizes[1] == a.W && is_contiguous(*scores),
+                    "scores must be a contiguous float32 [requests, beams] tensor on the logits' device");
+        a.scores = static_cast<const float*>(scores->data);
+        if (ended != nullptr && ended->ndim > 0) {
+            check_tensor_struct(ended, "ended");
+            DARIC_CHECK(ended->device == c.device && ended->elem_size == 1 && ended->dtype == DARIC_DTYPE_UINT8 &&
+                        ended->ndim == 2 && ended->sizes[0] == a.B && ended->sizes[1] == a.W && is_contiguous(*ended),
+                        "ended must be a contiguous bool [requests, beams] tensor on the logits' device");
+            DARIC_CHECK(end_token >= 0 && end_token < a.V, "end_token must be in the vocabulary, got ", end_token);
+            a.ended = static_cast<const uint8_t*>(ended->data);
+            a.end_token = static_cast<int32_t>(end_token);
+        }
+        if (a.B == 0) return;
+        const int64_t need = c.bytes();
+        DARIC_CHECK(workspace != nullptr && workspace_bytes >= need && aligned(workspace, 16),
+                    "workspace must be 16-byte aligned and hold ", need, " bytes, got ", workspace_bytes);
+        check_written({{out_scores, "out_scores"}, {parents, "parents"}, {tokens, "tokens"}, {workspace, need, "workspace"}},
+                      {{logits, "logits"}, {scores, "scores"}, {a.ended != nullptr ? ended : nullptr, "ended"}});
+        a.out_scores = static_cast<float*>(out_scores->data);
+        a.parents = static_cast<int32_t*>(parents->data);
+        a.tokens = static_cast<int32_t*>(tokens->data);
+        a.part = static_cast<BeamCandidate*>(workspace);
+        a.part_ms = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + c.list_bytes());
+        DeviceGuard guard(c.device);
+        launch_select_beams(a, c.kind, c.regs, as_stream(stream));
+    });
+}
+
+int daric_reorder_beams(const daric_tensor* layers, int64_t n_layers, int page_first, daric_tensor* block_table,
+                        const daric_tensor* parents, const daric_beams* beams, int64_t n, uint64_t stream) {
+    return guarded([&] {
+        DARIC_CHECK(n_layers > 0 && layers != nullptr, "layers must not be empty");
+        for (int64_t i = 0; i < n_layers; ++i) check_tensor_struct(&layers[i], "kv layer");
+        check_same_layers(layers, n_layers);
+        const daric_tensor& t = layers[0];
+        DARIC_CHECK(t.device >= 0, "KV cache tensor must be on CUDA");
+        check_head_dim(t, "reorder_beams");
+        const KVGeom g = kv_geom(t, page_first != 0);
+        DARIC_CHECK(g.H > 0 && g.PS > 0 && g.num_blocks > 0, "KV cache must not be empty");
+        check_block_table(block_table, t.device);
+        const int64_t bt_n = numel(*block_table);
+        DARIC_CHECK(n >= 0 && (n == 0 || beams != nullptr), "beams must not be null");
+        check_tensor_struct(parents, "parents");
+        DARIC_CHECK(parents->device == t.device && parents->dtype == DARIC_DTYPE_INT32 && parents->ndim == 2 &&
+                    parents->sizes[0] == n && (parents->strides[1] == 1 || parents->sizes[1] <= 1) &&
+                    parents->strides[0] >= 0,
+                    "parents must be an int32 [requests, beams] tensor with contiguous rows on the layers' device");
+        int64_t unit = 16;
+        const int64_t es = t.elem_size;
+        const auto allows = [&](int64_t u) {
+            bool ok = (g.D * es) % u == 0 && (g.sb * es) % u == 0 && (g.ss * es) % u == 0 && (g.sh * es) % u == 0 &&
+                      (g.v_off < 0 || (g.v_off * es) % u == 0);
+            for (int64_t i = 0; ok && i < n_layers; ++i) ok = aligned(layers[i].data, u);
+            return ok;
+        };
+        while (unit > 1 && !allows(unit)) unit /= 2;
+        const int64_t token_units = (g.v_off >= 0 ? 2 : 1) * g.H * (g.D * es / unit);
+        DARIC_CHECK(token_units <= kIntMax / g.PS / 2, "a page of the cache is too large for reorder_beams");
+        std::vector<BeamLists> lists;
+        std::vector<std::pair<int64_t, int64_t>> ranges;
+        lists.reserve(n);
+        int64_t most_beams = 0, most_pages = 0, tiles = 0;
+        for (int64_t i = 0; i < n; ++i) {
+            const daric_beams& s = beams[i];
+            DARIC_CHECK(s.bt_offset >= 0 && s.stride >= 0 && s.n_beams >= 0 && s.n_tokens >= 0,
+                        "negative field of request ", i);
+            DARIC_CHECK(s.n_beams <= kReorderBeams, "reorder_beams takes up to ", kReorderBeams, " beams of a request, got ",
+                        s.n_beams);
+            DARIC_CHECK(s.n_beams <= parents->sizes[1], "request ", i, " has more beams than parents has columns");
+            DARIC_CHECK(s.n_tokens <= kMaxTokens, "request ", i, " is too long");
+            const int64_t pages = (s.n_tokens + g.PS - 1) / g.PS;
+            DARIC_CHECK(s.n_beams <= 1 || s.stride >= pages, "request ", i, ": the block lists of its beams overlap");
+            BeamLists x{};
+            x.bt_offset = s.bt_offset;
+            x.stride = s.stride;
+            x.n_beams = static_cast<int32_t>(s.n_beams);
+            x.n_tokens = static_cast<int32_t>(s.n_tokens);
+            x.tile_begin = static_cast<int32_t>(tiles);
+            if (s.n_beams > 0 && pages > 0) {
+                const int64_t rest = bt_n - s.bt_offset - pages;
+                DARIC_CHECK(s.bt_offset <= bt_n && rest >= 0 && (s.n_beams == 1 || s.stride <= rest / (s.n_beams - 1)),
+                            "request ", i, " reaches past the end of block_table");
+                ranges.emplace_back(s.bt_offset, (s.n_beams - 1) * s.stride + pages);
+            }
+            if (s.n_beams > 1) {
+                tiles += (s.n_tokens % g.PS * token_units + kReorderThreads - 1) / kReorderThreads;
+                most_pages = std::max(most_pages, s.n_tokens / g.PS);
+                most_beams = std::max(most_beams, s.n_beams);
+                DARIC_CHECK(tiles <= kMaxTiles, "too many rows in one reorder_beams call");
+            }
+            lists.push_back(x);
+        }
+        check_apart(ranges, "block list");
+        if (tiles == 0 && most_pages == 0) return;
+        DARIC_CHECK(n <= 65535, "too many requests in one reorder_beams call");
+        std::vector<const void*> data;
+        for (int64_t i = 0; i < n_layers; ++i) data.push_back(layers[i].data);
+        std::sort(data.begin(), data.end());
+        DARIC_CHECK(std::adjacent_find(data.begin(), data.end()) == data.end(), "a layer is given twice");
+        check_written({{block_table, "block_table"}}, {{parents, "parents"}});
+        for (int64_t i = 0; i < n_layers; ++i)
+            check_written({{&layers[i], "a layer"}}, {{block_table, "block_table"}, {parents, "parents"}});
+        DeviceGuard guard(t.device);
+        const hipStream_t st = as_stream(stream);
+        const size_t cb = lists.size() * sizeof(BeamLists);
+        std::vector<uint8_t> blob(cb + n_layers * sizeof(uint8_t*));
+        std::memcpy(blob.data(), lists.data(), cb);
+        const auto ptrs = layer_ptrs(layers, n_layers);
+        std::memcpy(blob.data() + cb, ptrs.data(), n_layers * sizeof(uint8_t*));
+        DescHandOver ho(t.device, blob.data(), blob.size(), st);
+        launch_reorder(ho.arg(), static_cast<int>(cb), static_cast<int>(n_layers), g, static_cast<int>(es),
+                       static_cast<int>(unit), static_cast<int32_t*>(block_table->data),
+                       static_cast<const int32_t*>(parents->data), parents->strides[0], static_cast<int>(n),
+                       static_cast<int>(most_beams), most_pages, tiles, st);
     });
 }
 

@@ -7,13 +7,17 @@ signatures; the rest are additions.
 """
 from daric_amd.cache_ops import (  # noqa: F401
     CacheCopier,
+    append_tokens,
     attend_pages,
     batched_memcpy_d2h,
     batched_memcpy_h2d,
     evict_tokens,
     kv_deviation,
     merge_rows,
+    reorder_beams,
     rerotate_pages,
+    rotate_rows,
+    select_beams,
     select_merge,
     timing_enable,
     timing_read,

@@ -483,6 +483,88 @@ int daric_evict_tokens(const daric_tensor* layers, int64_t n_layers, int page_fi
                        const daric_eviction* evictions, int64_t n_evictions, daric_tensor* kept,
                        daric_tensor* workspace, uint64_t stream);
 
+/* ---------------------------------------------------------------------- */
+/* New rows of a step: rotary positions and the append to the paged cache   */
+/* (new entry points; the reference leaves both to vLLM).                   */
+/* ---------------------------------------------------------------------- */
+
+/* out[r, h] = rows[r, h] with pair i of its first rotary_dim values turned by the
+ * angle positions[r] * inv_freq[i]: (x1, x2) -> (x1 c - x2 s, x2 c + x1 s), c and s
+ * its cosine and sine times attention_scale (finite; 1 but for scaled tables). The
+ * other values are copied. Angles are computed and reduced in fp64, the rotation in
+ * fp32, rounded once.
+ * rows: [T, H, D] bfloat16, float16 or float32, the values of a head contiguous, other
+ * strides free (not negative). positions: contiguous int64 [T] on the device, any
+ * sign. out: rows itself (whose elements then share no memory), or a contiguous tensor
+ * of its shape and type that overlaps nothing that the call reads. */
+int daric_rotate_rows(const daric_tensor* rows, const daric_tensor* positions, const daric_rope* rope,
+                      float attention_scale, daric_tensor* out, uint64_t stream);
+
+/* Writes row i of each sequence's rows into the cache as its token n_ctx + i: page
+ * block_table[bt_offset + (n_ctx + i) / PS], slot (n_ctx + i) % PS, K rotated as by
+ * daric_rotate_rows to positions[row] (NULL: to n_ctx + i; rope NULL: not rotated), V as
+ * it is; and q rotated alike into q_out. Sequences as in daric_attend_pages, which reads
+ * what this call writes (col_start is not used). A token whose page id is 0 or outside
+ * [1, num_blocks) is not written. Rows of no sequence: nothing of them is written, their
+ * row of q_out included. No row may be in two sequences, and no slot may be
+ * written by two rows.
+ * layer: one paged cache, bfloat16, float16 or e4m3, head_dim from 2 on. k, v: [T, H, D] rows of its type, or
+ * bfloat16 or float16 for an e4m3 cache, strides as daric_rotate_rows' rows; v is NULL for
+ * a 3-D (MLA) cache, whose rows are k's one head. An e4m3 cache takes the saturating
+ * round-to-nearest-even code of the rotated fp32 value / scale[h], the quotient
+ * correctly rounded; k_scale, v_scale: NULL (1) or contiguous fp32 [H], for such a cache
+ * only. q: NULL, or [T, Hq, D] rows of k's type; q_out: as daric_rotate_rows' out.
+ * k, v and q may be parts of one joint projection, q_out q in it. */
+int daric_append_tokens(const daric_tensor* layer, int page_first, const daric_tensor* block_table,
+                        const daric_tensor* k, const daric_tensor* v, const daric_sequence* sequences,
+                        int64_t n_sequences, const daric_tensor* positions, const daric_rope* rope,
+                        float attention_scale, const daric_tensor* q, daric_tensor* q_out,
+                        const daric_tensor* k_scale, const daric_tensor* v_scale, uint64_t stream);
+
+/* ---------------------------------------------------------------------- */
+/* Beam search over the paged cache (new entry points).                     */
+/* ---------------------------------------------------------------------- */
+
+/* For each request the k best candidates (beam w, token v), best first: the score of one
+ * is scores[b, w] + logits[b, w, v] - log(sum over the vocabulary of exp(logits[b, w])),
+ * ties go to the lower w, then the lower v. A beam whose `ended` is not 0 offers end_token
+ * alone, at the score scores[b, w]. Candidates whose score is -inf or NaN are not there
+ * (masked logits, beams of score -inf; all of a row that holds +inf or NaN); places
+ * that none is left for get score -inf, parent -1 and token -1.
+ * logits: [B, W, V] bfloat16, float16 or float32, rows contiguous, other strides free
+ * (not negative), W <= 64. scores: contiguous fp32 [B, W]. ended: NULL or contiguous uint8
+ * [B, W]. out_scores (fp32), parents, tokens (int32): contiguous [B, k], 1 <= k <= 64.
+ * workspace: at least the bytes that daric_select_workspace gives, in use until the
+ * call's work on `stream` is done. What is written overlaps neither each other nor what is
+ * read. Sums of exponentials are fp32 over up to 8192 values, joined in fp64, and scores are
+ * compared in fp64; the same call gives the same bits. */
+int daric_select_workspace(const daric_tensor* logits, int64_t k, int64_t* bytes);
+int daric_select_beams(const daric_tensor* logits, const daric_tensor* scores, const daric_tensor* ended,
+                       int64_t end_token, daric_tensor* out_scores, daric_tensor* parents, daric_tensor* tokens,
+                       void* workspace, int64_t workspace_bytes, uint64_t stream);
+
+/* A request's beams: beam w < n_beams holds n_tokens tokens, in the pages of its block
+ * list block_table[bt_offset + w * stride ...]. */
+typedef struct daric_beams {
+    int64_t bt_offset;
+    int64_t stride;
+    int64_t n_beams;
+    int64_t n_tokens;
+} daric_beams;
+
+/* Beam w of request i goes on from beam p = parents[i, w] (outside [0, n_beams): it stays):
+ * the first n_tokens / PS entries of its block list become p's, and the n_tokens % PS
+ * tokens of its last page take the rows of p's last page, in every layer, K and V, all
+ * at once (beams may exchange places). The last page is each beam's own: its id stays, and
+ * no other beam's or request's list may hold it there; full pages may be shared. Rows whose
+ * page id, or whose parent's, is 0 or outside [1, num_blocks) are not moved. Which full
+ * pages no list names any more is the caller's to find.
+ * layers: caches of any type and layout, head_dim from 2 on, none given twice. parents: int32 [n, columns], rows
+ * contiguous (daric_select_beams' parents, or their first columns). Up to 32 beams of a
+ * request; block lists do not overlap. block_table is written. */
+int daric_reorder_beams(const daric_tensor* layers, int64_t n_layers, int page_first, daric_tensor* block_table,
+                        const daric_tensor* parents, const daric_beams* beams, int64_t n_beams, uint64_t stream);
+
 #ifdef __cplusplus
 }
 #endif

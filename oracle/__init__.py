@@ -14,6 +14,8 @@ function on the path, each citing the reference file:line it follows:
              kernels; the reference has no such kernel)
   attend.py  attention over the paged cache, token weights and eviction, in 64
              bits (spec of the attention kernels; no reference kernel)
+  decode.py  rotary positions, the append to the paged cache and beam search, in 64
+             bits (spec of the append and beam kernels; no reference kernel)
   kvio.py    store/load record format and copy plan of the daric-store GPU I/O
              (daric/management/service/gpu_kv_io.py)
   c/oracle_copy.c + native.py

@@ -1,0 +1,331 @@
+"""New rows and beam search without a GPU: the oracle against facts that do not
+restate its formulas, the rotary frequencies, and every refusal of the C ABI and the
+Python layer (fake device pointers; each case fails before any device call)."""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from daric_amd import _lib, cache_ops, rotary
+from oracle import decode as odec
+from oracle import rope as orope
+from tests.gpu_util import make_layer
+from tests.test_capi_cpu import fake
+
+lib = pytest.fixture(scope="module")(lambda: _lib.load())
+r = ctypes.byref
+
+
+# ------------------------------------------------------------------ the oracle
+@pytest.mark.parametrize("neox", [True, False])
+def test_oracle_rotation_is_a_complex_product(neox):
+    rng = np.random.default_rng(1)
+    f = orope.default_inv_freq(12, 10000.0)
+    x = rng.normal(size=(5, 2, 16))
+    p = np.array([0, 1, 777, -3, 10 ** 6])
+    out, off = odec.rotate(x, p, f, 12, neox, 1.25)
+    z = x[..., :6] + 1j * x[..., 6:12] if neox else x[..., 0:12:2] + 1j * x[..., 1:12:2]
+    z = z * 1.25 * np.exp(1j * p[:, None, None].astype(float) * np.asarray(f, np.float64))
+    got = out[..., :6] + 1j * out[..., 6:12] if neox else out[..., 0:12:2] + 1j * out[..., 1:12:2]
+    assert np.allclose(got, z, atol=1e-12) and (out[..., 12:] == x[..., 12:]).all()
+    assert (off[..., :12] > 0).all() and (off[..., 12:] == 0).all()
+    back, _ = odec.rotate(out, -p, f, 12, neox, 0.8)
+    assert np.allclose(back, x, atol=1e-9)
+    # the rotation by positions agrees with the cached rows' rotation by a shift
+    two, _ = odec.rotate(odec.rotate(x, p, f, 12, neox)[0], np.full(5, 40), f, 12, neox)
+    assert np.allclose(two, odec.rotate(x, p + 40, f, 12, neox)[0], atol=1e-9)
+
+
+def test_oracle_append_places_rows():
+    layer, pf = make_layer("nhd", 6, 4, 1, 2, torch.float16, torch.Generator().manual_seed(0))
+    k = torch.arange(12, dtype=torch.float16).view(6, 1, 2)
+    where, pos, kk, vv, _ = odec.append(layer, pf, [3, 0, 5, 9], k, k, [(0, 1, 3, 2), (2, 4, 2, 3)])
+    assert where == [(1, 3, 2), (2, 3, 3), (4, 5, 3)]            # token 4 is on the null page, 9 is no page
+    assert pos.tolist() == [0, 2, 3, 4, 3, 4] and (kk == k.double().numpy()).all() and (vv == kk).all()
+
+
+def test_oracle_selection_is_a_search_over_log_softmax():
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn(2, 3, 40, generator=g)
+    s = torch.randn(2, 3, generator=g)
+    got = odec.select(x, s, 5)
+    flat = (x.double().log_softmax(-1) + s.double()[..., None]).flatten(1)
+    best, at = flat.topk(5)
+    assert np.allclose(got[0], best.numpy()) and (got[1] == at.numpy() // 40).all() and (got[2] == at.numpy() % 40).all()
+    # ties: the lower beam, then the lower token; an ended beam's one candidate; nothing behind
+    x = torch.zeros(1, 2, 4)
+    assert odec.select(x, [[0.0, 0.0]], 5)[1:][0].tolist() == [[0, 0, 0, 0, 1]]
+    assert odec.select(x, [[0.0, 0.0]], 5)[2].tolist() == [[0, 1, 2, 3, 0]]
+    got = odec.select(x, [[-1.0, -math.inf]], 3, ended=[[True, False]], end_token=2)
+    assert got[0].tolist() == [[-1.0, -math.inf, -math.inf]] and got[1].tolist() == [[0, -1, -1]] and got[2].tolist() == [[2, -1, -1]]
+    x[0, 0, 1] = math.nan
+    assert odec.select(x, [[0.0, 0.0]], 1)[1].tolist() == [[1]]
+
+
+def test_oracle_reorder_follows_parents():
+    layer, pf = make_layer("nhd", 9, 2, 1, 2, torch.float16, torch.Generator().manual_seed(1))
+    before = layer.clone()
+    bt = np.array([1, 2, 3, 1, 4, 5, 1, 6, 7], np.int32)         # three beams of five tokens, page 1 shared
+    odec.reorder([layer], pf, bt, [[1, 0, -1]], [(0, 3, 3, 5)])
+    assert bt.tolist() == [1, 4, 3, 1, 2, 5, 1, 6, 7]            # full pages exchanged, last pages stay
+    k, kb = layer[0], before[0]
+    assert torch.equal(k[3, 0], kb[5, 0]) and torch.equal(k[5, 0], kb[3, 0]) and torch.equal(k[3, 1], kb[3, 1])
+    assert torch.equal(k[7], kb[7]) and torch.equal(k[2], kb[2])
+
+
+# ------------------------------------------------------------- frequencies
+def test_frequencies_of_scaled_models():
+    f, m = rotary.rotary_frequencies(128, 500000.0)
+    assert m == 1.0 and f.dtype == torch.float32
+    want = 500000.0 ** (-np.arange(0, 128, 2) / 128)
+    assert np.allclose(f.numpy(), want, rtol=2.0 ** -24, atol=0)
+    lin, _ = rotary.rotary_frequencies(128, 500000.0, {"type": "linear", "factor": 4.0})
+    assert torch.equal(lin, f / 4)
+    dyn = {"type": "dynamic", "factor": 2.0, "original_max_position_embeddings": 2048}
+    assert torch.equal(rotary.rotary_frequencies(64, 10000.0, dyn, seq_len=2048)[0], rotary.rotary_frequencies(64)[0])
+    longer = rotary.rotary_frequencies(64, 10000.0, dyn, seq_len=4096)[0]
+    # the slowest pair is stretched by the whole ratio, 2 * 4096 / 2048 - 1 = 3, the fastest not at all
+    plain = rotary.rotary_frequencies(64)[0]
+    assert longer[0] == 1 and np.isclose(float(plain[-1] / longer[-1]), 3.0, rtol=1e-6)
+    l3 = {"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0,
+          "original_max_position_embeddings": 8192}
+    g, m = rotary.rotary_frequencies(128, 500000.0, l3)
+    wave = 2 * np.pi / want
+    ratio = f.numpy() / g.numpy()
+    assert m == 1.0 and np.allclose(ratio[wave < 8192 / 4], 1) and np.allclose(ratio[wave > 8192], 8)
+    mid = (wave >= 8192 / 4) & (wave <= 8192)
+    assert mid.any() and (ratio[mid] >= 1).all() and (ratio[mid] <= 8).all() and (np.diff(ratio) >= -1e-6).all()
+    y, m = rotary.rotary_frequencies(64, 10000.0, {"type": "yarn", "factor": 4.0, "original_max_position_embeddings": 4096})
+    p = rotary.rotary_frequencies(64)[0]
+    assert np.isclose(m, 0.1 * math.log(4.0) + 1) and y[0] == p[0] and np.isclose(float(p[-1] / y[-1]), 4.0)
+    assert rotary.rotary_frequencies(64, 10000.0, {"type": "yarn", "factor": 4.0, "attention_factor": 1.5,
+                                                   "original_max_position_embeddings": 4096})[1] == 1.5
+
+
+@pytest.mark.parametrize("args,text", [
+    ((7,), "positive and even"), ((0,), "positive and even"), ((8, -1.0), "base must be"),
+    ((8, 10000.0, {"type": "linear"}), "finite factor"), ((8, 10000.0, {"type": "linear", "factor": 0}), "must be positive"),
+    ((8, 10000.0, {"type": "spiral", "factor": 2.0}), "unknown rotary scaling"),
+    ((8, 10000.0, {"type": "llama3", "factor": 2.0, "low_freq_factor": 4.0, "high_freq_factor": 1.0,
+                   "original_max_position_embeddings": 64}), "below high_freq_factor"),
+    ((8, 10000.0, {"type": "yarn", "factor": 2.0}), "original_max_position_embeddings")])
+def test_frequency_refusals(args, text):
+    with pytest.raises(ValueError, match=text):
+        rotary.rotary_frequencies(*args)
+
+
+# ------------------------------------------------------------------ the C ABI
+def rope(R=64, ptr=0x90000000, neox=1):
+    x = _lib.DaricRope()
+    x.inv_freq, x.rotary_dim, x.is_neox = ptr, R, neox
+    return x
+
+
+def ref(t):
+    return r(t) if t is not None else None
+
+
+def test_rotation_refusals(lib):
+    rows = fake((10, 8, 64), torch.bfloat16, ptr=0x30000000)
+    out = fake((10, 8, 64), torch.bfloat16, ptr=0x40000000)
+    pos = fake((10,), torch.int64, ptr=0x50000000)
+
+    def run(x=rows, p=pos, ro=rope(), m=1.0, o=out):
+        st = lib.daric_rotate_rows(ref(x), ref(p), ref(ro), m, ref(o), ctypes.c_uint64(0))
+        assert st != 0
+        return lib.daric_last_error().decode()
+
+    assert "bfloat16, float16 or float32" in run(x=fake((10, 8, 64), torch.uint8))
+    assert "must be [T, H, D]" in run(x=fake((10, 512), torch.bfloat16))
+    assert "must be [T, H, D]" in run(x=fake((10, 8, 64), torch.bfloat16, strides=(512, 1, 8)))
+    assert "negative strides" in run(x=fake((10, 8, 64), torch.bfloat16, strides=(-512, 64, 1)))
+    assert "too large" in run(x=fake((10, 2 ** 20, 64), torch.bfloat16))
+    assert "rows must be on CUDA" in run(x=fake((10, 8, 64), torch.bfloat16, device=-1))
+    assert "positions must be" in run(p=fake((10,), torch.int32))
+    assert "positions must be" in run(p=fake((9,), torch.int64))
+    assert "positions must be" in run(p=fake((10,), torch.int64, device=1))
+    assert "rope parameters" in run(ro=None)
+    assert "inv_freq must not be null" in run(ro=rope(ptr=None))
+    assert "rotary_dim must be" in run(ro=rope(66)) and "rotary_dim must be" in run(ro=rope(7)) and "rotary_dim must be" in run(ro=rope(0))
+    assert "at most 512" in run(ro=rope(1024))
+    assert "attention_scale must be finite" in run(m=math.nan) and "attention_scale must be finite" in run(m=math.inf)
+    assert "out must be rows itself or" in run(o=fake((10, 8, 64), torch.float16, ptr=0x40000000))
+    assert "out must be rows itself or" in run(o=fake((10, 8, 64), torch.bfloat16, ptr=0x40000000, strides=(1024, 64, 1)))
+    assert "out must be rows itself or" in run(o=fake((10, 4, 64), torch.bfloat16, ptr=0x40000000))
+    assert "out must not overlap rows" in run(o=fake((10, 8, 64), torch.bfloat16, ptr=0x30000080))
+    assert "out must not overlap positions" in run(o=fake((10, 8, 64), torch.bfloat16, ptr=0x50000000))
+    assert "out must not overlap inv_freq" in run(o=fake((10, 8, 64), torch.bfloat16, ptr=0x8fffffe0))
+    one = fake((10, 8, 64), torch.bfloat16, ptr=0x30000000, strides=(0, 64, 1))
+    assert "share memory" in run(x=one, o=one)
+    none = fake((0, 8, 64), torch.bfloat16)
+    assert lib.daric_rotate_rows(r(none), r(fake((0,), torch.int64)), r(rope()), 1.0, r(none), ctypes.c_uint64(0)) == 0
+
+
+def test_append_refusals(lib):
+    layer, f8 = fake((2, 8, 16, 4, 64), torch.bfloat16), fake((2, 8, 16, 4, 64), torch.uint8)
+    bt = fake((8,), torch.int32, ptr=0x20000000)
+    k, v = fake((10, 4, 64), torch.bfloat16, ptr=0x30000000), fake((10, 4, 64), torch.bfloat16, ptr=0x38000000)
+    q, out = fake((10, 8, 64), torch.bfloat16, ptr=0x40000000), fake((10, 8, 64), torch.bfloat16, ptr=0x48000000)
+    ok = (0, 0, 10, 100, 0)
+
+    def run(lay=layer, pf=0, bt_=bt, k_=k, v_=v, s=(ok,), pos=None, ro=rope(), m=1.0, q_=None, o=None, ks=None, vs=None):
+        a = np.array(s, np.int64).reshape(-1, 5)
+        st = lib.daric_append_tokens(ref(lay), pf, ref(bt_), ref(k_), ref(v_), a.ctypes.data, len(a), ref(pos), ref(ro), m,
+                                     ref(q_), ref(o), ref(ks), ref(vs), ctypes.c_uint64(0))
+        assert st != 0
+        return lib.daric_last_error().decode()
+
+    assert "unsupported KV cache dtype" in run(lay=fake((2, 8, 16, 4, 64), torch.float32))
+    assert "Unsupported KV cache rank" in run(lay=fake((8, 64), torch.bfloat16))
+    assert "must not be empty" in run(lay=fake((2, 0, 16, 4, 64), torch.bfloat16))
+    assert "head_dim from 2 on" in run(lay=fake((2, 8, 16, 4, 1), torch.bfloat16))
+    assert "block_table must be a 1-D contiguous int32" in run(bt_=fake((8,), torch.int64))
+    assert "k must have the cache's element type" in run(k_=fake((10, 4, 64), torch.float16))
+    assert "k must have the cache's element type" in run(k_=fake((10, 4, 64), torch.float32))
+    assert "k must be [T, 4, 64] rows" in run(k_=fake((10, 8, 64), torch.bfloat16))
+    assert "k must be [T, 4, 64] rows" in run(k_=fake((10, 4, 32), torch.bfloat16))
+    assert "v must be [T, 4, 64] rows" in run(v_=fake((9, 4, 64), torch.bfloat16))
+    assert "v must be [T, 4, 64] rows" in run(lay=f8, v_=fake((10, 4, 64), torch.float16))
+    assert "v must not be null" in run(v_=None)
+    assert "v must be None" in run(lay=fake((8, 16, 64), torch.bfloat16), pf=1, k_=fake((10, 1, 64), torch.bfloat16),
+                                   v_=fake((10, 1, 64), torch.bfloat16))
+    assert "negative field of sequence 1" in run(s=((0, 0, 1, 4, 0), (0, 1, 1, -4, 50)))
+    assert "rows exceed k" in run(s=((0, 5, 6, 4, 0),))
+    assert "is too long" in run(s=((0, 0, 1, 2 ** 31, 0),)) and "is too long" in run(s=((0, 0, 1, 2 ** 62, 0),))
+    assert "row 4 is in two sequences" in run(s=((0, 4, 2, 4, 50), (0, 0, 5, 4, 0)))
+    assert "reaches past the end of block_table" in run(s=((2, 0, 10, 100, 0),))
+    assert "reaches past the end of block_table" in run(s=((2 ** 62, 0, 1, 0, 0),))
+    assert "positions must be" in run(pos=fake((9,), torch.int64))
+    assert "no greater than head_dim" in run(ro=rope(66))
+    assert "attention_scale must be finite" in run(m=math.nan)
+    assert "q needs inv_freq" in run(ro=None, q_=q, o=out)
+    assert "q must be [T, Hq, 64] rows" in run(q_=fake((10, 8, 32), torch.bfloat16), o=out)
+    assert "q must be [T, Hq, 64] rows" in run(q_=fake((10, 8, 64), torch.float16), o=out)
+    assert "q_out must not be null" in run(q_=q)
+    assert "q_out must be q itself or" in run(q_=q, o=fake((10, 8, 64), torch.bfloat16, strides=(1024, 64, 1)))
+    assert "k_scale applies to fp8" in run(ks=fake((4,), torch.float32)) and "v_scale applies to fp8" in run(vs=fake((4,), torch.float32))
+    assert "k_scale must be a contiguous float32 [H]" in run(lay=f8, ks=fake((5,), torch.float32))
+    # written memory that the call reads or writes elsewhere
+    assert "the layer must not overlap k" in run(k_=fake((10, 4, 64), torch.bfloat16, ptr=0x10000100))
+    assert "the layer must not overlap v" in run(v_=fake((10, 4, 64), torch.bfloat16, ptr=0x10000100))
+    assert "the layer must not overlap block_table" in run(bt_=fake((8,), torch.int32, ptr=0x10000100))
+    assert "the layer must not overlap q_out" in run(q_=q, o=fake((10, 8, 64), torch.bfloat16, ptr=0x10000100))
+    assert "q_out must not overlap q" in run(q_=q, o=fake((10, 8, 64), torch.bfloat16, ptr=0x40000080))
+    assert "q_out must not overlap k" in run(q_=q, o=fake((10, 8, 64), torch.bfloat16, ptr=0x30000080))
+    assert "q_out must not overlap positions" in run(q_=q, o=out, pos=fake((10,), torch.int64, ptr=0x48000010))
+    # q in place in a joint projection is apart from k and v beside it, not from what overlaps it
+    joint = [fake((10, n, 64), torch.bfloat16, ptr=0x50000000 + 128 * at, strides=(1024, 64, 1)) for n, at in ((8, 0), (4, 8), (4, 12))]
+    a = np.array([(0, 0, 0, 100, 0)], np.int64)
+    assert lib.daric_append_tokens(r(layer), 0, r(bt), r(joint[1]), r(joint[2]), a.ctypes.data, 1, None, r(rope()), 1.0,
+                                   r(joint[0]), r(joint[0]), None, None, ctypes.c_uint64(0)) == 0      # no rows: no device call
+    over = fake((10, 4, 64), torch.bfloat16, ptr=0x50000000 + 128 * 7, strides=(1024, 64, 1))
+    assert "q_out must not overlap k" in run(k_=over, v_=joint[2], q_=joint[0], o=joint[0])
+    wraps = fake((10, 4, 64), torch.bfloat16, ptr=0x50000000 + 128 * 14, strides=(1024, 64, 1))
+    assert "q_out must not overlap v" in run(k_=joint[1], v_=wraps, q_=joint[0], o=joint[0])
+
+
+def test_selection_refusals(lib):
+    x = fake((2, 4, 1000), torch.bfloat16, ptr=0x30000000)
+    sc, out = fake((2, 4), torch.float32, ptr=0x40000000), fake((2, 6), torch.float32, ptr=0x50000000)
+    par, tok = fake((2, 6), torch.int32, ptr=0x51000000), fake((2, 6), torch.int32, ptr=0x52000000)
+    end = fake((2, 4), torch.uint8, ptr=0x53000000)
+
+    def run(x_=x, sc_=sc, end_=None, et=2, out_=out, par_=par, tok_=tok, work=0x60000000, size=None):
+        need = ctypes.c_int64(0)
+        if size is None and lib.daric_select_workspace(ref(x_), par_.sizes[1], r(need)) != 0:
+            return lib.daric_last_error().decode()
+        st = lib.daric_select_beams(ref(x_), ref(sc_), ref(end_), et, ref(out_), ref(par_), ref(tok_), work,
+                                    need.value if size is None else size, ctypes.c_uint64(0))
+        assert st != 0
+        return lib.daric_last_error().decode()
+
+    assert "bfloat16, float16 or float32" in run(x_=fake((2, 4, 1000), torch.uint8))
+    assert "must be [requests, beams, vocabulary]" in run(x_=fake((8, 1000), torch.bfloat16))
+    assert "must be [requests, beams, vocabulary]" in run(x_=fake((2, 4, 1000), torch.bfloat16, strides=(1, 2, 8)))
+    assert "must be [requests, beams, vocabulary]" in run(x_=fake((2, 4, 1000), torch.bfloat16, strides=(-4000, 1000, 1)))
+    assert "must be [requests, beams, vocabulary]" in run(x_=fake((2, 4, 0), torch.bfloat16))
+    assert "logits must be on CUDA" in run(x_=fake((2, 4, 1000), torch.bfloat16, device=-1))
+    assert "up to 64 beams" in run(x_=fake((2, 65, 1000), torch.bfloat16))
+    for k in (0, 65):
+        wide = [fake((2, k), t, ptr=0x55000000) for t in (torch.float32, torch.int32, torch.int32)]
+        assert "1 to 64 candidates" in run(out_=wide[0], par_=wide[1], tok_=wide[2])
+    assert "vocabulary is too large" in run(x_=fake((2, 64, 2 ** 24), torch.bfloat16))
+    assert "too many rows" in run(x_=fake((2 ** 24, 4, 100000), torch.bfloat16))
+    assert "scores must be" in run(sc_=fake((2, 3), torch.float32)) and "scores must be" in run(sc_=fake((2, 4), torch.float16))
+    assert "ended must be" in run(end_=fake((2, 4), torch.int32)) and "ended must be" in run(end_=fake((4,), torch.uint8))
+    assert "end_token must be in the vocabulary" in run(end_=end, et=1000)
+    assert "end_token must be in the vocabulary" in run(end_=end, et=-1)
+    assert "out_scores must be" in run(out_=fake((2, 5), torch.float32))
+    assert "tokens must be" in run(tok_=fake((2, 6), torch.int64))
+    assert "workspace must be 16-byte aligned" in run(work=None) and "workspace must be 16-byte aligned" in run(work=0x60000004)
+    assert "workspace must be 16-byte aligned" in run(size=16)
+    assert "parents must not overlap tokens" in run(tok_=fake((2, 6), torch.int32, ptr=0x51000010))
+    assert "out_scores must not overlap scores" in run(out_=fake((2, 6), torch.float32, ptr=0x40000010))
+    assert "workspace must not overlap logits" in run(work=0x30000010)
+    none = [fake((0, 6), t) for t in (torch.float32, torch.int32, torch.int32)]
+    assert lib.daric_select_beams(r(fake((0, 4, 10), torch.float32)), r(fake((0, 4), torch.float32)), None, 0, r(none[0]),
+                                  r(none[1]), r(none[2]), None, 0, ctypes.c_uint64(0)) == 0
+
+
+def test_reorder_refusals(lib):
+    layers = (_lib.DaricTensor * 2)(*[fake((2, 8, 16, 4, 64), torch.bfloat16, ptr=0x10000000 * (i + 1)) for i in range(2)])
+    bt = fake((40,), torch.int32, ptr=0x30000000)
+    par = fake((1, 4), torch.int32, ptr=0x40000000)
+
+    def run(s=((0, 10, 4, 100),), lay=layers, bt_=bt, par_=par, pf=0, n=None):
+        a = np.array(s, np.int64).reshape(-1, 4)
+        st = lib.daric_reorder_beams(lay, 2, pf, r(bt_), ref(par_), a.ctypes.data, len(a), ctypes.c_uint64(0))
+        assert st != 0
+        return lib.daric_last_error().decode()
+
+    assert "negative field of request 0" in run(s=((0, 10, 4, -1),))
+    assert "up to 32 beams" in run(s=((0, 10, 33, 5),))
+    assert "more beams than parents has columns" in run(s=((0, 10, 5, 5),))
+    assert "is too long" in run(s=((0, 10, 4, 2 ** 31),))
+    assert "block lists of its beams overlap" in run(s=((0, 6, 4, 100),))
+    assert "reaches past the end of block_table" in run(s=((5, 10, 4, 100),))
+    assert "reaches past the end of block_table" in run(s=((0, 2 ** 62, 4, 100),))
+    assert "reaches past the end of block_table" in run(s=((2 ** 62, 10, 4, 100),))
+    two = fake((2, 4), torch.int32, ptr=0x40000000)
+    assert "block list 20 is in two sequences" in run(s=((0, 10, 3, 40), (20, 10, 2, 30)), par_=two)
+    assert "parents must be" in run(par_=two) and "parents must be" in run(par_=fake((1, 4), torch.int64))
+    assert "parents must be" in run(par_=fake((1, 4), torch.int32, device=1)) and "parents must be" in run(par_=fake((4,), torch.int32))
+    assert "parents must be" in run(par_=fake((1, 4), torch.int32, strides=(4, 2)))
+    assert "block_table must be a 1-D contiguous int32" in run(bt_=fake((40,), torch.int64))
+    assert "block_table must not overlap parents" in run(par_=fake((1, 4), torch.int32, ptr=0x30000010))
+    assert "a layer must not overlap block_table" in run(bt_=fake((40,), torch.int32, ptr=0x10000010))
+    twice = (_lib.DaricTensor * 2)(layers[0], layers[0])
+    assert "a layer is given twice" in run(lay=twice)
+    other = (_lib.DaricTensor * 2)(layers[0], fake((2, 8, 16, 4, 32), torch.bfloat16))
+    assert "must share shape" in run(lay=other)
+    # nothing to move: no beams, one beam, no tokens
+    for s in ((), ((0, 10, 0, 100),), ((0, 10, 1, 100),), ((0, 10, 4, 0),)):
+        a = np.array(s, np.int64).reshape(-1, 4)
+        p = fake((len(a), 4), torch.int32, ptr=0x40000000)
+        assert lib.daric_reorder_beams(layers, 2, 0, r(bt), r(p), a.ctypes.data, len(a), ctypes.c_uint64(0)) == 0
+
+
+# ------------------------------------------------------------ the Python layer
+def test_python_refusals():
+    x = torch.zeros(2, 2, 8, dtype=torch.bfloat16)
+    f, p = torch.ones(4), torch.zeros(2, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="inv_freq must be a float32 device tensor"):
+        cache_ops.rotate_rows(x, p, f, 8)
+    layer, bt = torch.zeros(2, 3, 4, 2, 8, dtype=torch.bfloat16), torch.ones(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="sequences must be"):
+        cache_ops.append_tokens(layer, False, bt, x, x, [(0, 0)])
+    with pytest.raises(RuntimeError, match="must be on CUDA"):
+        cache_ops.append_tokens(layer, False, bt, x, x, [(0, 0, 2, 0)])
+    with pytest.raises(RuntimeError, match="logits must be on CUDA"):
+        cache_ops.select_beams(torch.zeros(1, 2, 8), torch.zeros(1, 2))
+    with pytest.raises(ValueError, match="beams must be"):
+        cache_ops.reorder_beams([layer], False, bt, torch.zeros(1, 2, dtype=torch.int32), [(0, 1, 2)])
+    with pytest.raises(RuntimeError, match="must be on CUDA"):
+        cache_ops.reorder_beams([layer], False, bt, torch.zeros(1, 2, dtype=torch.int32), [(0, 1, 2, 1)])
+    g = torch.zeros(2, 2, 8, requires_grad=True)
+    for call in (lambda: cache_ops.rotate_rows(g, p, f, 8), lambda: cache_ops.append_tokens(layer, False, bt, g, x, [(0, 0, 2, 0)]),
+                 lambda: cache_ops.select_beams(g, torch.zeros(2, 2))):
+        with pytest.raises(RuntimeError, match="has no backward pass"):
+            call()
