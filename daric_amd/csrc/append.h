@@ -57,7 +57,8 @@ inline int append_vec(int64_t half, int64_t rest, int most) {
     return v;
 }
 
-// from: ElemKind of the rows or kF32; to: kE4M3 for an e4m3 cache, else `from`.
-void launch_append(const DescArg& d, const AppendArgs& a, int from, int to, int vec, int64_t tiles, hipStream_t stream);
+// from: ElemKind of the rows or kF32; to: kE4M3 for an e4m3 cache, else `from`. past: 16-byte
+// stores go past the caches.
+void launch_append(const DescArg& d, const AppendArgs& a, int from, int to, int vec, bool past, int64_t tiles, hipStream_t stream);
 
 }  // namespace daric

@@ -67,8 +67,14 @@ struct Values {
             w[0] = *reinterpret_cast<const uint16_t*>(p);
         }
     }
+    // PAST: past the caches (16-byte stores)
+    template <bool PAST>
     __device__ __forceinline__ void store(uint8_t* p) const {
-        if constexpr (kBytes == 16) *reinterpret_cast<u32x4*>(p) = u32x4{w[0], w[1], w[2], w[3]};
+        if constexpr (kBytes == 16) {
+            const u32x4 x = {w[0], w[1], w[2], w[3]};
+            if constexpr (PAST) __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>(p));
+            else *reinterpret_cast<u32x4*>(p) = x;
+        }
         else if constexpr (kBytes == 8) *reinterpret_cast<u32x2*>(p) = u32x2{w[0], w[1]};
         else if constexpr (kBytes == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
         else if constexpr (kBytes == 2) *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(w[0]);
@@ -105,7 +111,7 @@ struct Values {
     }
 };
 
-template <int FROM, int TO, int VEC>
+template <int FROM, int TO, int VEC, bool PAST>
 __global__ __launch_bounds__(kThreads) void append_kernel(DescArg d, AppendArgs a) {
     extern __shared__ __align__(16) float s_turn[];      // cosines and sines, [tile][R / 2] each
     __shared__ int64_t s_slot[kThreads / 2];             // K element of each row's token, -1: nowhere
@@ -204,8 +210,8 @@ __global__ __launch_bounds__(kThreads) void append_kernel(DescArg d, AppendArgs 
                 it.y.pack(y);
             }
             uint8_t* p = a.q_out + ((row0 + it.tok) * a.out_row + it.head * a.out_head) * (From::kBytes / VEC);
-            it.x.store(p + u * (From::kBytes / VEC));
-            if (it.second) it.y.store(p + v * (From::kBytes / VEC));
+            it.x.template store<PAST>(p + u * (From::kBytes / VEC));
+            if (it.second) it.y.template store<PAST>(p + v * (From::kBytes / VEC));
             return;
         }
         if constexpr (FROM != kF32) {
@@ -237,8 +243,8 @@ __global__ __launch_bounds__(kThreads) void append_kernel(DescArg d, AppendArgs 
                 xo = it.x;
                 yo = it.y;
             }
-            xo.store(p + u * (To::kBytes / VEC));
-            if (it.second) yo.store(p + v * (To::kBytes / VEC));
+            xo.template store<PAST>(p + u * (To::kBytes / VEC));
+            if (it.second) yo.template store<PAST>(p + v * (To::kBytes / VEC));
         }
     };
 
@@ -277,20 +283,22 @@ __global__ __launch_bounds__(kThreads) void append_kernel(DescArg d, AppendArgs 
 
 }  // namespace
 
-void launch_append(const DescArg& d, const AppendArgs& a, int from, int to, int vec, int64_t tiles, hipStream_t stream) {
+void launch_append(const DescArg& d, const AppendArgs& a, int from, int to, int vec, bool past, int64_t tiles, hipStream_t stream) {
     const size_t lds = static_cast<size_t>(a.tile) * a.R * sizeof(float);
-#define DARIC_AP(F, T, V) DARIC_LAUNCH((append_kernel<F, T, V>), static_cast<unsigned>(tiles), kThreads, lds, stream, d, a)
+#define DARIC_AP(F, T, V, P) DARIC_LAUNCH((append_kernel<F, T, V, P>), static_cast<unsigned>(tiles), kThreads, lds, stream, d, a)
 #define DARIC_AV(F, T)                    \
     do {                                  \
-        if (vec == 8) DARIC_AP(F, T, 8);  \
-        else if (vec == 4) DARIC_AP(F, T, 4); \
-        else if (vec == 2) DARIC_AP(F, T, 2); \
-        else DARIC_AP(F, T, 1);           \
+        if (vec == 8 && past) DARIC_AP(F, T, 8, true); \
+        else if (vec == 8) DARIC_AP(F, T, 8, false);   \
+        else if (vec == 4) DARIC_AP(F, T, 4, false);   \
+        else if (vec == 2) DARIC_AP(F, T, 2, false);   \
+        else DARIC_AP(F, T, 1, false);                 \
     } while (0)
     if (from == kF32) {
-        if (vec == 4) DARIC_AP(kF32, kF32, 4);
-        else if (vec == 2) DARIC_AP(kF32, kF32, 2);
-        else DARIC_AP(kF32, kF32, 1);
+        if (vec == 4 && past) DARIC_AP(kF32, kF32, 4, true);
+        else if (vec == 4) DARIC_AP(kF32, kF32, 4, false);
+        else if (vec == 2) DARIC_AP(kF32, kF32, 2, false);
+        else DARIC_AP(kF32, kF32, 1, false);
     } else if (to == kE4M3) {
         if (from == kBF16) DARIC_AV(kBF16, kE4M3);
         else DARIC_AV(kF16, kE4M3);

@@ -3,8 +3,7 @@
 //
 // A candidate's score is the beam's plus x - lse, lse = log sum exp(x) of its row of
 // logits. Within a row scores are ordered as the logits are, so the choice needs one
-// pass over them: a wavefront takes a split of a row into registers (`REGS` words a
-// lane), reduces its maximum and its sum of exponentials, and leaves the split's k
+// pass over them: a wavefront takes a split of a row, 8 KiB, into registers, reduces its maximum and its sum of exponentials, and leaves the split's k
 // best logits in order, ties to the lower token. select_join_kernel, a wavefront per
 // request, joins the splits' sums to each beam's lse in fp64 and merges the lists by
 // score: k times the best of their heads.
@@ -43,65 +42,90 @@ struct Rank {
     }
 };
 
-template <int KIND, int REGS>
+// A lane's share of a split of a row: kSplitBytes / 64, in units of 16 bytes. Value j of unit r is
+// value (r * 64 + lane) * kUnit + j of the split; behind its end stands -inf.
+template <int KIND>
 struct Split {
     static constexpr int kPerReg = KIND == kF32 ? 1 : 2;
-    static constexpr int kUnit = 4 * kPerReg;          // values of a 16-byte access
-    static constexpr int kValues = REGS * kPerReg;     // of a lane
-    uint32_t w[REGS];
-    int lane;
-    // Value j of the lane is value (j / kUnit * 64 + lane) * kUnit + j % kUnit of the split.
-    __device__ __forceinline__ int index(int j) const { return (j / kUnit * 64 + lane) * kUnit + j % kUnit; }
-    __device__ __forceinline__ float at(int j) const {
-        if constexpr (KIND == kF32) return u2f(w[j]);
-        else if constexpr (KIND == kBF16) return u2f((j & 1) != 0 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
-        else return f16_to_f32((j & 1) != 0 ? w[j / 2] >> 16 : w[j / 2] & 0xffffu);
-    }
-    // n values from p, of any element-aligned address; -inf behind them.
-    __device__ __forceinline__ void load(const uint8_t* p, int64_t n) {
+    static constexpr int kBytes = 4 / kPerReg;         // of a value
+    static constexpr int kUnit = 4 * kPerReg;          // values of a unit
+    static constexpr int kUnits = kSplitBytes / 1024;
+    static constexpr int kTotal = 64 * kUnits * kUnit;
+    const uint8_t* p;                                  // of the split's values, at any element
+    int n, lane;                                       // values that are there
+
+    __device__ __forceinline__ int index(int r) const { return (r * 64 + lane) * kUnit; }
+    __device__ __forceinline__ u32x4 words(int r) const {
         constexpr uint32_t kNone = KIND == kF32 ? 0xff800000u : KIND == kBF16 ? 0xff80ff80u : 0xfc00fc00u;
-        constexpr int kBytes = 4 / kPerReg;
-#pragma unroll
-        for (int r = 0; r < REGS / 4; ++r) {
-            const int64_t i = (static_cast<int64_t>(r) * 64 + lane) * kUnit;
-            if (i + kUnit <= n) {
-                u32x4 x;
-                __builtin_memcpy(&x, p + i * kBytes, 16);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) w[4 * r + j] = x[j];
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    uint32_t x = kNone;
-                    if constexpr (KIND == kF32) {
-                        if (i + j < n) __builtin_memcpy(&x, p + (i + j) * kBytes, 4);
-                    } else {
-                        uint16_t h;
-                        if (i + 2 * j < n) {
-                            __builtin_memcpy(&h, p + (i + 2 * j) * kBytes, 2);
-                            x = (x & 0xffff0000u) | h;
-                        }
-                        if (i + 2 * j + 1 < n) {
-                            __builtin_memcpy(&h, p + (i + 2 * j + 1) * kBytes, 2);
-                            x = (x & 0xffffu) | static_cast<uint32_t>(h) << 16;
-                        }
-                    }
-                    w[4 * r + j] = x;
-                }
-            }
+        const int i = index(r);
+        u32x4 w;
+        if (i + kUnit <= n) {
+            __builtin_memcpy(&w, p + static_cast<int64_t>(i) * kBytes, 16);
+            return w;
         }
+        w = u32x4{kNone, kNone, kNone, kNone};
+        for (int j = 0; j < kUnit; ++j) {
+            if (i + j >= n) break;
+            uint32_t x = 0;
+            __builtin_memcpy(&x, p + static_cast<int64_t>(i + j) * kBytes, kBytes);
+            const int at = j / kPerReg;
+            const uint32_t old = at == 0 ? w[0] : at == 1 ? w[1] : at == 2 ? w[2] : w[3];
+            const uint32_t mixed = kPerReg == 1 ? x : (j & 1) != 0 ? (old & 0xffffu) | x << 16 : (old & 0xffff0000u) | x;
+            w[0] = at == 0 ? mixed : w[0];
+            w[1] = at == 1 ? mixed : w[1];
+            w[2] = at == 2 ? mixed : w[2];
+            w[3] = at == 3 ? mixed : w[3];
+        }
+        return w;
+    }
+    static __device__ __forceinline__ float value(const u32x4& w, int j) {
+        const uint32_t x = w[j / kPerReg];
+        if constexpr (KIND == kF32) return u2f(x);
+        else if constexpr (KIND == kBF16) return u2f((j & 1) != 0 ? x & 0xffff0000u : x << 16);
+        else return f16_to_f32((j & 1) != 0 ? x >> 16 : x & 0xffffu);
     }
 };
 
+// Lane i's value of lane i - n of its row of 16 (CTRL row_shr:n), or lane 15's or 31's
+// passed on to the rows behind (row_bcast); `old` where there is none.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ float dpp(float old, float x) {
+#ifdef __HIP_DEVICE_COMPILE__
+    return u2f(static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(f2u(old)), static_cast<int>(f2u(x)), CTRL, ROWS, 0xf, false)));
+#else
+    return old + x;
+#endif
+}
+__device__ __forceinline__ float lane63(float x) {
+    return u2f(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(f2u(x)), 63)));
+}
 __device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o, 64));
-    return x;
+    x = fmaxf(x, dpp<0x111>(x, x));
+    x = fmaxf(x, dpp<0x112>(x, x));
+    x = fmaxf(x, dpp<0x114>(x, x));
+    x = fmaxf(x, dpp<0x118>(x, x));
+    x = fmaxf(x, dpp<0x142, 0xa>(x, x));
+    x = fmaxf(x, dpp<0x143, 0xc>(x, x));
+    return lane63(x);
 }
 __device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
-    return x;
+    x += dpp<0x111>(0.0f, x);
+    x += dpp<0x112>(0.0f, x);
+    x += dpp<0x114>(0.0f, x);
+    x += dpp<0x118>(0.0f, x);
+    x += dpp<0x142, 0xa>(0.0f, x);
+    x += dpp<0x143, 0xc>(0.0f, x);
+    return lane63(x);
+}
+// Larger of three; a NaN is passed over.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+#ifdef __HIP_DEVICE_COMPILE__
+    float m;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(m) : "v"(a), "v"(b), "v"(c));
+    return m;
+#else
+    return fmaxf(fmaxf(a, b), c);
+#endif
 }
 
 // The largest t of `bits` leading bits for which count(t) >= k (0 if none).
@@ -115,31 +139,39 @@ __device__ __forceinline__ uint32_t largest_with(int bits, int k, Count&& count)
     return t;
 }
 
-template <int KIND, int REGS>
+template <int KIND>
 __global__ __launch_bounds__(kSplitThreads) void select_split_kernel(SelectArgs a) {
     __shared__ uint64_t s_list[kSplitsPerBlock][kListed];
-    using S = Split<KIND, REGS>;
-    constexpr int kBytes = 4 / S::kPerReg;
-    constexpr int kTotal = S::kValues * 64;
+    using S = Split<KIND>;
+    using R = Rank<KIND>;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
     const int lane = static_cast<int>(threadIdx.x) & 63;
-    const int64_t unit = static_cast<int64_t>(blockIdx.x) * kSplitsPerBlock + wave;
-    const int64_t rows = static_cast<int64_t>(a.B) * a.W;
+    const uint32_t unit = blockIdx.x * kSplitsPerBlock + wave;
+    const uint32_t rows = static_cast<uint32_t>(a.B) * a.W;
     if (unit >= rows * a.splits) return;
-    const int64_t row = unit / a.splits;
+    const uint32_t row = a.d_splits.div(unit);
     const int split = static_cast<int>(unit - row * a.splits);
     // rows that offer no logit: their beam has ended, or has no score
     if (a.ended != nullptr && a.ended[row] != 0) return;
     if (!(a.scores[row] > -__builtin_huge_valf())) return;
-    const int64_t b = row / a.W, w = row - b * a.W;
-    const int64_t v0 = static_cast<int64_t>(split) * kTotal;
+    const uint32_t b = a.d_beams.div(row), w = row - b * a.W;
+    const int64_t v0 = static_cast<int64_t>(split) * S::kTotal;
     S v;
+    v.p = a.logits + (b * a.batch + w * a.row + v0) * S::kBytes;
+    v.n = static_cast<int>(min(a.V - v0, static_cast<int64_t>(S::kTotal)));
     v.lane = lane;
-    v.load(a.logits + (b * a.batch + w * a.row + v0) * kBytes, a.V - v0);
-
-    float top = -__builtin_huge_valf();
+    u32x4 x[S::kUnits];
 #pragma unroll
-    for (int j = 0; j < S::kValues; ++j) top = fmaxf(top, v.at(j));
+    for (int r = 0; r < S::kUnits; ++r) x[r] = v.words(r);
+
+    float best[S::kUnits], top = -__builtin_huge_valf();   // of each unit, of all
+#pragma unroll
+    for (int r = 0; r < S::kUnits; ++r) {
+        best[r] = -__builtin_huge_valf();
+#pragma unroll
+        for (int j = 0; j < S::kUnit; j += 2) best[r] = max3(best[r], S::value(x[r], j), S::value(x[r], j + 1));
+        top = fmaxf(top, best[r]);
+    }
     const float most = wave_max(top);
     // a split of nothing but -inf: 0 in its place, so that the sum is 0, or NaN if it holds one
     const float ref = most > -__builtin_huge_valf() ? most : 0.0f;
@@ -147,88 +179,107 @@ __global__ __launch_bounds__(kSplitThreads) void select_split_kernel(SelectArgs 
     constexpr float kLog2eRest = static_cast<float>(1.44269504088896340736 - static_cast<double>(kLog2e));
     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int j = 0; j < S::kValues; ++j) {
-        const float x = v.at(j) - ref;
-        sum[j % 4] += __builtin_amdgcn_exp2f(__builtin_fmaf(x, kLog2e, x * kLog2eRest));
+    for (int r = 0; r < S::kUnits; ++r) {
+#pragma unroll
+        for (int j = 0; j < S::kUnit; ++j) {
+            const float d = S::value(x[r], j) - ref;
+            sum[j % 4] += __builtin_amdgcn_exp2f(__builtin_fmaf(d, kLog2e, d * kLog2eRest));
+        }
     }
     const float total = wave_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
     if (lane == 0) {
-        a.part_ms[unit * 2] = most;
-        a.part_ms[unit * 2 + 1] = total;
+        a.part_ms[static_cast<int64_t>(unit) * 2] = most;
+        a.part_ms[static_cast<int64_t>(unit) * 2 + 1] = total;
     }
 
     // At least k of the split's values are as large as the k-th largest of the lanes'
     // maxima: few more than k where they are spread over the lanes.
-    using R = Rank<KIND>;
     const uint32_t mine = R::of(top);
     uint32_t least = largest_with(R::kBits, a.k, [&](uint32_t t) { return __popcll(__ballot(mine >= t)); });
     least = max(least, R::kLeast);
-    int found = 0;
-#pragma unroll
-    for (int j = 0; j < S::kValues; ++j) found += __popcll(__ballot(R::of(v.at(j)) >= least));
     uint64_t* const list = s_list[wave];
-    const auto entry = [&](int j) { return static_cast<uint64_t>(R::of(v.at(j))) << 32 | static_cast<uint32_t>(~v.index(j)); };
     const unsigned long long below = (1ull << lane) - 1;
+    int found = 0;
+    {
+        // the units that hold any are read again, each lane's next one at a time: picking
+        // them out of the registers would be code for every value
+        const float bound = R::value(least);
+        uint32_t holds = 0;
+#pragma unroll
+        for (int r = 0; r < S::kUnits; ++r) holds |= best[r] >= bound ? 1u << r : 0u;
+        while (__ballot(holds != 0) != 0) {
+            u32x4 u = {0, 0, 0, 0};
+            int at0 = 0;
+            const bool has = holds != 0;
+            if (has) {
+                const int r = __ffs(static_cast<int>(holds)) - 1;
+                holds &= holds - 1;
+                at0 = v.index(r);
+                u = v.words(r);
+            }
+#pragma unroll
+            for (int j = 0; j < S::kUnit; ++j) {
+                const float f = S::value(u, j);
+                const bool is = has && f >= bound;
+                const unsigned long long some = __ballot(is);
+                if (some == 0) continue;
+                const int at = found + __popcll(some & below);
+                if (is && at < kListed) list[at] = static_cast<uint64_t>(R::of(f)) << 32 | static_cast<uint32_t>(~(at0 + j));
+                found += __popcll(some);
+            }
+        }
+    }
     if (found > kListed) {
         // Few lanes hold them, or many are alike: the k-th largest value itself, all
-        // above it, and the first of those equal to it.
-        least = largest_with(R::kBits, a.k, [&](uint32_t t) {
+        // above it, and the first of those equal to it, from the values read again.
+        const auto count = [&](int r, auto&& test) {
+            const u32x4 u = v.words(r);
             int n = 0;
 #pragma unroll
-            for (int j = 0; j < S::kValues; ++j) n += __popcll(__ballot(R::of(v.at(j)) >= t));
+            for (int j = 0; j < S::kUnit; ++j) n += test(R::of(S::value(u, j))) ? 1 : 0;
             return n;
+        };
+        const auto upto = [&](int n) {                 // sum over the lanes up to this one
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int y = __shfl_up(n, o, 64);
+                if (lane >= o) n += y;
+            }
+            return n;
+        };
+        least = largest_with(R::kBits, a.k, [&](uint32_t t) {
+            int n = 0;
+            for (int r = 0; r < S::kUnits; ++r) n += count(r, [&](uint32_t q) { return q >= t; });
+            return __shfl(upto(n), 63, 64);
         });
         least = max(least, R::kLeast);
         found = 0;
-#pragma unroll
-        for (int j = 0; j < S::kValues; ++j) {
-            const bool is = R::of(v.at(j)) > least;
-            const unsigned long long some = __ballot(is);
-            if (is) list[found + __popcll(some & below)] = entry(j);
-            found += __popcll(some);
-        }
-        int open = a.k - found;                        // places for those equal to it, in order
-#pragma unroll
-        for (int r = 0; r < REGS / 4; ++r) {
-            int n = 0;
-#pragma unroll
-            for (int j = 0; j < S::kUnit; ++j) n += R::of(v.at(r * S::kUnit + j)) == least ? 1 : 0;
-            int upto = n;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const int x = __shfl_up(upto, o, 64);
-                if (lane >= o) upto += x;
-            }
-            int at = upto - n;
+        int open = a.k;                                // places for those equal to it, in order
+        for (int r = 0; r < S::kUnits; ++r) open -= __shfl(upto(count(r, [&](uint32_t q) { return q > least; })), 63, 64);
+        for (int r = 0; r < S::kUnits; ++r) {
+            const u32x4 u = v.words(r);
+            const int equal = upto(count(r, [&](uint32_t q) { return q == least; }));
+            int before = equal - count(r, [&](uint32_t q) { return q == least; });
 #pragma unroll
             for (int j = 0; j < S::kUnit; ++j) {
-                if (R::of(v.at(r * S::kUnit + j)) == least) {
-                    if (at < open) list[found + at] = entry(r * S::kUnit + j);
-                    ++at;
-                }
+                const uint32_t q = R::of(S::value(u, j));
+                const bool is = q > least || (q == least && before < open);
+                before += q == least ? 1 : 0;
+                const unsigned long long some = __ballot(is);
+                if (is) list[found + __popcll(some & below)] = static_cast<uint64_t>(q) << 32 | static_cast<uint32_t>(~(v.index(r) + j));
+                found += __popcll(some);
             }
-            const int all = min(__shfl(upto, 63, 64), open);
-            found += all;
-            open -= all;
-        }
-    } else {
-        int at = 0;
-#pragma unroll
-        for (int j = 0; j < S::kValues; ++j) {
-            const bool is = R::of(v.at(j)) >= least;
-            const unsigned long long some = __ballot(is);
-            if (some == 0) continue;
-            if (is) list[at + __popcll(some & below)] = entry(j);
-            at += __popcll(some);
+            open -= min(open, __shfl(equal, 63, 64));
         }
     }
     __builtin_amdgcn_wave_barrier();
     __threadfence_block();
     // a candidate's place is the number of better ones
-    BeamCandidate* const out = a.part + unit * a.k;
+    BeamCandidate* const out = a.part + static_cast<int64_t>(unit) * a.k;
     for (int i = lane; i < found; i += 64) {
         const uint64_t key = list[i];
         int place = 0;
+#pragma unroll 4
         for (int j = 0; j < found; ++j) place += list[j] > key ? 1 : 0;
         if (place < a.k) {
             out[place].x = R::value(static_cast<uint32_t>(key >> 32));
@@ -245,27 +296,41 @@ __device__ __forceinline__ uint32_t score_rank(double s) {
 }
 
 // A workgroup per request. The k-th best of the lists' heads is at most the k-th best of
-// all: the candidates from it on, few more than k, are ranked in LDS. Where they are too
-// many (scores alike), the first wavefront takes k times the best of the heads.
-constexpr int kJoinThreads = 256;
+// all: the lists whose head is as good, and of them the candidates that are, few more than
+// k, are ranked in LDS. Where they are too many (scores alike), the first wavefront takes k
+// times the best of the heads. Bound by latency: three rounds of loads.
+constexpr int kJoinThreads = 512;
 constexpr int kJoined = 512;
 constexpr int kHeadsPerLane = 8;      // of the first wavefront: lists beyond are not asked for the threshold
-__global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a, int lists_per_lane) {
+__global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a, int lists_per_lane, FastDiv k_div) {
     extern __shared__ uint8_t s_at[];                  // [lists_per_lane][64]: candidates taken from each list
-    __shared__ double s_base[kMaxBeams];               // score - lse of each beam
-    __shared__ double s_score[kJoined];
-    __shared__ int64_t s_where[kJoined];
+    __shared__ double s_base[kMaxBeams];               // score - lse of each beam; of one at its end, its score
+    __shared__ uint8_t s_ended[kMaxBeams];
+    __shared__ uint32_t s_heads[kHeadsPerLane * 64];
+    struct Found {
+        double score;
+        int64_t where;
+    };
+    __shared__ __align__(16) Found s_found[kJoined];
+    __shared__ int s_lists[kJoined];
     __shared__ uint32_t s_least;
-    __shared__ int s_count;
+    __shared__ int s_count, s_n_lists;
     const int64_t b = blockIdx.x;
     const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = tid >> 6;
     const int64_t row0 = b * a.W;
     const double kNone = -__builtin_huge_val();
-    const auto ended = [&](int w) { return a.ended != nullptr && a.ended[row0 + w] != 0; };
-    const auto alive = [&](int w) { return a.scores[row0 + w] > -__builtin_huge_valf(); };
+    const int lists = a.W * a.splits;
+    const BeamCandidate* const part = a.part + row0 * a.splits * a.k;
+    constexpr int kMine = kHeadsPerLane * 64 / kJoinThreads;
+    BeamCandidate head[kMine];                         // what rows without logits left there is not used
+#pragma unroll
+    for (int n = 0; n < kMine; ++n)
+        if (n * kJoinThreads + tid < lists) head[n] = part[static_cast<int64_t>(n * kJoinThreads + tid) * a.k];
     for (int w = wave; w < a.W; w += kJoinThreads / 64) {
-        double base = a.scores[row0 + w];
-        if (!ended(w) && alive(w)) {
+        const float score = a.scores[row0 + w];
+        const bool at_end = a.ended != nullptr && a.ended[row0 + w] != 0;
+        double base = score;
+        if (!at_end) {
             const float* ms = a.part_ms + (row0 + w) * a.splits * 2;
             float most = -__builtin_huge_valf();
             for (int i = lane; i < a.splits; i += 64) most = fmaxf(most, ms[2 * i]);
@@ -275,69 +340,81 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a,
                 sum += static_cast<double>(ms[2 * i + 1]) * exp(static_cast<double>(ms[2 * i]) - static_cast<double>(most));
 #pragma unroll
             for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-            base -= static_cast<double>(most) + log(sum);
+            // a beam without a score left no sums
+            base = score > -__builtin_huge_valf() ? base - (static_cast<double>(most) + log(sum)) : kNone;
         }
-        if (lane == 0) s_base[w] = base;
+        if (lane == 0) {
+            s_base[w] = base;
+            s_ended[w] = at_end ? 1 : 0;
+        }
     }
-    if (tid == 0) s_count = 0;
+    if (tid == 0) s_count = s_n_lists = 0;
     __syncthreads();
-    const int lists = a.W * a.splits;
-    // Candidate `at` of a list: its score, -inf where there is none (NaN too), and its
-    // beam and token in one number, which orders ties.
-    const auto look = [&](int list, int at, double* score, int64_t* where) {
-        *score = kNone;
-        *where = 0;
-        const int w = list / a.splits, s = list - w * a.splits;
-        int token = a.end_token;
-        double x = 0.0;
-        if (ended(w)) {
-            if (s > 0 || at > 0) return;
-        } else {
-            if (at >= a.k || !alive(w)) return;
-            const BeamCandidate c = a.part[(row0 * a.splits + list) * a.k + at];
-            token = c.token;
-            if (token < 0) return;
-            x = c.x;
-        }
-        const double v = s_base[w] + x;
-        if (!(v > kNone)) return;
-        *score = v;
-        *where = static_cast<int64_t>(w) << 32 | token;
+    // A list's candidate (number `at` of it): its score, -inf where there is none (NaN too),
+    // and its beam and token in one number, which orders ties.
+    const auto judge = [&](int list, int at, const BeamCandidate& c, double* score, int64_t* where) {
+        const int w = static_cast<int>(a.d_splits.div(static_cast<uint32_t>(list)));
+        const bool at_end = s_ended[w] != 0;
+        const bool first = list == w * a.splits && at == 0;
+        const int token = at_end ? a.end_token : c.token;
+        const double v = at_end ? s_base[w] : s_base[w] + static_cast<double>(c.x);
+        const bool is = (at_end ? first : token >= 0) && v > kNone;
+        *score = is ? v : kNone;
+        *where = static_cast<int64_t>(w) << 32 | static_cast<uint32_t>(token);
     };
+    const auto look = [&](int list, int at, double* score, int64_t* where) {
+        BeamCandidate c{0.0f, -1};
+        if (at < a.k) c = part[static_cast<int64_t>(list) * a.k + at];
+        judge(list, at, c, score, where);
+    };
+    const auto rank_of_list = [&](int list, const BeamCandidate& c) {
+        double s;
+        int64_t at;
+        judge(list, 0, c, &s, &at);
+        return s > kNone ? score_rank(s) : 0u;
+    };
+    uint32_t rank[kMine];
+#pragma unroll
+    for (int n = 0; n < kMine; ++n) {
+        rank[n] = n * kJoinThreads + tid < lists ? rank_of_list(n * kJoinThreads + tid, head[n]) : 0u;
+        s_heads[n * kJoinThreads + tid] = rank[n];
+    }
+    __syncthreads();
     if (wave == 0) {
-        uint32_t head[kHeadsPerLane];
+        // of the best of each lane's heads, in 20 bits: eight of a score's mantissa
+        uint32_t h = 0;
 #pragma unroll
-        for (int n = 0; n < kHeadsPerLane; ++n) {
-            double s = kNone;
-            int64_t at;
-            if (n * 64 + lane < lists) look(n * 64 + lane, 0, &s, &at);
-            head[n] = s > kNone ? score_rank(s) : 0u;
-        }
-        // 20 bits: eight of a score's mantissa
-        const uint32_t least = largest_with(20, a.k, [&](uint32_t t) {
-            int c = 0;
-#pragma unroll
-            for (int n = 0; n < kHeadsPerLane; ++n) c += __popcll(__ballot(head[n] >= t));
-            return c;
-        });
+        for (int n = 0; n < kHeadsPerLane; ++n) h = max(h, s_heads[n * 64 + lane]);
+        const uint32_t least = largest_with(20, a.k, [&](uint32_t t) { return __popcll(__ballot(h >= t)); });
         if (lane == 0) s_least = max(least, 1u);
     }
     __syncthreads();
     const uint32_t least = s_least;
-    for (int i = tid; i < lists * a.k; i += kJoinThreads) {
-        const int list = i / a.k;
-        double s;
-        int64_t at;
-        look(list, i - list * a.k, &s, &at);
-        if (s > kNone && score_rank(s) >= least) {
-            const int p = atomicAdd(&s_count, 1);
-            if (p < kJoined) {
-                s_score[p] = s;
-                s_where[p] = at;
+    const auto enlist = [&](int list, uint32_t r) {
+        if (r < least) return;
+        const int p = atomicAdd(&s_n_lists, 1);
+        if (p < kJoined) s_lists[p] = list;
+    };
+#pragma unroll
+    for (int n = 0; n < kMine; ++n) enlist(n * kJoinThreads + tid, rank[n]);
+    for (int i = kMine * kJoinThreads + tid; i < lists; i += kJoinThreads)
+        enlist(i, rank_of_list(i, part[static_cast<int64_t>(i) * a.k]));
+    __syncthreads();
+    const int n_lists = s_n_lists;
+    if (n_lists <= kJoined) {
+        for (int i = tid; i < n_lists * a.k; i += kJoinThreads) {
+            const int l = static_cast<int>(k_div.div(static_cast<uint32_t>(i)));
+            double s;
+            int64_t at;
+            look(s_lists[l], i - l * a.k, &s, &at);
+            if (s > kNone && score_rank(s) >= least) {
+                const int p = atomicAdd(&s_count, 1);
+                if (p < kJoined) s_found[p] = Found{s, at};
             }
         }
+        __syncthreads();
     }
-    __syncthreads();
+    const bool ranked = n_lists <= kJoined && s_count <= kJoined;
     const int count = s_count;
     const auto write = [&](int c, double s, int64_t at) {
         const int64_t o = b * a.k + c;
@@ -346,13 +423,17 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a,
         a.parents[o] = none ? -1 : static_cast<int32_t>(at >> 32);
         a.tokens[o] = none ? -1 : static_cast<int32_t>(at);
     };
-    if (count <= kJoined) {
-        for (int i = tid; i < count; i += kJoinThreads) {
-            const double s = s_score[i];
-            const int64_t at = s_where[i];
+    if (ranked) {
+        // a candidate's place is the number of better ones, counted by eight lanes
+        for (int i0 = 0; i0 < count; i0 += kJoinThreads / 8) {
+            const int i = i0 + (tid >> 3);
+            const Found f = s_found[min(i, count - 1)];
             int place = 0;
-            for (int j = 0; j < count; ++j) place += s_score[j] > s || (s_score[j] == s && s_where[j] < at) ? 1 : 0;
-            if (place < a.k) write(place, s, at);
+            for (int j = tid & 7; j < count; j += 8)
+                place += s_found[j].score > f.score || (s_found[j].score == f.score && s_found[j].where < f.where) ? 1 : 0;
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) place += __shfl_xor(place, o, 64);
+            if (i < count && (tid & 7) == 0 && place < a.k) write(place, f.score, f.where);
         }
         for (int c = count + tid; c < a.k; c += kJoinThreads) write(c, kNone, 0);
         return;
@@ -402,14 +483,43 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a,
 // page, its own, takes the rows of p_w's. A lane holds one unit of the rows of all
 // the beams of a request: it reads the parents' before it writes any, so beams may
 // exchange places, and no other lane touches those bytes. Bound by memory.
+// The ids of full pages: a lane holds one place of all the lists of a request.
+template <int W>
+__device__ __forceinline__ void reorder_lists(const BeamLists& s, int32_t* block_table, const int32_t* __restrict__ parents,
+                                              int page_size, int block, int64_t* s_from) {
+    const int tid = static_cast<int>(threadIdx.x);
+    if (tid < s.n_beams) {
+        const int p = parents[tid];
+        s_from[tid] = p >= 0 && p < s.n_beams && p != tid ? p : -1;
+    }
+    __syncthreads();
+    const int at = block * kReorderThreads + tid;
+    if (at >= s.n_tokens / page_size) return;
+    int32_t* list = block_table + s.bt_offset + at;
+    int32_t id[W];
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+        if (w < s.n_beams && s_from[w] >= 0) id[w] = list[s_from[w] * s.stride];
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+        if (w < s.n_beams && s_from[w] >= 0) list[w * s.stride] = id[w];
+}
+
 template <typename U, int W>
-__global__ __launch_bounds__(kReorderThreads) void reorder_rows_kernel(DescArg d, int layer_off, LayerMinor lm, KVGeom g,
-                                                                       int es, const int32_t* block_table,
+__global__ __launch_bounds__(kReorderThreads) void reorder_kernel(DescArg d, int layer_off, LayerMinor lm, KVGeom g,
+                                                                       int es, int32_t* block_table,
                                                                        const int32_t* __restrict__ parents,
                                                                        int64_t parent_stride, int n_lists,
                                                                        FastDiv inner, FastDiv mid, int token_inner,
-                                                                       int head_units) {
+                                                                       int head_units, unsigned row_blocks,
+                                                                       unsigned page_blocks) {
     __shared__ int64_t s_from[kReorderBeams], s_to[kReorderBeams];   // bytes of the pages, -1: beam stays
+    if (blockIdx.x >= row_blocks) {
+        const unsigned i = blockIdx.x - row_blocks, list = i / page_blocks;
+        reorder_lists<W>(desc_load(desc_at<BeamLists>(d, 0) + list), block_table, parents + list * parent_stride, g.PS,
+                         static_cast<int>(i - list * page_blocks), s_from);
+        return;
+    }
     int l;
     int64_t item;
     lm.at(l, item);
@@ -461,48 +571,18 @@ __global__ __launch_bounds__(kReorderThreads) void reorder_rows_kernel(DescArg d
         if (w < s.n_beams && s_from[w] >= 0) *reinterpret_cast<U*>(base + s_to[w]) = x[w];
 }
 
-// The ids of full pages: a lane holds one place of all the lists of a request.
-template <int W>
-__global__ __launch_bounds__(kReorderThreads) void reorder_lists_kernel(DescArg d, int32_t* block_table,
-                                                                        const int32_t* __restrict__ parents,
-                                                                        int64_t parent_stride, int page_size) {
-    __shared__ int s_from[kReorderBeams];
-    const BeamLists s = desc_load(desc_at<BeamLists>(d, 0) + blockIdx.y);
-    const int tid = static_cast<int>(threadIdx.x);
-    if (tid < s.n_beams) {
-        const int p = parents[blockIdx.y * parent_stride + tid];
-        s_from[tid] = p >= 0 && p < s.n_beams && p != tid ? p : -1;
-    }
-    __syncthreads();
-    const int at = static_cast<int>(blockIdx.x) * kReorderThreads + tid;
-    if (at >= s.n_tokens / page_size) return;
-    int32_t* list = block_table + s.bt_offset + at;
-    int32_t id[W];
-#pragma unroll
-    for (int w = 0; w < W; ++w)
-        if (w < s.n_beams && s_from[w] >= 0) id[w] = list[s_from[w] * s.stride];
-#pragma unroll
-    for (int w = 0; w < W; ++w)
-        if (w < s.n_beams && s_from[w] >= 0) list[w * s.stride] = id[w];
-}
-
 }  // namespace
 
-void launch_select_beams(const SelectArgs& a, int kind, int regs, hipStream_t stream) {
+void launch_select_beams(const SelectArgs& a, int kind, hipStream_t stream) {
     const int64_t units = static_cast<int64_t>(a.B) * a.W * a.splits;
     const unsigned blocks = static_cast<unsigned>((units + kSplitsPerBlock - 1) / kSplitsPerBlock);
-#define DARIC_SS(K)                                                                                   \
-    do {                                                                                              \
-        if (regs == 16) DARIC_LAUNCH((select_split_kernel<K, 16>), blocks, kSplitThreads, 0, stream, a); \
-        else DARIC_LAUNCH((select_split_kernel<K, 64>), blocks, kSplitThreads, 0, stream, a);         \
-    } while (0)
-    if (kind == kBF16) DARIC_SS(kBF16);
-    else if (kind == kF16) DARIC_SS(kF16);
-    else DARIC_SS(kF32);
-#undef DARIC_SS
+    if (kind == kBF16) DARIC_LAUNCH((select_split_kernel<kBF16>), blocks, kSplitThreads, 0, stream, a);
+    else if (kind == kF16) DARIC_LAUNCH((select_split_kernel<kF16>), blocks, kSplitThreads, 0, stream, a);
+    else DARIC_LAUNCH((select_split_kernel<kF32>), blocks, kSplitThreads, 0, stream, a);
     check_launch("select_beams");
     const int per_lane = (a.W * a.splits + 63) / 64;
-    DARIC_LAUNCH(select_join_kernel, static_cast<unsigned>(a.B), kJoinThreads, static_cast<size_t>(per_lane) * 64, stream, a, per_lane);
+    DARIC_LAUNCH(select_join_kernel, static_cast<unsigned>(a.B), kJoinThreads, static_cast<size_t>(per_lane) * 64, stream, a, per_lane,
+                 FastDiv(static_cast<uint32_t>(a.k)));
     check_launch("select_beams join");
 }
 
@@ -512,9 +592,15 @@ void launch_reorder(const DescArg& d, int layer_off, int n_layers, const KVGeom&
     const int head_units = g.D * es / unit;
     const FastDiv inner(static_cast<uint32_t>(head_units)), mid(static_cast<uint32_t>(g.H));
     const int token_inner = g.ss < g.sh ? 1 : 0;
-    for_layer_minor(n_layers, tiles, [&](const LayerMinor& lm, unsigned blocks) {
-#define DARIC_RW(U, W) DARIC_LAUNCH((reorder_rows_kernel<U, W>), blocks, kReorderThreads, 0, stream, d, layer_off, lm, g, \
-                                    es, block_table, parents, parent_stride, n_lists, inner, mid, token_inner, head_units)
+    // the lists' blocks stand behind the rows' of one launch: they write other places of
+    // block_table than the rows' read
+    const unsigned page_blocks = static_cast<unsigned>((most_pages + kReorderThreads - 1) / kReorderThreads);
+    unsigned list_blocks = page_blocks * static_cast<unsigned>(n_lists);
+    const auto launch = [&](const LayerMinor& lm, unsigned row_blocks) {
+        const unsigned blocks = row_blocks + list_blocks;
+#define DARIC_RW(U, W) DARIC_LAUNCH((reorder_kernel<U, W>), blocks, kReorderThreads, 0, stream, d, layer_off, lm, g, es, \
+                                    block_table, parents, parent_stride, n_lists, inner, mid, token_inner, head_units, \
+                                    row_blocks, std::max(1u, page_blocks))
 #define DARIC_RU(U)                                 \
     do {                                            \
         if (most_beams <= 4) DARIC_RW(U, 4);        \
@@ -530,12 +616,10 @@ void launch_reorder(const DescArg& d, int layer_off, int n_layers, const KVGeom&
 #undef DARIC_RU
 #undef DARIC_RW
         check_launch("reorder_beams");
-    });
-    if (most_pages == 0) return;
-    const dim3 grid(static_cast<unsigned>((most_pages + kReorderThreads - 1) / kReorderThreads), static_cast<unsigned>(n_lists));
-    if (most_beams <= 8) DARIC_LAUNCH((reorder_lists_kernel<8>), grid, kReorderThreads, 0, stream, d, block_table, parents, parent_stride, g.PS);
-    else DARIC_LAUNCH((reorder_lists_kernel<32>), grid, kReorderThreads, 0, stream, d, block_table, parents, parent_stride, g.PS);
-    check_launch("reorder_beams lists");
+        list_blocks = 0;
+    };
+    for_layer_minor(n_layers, tiles, launch);
+    if (list_blocks > 0) launch(LayerMinor{}, 0);
 }
 
 }  // namespace daric

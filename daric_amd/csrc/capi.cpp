@@ -2128,15 +2128,22 @@ void set_rotation(AppendArgs& a, const daric_rope* rope, float m) {
     a.m = m;
 }
 
-// Rows of a workgroup: as many as have their angles computed in one round of its
-// lanes and the rest of a few, but no more than leave the chip full.
-constexpr int64_t kAppendGroups = 1024;
-int64_t append_tile(int64_t rows, int R) {
-    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(8, 512 / std::max(R, 64)));
+// Rows of a workgroup, `items` accesses each: one while there are workgroups for fewer than
+// kAppendGroups more, then as many as leave so many, up to kAppendItems accesses. MI355X, 1,
+// 2 and 4 rows of 40 x 128 bf16: 256 rows 5.1, 7.1 and 8.0 us, 1024 6.7, 7.5 and 9.9, 2048
+// 11.4, 9.9 and 10.8, 3500 16.1, 15.4 and 14.5, 16384 78, 68 and 66 (8 rows: 70).
+constexpr int64_t kAppendGroups = 1024, kAppendItems = 2048, kAppendTile = 32;
+int64_t append_tile(int64_t rows, int64_t items, int R) {
     int64_t tile = 1;
-    while (tile < most && rows / (2 * tile) >= kAppendGroups) tile *= 2;
+    while (tile < kAppendTile && rows / (2 * tile) >= kAppendGroups && 2 * tile * items <= kAppendItems &&
+           2 * tile * R <= 4096)
+        tile *= 2;
     return tile;
 }
+// Bytes of rows and codes from which they are written past the caches. MI355X, q of 40 x 128
+// bf16: 10 MB 8.4 -> 7.5 us, 21 MB 11.5 -> 9.9, 36 MB 20.2 -> 14.5, 168 MB 72 -> 66; at 3 MB
+// alike, and there what reads them next finds them in the caches.
+constexpr int64_t kAppendPast = 8 << 20;
 
 // Finishes the arguments and launches over the sequences.
 void append(AppendArgs& a, std::vector<AppendSeq>& seqs, int from, int to, int device, int64_t rows, hipStream_t stream) {
@@ -2165,7 +2172,8 @@ void append(AppendArgs& a, std::vector<AppendSeq>& seqs, int from, int to, int d
     a.d_rot = FastDiv(static_cast<uint32_t>(a.rot_items));
     a.d_copy = FastDiv(static_cast<uint32_t>(a.copy_items));
     a.d_half = FastDiv(static_cast<uint32_t>(std::max(1, a.R / 2)));
-    const int64_t tile = append_tile(rows, a.R);
+    const int64_t tile = append_tile(rows, per, a.R);
+    const bool past = rows * a.D * (static_cast<int64_t>(a.Hq) * es + a.g.H * (a.g.v_off >= 0 ? 2 : 1) * ces) >= kAppendPast;
     int64_t tiles = 0;
     a.one_tile = 1;
     for (AppendSeq& s : seqs) {
@@ -2179,7 +2187,7 @@ void append(AppendArgs& a, std::vector<AppendSeq>& seqs, int from, int to, int d
     DeviceGuard guard(device);
     const size_t bytes = seqs.size() * sizeof(AppendSeq);
     DescHandOver ho(device, seqs.data(), bytes, stream, a.one_tile != 0 && bytes <= 16 * 1024);
-    launch_append(ho.arg(), a, from, to, vec, tiles, stream);
+    launch_append(ho.arg(), a, from, to, vec, past, tiles, stream);
 }
 
 }  // namespace
@@ -2326,17 +2334,9 @@ int daric_append_tokens(const daric_tensor* layer, int page_first, const daric_t
 
 namespace {
 
-// Registers of a split's lane: 16 where splits of 64 would leave half the chip's wavefronts
-// idle.
-int select_regs(int64_t B, int64_t W, int64_t V, int es) {
-    const int64_t big = split_values(64, es), small = split_values(16, es);
-    const bool few = B * W * ((V + big - 1) / big) < 512;
-    return few && W * ((V + small - 1) / small) <= 4096 ? 16 : 64;
-}
-
 struct SelectCall {
     SelectArgs a{};
-    int kind = -1, regs = 64, device = -1;
+    int kind = -1, device = -1;
     int64_t units() const { return static_cast<int64_t>(a.B) * a.W * a.splits; }
     int64_t list_bytes() const { return units() * a.k * static_cast<int64_t>(sizeof(BeamCandidate)); }
     int64_t bytes() const { return list_bytes() + units() * 2 * static_cast<int64_t>(sizeof(float)); }
@@ -2356,8 +2356,7 @@ SelectCall select_call(const daric_tensor* logits, int64_t k) {
     DARIC_CHECK(W <= kMaxBeams, "select_beams takes up to ", kMaxBeams, " beams of a request, got ", W);
     DARIC_CHECK(k >= 1 && k <= kMaxCandidates, "select_beams chooses 1 to ", kMaxCandidates, " candidates, got ", k);
     DARIC_CHECK(V <= kMaxTokens, "the vocabulary is too large");
-    c.regs = select_regs(B, W, V, logits->elem_size);
-    const int64_t per = split_values(c.regs, logits->elem_size);
+    const int64_t per = kSplitBytes / logits->elem_size;
     const int64_t splits = (V + per - 1) / per;
     DARIC_CHECK(W * splits <= 32768, "the vocabulary is too large for ", W, " beams");
     DARIC_CHECK(B * W * splits <= kMaxTiles && B <= kMaxTiles, "too many rows in one select_beams call");
@@ -2370,6 +2369,8 @@ SelectCall select_call(const daric_tensor* logits, int64_t k) {
     a.V = V;
     a.k = static_cast<int32_t>(k);
     a.splits = static_cast<int32_t>(splits);
+    a.d_splits = FastDiv(static_cast<uint32_t>(splits));
+    a.d_beams = FastDiv(static_cast<uint32_t>(W));
     return c;
 }
 
@@ -2427,7 +2428,7 @@ int daric_select_beams(const daric_tensor* logits, const daric_tensor* scores, c
         a.part = static_cast<BeamCandidate*>(workspace);
         a.part_ms = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + c.list_bytes());
         DeviceGuard guard(c.device);
-        launch_select_beams(a, c.kind, c.regs, as_stream(stream));
+        launch_select_beams(a, c.kind, as_stream(stream));
     });
 }
 
@@ -2497,7 +2498,7 @@ int daric_reorder_beams(const daric_tensor* layers, int64_t n_layers, int page_f
         }
         check_apart(ranges, "block list");
         if (tiles == 0 && most_pages == 0) return;
-        DARIC_CHECK(n <= 65535, "too many requests in one reorder_beams call");
+        DARIC_CHECK((most_pages / kReorderThreads + 1) * n <= kMaxTiles / 2, "too many requests in one reorder_beams call");
         std::vector<const void*> data;
         for (int64_t i = 0; i < n_layers; ++i) data.push_back(layers[i].data);
         std::sort(data.begin(), data.end());
