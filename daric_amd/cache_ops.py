@@ -26,9 +26,10 @@ from __future__ import annotations
 
 import array
 import ctypes
+import struct
 from collections.abc import Sequence
 from contextlib import nullcontext
-from itertools import chain, repeat
+from itertools import chain
 from typing import Optional
 
 import numpy as np
@@ -81,6 +82,9 @@ def _on_stream(stream: int, device: torch.device):
     if stream == _resolve_stream(0, device):
         return nullcontext()
     return torch.cuda.stream(_ext_stream(stream, device))
+
+
+_HERE = nullcontext()
 
 
 def _record(stream: int, device: torch.device, *tensors) -> None:
@@ -493,19 +497,26 @@ def _sequences(seqs):
     return _tuples(seqs, (5, 4), _SEQUENCES)
 
 
+_ROW_STRUCTS: dict = {}
+
+
 def _rows_of_ints(entries, widths, what: str):
-    """(address of int64 [n, widths[0]], n, keep-alive) of integer tuples, as _tuples, where
-    widths[1], if there is one, is one less. Lists of equal tuples without a Python-level loop or numpy: 48 of
-    four ints take 4.0 us on the host, through numpy 9.5 (MI355X host)."""
+    """(int64 [n, widths[0]] as bytes or its address, n, keep-alive) of integer tuples, as
+    _tuples, where widths[1], if there is one, is one less. Lists without a Python-level loop
+    or numpy: 48 tuples of four ints take 5 us on the host, through numpy 17."""
     if type(entries) is list and entries:
-        n = len(entries[0]) if type(entries[0]) is tuple else 0
-        if n in widths and set(map(type, entries)) == {tuple} and set(map(len, entries)) == {n}:
-            try:
-                flat = array.array("q", list(chain.from_iterable(
-                    entries if n == widths[0] else zip(*zip(*entries), repeat(0)))))
-                return flat.buffer_info()[0], len(entries), flat
-            except TypeError:       # not ints: numpy converts or refuses them
-                pass
+        try:
+            n, width = len(entries), len(entries[0])
+            if n <= 1024 and width in widths and set(map(len, entries)) == {width}:
+                pack = _ROW_STRUCTS.get((n, width, widths))
+                if pack is None:
+                    if len(_ROW_STRUCTS) >= 256:
+                        _ROW_STRUCTS.clear()
+                    row = f"{width}q{8 * (widths[0] - width)}x"
+                    pack = _ROW_STRUCTS[(n, width, widths)] = struct.Struct("@" + row * n).pack
+                return pack(*chain.from_iterable(entries)), n, None
+        except (TypeError, struct.error):       # not ints: numpy converts or refuses them
+            pass
     return _tuples(entries, widths, what)
 
 
@@ -526,8 +537,11 @@ def _scale(scale: Optional[float], q: torch.Tensor) -> float:
 def _no_backward(what: str, *tensors) -> None:
     """These calls have no backward pass: an input that asks for a gradient is
     refused, not answered by an output that silently has none."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad(), or detach what requires a gradient")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad(), or detach what "
+                                   "requires a gradient")
 
 
 def _layer_desc(layer: torch.Tensor):
@@ -650,7 +664,7 @@ def rotate_rows(rows: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Ten
     rope = _rope(inv_freq, rotary_dim, is_neox_style, dev)
     given = out                 # what is made here belongs to `st` already
     if out is None:
-        with _on_stream(st, dev):
+        with _on_stream(st, dev) if stream else _HERE:
             out = torch.empty(rows.shape, dtype=rows.dtype, device=dev)
     check(load().daric_rotate_rows(packed(rows), packed(positions), ctypes.byref(rope), float(attention_scale), packed(out), st))
     _record(st, dev, rows, positions, inv_freq, given)
@@ -683,7 +697,7 @@ def append_tokens(layer: torch.Tensor, page_first: bool, block_table: torch.Tens
         q_out = None
     given = q_out               # what is made here belongs to `st` already
     if q is not None and q_out is None:
-        with _on_stream(st, dev):
+        with _on_stream(st, dev) if stream else _HERE:
             q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     check(load().daric_append_tokens(packed(layer), 1 if page_first else 0, packed(block_table), packed(k), _packed(v),
                                      addr, n, _packed(positions), ctypes.byref(rope) if rope is not None else None,
@@ -712,7 +726,7 @@ def select_beams(logits: torch.Tensor, scores: torch.Tensor, k: Optional[int] = 
     lib, need = load(), ctypes.c_int64()
     check(lib.daric_select_workspace(ld, k, ctypes.byref(need)))
     shape = (logits.shape[0], k)
-    with _on_stream(st, dev):
+    with _on_stream(st, dev) if stream else _HERE:
         out = torch.empty(shape, dtype=torch.float32, device=dev)
         parents = torch.empty(shape, dtype=torch.int32, device=dev)
         tokens = torch.empty(shape, dtype=torch.int32, device=dev)

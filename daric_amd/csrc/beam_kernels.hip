@@ -486,7 +486,7 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a,
 // The ids of full pages: a lane holds one place of all the lists of a request.
 template <int W>
 __device__ __forceinline__ void reorder_lists(const BeamLists& s, int32_t* block_table, const int32_t* __restrict__ parents,
-                                              int page_size, int block, int64_t* s_from) {
+                                              int page_size, int block, int* s_from) {
     const int tid = static_cast<int>(threadIdx.x);
     if (tid < s.n_beams) {
         const int p = parents[tid];
@@ -513,7 +513,8 @@ __global__ __launch_bounds__(kReorderThreads) void reorder_kernel(DescArg d, int
                                                                        FastDiv inner, FastDiv mid, int token_inner,
                                                                        int head_units, unsigned row_blocks,
                                                                        unsigned page_blocks) {
-    __shared__ int64_t s_from[kReorderBeams], s_to[kReorderBeams];   // bytes of the pages, -1: beam stays
+    __shared__ int s_from[kReorderBeams], s_to[kReorderBeams];       // pages; to 0: beam stays
+    __shared__ int s_moves;
     if (blockIdx.x >= row_blocks) {
         const unsigned i = blockIdx.x - row_blocks, list = i / page_blocks;
         reorder_lists<W>(desc_load(desc_at<BeamLists>(d, 0) + list), block_table, parents + list * parent_stride, g.PS,
@@ -528,29 +529,38 @@ __global__ __launch_bounds__(kReorderThreads) void reorder_kernel(DescArg d, int
     const BeamLists s = desc_load(lists + li);
     const int full = s.n_tokens / g.PS, rest = s.n_tokens - full * g.PS;
     const int tid = static_cast<int>(threadIdx.x);
-    if (tid < s.n_beams) {
-        const int32_t* last = block_table + s.bt_offset + full;
-        const int p = parents[li * parent_stride + tid];
-        s_from[tid] = -1;
-        if (p >= 0 && p < s.n_beams && p != tid) {
-            const int from = last[p * s.stride], to = last[tid * s.stride];
-            if (from > 0 && from < g.num_blocks && to > 0 && to < g.num_blocks && from != to) {
-                s_from[tid] = static_cast<int64_t>(from) * g.sb * es;
-                s_to[tid] = static_cast<int64_t>(to) * g.sb * es;
+    if (tid < W) {
+        int from = 0, to = 0;
+        if (tid < s.n_beams) {
+            const int32_t* last = block_table + s.bt_offset + full;
+            const int p = parents[li * parent_stride + tid];
+            if (p >= 0 && p < s.n_beams && p != tid) {
+                from = last[p * s.stride];
+                to = last[tid * s.stride];
+                if (from <= 0 || from >= g.num_blocks || to <= 0 || to >= g.num_blocks || from == to) from = to = 0;
             }
         }
+        // beams that stay read what the first that moves does, and write nothing: loads
+        // without branches, all in flight together
+        const unsigned long long moves = __ballot(from != 0);
+        const int first = __shfl(from, __ffsll(static_cast<long long>(moves | 1ull << 63)) - 1, 64);
+        s_from[tid] = from != 0 ? from : first;
+        s_to[tid] = to;
+        if (tid == 0) s_moves = moves != 0 ? 1 : 0;
     }
     __syncthreads();
-    // unit -> (K or V, outer, inner, unit of the row); tokens are the inner index of
-    // head-major pages, heads of the others
-    const int units = (g.v_off >= 0 ? 2 : 1) * rest * g.H * head_units;
-    const int i = (static_cast<int>(item) - s.tile_begin) * kReorderThreads + tid;
+    if (s_moves == 0) return;
+    // a workgroup's units are K's or V's: (outer, inner, unit of the row); tokens are the
+    // inner index of head-major pages, heads of the others
+    const int units = rest * g.H * head_units;
+    const int blocks = (units + kReorderThreads - 1) / kReorderThreads;
+    int block = static_cast<int>(item) - s.tile_begin;
+    const bool v = block >= blocks;
+    block -= v ? blocks : 0;
+    const int i = block * kReorderThreads + tid;
     if (i >= units) return;
-    const int per_plane = rest * g.H * head_units;
-    const int v = i >= per_plane ? 1 : 0;
-    int r = i - v * per_plane;
-    const int row = static_cast<int>(inner.div(static_cast<uint32_t>(r)));       // head_units
-    const int u = r - row * head_units;
+    const int row = static_cast<int>(inner.div(static_cast<uint32_t>(i)));       // head_units
+    const int u = i - row * head_units;
     int token, head;
     if (token_inner) {
         head = row / rest;
@@ -559,16 +569,19 @@ __global__ __launch_bounds__(kReorderThreads) void reorder_kernel(DescArg d, int
         token = static_cast<int>(mid.div(static_cast<uint32_t>(row)));           // H
         head = row - token * g.H;
     }
-    uint8_t* base = desc_at<uint8_t*>(d, layer_off)[l] +
-                    (static_cast<int64_t>(token) * g.ss + static_cast<int64_t>(head) * g.sh + (v != 0 ? g.v_off : 0)) * es +
-                    static_cast<int64_t>(u) * static_cast<int>(sizeof(U));
+    uint8_t* const plane = desc_at<uint8_t*>(d, layer_off)[l] + (v ? g.v_off * es : 0);
+    const int64_t at = (static_cast<int64_t>(token) * g.ss + static_cast<int64_t>(head) * g.sh) * es +
+                       static_cast<int64_t>(u) * static_cast<int>(sizeof(U));
+    const int64_t page = g.sb * es;
     U x[W];
 #pragma unroll
     for (int w = 0; w < W; ++w)
-        if (w < s.n_beams && s_from[w] >= 0) x[w] = *reinterpret_cast<const U*>(base + s_from[w]);
+        x[w] = *reinterpret_cast<const U*>(plane + __builtin_amdgcn_readfirstlane(s_from[w]) * page + at);
 #pragma unroll
-    for (int w = 0; w < W; ++w)
-        if (w < s.n_beams && s_from[w] >= 0) *reinterpret_cast<U*>(base + s_to[w]) = x[w];
+    for (int w = 0; w < W; ++w) {
+        const int to = __builtin_amdgcn_readfirstlane(s_to[w]);
+        if (to != 0) *reinterpret_cast<U*>(plane + to * page + at) = x[w];
+    }
 }
 
 }  // namespace

@@ -2460,7 +2460,8 @@ int daric_reorder_beams(const daric_tensor* layers, int64_t n_layers, int page_f
             return ok;
         };
         while (unit > 1 && !allows(unit)) unit /= 2;
-        const int64_t token_units = (g.v_off >= 0 ? 2 : 1) * g.H * (g.D * es / unit);
+        const int64_t planes = g.v_off >= 0 ? 2 : 1;
+        const int64_t token_units = g.H * (g.D * es / unit);       // of K, or of V
         DARIC_CHECK(token_units <= kIntMax / g.PS / 2, "a page of the cache is too large for reorder_beams");
         std::vector<BeamLists> lists;
         std::vector<std::pair<int64_t, int64_t>> ranges;
@@ -2489,7 +2490,7 @@ int daric_reorder_beams(const daric_tensor* layers, int64_t n_layers, int page_f
                 ranges.emplace_back(s.bt_offset, (s.n_beams - 1) * s.stride + pages);
             }
             if (s.n_beams > 1) {
-                tiles += (s.n_tokens % g.PS * token_units + kReorderThreads - 1) / kReorderThreads;
+                tiles += planes * ((s.n_tokens % g.PS * token_units + kReorderThreads - 1) / kReorderThreads);
                 most_pages = std::max(most_pages, s.n_tokens / g.PS);
                 most_beams = std::max(most_beams, s.n_beams);
                 DARIC_CHECK(tiles <= kMaxTiles, "too many rows in one reorder_beams call");
