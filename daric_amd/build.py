@@ -29,7 +29,7 @@ BUILD = os.path.join(ROOT, "_build")
 LIB = os.path.join(LIBDIR, "libdaric_cache_ops.so")
 HOSTTEST_LIB = os.path.join(LIBDIR, "libdaric_hosttest.so")
 
-SOURCES = ["capi.cpp", "runtime.cpp", "copy_kernels.hip", "rope_kernels.hip", "select_kernels.hip",
+SOURCES = ["capi.cpp", "runtime.cpp", "pyviews.cpp", "copy_kernels.hip", "rope_kernels.hip", "select_kernels.hip",
            "token_kernels.hip", "noalloc.hip", "attend_bf16.hip", "attend_f16.hip", "attend_e4m3_bf16.hip",
            "attend_e4m3_f16.hip", "evict_kernels.hip", "append_kernels.hip", "beam_kernels.hip"]
 

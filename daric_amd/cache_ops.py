@@ -30,13 +30,14 @@ import struct
 from collections.abc import Sequence
 from contextlib import nullcontext
 from itertools import chain
+from operator import attrgetter
 from typing import Optional
 
 import numpy as np
 import torch
 
 from . import _lib
-from ._lib import I64, DaricChunk, DaricRope, check, desc, load, packed, str_array
+from ._lib import I64, DaricChunk, DaricRope, check, desc, layer_views, load, str_array, views
 
 __all__ = [
     "CacheCopier", "batched_memcpy_d2h", "batched_memcpy_h2d", "rerotate_pages",
@@ -85,6 +86,7 @@ def _on_stream(stream: int, device: torch.device):
 
 
 _HERE = nullcontext()
+_REQUIRES_GRAD = attrgetter("requires_grad")
 
 
 def _record(stream: int, device: torch.device, *tensors) -> None:
@@ -520,10 +522,6 @@ def _rows_of_ints(entries, widths, what: str):
     return _tuples(entries, widths, what)
 
 
-def _packed(t: Optional[torch.Tensor]):
-    return packed(t) if t is not None else None
-
-
 def _ref(t: Optional[torch.Tensor]):
     return ctypes.byref(desc(t)) if t is not None else None
 
@@ -666,7 +664,8 @@ def rotate_rows(rows: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Ten
     if out is None:
         with _on_stream(st, dev) if stream else _HERE:
             out = torch.empty(rows.shape, dtype=rows.dtype, device=dev)
-    check(load().daric_rotate_rows(packed(rows), packed(positions), ctypes.byref(rope), float(attention_scale), packed(out), st))
+    (rd, pd, od), _keep = views(rows, positions, out)
+    check(load().daric_rotate_rows(rd, pd, ctypes.byref(rope), float(attention_scale), od, st))
     _record(st, dev, rows, positions, inv_freq, given)
     return out
 
@@ -699,9 +698,10 @@ def append_tokens(layer: torch.Tensor, page_first: bool, block_table: torch.Tens
     if q is not None and q_out is None:
         with _on_stream(st, dev) if stream else _HERE:
             q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    check(load().daric_append_tokens(packed(layer), 1 if page_first else 0, packed(block_table), packed(k), _packed(v),
-                                     addr, n, _packed(positions), ctypes.byref(rope) if rope is not None else None,
-                                     float(attention_scale), _packed(q), _packed(q_out), _packed(k_scale), _packed(v_scale), st))
+    (ld, bt, kd, vd, pd, qd, od, ks, vs), _views = views(layer, block_table, k, v, positions, q, q_out, k_scale, v_scale)
+    check(load().daric_append_tokens(ld, 1 if page_first else 0, bt, kd, vd, addr, n, pd,
+                                     ctypes.byref(rope) if rope is not None else None, float(attention_scale), qd, od,
+                                     ks, vs, st))
     _record(st, dev, block_table, k, v, positions, inv_freq, q, given, k_scale, v_scale)
     return q_out
 
@@ -722,18 +722,18 @@ def select_beams(logits: torch.Tensor, scores: torch.Tensor, k: Optional[int] = 
     if k is None:
         k = logits.shape[1] if logits.dim() == 3 else 1
     k = int(k)
-    ld = packed(logits)
-    lib, need = load(), ctypes.c_int64()
-    check(lib.daric_select_workspace(ld, k, ctypes.byref(need)))
-    shape = (logits.shape[0], k)
+    shape = (logits.shape[0] if logits.dim() else 0, k)
     with _on_stream(st, dev) if stream else _HERE:
         out = torch.empty(shape, dtype=torch.float32, device=dev)
         parents = torch.empty(shape, dtype=torch.int32, device=dev)
         tokens = torch.empty(shape, dtype=torch.int32, device=dev)
-        work = torch.empty(need.value, dtype=torch.uint8, device=dev)
     end = ended.view(torch.uint8) if ended is not None and ended.dtype == torch.bool else ended
-    check(lib.daric_select_beams(ld, packed(scores), _packed(end), int(end_token), packed(out), packed(parents),
-                                 packed(tokens), work.data_ptr(), need.value, st))
+    (ld, sd, ed, od, pd, td), _views = views(logits, scores, end, out, parents, tokens)
+    lib, need = load(), ctypes.c_int64()
+    check(lib.daric_select_workspace(ld, k, ctypes.byref(need)))
+    with _on_stream(st, dev) if stream else _HERE:
+        work = torch.empty(need.value, dtype=torch.uint8, device=dev)
+    check(lib.daric_select_beams(ld, sd, ed, int(end_token), od, pd, td, work.data_ptr(), need.value, st))
     _record(st, dev, logits, scores, end)
     return out, parents, tokens
 
@@ -748,12 +748,13 @@ def reorder_beams(layers: Sequence[torch.Tensor], page_first: bool, block_table:
     every layer at once. Up to 32 beams of a request; caches of any type and
     layout."""
     layers = list(layers)
-    _no_backward("reorder_beams", *layers)
+    if torch.is_grad_enabled() and any(map(_REQUIRES_GRAD, layers)):
+        _no_backward("reorder_beams", *layers)
     dev = layers[0].device
     st = _resolve_stream(stream, dev)
     addr, n, _keep = _rows_of_ints(beams, (4,), "beams must be (bt_offset, stride, n_beams, n_tokens) entries of ints")
-    check(load().daric_reorder_beams(_layer_array(layers), len(layers), 1 if page_first else 0, packed(block_table),
-                                     packed(parents), addr, n, st))
+    (bt, pd), _views = views(block_table, parents)
+    check(load().daric_reorder_beams(layer_views(layers), len(layers), 1 if page_first else 0, bt, pd, addr, n, st))
     _record(st, dev, block_table, parents)
 
 

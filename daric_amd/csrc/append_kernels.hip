@@ -111,15 +111,18 @@ struct Values {
     }
 };
 
-template <int FROM, int TO, int VEC, bool PAST>
-__global__ __launch_bounds__(kThreads) void append_kernel(DescArg d, AppendArgs a) {
+__device__ __forceinline__ DescPtr<AppendSeq> sequences(const DescArg& d) { return desc_at<AppendSeq>(d, 0); }
+__device__ __forceinline__ DescPtr<AppendSeq> sequences(const FewSeqs& d) { return (DescPtr<AppendSeq>)d.s; }
+
+template <int FROM, int TO, int VEC, bool PAST, class Desc>
+__global__ __launch_bounds__(kThreads) void append_kernel(Desc d, AppendArgs a) {
     extern __shared__ __align__(16) float s_turn[];      // cosines and sines, [tile][R / 2] each
     __shared__ int64_t s_slot[kThreads / 2];             // K element of each row's token, -1: nowhere
     using From = Values<FROM, VEC>;
     using To = Values<TO, VEC>;
     const int tid = static_cast<int>(threadIdx.x);
     const int block = static_cast<int>(blockIdx.x);
-    const DescPtr<AppendSeq> seqs = desc_at<AppendSeq>(d, 0);
+    const DescPtr<AppendSeq> seqs = sequences(d);
     const int si = a.one_tile ? block : find_by_tile(seqs, a.n_seqs, block);
     const AppendSeq s = desc_load(seqs + si);
     const int t0 = (block - s.tile_begin) * a.tile;
@@ -281,11 +284,10 @@ __global__ __launch_bounds__(kThreads) void append_kernel(DescArg d, AppendArgs 
     }
 }
 
-}  // namespace
-
-void launch_append(const DescArg& d, const AppendArgs& a, int from, int to, int vec, bool past, int64_t tiles, hipStream_t stream) {
+template <class Desc>
+void launch(const Desc& d, const AppendArgs& a, int from, int to, int vec, bool past, int64_t tiles, hipStream_t stream) {
     const size_t lds = static_cast<size_t>(a.tile) * a.R * sizeof(float);
-#define DARIC_AP(F, T, V, P) DARIC_LAUNCH((append_kernel<F, T, V, P>), static_cast<unsigned>(tiles), kThreads, lds, stream, d, a)
+#define DARIC_AP(F, T, V, P) DARIC_LAUNCH((append_kernel<F, T, V, P, Desc>), static_cast<unsigned>(tiles), kThreads, lds, stream, d, a)
 #define DARIC_AV(F, T)                    \
     do {                                  \
         if (vec == 8 && past) DARIC_AP(F, T, 8, true); \
@@ -307,6 +309,15 @@ void launch_append(const DescArg& d, const AppendArgs& a, int from, int to, int 
 #undef DARIC_AV
 #undef DARIC_AP
     check_launch("append_tokens");
+}
+
+}  // namespace
+
+void launch_append(const FewSeqs& d, const AppendArgs& a, int from, int to, int vec, bool past, int64_t tiles, hipStream_t stream) {
+    launch(d, a, from, to, vec, past, tiles, stream);
+}
+void launch_append(const DescArg& d, const AppendArgs& a, int from, int to, int vec, bool past, int64_t tiles, hipStream_t stream) {
+    launch(d, a, from, to, vec, past, tiles, stream);
 }
 
 }  // namespace daric

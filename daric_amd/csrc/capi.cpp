@@ -2185,6 +2185,12 @@ void append(AppendArgs& a, std::vector<AppendSeq>& seqs, int from, int to, int d
     a.tile = static_cast<int32_t>(tile);
     a.n_seqs = static_cast<int32_t>(seqs.size());
     DeviceGuard guard(device);
+    if (seqs.size() <= static_cast<size_t>(FewSeqs::kMost)) {
+        FewSeqs few{};
+        std::copy(seqs.begin(), seqs.end(), few.s);
+        launch_append(few, a, from, to, vec, past, tiles, stream);
+        return;
+    }
     const size_t bytes = seqs.size() * sizeof(AppendSeq);
     DescHandOver ho(device, seqs.data(), bytes, stream, a.one_tile != 0 && bytes <= 16 * 1024);
     launch_append(ho.arg(), a, from, to, vec, past, tiles, stream);

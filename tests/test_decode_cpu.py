@@ -308,6 +308,46 @@ def test_reorder_refusals(lib):
 
 
 # ------------------------------------------------------------ the Python layer
+def test_views_of_tensors_are_their_attributes():
+    """Through torch's own function and one by one: the same bytes."""
+    base = torch.zeros(4, 40, 2, 16)
+    ts = [base, None, base[:, ::2, 1:, 3], base.permute(2, 0, 3, 1), base[:0], torch.zeros(()), torch.zeros(3, 3, requires_grad=True).t(),
+          base[:1].expand(5, 40, 2, 16)] + [torch.zeros(1, 3, 1, dtype=t)[:, 1:] for t in (*_lib.DTYPE_CODES, torch.bool, torch.float64)]
+    for some in (ts[:8], ts[8:], [None] * 3, []):
+        at, arr = _lib.views(*some)
+        assert len(at) == len(some)
+        for i, (a, t) in enumerate(zip(at, some)):
+            assert (a is None) == (t is None)
+            if t is not None:
+                assert a == ctypes.addressof(arr[i]) and bytes(arr[i]) == _lib.packed(t), (t.dtype, t.shape, t.stride())
+    slow = _lib._Views()
+    assert slow.fill is not None or not hasattr(torch.Tensor, "__dlpack_c_exchange_api__")
+    slow.fill = None
+    one = [t for t in ts if t is not None]
+    assert bytes(slow.of(one)) == bytes(_lib.layer_views(one))
+    for bad in (3, "x", np.zeros(3)):
+        with pytest.raises(Exception):
+            _lib.views(torch.zeros(3), bad)
+    with pytest.raises(RuntimeError, match="rank"):
+        _lib.views(torch.zeros([1] * 9))
+
+
+def test_rows_of_ints():
+    take = lambda e: cache_ops._rows_of_ints(e, (5, 4), "refused")
+    def values(e):
+        at, n, keep = take(e)
+        if isinstance(at, bytes):
+            return np.frombuffer(at, np.int64).reshape(n, 5).tolist()
+        return keep.tolist() if n else []
+    assert values([(1, 2, 3, 4), (5, 6, 7, 2 ** 62)]) == [[1, 2, 3, 4, 0], [5, 6, 7, 2 ** 62, 0]]
+    assert values([(1, 2, 3, 4, 5)] * 2000) == [[1, 2, 3, 4, 5]] * 2000
+    assert values([[1, 2, 3, 4]]) == values(np.array([[1, 2, 3, 4]])) == values(((1, 2, 3, np.int64(4)),)) == [[1, 2, 3, 4, 0]]
+    assert values([]) == values(()) == []
+    for bad in ([(1, 2, 3)], [(1, 2, 3, 4.0)], [(1, 2, 3, 4), (1, 2, 3)], [(1, 2, 3, "4")], [1, 2], [(1, 2, 3, 4), (1, 2, 3, 4, 5)], [None]):
+        with pytest.raises((ValueError, TypeError)):
+            take(bad)
+
+
 def test_python_refusals():
     x = torch.zeros(2, 2, 8, dtype=torch.bfloat16)
     f, p = torch.ones(4), torch.zeros(2, dtype=torch.int64)
