@@ -13,6 +13,8 @@
 // to 48 bits, rounded once, and what follows the splits' fp32 sums is fp64.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "append.h"
 #include "beams.h"
 #include "elem.h"
@@ -25,6 +27,9 @@ namespace {
 constexpr int kSplitThreads = 256;                     // wavefronts of a workgroup work apart
 constexpr int kSplitsPerBlock = kSplitThreads / 64;
 constexpr int kListed = 512;                           // candidates that a wavefront ranks
+// Candidates up to which thresholds are taken of one maximum a lane, with one test a step:
+// the looser, the more of the 64 lanes are asked for.
+constexpr int kFewCandidates = 16;
 
 // Order of a type's values as unsigned numbers, in the leading bits that they differ
 // in as fp32; -0 as +0, NaN as -inf.
@@ -40,7 +45,24 @@ struct Rank {
     static __device__ __forceinline__ float value(uint32_t r) {
         return u2f((r & 0x80000000u) ? r & 0x7fffffffu : ~r & kMask);
     }
+    // A value and its place in a split (lower places first) as one number: a rank of 19
+    // bits and a place below 2^12 fit in one word.
+    static constexpr int kPlaceBits = 12;
+    using Key = typename std::conditional<KIND == kF32, uint64_t, uint32_t>::type;
+    static __device__ __forceinline__ Key key(uint32_t rank, int place) {
+        if constexpr (KIND == kF32) return static_cast<uint64_t>(rank) << 32 | static_cast<uint32_t>(~place);
+        else return rank | ((1u << kPlaceBits) - 1 - static_cast<uint32_t>(place));
+    }
+    static __device__ __forceinline__ uint32_t rank(Key k) {
+        if constexpr (KIND == kF32) return static_cast<uint32_t>(k >> 32);
+        else return k & kMask;
+    }
+    static __device__ __forceinline__ int place(Key k) {
+        if constexpr (KIND == kF32) return static_cast<int>(~static_cast<uint32_t>(k));
+        else return static_cast<int>((1u << kPlaceBits) - 1 - (k & ((1u << kPlaceBits) - 1)));
+    }
 };
+static_assert(kSplitBytes / 2 <= 1 << Rank<kF16>::kPlaceBits && Rank<kF16>::kBits + Rank<kF16>::kPlaceBits <= 32, "keys of 16-bit values");
 
 // A lane's share of a split of a row: kSplitBytes / 64, in units of 16 bytes. Value j of unit r is
 // value (r * 64 + lane) * kUnit + j of the split; behind its end stands -inf.
@@ -78,6 +100,17 @@ struct Split {
         }
         return w;
     }
+    // Value j of a unit and its place as one word or two, which cost less than its key.
+    using Raw = typename std::conditional<KIND == kF32, uint64_t, uint32_t>::type;
+    static __device__ __forceinline__ Raw raw(const u32x4& w, int j, int place) {
+        const uint32_t x = w[j / kPerReg];
+        if constexpr (KIND == kF32) return static_cast<uint64_t>(static_cast<uint32_t>(place)) << 32 | x;
+        else return static_cast<uint32_t>(place) << 16 | ((j & 1) != 0 ? x >> 16 : x & 0xffffu);
+    }
+    static __device__ __forceinline__ float raw_value(Raw r) {
+        return value(u32x4{static_cast<uint32_t>(r), 0, 0, 0}, 0);
+    }
+    static __device__ __forceinline__ int raw_place(Raw r) { return static_cast<int>(r >> (KIND == kF32 ? 32 : 16)); }
     static __device__ __forceinline__ float value(const u32x4& w, int j) {
         const uint32_t x = w[j / kPerReg];
         if constexpr (KIND == kF32) return u2f(x);
@@ -128,10 +161,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 #endif
 }
 
-// The largest t of `bits` leading bits for which count(t) >= k (0 if none).
-template <class Count>
+// The largest t of `bits` leading bits for which count(t) >= k (0 if none). UNROLL 1 in a
+// kernel that runs through its code once, and waits for the code itself.
+template <int UNROLL, class Count>
 __device__ __forceinline__ uint32_t largest_with(int bits, int k, Count&& count) {
     uint32_t t = 0;
+#pragma unroll UNROLL
     for (int b = 31; b > 31 - bits; --b) {
         const uint32_t u = t | (1u << b);
         if (count(u) >= k) t = u;
@@ -141,9 +176,10 @@ __device__ __forceinline__ uint32_t largest_with(int bits, int k, Count&& count)
 
 template <int KIND>
 __global__ __launch_bounds__(kSplitThreads) void select_split_kernel(SelectArgs a) {
-    __shared__ uint64_t s_list[kSplitsPerBlock][kListed];
     using S = Split<KIND>;
     using R = Rank<KIND>;
+    using Key = typename R::Key;
+    __shared__ __align__(16) Key s_list[kSplitsPerBlock][kListed + 4];
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
     const int lane = static_cast<int>(threadIdx.x) & 63;
     const uint32_t unit = blockIdx.x * kSplitsPerBlock + wave;
@@ -192,46 +228,66 @@ __global__ __launch_bounds__(kSplitThreads) void select_split_kernel(SelectArgs 
         a.part_ms[static_cast<int64_t>(unit) * 2 + 1] = total;
     }
 
-    // At least k of the split's values are as large as the k-th largest of the lanes'
-    // maxima: few more than k where they are spread over the lanes.
-    const uint32_t mine = R::of(top);
-    uint32_t least = largest_with(R::kBits, a.k, [&](uint32_t t) { return __popcll(__ballot(mine >= t)); });
+    // At least k of the split's values are as large as the k-th largest of the lanes' maxima,
+    // few more than k where those are few of the lanes; for larger k, of the units' maxima.
+    uint32_t least;
+    if (a.k <= kFewCandidates) {
+        const uint32_t mine = R::of(top);
+        least = largest_with<32>(R::kBits, a.k, [&](uint32_t t) { return __popcll(__ballot(mine >= t)); });
+    } else {
+        uint32_t mine[S::kUnits];
+#pragma unroll
+        for (int r = 0; r < S::kUnits; ++r) mine[r] = R::of(best[r]);
+        least = largest_with<32>(R::kBits, a.k, [&](uint32_t t) {
+            int c = 0;
+#pragma unroll
+            for (int r = 0; r < S::kUnits; ++r) c += __popcll(__ballot(mine[r] >= t));
+            return c;
+        });
+    }
     least = max(least, R::kLeast);
-    uint64_t* const list = s_list[wave];
+    Key* const list = s_list[wave];
     const unsigned long long below = (1ull << lane) - 1;
     int found = 0;
     {
-        // the units that hold any are read again, each lane's next one at a time: picking
-        // them out of the registers would be code for every value
+        // The units that hold any, each lane's next one at a time, chosen from the registers by
+        // selects: read again from memory they kept a wavefront at its end waiting.
         const float bound = R::value(least);
         uint32_t holds = 0;
 #pragma unroll
         for (int r = 0; r < S::kUnits; ++r) holds |= best[r] >= bound ? 1u << r : 0u;
         while (__ballot(holds != 0) != 0) {
-            u32x4 u = {0, 0, 0, 0};
-            int at0 = 0;
-            const bool has = holds != 0;
-            if (has) {
-                const int r = __ffs(static_cast<int>(holds)) - 1;
-                holds &= holds - 1;
-                at0 = v.index(r);
-                u = v.words(r);
+            const int r = holds != 0 ? __ffs(static_cast<int>(holds)) - 1 : 0;
+            const float mine = holds != 0 ? bound : __builtin_nanf("");     // no value is as large
+            holds &= holds - 1;
+            static_assert(S::kUnits == 8, "a unit is chosen by three bits");
+            u32x4 u;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const uint32_t a0 = (r & 1) != 0 ? x[1][c] : x[0][c], a1 = (r & 1) != 0 ? x[3][c] : x[2][c];
+                const uint32_t a2 = (r & 1) != 0 ? x[5][c] : x[4][c], a3 = (r & 1) != 0 ? x[7][c] : x[6][c];
+                const uint32_t b0 = (r & 2) != 0 ? a1 : a0, b1 = (r & 2) != 0 ? a3 : a2;
+                u[c] = (r & 4) != 0 ? b1 : b0;
             }
+            const int at0 = v.index(r);
 #pragma unroll
             for (int j = 0; j < S::kUnit; ++j) {
-                const float f = S::value(u, j);
-                const bool is = has && f >= bound;
+                const bool is = S::value(u, j) >= mine;
                 const unsigned long long some = __ballot(is);
                 if (some == 0) continue;
                 const int at = found + __popcll(some & below);
-                if (is && at < kListed) list[at] = static_cast<uint64_t>(R::of(f)) << 32 | static_cast<uint32_t>(~(at0 + j));
+                if (is && at < kListed) list[at] = S::raw(u, j, at0 + j);
                 found += __popcll(some);
             }
         }
+        for (int i = lane; i < min(found, kListed); i += 64) {
+            const Key k = list[i];
+            list[i] = R::key(R::of(S::raw_value(k)), S::raw_place(k));
+        }
     }
     if (found > kListed) {
-        // Few lanes hold them, or many are alike: the k-th largest value itself, all
-        // above it, and the first of those equal to it, from the values read again.
+        // Few lanes hold them, or many are alike: the k-th largest value itself, and from the
+        // values read again all above it and the first of those equal to it.
         const auto count = [&](int r, auto&& test) {
             const u32x4 u = v.words(r);
             int n = 0;
@@ -247,10 +303,16 @@ __global__ __launch_bounds__(kSplitThreads) void select_split_kernel(SelectArgs 
             }
             return n;
         };
-        least = largest_with(R::kBits, a.k, [&](uint32_t t) {
+        least = largest_with<1>(R::kBits, a.k, [&](uint32_t t) {
+            if (t < R::kLeast) return a.k;             // all are as large, and enough
+            const float from = R::value(t);
             int n = 0;
-            for (int r = 0; r < S::kUnits; ++r) n += count(r, [&](uint32_t q) { return q >= t; });
-            return __shfl(upto(n), 63, 64);
+#pragma unroll
+            for (int r = 0; r < S::kUnits; ++r) {
+#pragma unroll
+                for (int j = 0; j < S::kUnit; ++j) n += __popcll(__ballot(S::value(x[r], j) >= from));
+            }
+            return n;
         });
         least = max(least, R::kLeast);
         found = 0;
@@ -266,25 +328,27 @@ __global__ __launch_bounds__(kSplitThreads) void select_split_kernel(SelectArgs 
                 const bool is = q > least || (q == least && before < open);
                 before += q == least ? 1 : 0;
                 const unsigned long long some = __ballot(is);
-                if (is) list[found + __popcll(some & below)] = static_cast<uint64_t>(q) << 32 | static_cast<uint32_t>(~(v.index(r) + j));
+                if (is) list[found + __popcll(some & below)] = R::key(q, v.index(r) + j);
                 found += __popcll(some);
             }
             open -= min(open, __shfl(equal, 63, 64));
         }
     }
+    // a candidate's place is the number of better ones
+    if (lane < 4) list[found + lane] = 0;              // read with the last of them, better than none
     __builtin_amdgcn_wave_barrier();
     __threadfence_block();
-    // a candidate's place is the number of better ones
     BeamCandidate* const out = a.part + static_cast<int64_t>(unit) * a.k;
     for (int i = lane; i < found; i += 64) {
-        const uint64_t key = list[i];
+        const Key key = list[i];
         int place = 0;
-#pragma unroll 4
-        for (int j = 0; j < found; ++j) place += list[j] > key ? 1 : 0;
-        if (place < a.k) {
-            out[place].x = R::value(static_cast<uint32_t>(key >> 32));
-            out[place].token = static_cast<int32_t>(v0 + static_cast<int32_t>(~static_cast<uint32_t>(key)));
+        for (int j = 0; j < found; j += 4) {
+            Key o[4];
+            __builtin_memcpy(o, __builtin_assume_aligned(list + j, 16), sizeof(o));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) place += o[e] > key ? 1 : 0;
         }
+        if (place < a.k) out[place] = BeamCandidate{R::value(R::rank(key)), static_cast<int32_t>(v0 + R::place(key))};
     }
     for (int i = found + lane; i < a.k; i += 64) out[i].token = -1;
 }
@@ -297,23 +361,28 @@ __device__ __forceinline__ uint32_t score_rank(double s) {
 
 // A workgroup per request. The k-th best of the lists' heads is at most the k-th best of
 // all: the lists whose head is as good, and of them the candidates that are, few more than
-// k, are ranked in LDS. Where they are too many (scores alike), the first wavefront takes k
-// times the best of the heads. Bound by latency: three rounds of loads.
+// k, are ranked in LDS. Where one beam's lists hold most, they may be many: a rank that
+// leaves few of them is found then bit by bit, and they are taken again from it on. Where they are too many
+// for that (scores alike), each wavefront takes k times the best head of its share of the
+// lists, and those are ranked. Bound by latency: three rounds of loads.
 constexpr int kJoinThreads = 512;
-constexpr int kJoined = 512;
-constexpr int kHeadsPerLane = 8;      // of the first wavefront: lists beyond are not asked for the threshold
-__global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a, int lists_per_lane, FastDiv k_div) {
-    extern __shared__ uint8_t s_at[];                  // [lists_per_lane][64]: candidates taken from each list
+constexpr int kJoined = kJoinThreads / 64 * kMaxCandidates;
+constexpr int kJoinLists = 2048;      // lists whose candidates are looked through
+constexpr int kHalved = 4096;         // candidates of which a few are found so
+constexpr int kHeadsPerLane = 16;     // of the first wavefront: lists beyond are not asked for the threshold
+__global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a, int lists_per_lane) {
+    extern __shared__ uint8_t s_at[];                  // [lists_per_lane][kJoinThreads]: candidates taken from each list
     __shared__ double s_base[kMaxBeams];               // score - lse of each beam; of one at its end, its score
     __shared__ uint8_t s_ended[kMaxBeams];
-    __shared__ uint32_t s_heads[kHeadsPerLane * 64];
+    __shared__ uint32_t s_rank[kHalved];               // of the lists' heads, then of the candidates
     struct Found {
         double score;
         int64_t where;
     };
     __shared__ __align__(16) Found s_found[kJoined];
-    __shared__ int s_lists[kJoined];
+    __shared__ uint16_t s_lists[kJoinLists];
     __shared__ uint32_t s_least;
+    __shared__ int s_sums[2][kJoinThreads / 64];
     __shared__ int s_count, s_n_lists;
     const int64_t b = blockIdx.x;
     const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = tid >> 6;
@@ -326,24 +395,26 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a,
 #pragma unroll
     for (int n = 0; n < kMine; ++n)
         if (n * kJoinThreads + tid < lists) head[n] = part[static_cast<int64_t>(n * kJoinThreads + tid) * a.k];
-    for (int w = wave; w < a.W; w += kJoinThreads / 64) {
+    // sixteen lanes a beam
+    for (int w = tid >> 4; w < a.W; w += kJoinThreads / 16) {
         const float score = a.scores[row0 + w];
         const bool at_end = a.ended != nullptr && a.ended[row0 + w] != 0;
         double base = score;
         if (!at_end) {
             const float* ms = a.part_ms + (row0 + w) * a.splits * 2;
             float most = -__builtin_huge_valf();
-            for (int i = lane; i < a.splits; i += 64) most = fmaxf(most, ms[2 * i]);
-            most = wave_max(most);
+            for (int i = tid & 15; i < a.splits; i += 16) most = fmaxf(most, ms[2 * i]);
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
             double sum = 0.0;
-            for (int i = lane; i < a.splits; i += 64)
+            for (int i = tid & 15; i < a.splits; i += 16)
                 sum += static_cast<double>(ms[2 * i + 1]) * exp(static_cast<double>(ms[2 * i]) - static_cast<double>(most));
 #pragma unroll
-            for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+            for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
             // a beam without a score left no sums
             base = score > -__builtin_huge_valf() ? base - (static_cast<double>(most) + log(sum)) : kNone;
         }
-        if (lane == 0) {
+        if ((tid & 15) == 0) {
             s_base[w] = base;
             s_ended[w] = at_end ? 1 : 0;
         }
@@ -377,45 +448,127 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a,
 #pragma unroll
     for (int n = 0; n < kMine; ++n) {
         rank[n] = n * kJoinThreads + tid < lists ? rank_of_list(n * kJoinThreads + tid, head[n]) : 0u;
-        s_heads[n * kJoinThreads + tid] = rank[n];
+        s_rank[n * kJoinThreads + tid] = rank[n];
     }
     __syncthreads();
     if (wave == 0) {
-        // of the best of each lane's heads, in 20 bits: eight of a score's mantissa
-        uint32_t h = 0;
+        // in 20 bits: eight of a score's mantissa; of one maximum a lane, or of four
+        uint32_t h[4], least;
 #pragma unroll
-        for (int n = 0; n < kHeadsPerLane; ++n) h = max(h, s_heads[n * 64 + lane]);
-        const uint32_t least = largest_with(20, a.k, [&](uint32_t t) { return __popcll(__ballot(h >= t)); });
+        for (int g = 0; g < 4; ++g) {
+            h[g] = 0;
+#pragma unroll
+            for (int n = g; n < kHeadsPerLane; n += 4) h[g] = max(h[g], s_rank[n * 64 + lane]);
+        }
+        if (a.k <= kFewCandidates) {
+            const uint32_t best = max(max(h[0], h[1]), max(h[2], h[3]));
+            least = largest_with<1>(20, a.k, [&](uint32_t t) { return __popcll(__ballot(best >= t)); });
+        } else {
+            least = largest_with<1>(20, a.k, [&](uint32_t t) {
+                return __popcll(__ballot(h[0] >= t)) + __popcll(__ballot(h[1] >= t)) + __popcll(__ballot(h[2] >= t)) +
+                       __popcll(__ballot(h[3] >= t));
+            });
+        }
         if (lane == 0) s_least = max(least, 1u);
     }
     __syncthreads();
-    const uint32_t least = s_least;
+    uint32_t least = s_least;
     const auto enlist = [&](int list, uint32_t r) {
         if (r < least) return;
         const int p = atomicAdd(&s_n_lists, 1);
-        if (p < kJoined) s_lists[p] = list;
+        if (p < kJoinLists) s_lists[p] = static_cast<uint16_t>(list);
     };
 #pragma unroll
     for (int n = 0; n < kMine; ++n) enlist(n * kJoinThreads + tid, rank[n]);
     for (int i = kMine * kJoinThreads + tid; i < lists; i += kJoinThreads)
         enlist(i, rank_of_list(i, part[static_cast<int64_t>(i) * a.k]));
     __syncthreads();
+    // The candidates from `least` on: how many, their ranks, and the first of them.
     const int n_lists = s_n_lists;
-    if (n_lists <= kJoined) {
-        for (int i = tid; i < n_lists * a.k; i += kJoinThreads) {
-            const int l = static_cast<int>(k_div.div(static_cast<uint32_t>(i)));
-            double s;
-            int64_t at;
-            look(s_lists[l], i - l * a.k, &s, &at);
-            if (s > kNone && score_rank(s) >= least) {
-                const int p = atomicAdd(&s_count, 1);
-                if (p < kJoined) s_found[p] = Found{s, at};
+    const auto take = [&]() {
+        // sixteen lanes a list, which is in order: on while all of them are good enough
+        for (int l = tid >> 4; l < n_lists; l += kJoinThreads / 16) {
+            for (int at0 = 0; at0 < a.k; at0 += 16) {
+                double s;
+                int64_t at;
+                look(s_lists[l], at0 + (tid & 15), &s, &at);
+                const uint32_t r = s > kNone ? score_rank(s) : 0u;
+                const bool is = r >= least;
+                if (is) {
+                    const int p = atomicAdd(&s_count, 1);
+                    if (p < kHalved) s_rank[p] = r;
+                    if (p < kJoined) s_found[p] = Found{s, at};
+                }
+                if ((__ballot(is) >> (lane & 48) & 0xffffull) != 0xffffull) break;
             }
         }
         __syncthreads();
+        return s_count;
+    };
+    int count = n_lists <= kJoinLists ? take() : kHalved + 1;
+    if (count > kJoined && count <= kHalved) {
+        // the largest t of leading bits that leaves k of them, or the first that leaves few
+        uint32_t t = 0;
+        for (int bit = 31, turn = 0; bit >= 0; --bit, turn ^= 1) {
+            const uint32_t u = t | 1u << bit;
+            int c = 0;
+            for (int i = tid; i < (count + 63) / 64 * 64; i += kJoinThreads) c += __popcll(__ballot(i < count && s_rank[i] >= u));
+            if (lane == 0) s_sums[turn][wave] = c;
+            __syncthreads();
+            c = 0;
+#pragma unroll
+            for (int w = 0; w < kJoinThreads / 64; ++w) c += s_sums[turn][w];
+            if (c >= a.k) t = u;
+            if (c >= a.k && c <= kJoined / 2) break;
+        }
+        least = t;
+        __syncthreads();
+        if (tid == 0) s_count = 0;
+        __syncthreads();
+        count = take();
     }
-    const bool ranked = n_lists <= kJoined && s_count <= kJoined;
-    const int count = s_count;
+    if (count > kJoined) {
+        // lists n * kJoinThreads + tid are the lane's
+        for (int i = 0; i < lists_per_lane; ++i) s_at[i * kJoinThreads + tid] = 0;
+        double best = kNone;
+        int64_t where = 0;
+        int mine = 0;                                  // which of the lane's lists its best heads
+        const auto heads = [&]() {
+            best = kNone;
+            for (int n = 0; n < lists_per_lane && n * kJoinThreads + tid < lists; ++n) {
+                double s;
+                int64_t at;
+                look(n * kJoinThreads + tid, s_at[n * kJoinThreads + tid], &s, &at);
+                if (s > best || (s == best && s > kNone && at < where)) {
+                    best = s;
+                    where = at;
+                    mine = n;
+                }
+            }
+        };
+        heads();
+        __syncthreads();                               // the candidates of the first attempt are read no more
+        for (int c = 0; c < a.k; ++c) {
+            double top = best;
+            int64_t at = where;
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) {
+                const double s = __shfl_xor(top, o, 64);
+                const int64_t p = __shfl_xor(at, o, 64);
+                if (s > top || (s == top && p < at)) {
+                    top = s;
+                    at = p;
+                }
+            }
+            if (lane == 0) s_found[c * (kJoinThreads / 64) + wave] = Found{top, at};
+            if (top > kNone && best == top && where == at) {
+                ++s_at[mine * kJoinThreads + tid];
+                heads();
+            }
+        }
+        __syncthreads();
+        count = a.k * (kJoinThreads / 64);
+    }
     const auto write = [&](int c, double s, int64_t at) {
         const int64_t o = b * a.k + c;
         const bool none = !(s > kNone);
@@ -423,58 +576,22 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a,
         a.parents[o] = none ? -1 : static_cast<int32_t>(at >> 32);
         a.tokens[o] = none ? -1 : static_cast<int32_t>(at);
     };
-    if (ranked) {
-        // a candidate's place is the number of better ones, counted by eight lanes
-        for (int i0 = 0; i0 < count; i0 += kJoinThreads / 8) {
-            const int i = i0 + (tid >> 3);
-            const Found f = s_found[min(i, count - 1)];
-            int place = 0;
-            for (int j = tid & 7; j < count; j += 8)
-                place += s_found[j].score > f.score || (s_found[j].score == f.score && s_found[j].where < f.where) ? 1 : 0;
+    // a candidate's place is the number of better ones, counted by eight lanes; those that
+    // are none of a wavefront that ran out of them stand behind all others, by their entry
+    for (int i0 = 0; i0 < count; i0 += kJoinThreads / 8) {
+        const int i = i0 + (tid >> 3);
+        const Found f = s_found[min(i, count - 1)];
+        int place = 0;
+#pragma unroll 4
+        for (int j = tid & 7; j < count; j += 8) {
+            const Found o = s_found[j];
+            place += o.score > f.score || (o.score == f.score && (o.score > kNone ? o.where < f.where : j < i)) ? 1 : 0;
+        }
 #pragma unroll
-            for (int o = 1; o < 8; o <<= 1) place += __shfl_xor(place, o, 64);
-            if (i < count && (tid & 7) == 0 && place < a.k) write(place, f.score, f.where);
-        }
-        for (int c = count + tid; c < a.k; c += kJoinThreads) write(c, kNone, 0);
-        return;
+        for (int o = 1; o < 8; o <<= 1) place += __shfl_xor(place, o, 64);
+        if (i < count && (tid & 7) == 0 && place < a.k) write(place, f.score, f.where);
     }
-    if (wave != 0) return;
-    for (int i = 0; i < lists_per_lane; ++i) s_at[i * 64 + lane] = 0;
-    double best = kNone;
-    int64_t where = 0;
-    int mine = 0;                                      // which of the lane's lists its best heads
-    const auto heads = [&]() {
-        best = kNone;
-        for (int n = 0; n < lists_per_lane && n * 64 + lane < lists; ++n) {
-            double s;
-            int64_t at;
-            look(n * 64 + lane, s_at[n * 64 + lane], &s, &at);
-            if (s > best || (s == best && s > kNone && at < where)) {
-                best = s;
-                where = at;
-                mine = n;
-            }
-        }
-    };
-    heads();
-    for (int c = 0; c < a.k; ++c) {
-        double top = best;
-        int64_t at = where;
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            const double s = __shfl_xor(top, o, 64);
-            const int64_t p = __shfl_xor(at, o, 64);
-            if (s > top || (s == top && p < at)) {
-                top = s;
-                at = p;
-            }
-        }
-        if (lane == 0) write(c, top, at);
-        if (top > kNone && best == top && where == at) {
-            ++s_at[mine * 64 + lane];
-            heads();
-        }
-    }
+    for (int c = count + tid; c < a.k; c += kJoinThreads) write(c, kNone, 0);
 }
 
 // ------------------------------------------------------------------- reorder
@@ -593,9 +710,8 @@ void launch_select_beams(const SelectArgs& a, int kind, hipStream_t stream) {
     else if (kind == kF16) DARIC_LAUNCH((select_split_kernel<kF16>), blocks, kSplitThreads, 0, stream, a);
     else DARIC_LAUNCH((select_split_kernel<kF32>), blocks, kSplitThreads, 0, stream, a);
     check_launch("select_beams");
-    const int per_lane = (a.W * a.splits + 63) / 64;
-    DARIC_LAUNCH(select_join_kernel, static_cast<unsigned>(a.B), kJoinThreads, static_cast<size_t>(per_lane) * 64, stream, a, per_lane,
-                 FastDiv(static_cast<uint32_t>(a.k)));
+    const int per_lane = (a.W * a.splits + kJoinThreads - 1) / kJoinThreads;
+    DARIC_LAUNCH(select_join_kernel, static_cast<unsigned>(a.B), kJoinThreads, static_cast<size_t>(per_lane) * kJoinThreads, stream, a, per_lane);
     check_launch("select_beams join");
 }
 

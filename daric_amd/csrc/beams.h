@@ -15,7 +15,7 @@ constexpr int kMaxBeams = 64;          // of a request, in a choice
 constexpr int kSplitBytes = 8192;
 
 // A candidate of a split of a row: its logit and its token (-1: none).
-struct BeamCandidate {
+struct alignas(8) BeamCandidate {
     float x;
     int32_t token;
 };
