@@ -353,14 +353,18 @@ __global__ __launch_bounds__(kSplitThreads) void select_split_kernel(SelectArgs 
     for (int i = found + lane; i < a.k; i += 64) out[i].token = -1;
 }
 
-// The order of scores as unsigned numbers, of their leading 32 bits.
-__device__ __forceinline__ uint32_t score_rank(double s) {
+// The order of scores as unsigned numbers, and its leading 32 bits.
+__device__ __forceinline__ uint64_t score_key(double s) {
     const uint64_t b = __builtin_bit_cast(uint64_t, s);
-    return static_cast<uint32_t>(((b >> 63) != 0 ? ~b : (b | 1ull << 63)) >> 32);
+    return (b >> 63) != 0 ? ~b : (b | 1ull << 63);
 }
+__device__ __forceinline__ double key_score(uint64_t k) {
+    return __builtin_bit_cast(double, (k >> 63) != 0 ? k & ~(1ull << 63) : ~k);
+}
+__device__ __forceinline__ uint32_t score_rank(double s) { return static_cast<uint32_t>(score_key(s) >> 32); }
 
-// A workgroup per request. The k-th best of the lists' heads is at most the k-th best of
-// all: the lists whose head is as good, and of them the candidates that are, few more than
+// A workgroup per request. The k-th best of the lists' heads, one or the first few, is at
+// most the k-th best of all: the lists whose head is as good, and of them the candidates that are, few more than
 // k, are ranked in LDS. Where one beam's lists hold most, they may be many: a rank that
 // leaves few of them is found then bit by bit, and they are taken again from it on. Where they are too many
 // for that (scores alike), each wavefront takes k times the best head of its share of the
@@ -368,16 +372,16 @@ __device__ __forceinline__ uint32_t score_rank(double s) {
 constexpr int kJoinThreads = 512;
 constexpr int kJoined = kJoinThreads / 64 * kMaxCandidates;
 constexpr int kJoinLists = 2048;      // lists whose candidates are looked through
-constexpr int kHalved = 4096;         // candidates of which a few are found so
-constexpr int kHeadsPerLane = 16;     // of the first wavefront: lists beyond are not asked for the threshold
-__global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a, int lists_per_lane) {
+constexpr int kHalved = 4096;         // candidates of which a few are found so; room for the heads, too
+constexpr int kHeadsPerLane = 64;     // of the first wavefront: what is beyond is not asked for the threshold
+__global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a, int lists_per_lane, int log2_heads) {
     extern __shared__ uint8_t s_at[];                  // [lists_per_lane][kJoinThreads]: candidates taken from each list
     __shared__ double s_base[kMaxBeams];               // score - lse of each beam; of one at its end, its score
     __shared__ uint8_t s_ended[kMaxBeams];
     __shared__ uint32_t s_rank[kHalved];               // of the lists' heads, then of the candidates
     struct Found {
-        double score;
-        int64_t where;
+        uint64_t key;                                  // of the score; 0: none
+        uint64_t tie;                                  // larger is better among equal scores: ~where
     };
     __shared__ __align__(16) Found s_found[kJoined];
     __shared__ uint16_t s_lists[kJoinLists];
@@ -390,11 +394,16 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a,
     const double kNone = -__builtin_huge_val();
     const int lists = a.W * a.splits;
     const BeamCandidate* const part = a.part + row0 * a.splits * a.k;
-    constexpr int kMine = kHeadsPerLane * 64 / kJoinThreads;
+    constexpr int kMine = 2;                           // of a lane's samples, read ahead
+    // the first 2^log2_heads candidates of each list, from which the threshold is taken
+    const int samples = lists << log2_heads;
+    const auto sample_at = [&](int i) {
+        return static_cast<int64_t>(i >> log2_heads) * a.k + (i & ((1 << log2_heads) - 1));
+    };
     BeamCandidate head[kMine];                         // what rows without logits left there is not used
 #pragma unroll
     for (int n = 0; n < kMine; ++n)
-        if (n * kJoinThreads + tid < lists) head[n] = part[static_cast<int64_t>(n * kJoinThreads + tid) * a.k];
+        if (n * kJoinThreads + tid < samples) head[n] = part[sample_at(n * kJoinThreads + tid)];
     // sixteen lanes a beam
     for (int w = tid >> 4; w < a.W; w += kJoinThreads / 16) {
         const float score = a.scores[row0 + w];
@@ -438,27 +447,32 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a,
         if (at < a.k) c = part[static_cast<int64_t>(list) * a.k + at];
         judge(list, at, c, score, where);
     };
-    const auto rank_of_list = [&](int list, const BeamCandidate& c) {
+    const auto rank_of = [&](int list, int n, const BeamCandidate& c) {
         double s;
         int64_t at;
-        judge(list, 0, c, &s, &at);
+        judge(list, n, c, &s, &at);
         return s > kNone ? score_rank(s) : 0u;
     };
-    uint32_t rank[kMine];
+    const auto sample_rank = [&](int i, const BeamCandidate& c) {
+        return rank_of(i >> log2_heads, i & ((1 << log2_heads) - 1), c);
+    };
 #pragma unroll
     for (int n = 0; n < kMine; ++n) {
-        rank[n] = n * kJoinThreads + tid < lists ? rank_of_list(n * kJoinThreads + tid, head[n]) : 0u;
-        s_rank[n * kJoinThreads + tid] = rank[n];
+        const int i = n * kJoinThreads + tid;
+        s_rank[i] = i < samples ? sample_rank(i, head[n]) : 0u;
     }
+    const int sampled = min(samples, kHeadsPerLane * 64);
+    for (int i = kMine * kJoinThreads + tid; i < (sampled + 63) / 64 * 64; i += kJoinThreads)
+        s_rank[i] = i < samples ? sample_rank(i, part[sample_at(i)]) : 0u;
     __syncthreads();
     if (wave == 0) {
         // in 20 bits: eight of a score's mantissa; of one maximum a lane, or of four
         uint32_t h[4], least;
+        for (int g = 0; g < 4; ++g) h[g] = 0;
+        for (int n = 0; n * 64 < samples && n < kHeadsPerLane; n += 4) {
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            h[g] = 0;
-#pragma unroll
-            for (int n = g; n < kHeadsPerLane; n += 4) h[g] = max(h[g], s_rank[n * 64 + lane]);
+            for (int g = 0; g < 4; ++g)
+                if ((n + g) * 64 < samples) h[g] = max(h[g], s_rank[(n + g) * 64 + lane]);
         }
         if (a.k <= kFewCandidates) {
             const uint32_t best = max(max(h[0], h[1]), max(h[2], h[3]));
@@ -478,10 +492,10 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a,
         const int p = atomicAdd(&s_n_lists, 1);
         if (p < kJoinLists) s_lists[p] = static_cast<uint16_t>(list);
     };
-#pragma unroll
-    for (int n = 0; n < kMine; ++n) enlist(n * kJoinThreads + tid, rank[n]);
-    for (int i = kMine * kJoinThreads + tid; i < lists; i += kJoinThreads)
-        enlist(i, rank_of_list(i, part[static_cast<int64_t>(i) * a.k]));
+    for (int i = tid; i < sampled; i += kJoinThreads)
+        if ((i & ((1 << log2_heads) - 1)) == 0) enlist(i >> log2_heads, s_rank[i]);
+    for (int i = kHeadsPerLane * 64 + tid; i < lists; i += kJoinThreads)
+        enlist(i, rank_of(i, 0, part[static_cast<int64_t>(i) * a.k]));
     __syncthreads();
     // The candidates from `least` on: how many, their ranks, and the first of them.
     const int n_lists = s_n_lists;
@@ -497,7 +511,7 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a,
                 if (is) {
                     const int p = atomicAdd(&s_count, 1);
                     if (p < kHalved) s_rank[p] = r;
-                    if (p < kJoined) s_found[p] = Found{s, at};
+                    if (p < kJoined) s_found[p] = Found{score_key(s), ~static_cast<uint64_t>(at)};
                 }
                 if ((__ballot(is) >> (lane & 48) & 0xffffull) != 0xffffull) break;
             }
@@ -560,7 +574,8 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a,
                     at = p;
                 }
             }
-            if (lane == 0) s_found[c * (kJoinThreads / 64) + wave] = Found{top, at};
+            const int to = c * (kJoinThreads / 64) + wave;
+            if (lane == 0) s_found[to] = top > kNone ? Found{score_key(top), ~static_cast<uint64_t>(at)} : Found{0, static_cast<uint64_t>(to)};
             if (top > kNone && best == top && where == at) {
                 ++s_at[mine * kJoinThreads + tid];
                 heads();
@@ -569,29 +584,34 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a,
         __syncthreads();
         count = a.k * (kJoinThreads / 64);
     }
-    const auto write = [&](int c, double s, int64_t at) {
+    // a candidate's place is the number of better ones, counted by eight lanes, four at a time
+    const int padded = (count + 31) & ~31;
+    if (tid < padded - count) s_found[count + tid] = Found{0, static_cast<uint64_t>(count + tid)};
+    __syncthreads();
+    const auto write = [&](int c, const Found& f) {
         const int64_t o = b * a.k + c;
-        const bool none = !(s > kNone);
-        a.out_scores[o] = none ? -__builtin_huge_valf() : static_cast<float>(s);
+        const bool none = f.key == 0;
+        const uint64_t at = ~f.tie;
+        a.out_scores[o] = none ? -__builtin_huge_valf() : static_cast<float>(key_score(f.key));
         a.parents[o] = none ? -1 : static_cast<int32_t>(at >> 32);
         a.tokens[o] = none ? -1 : static_cast<int32_t>(at);
     };
-    // a candidate's place is the number of better ones, counted by eight lanes; those that
-    // are none of a wavefront that ran out of them stand behind all others, by their entry
     for (int i0 = 0; i0 < count; i0 += kJoinThreads / 8) {
         const int i = i0 + (tid >> 3);
         const Found f = s_found[min(i, count - 1)];
         int place = 0;
-#pragma unroll 4
-        for (int j = tid & 7; j < count; j += 8) {
-            const Found o = s_found[j];
-            place += o.score > f.score || (o.score == f.score && (o.score > kNone ? o.where < f.where : j < i)) ? 1 : 0;
+        for (int j = tid & 7; j < padded; j += 32) {
+            Found o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = s_found[j + 8 * e];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) place += o[e].key > f.key || (o[e].key == f.key && o[e].tie > f.tie) ? 1 : 0;
         }
 #pragma unroll
         for (int o = 1; o < 8; o <<= 1) place += __shfl_xor(place, o, 64);
-        if (i < count && (tid & 7) == 0 && place < a.k) write(place, f.score, f.where);
+        if (i < count && (tid & 7) == 0 && place < a.k) write(place, f);
     }
-    for (int c = count + tid; c < a.k; c += kJoinThreads) write(c, kNone, 0);
+    for (int c = count + tid; c < a.k; c += kJoinThreads) write(c, Found{0, 0});
 }
 
 // ------------------------------------------------------------------- reorder
@@ -710,8 +730,13 @@ void launch_select_beams(const SelectArgs& a, int kind, hipStream_t stream) {
     else if (kind == kF16) DARIC_LAUNCH((select_split_kernel<kF16>), blocks, kSplitThreads, 0, stream, a);
     else DARIC_LAUNCH((select_split_kernel<kF32>), blocks, kSplitThreads, 0, stream, a);
     check_launch("select_beams");
-    const int per_lane = (a.W * a.splits + kJoinThreads - 1) / kJoinThreads;
-    DARIC_LAUNCH(select_join_kernel, static_cast<unsigned>(a.B), kJoinThreads, static_cast<size_t>(per_lane) * kJoinThreads, stream, a, per_lane);
+    const int lists = a.W * a.splits, per_lane = (lists + kJoinThreads - 1) / kJoinThreads;
+    // of a beam's few lists more than their best: twice as many as candidates are asked for,
+    // since one beam may hold all of them
+    int log2_heads = 0;
+    while ((a.splits << log2_heads) < 2 * a.k && (2 << log2_heads) <= a.k && (lists << (log2_heads + 1)) <= kHeadsPerLane * 64)
+        ++log2_heads;
+    DARIC_LAUNCH(select_join_kernel, static_cast<unsigned>(a.B), kJoinThreads, static_cast<size_t>(per_lane) * kJoinThreads, stream, a, per_lane, log2_heads);
     check_launch("select_beams join");
 }
 
