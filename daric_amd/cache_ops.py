@@ -692,8 +692,8 @@ def append_tokens(layer: torch.Tensor, page_first: bool, block_table: torch.Tens
     st = _resolve_stream(stream, dev)
     addr, n, _keep = _rows_of_ints(seqs, (5, 4), _SEQUENCES)
     rope = _rope(inv_freq, rotary_dim, is_neox_style, dev) if inv_freq is not None else None
-    if q is None:
-        q_out = None
+    if q is None and q_out is not None:
+        raise RuntimeError("q_out needs q")
     given = q_out               # what is made here belongs to `st` already
     if q is not None and q_out is None:
         with _on_stream(st, dev) if stream else _HERE:

@@ -2128,15 +2128,15 @@ void set_rotation(AppendArgs& a, const daric_rope* rope, float m) {
     a.m = m;
 }
 
-// Rows of a workgroup, `items` accesses each: one while there are workgroups for fewer than
-// kAppendGroups more, then as many as leave so many, up to kAppendItems accesses. MI355X, 1,
+// Rows of a workgroup, `items` accesses each: as many as give each lane one (kAppendLeast);
+// more while that leaves kAppendGroups workgroups, up to kAppendItems accesses. MI355X, 1,
 // 2 and 4 rows of 40 x 128 bf16: 256 rows 5.1, 7.1 and 8.0 us, 1024 6.7, 7.5 and 9.9, 2048
 // 11.4, 9.9 and 10.8, 3500 16.1, 15.4 and 14.5, 16384 78, 68 and 66 (8 rows: 70).
-constexpr int64_t kAppendGroups = 1024, kAppendItems = 2048, kAppendTile = 32;
+constexpr int64_t kAppendGroups = 1024, kAppendItems = 2048, kAppendLeast = 256, kAppendTile = 32;
 int64_t append_tile(int64_t rows, int64_t items, int R) {
     int64_t tile = 1;
-    while (tile < kAppendTile && rows / (2 * tile) >= kAppendGroups && 2 * tile * items <= kAppendItems &&
-           2 * tile * R <= 4096)
+    while (tile < kAppendTile && (rows / (2 * tile) >= kAppendGroups || tile * items < kAppendLeast) &&
+           2 * tile * items <= kAppendItems && 2 * tile * R <= 4096)
         tile *= 2;
     return tile;
 }

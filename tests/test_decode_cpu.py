@@ -358,6 +358,8 @@ def test_python_refusals():
         cache_ops.append_tokens(layer, False, bt, x, x, [(0, 0)])
     with pytest.raises(RuntimeError, match="must be on CUDA"):
         cache_ops.append_tokens(layer, False, bt, x, x, [(0, 0, 2, 0)])
+    with pytest.raises(RuntimeError, match="q_out needs q"):
+        cache_ops.append_tokens(layer, False, bt, x, x, [(0, 0, 2, 0)], q_out=x)
     with pytest.raises(RuntimeError, match="logits must be on CUDA"):
         cache_ops.select_beams(torch.zeros(1, 2, 8), torch.zeros(1, 2))
     with pytest.raises(ValueError, match="beams must be"):

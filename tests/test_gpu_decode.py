@@ -505,6 +505,48 @@ def test_reorder_missing_pages_and_long_lists(dev):
     check_reorder(dev, reorder_case([(2, 9)] * 3, ps=4, h=1, d=8, L=70), stream=torch.cuda.Stream().cuda_stream)
 
 
+# ------------------------------------------------------------- far offsets
+def test_offsets_past_32_bits(dev):
+    """Rows, pages and logits more than 2^32 elements into their tensors."""
+    f = torch.from_numpy(np.asarray(orope.default_inv_freq(64, 10000.0))).to(dev)
+    g = torch.Generator().manual_seed(3)
+    # rows far apart: element 2^32 is in row 4096
+    T, stride = 4200, 2 ** 20
+    wide = torch.empty(T * stride, dtype=torch.bfloat16, device=dev)
+    x = wide.as_strided((T, 2, 64), (stride, 64, 1))
+    host = torch.randn(T, 2, 64, generator=g).to(torch.bfloat16)
+    x.copy_(host)
+    pos = torch.arange(T, device=dev) * 3
+    out = cache_ops.rotate_rows(x, pos, f, 64)
+    want, off = odec.rotate(host, pos.cpu().numpy(), f.cpu().numpy(), 64)
+    close(out, want, off, torch.bfloat16)
+    cache_ops.rotate_rows(x, pos, f, 64, out=x)
+    assert torch.equal(x, out)
+    # the same memory as a paged cache: its last blocks' V lie past 2^32 values
+    NB, PS, H, D = 537000, 16, 4, 64
+    layer = wide[: 2 * NB * PS * H * D].view(2, NB, PS, H, D)
+    assert layer.stride(0) + (NB - 2) * layer.stride(1) > 2 ** 32
+    bt = torch.tensor([NB - 1, 5, NB - 2], dtype=torch.int32, device=dev)
+    layer[:, bt.long()] = 0
+    k, v = (torch.randn(40, H, D, generator=g).to(torch.bfloat16).to(dev) for _ in range(2))
+    cache_ops.append_tokens(layer, False, bt, k, v, [(0, 0, 40, 2)])
+    got = layer[:, bt.long()].flatten(1, 2)
+    assert torch.equal(got[0, 2:42], k) and torch.equal(got[1, 2:42], v)
+    assert not got[:, :2].any() and not got[:, 42:].any()
+    # two beams exchange the rows of their last pages, one at each end
+    lists = torch.tensor([NB - 1, 5], dtype=torch.int32, device=dev)
+    before = layer[:, lists.long()].clone()
+    cache_ops.reorder_beams([layer], False, lists, torch.tensor([[1, 0]], dtype=torch.int32, device=dev), [(0, 1, 2, 9)])
+    after = layer[:, lists.long()]
+    assert torch.equal(after[:, 0, :9], before[:, 1, :9]) and torch.equal(after[:, 1, :9], before[:, 0, :9])
+    assert torch.equal(after[:, :, 9:], before[:, :, 9:])
+    # logits of beams far apart
+    logits = wide.as_strided((2, 3, 5000), (2 ** 31 + 8, 2 ** 29 + 1, 1))
+    y, s = select_case(2, 3, 5000, torch.bfloat16, 4)
+    logits.copy_(y)
+    check_select(cache_ops.select_beams(logits, s.to(dev), 6), y, s, 6)
+
+
 # ------------------------------------------------------------- graphs, the loop
 def test_captured_steps_replay(dev):
     """A captured step of all four calls, replayed with other inputs and eager work between."""
