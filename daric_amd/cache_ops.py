@@ -648,8 +648,8 @@ def evict_tokens(layers: Sequence[torch.Tensor], page_first: bool, block_table: 
 def rotate_rows(rows: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, rotary_dim: int,
                 is_neox_style: bool = True, attention_scale: float = 1.0, out: Optional[torch.Tensor] = None,
                 stream: int = 0) -> torch.Tensor:
-    """Rotary positions of new rows ([T, H, D] bf16, fp16 or fp32: queries, keys, or
-    both heads after heads of a joint projection): pair i of the first rotary_dim values
+    """Rotary positions of new rows ([T, H, D] bf16, fp16 or fp32: queries, keys, or both
+    where their heads stand side by side): pair i of the first rotary_dim values
     turns by positions[t] * inv_freq[i] (int64 [T]; angles in fp64), cosine and sine
     times attention_scale; the other values are copied. Pairs are (i, i +
     rotary_dim / 2), or (2i, 2i + 1) with is_neox_style False. out: `rows` itself, or a
@@ -663,7 +663,7 @@ def rotate_rows(rows: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Ten
     given = out                 # what is made here belongs to `st` already
     if out is None:
         with _on_stream(st, dev) if stream else _HERE:
-            out = torch.empty(rows.shape, dtype=rows.dtype, device=dev)
+            out = rows.new_empty(rows.shape)
     (rd, pd, od), _keep = views(rows, positions, out)
     check(load().daric_rotate_rows(rd, pd, ctypes.byref(rope), float(attention_scale), od, st))
     _record(st, dev, rows, positions, inv_freq, given)
@@ -684,7 +684,8 @@ def append_tokens(layer: torch.Tensor, page_first: bool, block_table: torch.Tens
     differ); inv_freq None: nothing is rotated. rotary_dim, is_neox_style,
     attention_scale as in rotate_rows. An fp8 (e4m3) cache takes bf16 or fp16 rows as
     sat_rtne(x / scale) with its [H] fp32 k_scale / v_scale (None: 1). Tokens in pages
-    of id 0 are not written, nor is anything of rows of no sequence. Returns
+    of id 0 are not written, nor is anything of rows of no sequence; no slot may be
+    written by two rows of a call. Returns
     q_out (q itself, or a contiguous tensor, made if None), or None without q. No
     backward pass, as attend_pages."""
     _no_backward("append_tokens", layer, k, v, q, q_out, inv_freq, k_scale, v_scale)
@@ -697,7 +698,7 @@ def append_tokens(layer: torch.Tensor, page_first: bool, block_table: torch.Tens
     given = q_out               # what is made here belongs to `st` already
     if q is not None and q_out is None:
         with _on_stream(st, dev) if stream else _HERE:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+            q_out = q.new_empty(q.shape)
     (ld, bt, kd, vd, pd, qd, od, ks, vs), _views = views(layer, block_table, k, v, positions, q, q_out, k_scale, v_scale)
     check(load().daric_append_tokens(ld, 1 if page_first else 0, bt, kd, vd, addr, n, pd,
                                      ctypes.byref(rope) if rope is not None else None, float(attention_scale), qd, od,

@@ -71,10 +71,11 @@ typedef struct daric_tensor {
     int64_t strides[DARIC_MAX_DIMS];
 } daric_tensor;
 
-/* Rotary parameters for every re-rotation entry point.
+/* Rotary parameters for every rotating entry point.
  *  inv_freq   : device fp32 array of rotary_dim/2 inverse frequencies; the
  *               angle of pair i for a shift of d positions is the fp32 product
- *               (float)d * inv_freq[i].
+ *               (float)d * inv_freq[i]. Rows that are rotated to absolute positions
+ *               (daric_rotate_rows, daric_append_tokens) take it in fp64.
  *  rotary_dim : number of rotated dims at the start of each K head row (even).
  *  is_neox    : 1 pairs (i, i + rotary_dim/2); 0 pairs (2i, 2i+1) (GPT-J).
  * Same meaning as vLLM RotaryEmbedding.rotary_dim / is_neox_style consumed at

@@ -306,6 +306,7 @@ def check_select(got, x, scores, k, ended=None, end_token=-1):
     V = x.shape[2]
     s, p, t = (v.cpu().numpy() for v in got)
     live = np.isfinite(want[0])
+    assert (s[want[0] == np.inf] == np.inf).all()
     with np.errstate(all="ignore"):
         tol = 2 * E * np.abs(want[0]) + (V / 8192 + 48) * E
         # candidates of different beams are further apart than their scores may be off
@@ -313,7 +314,7 @@ def check_select(got, x, scores, k, ended=None, end_token=-1):
         close_by = live[:, 1:] & (want[1][:, 1:] != want[1][:, :-1]) & (apart < 2 * tol[:, 1:]) & (apart > 0)
     assert not close_by.any(), "the case's candidates are too close for a comparison"
     assert (p == want[1]).all() and (t == want[2]).all()
-    assert (np.abs(s - want[0])[live] <= tol[live]).all() and (s[~live] == -np.inf).all()
+    assert (np.abs(s[live] - want[0][live]) <= tol[live]).all() and (s[want[0] == -np.inf] == -np.inf).all()
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
@@ -388,6 +389,15 @@ def test_select_masks_and_numbers(dev):
     x = torch.nn.functional.pad(x, (0, 20000), value=-torch.inf)
     s = torch.tensor([[0.0, -0.25]])
     check_select(cache_ops.select_beams(x.to(dev), s.to(dev), 5), x, s, 5)
+
+
+def test_select_signed_zeros_and_infinite_scores(dev):
+    """Scores of -0 and +0 are alike, and +inf is a score."""
+    x = torch.zeros(2, 4, 50)
+    s = torch.tensor([[0.0, -0.0, 0.0, -0.0], [torch.inf, -1.0, -torch.inf, torch.inf]])
+    ended = torch.tensor([[True, True, True, True], [False, False, False, True]])
+    for k in (3, 6, 64):
+        check_select(cache_ops.select_beams(x.to(dev), s.to(dev), k, ended=ended.to(dev), end_token=7), x, s, k, ended, 7)
 
 
 def test_select_ended_beams(dev):
