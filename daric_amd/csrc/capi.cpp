@@ -2365,7 +2365,7 @@ SelectCall select_call(const daric_tensor* logits, int64_t k) {
     const int64_t per = kSplitBytes / logits->elem_size;
     const int64_t splits = (V + per - 1) / per;
     DARIC_CHECK(W * splits <= 32768, "the vocabulary is too large for ", W, " beams");
-    DARIC_CHECK(B * W * splits <= kMaxTiles && B <= kMaxTiles, "too many rows in one select_beams call");
+    DARIC_CHECK(B <= kMaxTiles && B * W * splits <= kMaxTiles, "too many rows in one select_beams call");
     SelectArgs& a = c.a;
     a.logits = static_cast<const uint8_t*>(logits->data);
     a.batch = logits->strides[0];
@@ -2490,8 +2490,8 @@ int daric_reorder_beams(const daric_tensor* layers, int64_t n_layers, int page_f
             x.n_tokens = static_cast<int32_t>(s.n_tokens);
             x.tile_begin = static_cast<int32_t>(tiles);
             if (s.n_beams > 0 && pages > 0) {
-                const int64_t rest = bt_n - s.bt_offset - pages;
-                DARIC_CHECK(s.bt_offset <= bt_n && rest >= 0 && (s.n_beams == 1 || s.stride <= rest / (s.n_beams - 1)),
+                const int64_t rest = s.bt_offset <= bt_n ? bt_n - s.bt_offset - pages : -1;
+                DARIC_CHECK(rest >= 0 && (s.n_beams == 1 || s.stride <= rest / (s.n_beams - 1)),
                             "request ", i, " reaches past the end of block_table");
                 ranges.emplace_back(s.bt_offset, (s.n_beams - 1) * s.stride + pages);
             }

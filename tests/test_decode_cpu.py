@@ -253,6 +253,7 @@ def test_selection_refusals(lib):
         assert "1 to 64 candidates" in run(out_=wide[0], par_=wide[1], tok_=wide[2])
     assert "vocabulary is too large" in run(x_=fake((2, 64, 2 ** 24), torch.bfloat16))
     assert "too many rows" in run(x_=fake((2 ** 24, 4, 100000), torch.bfloat16))
+    assert "too many rows" in run(x_=fake((2 ** 62, 4, 8), torch.bfloat16, strides=(0, 8, 1)))
     assert "scores must be" in run(sc_=fake((2, 3), torch.float32)) and "scores must be" in run(sc_=fake((2, 4), torch.float16))
     assert "ended must be" in run(end_=fake((2, 4), torch.int32)) and "ended must be" in run(end_=fake((4,), torch.uint8))
     assert "end_token must be in the vocabulary" in run(end_=end, et=1000)
@@ -288,6 +289,7 @@ def test_reorder_refusals(lib):
     assert "reaches past the end of block_table" in run(s=((5, 10, 4, 100),))
     assert "reaches past the end of block_table" in run(s=((0, 2 ** 62, 4, 100),))
     assert "reaches past the end of block_table" in run(s=((2 ** 62, 10, 4, 100),))
+    assert "reaches past the end of block_table" in run(s=((2 ** 63 - 1, 2 ** 31, 2, 2 ** 31 - 2000),))
     two = fake((2, 4), torch.int32, ptr=0x40000000)
     assert "block list 20 is in two sequences" in run(s=((0, 10, 3, 40), (20, 10, 2, 30)), par_=two)
     assert "parents must be" in run(par_=two) and "parents must be" in run(par_=fake((1, 4), torch.int64))
