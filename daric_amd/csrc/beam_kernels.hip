@@ -441,7 +441,7 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a,
     __syncthreads();
     // A list's candidate (number `at` of it): its score, -inf where there is none (NaN too),
     // and its beam and token in one number, which orders ties.
-    const auto judge = [&](int list, int at, const BeamCandidate& c, double* score, int64_t* where) {
+    const auto score_of = [&](int list, int at, const BeamCandidate& c, double* score, int64_t* where) {
         const int w = static_cast<int>(a.d_splits.div(static_cast<uint32_t>(list)));
         const bool at_end = s_ended[w] != 0;
         const bool first = list == w * a.splits && at == 0;
@@ -454,12 +454,12 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a,
     const auto look = [&](int list, int at, double* score, int64_t* where) {
         BeamCandidate c{0.0f, -1};
         if (at < a.k) c = part[static_cast<int64_t>(list) * a.k + at];
-        judge(list, at, c, score, where);
+        score_of(list, at, c, score, where);
     };
     const auto rank_of = [&](int list, int n, const BeamCandidate& c) {
         double s;
         int64_t at;
-        judge(list, n, c, &s, &at);
+        score_of(list, n, c, &s, &at);
         return s > kNone ? score_rank(s) : 0u;
     };
     const auto sample_rank = [&](int i, const BeamCandidate& c) {
