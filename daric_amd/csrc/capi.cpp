@@ -2365,7 +2365,8 @@ SelectCall select_call(const daric_tensor* logits, int64_t k) {
     const int64_t per = kSplitBytes / logits->elem_size;
     const int64_t splits = (V + per - 1) / per;
     DARIC_CHECK(W * splits <= 32768, "the vocabulary is too large for ", W, " beams");
-    DARIC_CHECK(B <= kMaxTiles && B * W * splits <= kMaxTiles, "too many rows in one select_beams call");
+    // the join's workgroups of 512 lanes count twice
+    DARIC_CHECK(B <= kMaxTiles / 2 && B * W * splits <= kMaxTiles, "too many rows in one select_beams call");
     SelectArgs& a = c.a;
     a.logits = static_cast<const uint8_t*>(logits->data);
     a.batch = logits->strides[0];

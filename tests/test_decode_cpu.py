@@ -270,6 +270,16 @@ def test_selection_refusals(lib):
                                   r(none[1]), r(none[2]), None, 0, ctypes.c_uint64(0)) == 0
 
 
+def test_selection_of_as_many_requests_as_a_launch_holds(lib):
+    """2^23 workgroups of 512 lanes are 2^32 lanes, one launch too large."""
+    need = ctypes.c_int64(0)
+    for B, fits in ((2 ** 23 - 1, True), (2 ** 23, False)):
+        x = fake((B, 1, 8), torch.bfloat16, strides=(0, 8, 1))
+        assert (lib.daric_select_workspace(r(x), 1, r(need)) == 0) is fits
+    assert "too many rows" in lib.daric_last_error().decode()
+    assert need.value == (2 ** 23 - 1) * 16               # a candidate, a maximum and a sum each
+
+
 def test_reorder_refusals(lib):
     layers = (_lib.DaricTensor * 2)(*[fake((2, 8, 16, 4, 64), torch.bfloat16, ptr=0x10000000 * (i + 1)) for i in range(2)])
     bt = fake((40,), torch.int32, ptr=0x30000000)
