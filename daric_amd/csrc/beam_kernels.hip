@@ -758,11 +758,12 @@ void launch_reorder(const DescArg& d, int layer_off, int n_layers, const KVGeom&
     const FastDiv inner(static_cast<uint32_t>(head_units)), mid(static_cast<uint32_t>(g.H));
     const int token_inner = g.ss < g.sh ? 1 : 0;
     // the lists' blocks stand behind the rows' of one launch: they write other places of
-    // block_table than the rows' read
+    // block_table than the rows' read; a launch that they do not fit in is followed by theirs
     const unsigned page_blocks = static_cast<unsigned>((most_pages + kReorderThreads - 1) / kReorderThreads);
     unsigned list_blocks = page_blocks * static_cast<unsigned>(n_lists);
     const auto launch = [&](const LayerMinor& lm, unsigned row_blocks) {
-        const unsigned blocks = row_blocks + list_blocks;
+        const bool fit = static_cast<int64_t>(row_blocks) + list_blocks <= kMaxGridBlocks;
+        const unsigned blocks = row_blocks + (fit ? list_blocks : 0);
 #define DARIC_RW(U, W) DARIC_LAUNCH((reorder_kernel<U, W>), blocks, kReorderThreads, 0, stream, d, layer_off, lm, g, es, \
                                     block_table, parents, parent_stride, n_lists, inner, mid, token_inner, head_units, \
                                     row_blocks, std::max(1u, page_blocks))
@@ -781,7 +782,7 @@ void launch_reorder(const DescArg& d, int layer_off, int n_layers, const KVGeom&
 #undef DARIC_RU
 #undef DARIC_RW
         check_launch("reorder_beams");
-        list_blocks = 0;
+        if (fit) list_blocks = 0;
     };
     for_layer_minor(n_layers, tiles, launch);
     if (list_blocks > 0) launch(LayerMinor{}, 0);

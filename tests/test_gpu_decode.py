@@ -327,6 +327,23 @@ def test_select(dev, dtype, B, W, V, k):
     check_select(got, x, s, k)
 
 
+def test_select_the_largest_vocabulary(dev):
+    """As many pieces of rows as a request may have: 64 beams of 2^20 fp32 logits."""
+    W, V, k = 64, 2 ** 20, 64
+    g = torch.Generator().manual_seed(9)
+    x = torch.randn(1, W, V, generator=g)
+    s = -torch.rand(1, W, generator=g)
+    got = cache_ops.select_beams(x.to(dev), s.to(dev), k)
+    torch.cuda.synchronize()
+    total = s.double()[0, :, None] + torch.log_softmax(x[0].double(), 1)
+    best, at = total.flatten().topk(k)
+    sc, par, tok = (v.cpu()[0] for v in got)
+    tol = 2 * E * best.abs() + (V / 8192 + 48) * E
+    assert (best[:-1] - best[1:] > 2 * tol[1:]).all(), "the case's candidates are too close for a comparison"
+    assert (par.long() == at // V).all() and (tok.long() == at % V).all()
+    assert ((sc.double() - best).abs() <= tol).all()
+
+
 def test_select_defaults_and_repeats(dev):
     x, s = select_case(3, 4, 5000, torch.bfloat16, 3)
     a = cache_ops.select_beams(x.to(dev), s.to(dev))
@@ -513,6 +530,25 @@ def test_reorder_missing_pages_and_long_lists(dev):
     check_reorder(dev, reorder_case([(3, 20001)], ps=2, h=1, d=4, L=2))
     check_reorder(dev, reorder_case([(2, 9)] * 300, ps=4, h=1, d=8, L=3), columns=3)
     check_reorder(dev, reorder_case([(2, 9)] * 3, ps=4, h=1, d=8, L=70), stream=torch.cuda.Stream().cuda_stream)
+
+
+def test_reorder_rows_and_lists_of_more_than_a_launch(dev):
+    """520000 requests of 32 workgroups of rows each, and one for their lists: 2^24 together
+    and more. The last pages are missing, which moves no rows."""
+    n, PS, H, D = 520000, 2, 256, 128
+    layer = torch.full((2, 4, PS, H, D), 7, dtype=torch.bfloat16, device=dev)
+    bt = torch.tensor([2, 0, 3, 0], dtype=torch.int32, device=dev).repeat(n)
+    parents = torch.tensor([[1, 0]], dtype=torch.int32, device=dev).expand(n, 2).contiguous()
+    parents[::2] = -1
+    beams = np.empty((n, 4), np.int64)
+    beams[:] = (0, 2, 2, 3)
+    beams[:, 0] = 4 * np.arange(n)
+    torch.cuda.synchronize()
+    cache_ops.reorder_beams([layer], False, bt, parents, beams)
+    torch.cuda.synchronize()
+    got = bt.view(-1, 2, 4).cpu()
+    assert (got[:, 0] == torch.tensor([2, 0, 3, 0])).all() and (got[:, 1] == torch.tensor([3, 0, 2, 0])).all()
+    assert (layer == 7).all()
 
 
 # ------------------------------------------------------------- far offsets
