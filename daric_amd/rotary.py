@@ -24,6 +24,22 @@ def _number(scaling: dict, name: str, default=None) -> float:
     return float(v)
 
 
+def _yarn_scale(scaling: dict, factor: float) -> float:
+    """The table's scale of a "yarn" scaling."""
+    if scaling.get("attention_factor") is not None:
+        return float(scaling["attention_factor"])
+
+    def g(s):
+        return 0.1 * s * math.log(factor) + 1 if factor > 1 else 1.0
+
+    part, whole = _number(scaling, "mscale", 0), _number(scaling, "mscale_all_dim", 0)
+    if part and whole:
+        return g(part) / g(whole)
+    if (part or whole) and g(part or 1) / g(whole) != g(1):
+        raise ValueError("rotary scaling takes mscale and mscale_all_dim together, or attention_factor in their place")
+    return g(1)
+
+
 def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[dict] = None,
                        seq_len: Optional[int] = None, device=None) -> tuple[torch.Tensor, float]:
     """(inv_freq fp32 [rotary_dim / 2], attention_scale). scaling: None, or a dict whose
@@ -37,7 +53,10 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional
       linearly in n / wavelength;
     - "yarn": dims that turn fewer than "beta_slow" (1) times over n positions are
       stretched by "factor", those of more than "beta_fast" (32) stay, between them mixed
-      linearly in the dim; attention_scale is "attention_factor", or 0.1 ln(factor) + 1.
+      linearly in the dim; attention_scale is "attention_factor", or g(1), or g(mscale) /
+      g(mscale_all_dim) where both are given, with g(s) = 0.1 s ln(factor) + 1 (1 for
+      factors up to 1). One of them without the other (or 0) is refused unless both readings
+      of it, g(1) and that ratio with g(0) = 1 for the missing one, agree.
     """
     R = int(rotary_dim)
     if R <= 0 or R % 2:
@@ -79,8 +98,7 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional
             lo, hi = max(math.floor(dim_of(fast)), 0), min(math.ceil(dim_of(slow)), R - 1)
             far = ((torch.arange(R // 2, dtype=torch.float64) - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
             f = f / factor * far + f * (1 - far)
-            given = scaling.get("attention_factor")
-            m = 0.1 * math.log(factor) + 1 if given is None and factor > 1 else 1.0 if given is None else float(given)
+            m = _yarn_scale(scaling, factor)
         else:
             raise ValueError(f"unknown rotary scaling {kind!r}")
     return f.to(torch.float32).to(device), m

@@ -104,6 +104,26 @@ def test_frequencies_of_scaled_models():
                                                    "original_max_position_embeddings": 4096})[1] == 1.5
 
 
+@pytest.mark.parametrize("scale,part,whole,want", [
+    (40.0, 1.0, 1.0, 1.0), (40.0, 0.707, 0.707, 1.0), (16.0, 1.0, 0.5, (0.1 * math.log(16) + 1) / (0.05 * math.log(16) + 1)),
+    (16.0, None, None, 0.1 * math.log(16) + 1), (16.0, 1.0, None, 0.1 * math.log(16) + 1), (16.0, 1, 0, 0.1 * math.log(16) + 1),
+    (16.0, 0.0, 0.0, 0.1 * math.log(16) + 1), (1.0, 0.5, None, 1.0), (0.5, 2.0, 3.0, 1.0)])
+def test_yarn_scale_of_two_parts(scale, part, whole, want):
+    """The table's scale is the ratio of the two parts' scales, which is 1 where they are alike."""
+    given = {k: v for k, v in (("mscale", part), ("mscale_all_dim", whole)) if v is not None}
+    yarn = {"type": "yarn", "factor": scale, "original_max_position_embeddings": 4096, **given}
+    assert np.isclose(rotary.rotary_frequencies(64, 10000.0, yarn)[1], want, rtol=1e-14, atol=0)
+    assert rotary.rotary_frequencies(64, 10000.0, {**yarn, "attention_factor": 1.5})[1] == 1.5
+
+
+@pytest.mark.parametrize("given", [{"mscale": 0.707}, {"mscale_all_dim": 1.0}, {"mscale": 0.707, "mscale_all_dim": 0.0},
+                                   {"mscale": "1"}, {"mscale": math.nan, "mscale_all_dim": 1.0}])
+def test_yarn_scale_refusals(given):
+    yarn = {"type": "yarn", "factor": 16.0, "original_max_position_embeddings": 4096, **given}
+    with pytest.raises(ValueError, match="mscale"):
+        rotary.rotary_frequencies(64, 10000.0, yarn)
+
+
 @pytest.mark.parametrize("args,text", [
     ((7,), "positive and even"), ((0,), "positive and even"), ((8, -1.0), "base must be"),
     ((8, 10000.0, {"type": "linear"}), "finite factor"), ((8, 10000.0, {"type": "linear", "factor": 0}), "must be positive"),
