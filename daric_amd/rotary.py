@@ -53,7 +53,7 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional
       linearly in n / wavelength;
     - "yarn": dims that turn fewer than "beta_slow" (1) times over n positions are
       stretched by "factor", those of more than "beta_fast" (32) stay, between them mixed
-      linearly in the dim; attention_scale is "attention_factor", or g(1), or g(mscale) /
+      linearly in the dim, the ends moved out to whole dims unless "truncate" is False; attention_scale is "attention_factor", or g(1), or g(mscale) /
       g(mscale_all_dim) where both are given, with g(s) = 0.1 s ln(factor) + 1 (1 for
       factors up to 1). One of them without the other (or 0) is refused unless both readings
       of it, g(1) and that ratio with g(0) = 1 for the missing one, agree.
@@ -95,7 +95,10 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional
             def dim_of(turns):          # the pair that turns so often over n positions
                 return R * math.log(n / (2 * math.pi * turns)) / (2 * math.log(base))
 
-            lo, hi = max(math.floor(dim_of(fast)), 0), min(math.ceil(dim_of(slow)), R - 1)
+            lo, hi = dim_of(fast), dim_of(slow)
+            if scaling.get("truncate", True):
+                lo, hi = math.floor(lo), math.ceil(hi)
+            lo, hi = max(lo, 0), min(hi, R - 1)
             far = ((torch.arange(R // 2, dtype=torch.float64) - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
             f = f / factor * far + f * (1 - far)
             m = _yarn_scale(scaling, factor)

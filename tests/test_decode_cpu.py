@@ -104,6 +104,28 @@ def test_frequencies_of_scaled_models():
                                                    "original_max_position_embeddings": 4096})[1] == 1.5
 
 
+@pytest.mark.parametrize("R,base,factor,n", [(64, 150000.0, 32.0, 4096), (128, 10000.0, 4.0, 4096), (64, 10000.0, 40.0, 4096),
+                                             (8, 1000.0, 4.0, 512), (16, 10.0, 2.0, 10 ** 6)])
+@pytest.mark.parametrize("given", [{}, {"truncate": True}, {"truncate": False}])
+def test_yarn_ramp(R, base, factor, n, given):
+    """Every pair, by the turns that it makes over n positions: its share of the stretched frequency
+    is linear in their logarithm from beta_fast down to beta_slow, and where the ends are whole dims
+    from the last dim of at least beta_fast turns to the first of at most beta_slow."""
+    got, _ = rotary.rotary_frequencies(R, base, {"type": "yarn", "factor": factor, "original_max_position_embeddings": n, **given})
+    dims = np.arange(-300, 300)
+    turns = n * base ** (-2.0 * dims / R) / (2 * np.pi)
+    if given.get("truncate", True):
+        first, last = max(dims[turns >= 32][-1], 0), min(dims[turns <= 1][0], R - 1)
+    else:
+        first, last = (np.interp(-np.log(t), -np.log(turns), dims) for t in (32.0, 1.0))
+        first, last = max(first, 0), min(last, R - 1)
+    i = np.arange(R // 2)
+    share = np.clip((i - first) / max(last - first, 1e-3), 0, 1)
+    f = base ** (-2.0 * i / R)
+    # a rounding to fp32, and a few of 64 bits
+    assert np.allclose(got.double().numpy(), f * (1 - share) + f / factor * share, rtol=2.0 ** -24 + 1e-11, atol=0)
+
+
 @pytest.mark.parametrize("scale,part,whole,want", [
     (40.0, 1.0, 1.0, 1.0), (40.0, 0.707, 0.707, 1.0), (16.0, 1.0, 0.5, (0.1 * math.log(16) + 1) / (0.05 * math.log(16) + 1)),
     (16.0, None, None, 0.1 * math.log(16) + 1), (16.0, 1.0, None, 0.1 * math.log(16) + 1), (16.0, 1, 0, 0.1 * math.log(16) + 1),
