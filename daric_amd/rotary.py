@@ -24,6 +24,25 @@ def _number(scaling: dict, name: str, default=None) -> float:
     return float(v)
 
 
+# What a scaling may hold: what the formulas below read (each kind its own), and what
+# says nothing about the frequencies of a given rotary_dim and base.
+_KNOWN = {"type", "rope_type", "factor", "original_max_position_embeddings", "low_freq_factor", "high_freq_factor",
+          "beta_fast", "beta_slow", "attention_factor", "mscale", "mscale_all_dim", "truncate", "rope_theta",
+          "partial_rotary_factor", "max_position_embeddings", "finetuned", "mrope_section", "mrope_interleaved"}
+
+
+def _kind(scaling: Optional[dict], base: float):
+    if scaling is None:
+        return None
+    for name in scaling:
+        if name not in _KNOWN:
+            raise ValueError(f"rotary scaling has {name!r}, whose effect on the frequencies is not known here")
+    if scaling.get("rope_theta") is not None and _number(scaling, "rope_theta") != base:
+        raise ValueError(f"rotary scaling has rope_theta {scaling['rope_theta']}, but base is {base}")
+    kind = scaling.get("rope_type")
+    return scaling.get("type") if kind is None else kind
+
+
 def _yarn_scale(scaling: dict, factor: float) -> float:
     """The table's scale of a "yarn" scaling."""
     if scaling.get("attention_factor") is not None:
@@ -57,6 +76,8 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional
       g(mscale_all_dim) where both are given, with g(s) = 0.1 s ln(factor) + 1 (1 for
       factors up to 1). One of them without the other (or 0) is refused unless both readings
       of it, g(1) and that ratio with g(0) = 1 for the missing one, agree.
+
+    Names that none of them knows are refused, and a "rope_theta" that is not `base`.
     """
     R = int(rotary_dim)
     if R <= 0 or R % 2:
@@ -66,7 +87,7 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional
     exponent = -torch.arange(0, R, 2, dtype=torch.float64) / R
     f = torch.tensor(float(base), dtype=torch.float64) ** exponent
     m = 1.0
-    kind = None if scaling is None else scaling.get("rope_type", scaling.get("type", "default"))
+    kind = _kind(scaling, base)
     if kind not in (None, "default"):
         factor = _number(scaling, "factor")
         if factor <= 0:

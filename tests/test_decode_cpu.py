@@ -146,6 +146,21 @@ def test_yarn_scale_refusals(given):
         rotary.rotary_frequencies(64, 10000.0, yarn)
 
 
+@pytest.mark.parametrize("kind", [{"type": "linear"}, {"rope_type": None, "type": "linear"}, {"rope_type": "linear", "type": "yarn"}])
+def test_scaling_names(kind):
+    """What changes no frequency may stand in a scaling, what may change one is refused if it is not known."""
+    plain = rotary.rotary_frequencies(64, 5e5)[0]
+    assert torch.equal(rotary.rotary_frequencies(64, 5e5, {**kind, "factor": 2.0, "rope_theta": 500000, "mrope_section": [16, 8, 8],
+                                                           "partial_rotary_factor": 0.5})[0], plain / 2)
+    assert torch.equal(rotary.rotary_frequencies(64, 5e5, {"rope_type": "default", "rope_theta": 5e5})[0], plain)
+    assert torch.equal(rotary.rotary_frequencies(64, 5e5, {})[0], plain)
+    for name in ("alpha", "extrapolation_factor", "long_factor", "attn_factor"):
+        with pytest.raises(ValueError, match=name):
+            rotary.rotary_frequencies(64, 5e5, {**kind, "factor": 2.0, name: 1.0})
+    with pytest.raises(ValueError, match="rope_theta 10000"):
+        rotary.rotary_frequencies(64, 5e5, {**kind, "factor": 2.0, "rope_theta": 10000.0})
+
+
 @pytest.mark.parametrize("args,text", [
     ((7,), "positive and even"), ((0,), "positive and even"), ((8, -1.0), "base must be"),
     ((8, 10000.0, {"type": "linear"}), "finite factor"), ((8, 10000.0, {"type": "linear", "factor": 0}), "must be positive"),
