@@ -205,6 +205,8 @@ class _Views:
         if ctypes.c_uint32.from_address(api).value != 1:
             return
         self.from_object = ctypes.c_uint64.from_address(api + 40).value
+        if not self.from_object:        # a table may leave it out
+            return
         self.none = id(None)
         self.fill = ctypes.PyDLL(LIB_PATH).daric_py_views
         self.fill.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_void_p]

@@ -401,6 +401,24 @@ def test_views_of_tensors_are_their_attributes():
         _lib.views(torch.zeros([1] * 9))
 
 
+def test_views_without_the_exchange_tables_function(monkeypatch):
+    """An exchange table that leaves the function out, or of another version, is not called."""
+    if not hasattr(torch.Tensor, "__dlpack_c_exchange_api__"):
+        pytest.skip("this torch has no exchange table")
+    name, c = b"dlpack_exchange_api", ctypes.pythonapi
+    get = ctypes.PYFUNCTYPE(ctypes.c_void_p, ctypes.py_object, ctypes.c_char_p)(("PyCapsule_GetPointer", c))
+    new = ctypes.PYFUNCTYPE(ctypes.py_object, ctypes.c_void_p, ctypes.c_char_p, ctypes.c_void_p)(("PyCapsule_New", c))
+    real = ctypes.string_at(get(torch.Tensor.__dlpack_c_exchange_api__, name), 48)
+    t = torch.zeros(2, 3)
+    for at, number, fits in ((40, 0, False), (0, 2, False), (40, int.from_bytes(real[40:], "little"), True)):
+        table = ctypes.create_string_buffer(real, 48)
+        ctypes.c_uint64.from_buffer(table, at).value = number
+        monkeypatch.setattr(torch.Tensor, "__dlpack_c_exchange_api__", new(ctypes.addressof(table), name, None))
+        views = _lib._Views()
+        assert (views.fill is not None) is fits
+        assert bytes(views.of([t])) == _lib.packed(t)
+
+
 def test_rows_of_ints():
     take = lambda e: cache_ops._rows_of_ints(e, (5, 4), "refused")
     def values(e):
