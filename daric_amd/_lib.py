@@ -69,10 +69,6 @@ class DaricEviction(ctypes.Structure):
                 ("n_first", c_int64), ("n_recent", c_int64)]
 
 
-class DaricBeams(ctypes.Structure):
-    _fields_ = [("bt_offset", c_int64), ("stride", c_int64), ("n_beams", c_int64), ("n_tokens", c_int64)]
-
-
 P = POINTER
 T = P(DaricTensor)
 B = c_void_p    # address of a daric_tensor
