@@ -35,6 +35,7 @@ from typing import Optional
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import I64, DaricChunk, DaricRope, check, desc, layer_views, load, str_array, views
@@ -86,6 +87,14 @@ def _on_stream(stream: int, device: torch.device):
 
 
 _HERE = nullcontext()
+
+
+def _in_dual_level() -> bool:
+    """Whether tensors may have forward-mode tangents. Where torch does not tell, they may:
+    asking each tensor takes a microsecond."""
+    return getattr(forward_ad, "_current_level", 0) >= 0
+
+
 _REQUIRES_GRAD = attrgetter("requires_grad")
 
 
@@ -533,13 +542,18 @@ def _scale(scale: Optional[float], q: torch.Tensor) -> float:
 
 
 def _no_backward(what: str, *tensors) -> None:
-    """These calls have no backward pass: an input that asks for a gradient is
-    refused, not answered by an output that silently has none."""
+    """These calls have no backward pass and carry no forward-mode tangents: an input that
+    asks for a gradient, or has a tangent, is refused, not answered by an output that
+    silently has none."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad(), or detach what "
                                    "requires a gradient")
+    if _in_dual_level():
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what} carries no forward-mode tangents: pass the primal of what has one")
 
 
 def _layer_desc(layer: torch.Tensor):
@@ -749,7 +763,7 @@ def reorder_beams(layers: Sequence[torch.Tensor], page_first: bool, block_table:
     every layer at once. Up to 32 beams of a request; caches of any type and
     layout."""
     layers = list(layers)
-    if torch.is_grad_enabled() and any(map(_REQUIRES_GRAD, layers)):
+    if _in_dual_level() or (torch.is_grad_enabled() and any(map(_REQUIRES_GRAD, layers))):
         _no_backward("reorder_beams", *layers)
     dev = layers[0].device
     st = _resolve_stream(stream, dev)

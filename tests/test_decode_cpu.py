@@ -458,3 +458,29 @@ def test_python_refusals():
                  lambda: cache_ops.select_beams(g, torch.zeros(2, 2))):
         with pytest.raises(RuntimeError, match="has no backward pass"):
             call()
+
+
+def test_forward_mode_tangents_are_refused():
+    """By every call that refuses a gradient; outside of a dual level nothing is asked."""
+    x = torch.zeros(2, 2, 8, dtype=torch.bfloat16)
+    f, p, bt = torch.ones(4), torch.zeros(2, dtype=torch.int64), torch.ones(2, dtype=torch.int32)
+    layer, w = torch.zeros(2, 3, 4, 2, 8, dtype=torch.bfloat16), torch.zeros(1, 2, 8)
+    seqs = [(0, 0, 2, 0)]
+    with torch.autograd.forward_ad.dual_level():
+        dual = lambda t: torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+        calls = [lambda: cache_ops.rotate_rows(dual(x), p, f, 8), lambda: cache_ops.rotate_rows(x, p, dual(f), 8),
+                 lambda: cache_ops.rotate_rows(x, p, f, 8, out=dual(x)),
+                 lambda: cache_ops.append_tokens(layer, False, bt, dual(x), x, seqs), lambda: cache_ops.append_tokens(layer, False, bt, x, dual(x), seqs),
+                 lambda: cache_ops.append_tokens(dual(layer), False, bt, x, x, seqs), lambda: cache_ops.append_tokens(layer, False, bt, x, x, seqs, q=dual(x)),
+                 lambda: cache_ops.select_beams(dual(w), torch.zeros(1, 2)), lambda: cache_ops.select_beams(w, dual(torch.zeros(1, 2))),
+                 lambda: cache_ops.reorder_beams([layer, dual(layer)], False, bt, torch.zeros(1, 2, dtype=torch.int32), [(0, 1, 2, 1)]),
+                 lambda: cache_ops.attend_pages(layer, False, bt, dual(x), seqs), lambda: cache_ops.weigh_tokens(layer, False, bt, dual(x), w[0, 0], seqs),
+                 lambda: cache_ops.evict_tokens([dual(layer)], False, bt, w, [(0, 0, 1, 1, 0, 0)])]
+        for call in calls:
+            for mode in (torch.enable_grad, torch.no_grad):        # tangents do not heed no_grad
+                with mode(), pytest.raises(RuntimeError, match="forward-mode tangents"):
+                    call()
+        with pytest.raises(RuntimeError, match="must be on CUDA"):  # primals pass on to the checks behind
+            cache_ops.append_tokens(layer, False, bt, x, x, seqs)
+        with pytest.raises(RuntimeError, match="must be on CUDA"):
+            cache_ops.reorder_beams([layer], False, bt, torch.zeros(1, 2, dtype=torch.int32), [(0, 1, 2, 1)])
