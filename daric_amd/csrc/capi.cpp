@@ -2266,9 +2266,9 @@ int daric_append_tokens(const daric_tensor* layer, int page_first, const daric_t
             a.v = check_head_rows(v, "v");
             like_cache(v, "v");
         } else {
-            DARIC_CHECK(v == nullptr || v->data == nullptr, "a 3-D (MLA) cache has no V rows: v must be None");
+            DARIC_CHECK(v == nullptr, "a 3-D (MLA) cache has no V rows: v must be None");
         }
-        const bool has_q = q != nullptr && q->ndim > 0;
+        const bool has_q = q != nullptr;
         if (has_q) {
             DARIC_CHECK(rope != nullptr, "q needs inv_freq: it is rotated only");
             a.q = check_head_rows(q, "q");
@@ -2283,7 +2283,7 @@ int daric_append_tokens(const daric_tensor* layer, int page_first, const daric_t
         set_rotation(a, rope, attention_scale);
         if (positions != nullptr) a.positions = check_positions(positions, t.device, T);
         const auto scales = [&](const daric_tensor* s, const char* what) -> const float* {
-            if (s == nullptr || s->data == nullptr) return nullptr;
+            if (s == nullptr) return nullptr;
             check_tensor_struct(s, what);
             DARIC_CHECK(ck == kE4M3, what, " applies to fp8 (e4m3) caches only");
             DARIC_CHECK(s->device == t.device && s->dtype == DARIC_DTYPE_FLOAT32 && is_contiguous(*s) &&
@@ -2414,7 +2414,7 @@ int daric_select_beams(const daric_tensor* logits, const daric_tensor* scores, c
                     scores->sizes[0] == a.B && scores->sizes[1] == a.W && is_contiguous(*scores),
                     "scores must be a contiguous float32 [requests, beams] tensor on the logits' device");
         a.scores = static_cast<const float*>(scores->data);
-        if (ended != nullptr && ended->ndim > 0) {
+        if (ended != nullptr) {
             check_tensor_struct(ended, "ended");
             DARIC_CHECK(ended->device == c.device && ended->elem_size == 1 && ended->dtype == DARIC_DTYPE_UINT8 &&
                         ended->ndim == 2 && ended->sizes[0] == a.B && ended->sizes[1] == a.W && is_contiguous(*ended),

@@ -283,6 +283,36 @@ def test_append_refusals(lib):
     assert "q_out must not overlap v" in run(k_=joint[1], v_=wraps, q_=joint[0], o=joint[0])
 
 
+def test_optional_tensors_without_dimensions_or_values_are_there(lib):
+    """A tensor of no dimensions, or of no values, is refused where one may be left out: it was
+    asked for, and is not what the call takes."""
+    layer, bt = fake((2, 8, 16, 4, 64), torch.uint8), fake((8,), torch.int32, ptr=0x20000000)
+    k, v = fake((10, 4, 64), torch.bfloat16, ptr=0x30000000), fake((10, 4, 64), torch.bfloat16, ptr=0x38000000)
+    a = np.array([(0, 0, 0, 100, 0)], np.int64)               # no rows: a call that is accepted ends before the device
+
+    def run(lay=layer, k_=k, v_=v, q=None, ks=None, vs=None, ro=rope(), pf=0):
+        if lib.daric_append_tokens(r(lay), pf, r(bt), r(k_), ref(v_), a.ctypes.data, 1, None, ref(ro), 1.0, ref(q), ref(q), ref(ks),
+                                   ref(vs), ctypes.c_uint64(0)) == 0:
+            return "taken"
+        return lib.daric_last_error().decode()
+
+    def none(dtype):
+        t = fake((0,), dtype)
+        t.data = None
+        return t
+
+    assert run() == "taken"
+    point = fake((), torch.bfloat16, ptr=0x40000000)
+    assert "q must be [T, H, D]" in run(q=point) and "q needs inv_freq" in run(q=point, ro=None)
+    assert "k_scale must be a contiguous" in run(ks=none(torch.float32)) and "v_scale must be a contiguous" in run(vs=none(torch.float32))
+    assert "v must be None" in run(lay=fake((8, 16, 64), torch.uint8), pf=1, k_=fake((10, 1, 64), torch.bfloat16), v_=none(torch.bfloat16))
+    x, sc = fake((0, 4, 1000), torch.bfloat16, ptr=0x30000000), fake((0, 4), torch.float32, ptr=0x40000000)
+    outs = [fake((0, 6), t, ptr=0x50000000) for t in (torch.float32, torch.int32, torch.int32)]
+    choose = lambda e: lib.daric_select_beams(r(x), r(sc), ref(e), 2, r(outs[0]), r(outs[1]), r(outs[2]), None, 0, ctypes.c_uint64(0))
+    assert choose(None) == 0 and choose(fake((0, 4), torch.uint8)) == 0
+    assert choose(fake((), torch.uint8, ptr=0x53000000)) != 0 and "ended must be" in lib.daric_last_error().decode()
+
+
 def test_selection_refusals(lib):
     x = fake((2, 4, 1000), torch.bfloat16, ptr=0x30000000)
     sc, out = fake((2, 4), torch.float32, ptr=0x40000000), fake((2, 6), torch.float32, ptr=0x50000000)
