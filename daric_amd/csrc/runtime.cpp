@@ -53,6 +53,10 @@ void check_tensor_struct(const daric_tensor* t, const char* what) {
     DARIC_CHECK(t != nullptr, what, " must not be null");
     DARIC_CHECK(t->ndim >= 0 && t->ndim <= DARIC_MAX_DIMS, what, " has an invalid rank: ", t->ndim);
     DARIC_CHECK(t->elem_size > 0, what, " has an invalid element size");
+    // a tensor that was only traced: a kernel would read from address 0 on
+    bool empty = false;
+    for (int i = 0; i < t->ndim; ++i) empty = empty || t->sizes[i] == 0;
+    DARIC_CHECK(t->data != nullptr || empty, what, " has no memory");
 }
 
 void check_launch(const char* what) {

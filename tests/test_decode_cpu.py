@@ -313,6 +313,32 @@ def test_optional_tensors_without_dimensions_or_values_are_there(lib):
     assert choose(fake((), torch.uint8, ptr=0x53000000)) != 0 and "ended must be" in lib.daric_last_error().decode()
 
 
+def test_tensors_without_memory_are_refused(lib):
+    """Such as a traced program's, whose address is null: no kernel is given one."""
+    def run(call, tensors, name):
+        args = {k: (fake(*t, ptr=0x10000000 * (i + 1)) if t is not None else None) for i, (k, t) in enumerate(tensors.items())}
+        args[name].data = None
+        assert call(**{k: ref(t) for k, t in args.items()}) != 0
+        assert "has no memory" in lib.daric_last_error().decode(), (name, lib.daric_last_error())
+
+    st, a = ctypes.c_uint64(0), np.array([(0, 0, 10, 100, 0)], np.int64)
+    bf, f32, i32 = torch.bfloat16, torch.float32, torch.int32
+    rows = lambda x, p, o: lib.daric_rotate_rows(x, p, r(rope()), 1.0, o, st)
+    for name in "xpo":
+        run(rows, dict(x=((10, 8, 64), bf), p=((10,), torch.int64), o=((10, 8, 64), bf)), name)
+    append = lambda l, b, k, v, p, q, o, s, z: lib.daric_append_tokens(l, 0, b, k, v, a.ctypes.data, 1, p, r(rope()), 1.0, q, o, s, z, st)
+    for name in "lbkvpqosz":
+        run(append, dict(l=((2, 8, 16, 4, 64), torch.uint8), b=((8,), i32), k=((10, 4, 64), bf), v=((10, 4, 64), bf), p=((10,), torch.int64),
+                         q=((10, 8, 64), bf), o=((10, 8, 64), bf), s=((4,), f32), z=((4,), f32)), name)
+    choose = lambda x, s, e, o, p, t: lib.daric_select_beams(x, s, e, 2, o, p, t, 0x70000000, 2 ** 20, st)
+    for name in "xseopt":
+        run(choose, dict(x=((2, 4, 1000), bf), s=((2, 4), f32), e=((2, 4), torch.uint8), o=((2, 6), f32), p=((2, 6), i32), t=((2, 6), i32)), name)
+    beams = np.array([(0, 10, 4, 100)], np.int64)
+    move = lambda l, b, p: lib.daric_reorder_beams(ctypes.cast(l, ctypes.POINTER(_lib.DaricTensor)), 1, 0, b, p, beams.ctypes.data, 1, st)
+    for name in "lbp":
+        run(move, dict(l=((2, 8, 16, 4, 64), bf), b=((40,), i32), p=((1, 4), i32)), name)
+
+
 def test_selection_refusals(lib):
     x = fake((2, 4, 1000), torch.bfloat16, ptr=0x30000000)
     sc, out = fake((2, 4), torch.float32, ptr=0x40000000), fake((2, 6), torch.float32, ptr=0x50000000)
