@@ -370,6 +370,26 @@ __device__ __forceinline__ double key_score(uint64_t k) {
 }
 __device__ __forceinline__ uint32_t score_rank(double s) { return static_cast<uint32_t>(score_key(s) >> 32); }
 
+// What orders candidates of equal scores, less is better: the beam, then the logit (the larger one
+// first), then the token. A score as large as a type's lowest value or infinite swallows the logits
+// of its beam in 64 bits, but the lists hold its likeliest tokens: so they stay in the lists' order.
+// 6 bits of beam; the tokens of 32-bit logits fit in 26 bits and leave their 32; those of 16-bit
+// ones, of which 19 bits differ, take 32 and leave 26.
+struct Place {
+    int token_bits;
+    __device__ explicit Place(int bits) : token_bits(bits) {}
+    __device__ __forceinline__ uint64_t of(int w, float x, int token) const {
+        const uint32_t b = f2u(x);
+        const uint32_t larger_first = (b & 0x80000000u) != 0 ? b : ~(b | 0x80000000u);
+        return static_cast<uint64_t>(w) << 58 | static_cast<uint64_t>(larger_first >> (token_bits - 26)) << token_bits |
+               static_cast<uint32_t>(token);
+    }
+    __device__ __forceinline__ int beam(uint64_t p) const { return static_cast<int>(p >> 58); }
+    __device__ __forceinline__ int token(uint64_t p) const { return static_cast<int>(p & ((1ull << token_bits) - 1)); }
+};
+static_assert(kMaxBeams <= 64 && kMaxSplits * (kSplitBytes / 4) <= 1ll << 26 && kMaxSplits * (kSplitBytes / 2) <= 1ll << 32,
+              "beams and tokens in a place");
+
 // A workgroup per request. The k-th best of the lists' heads, one or the first few of each,
 // is at most the k-th best of all: of the lists whose head is as good, the candidates that
 // are as good too, few more than k, are ranked in LDS. Where one beam's lists hold most of
@@ -390,7 +410,7 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a,
     __shared__ uint32_t s_rank[kHalved];               // of the lists' heads, then of the candidates
     struct Found {
         uint64_t key;                                  // of the score; 0: none
-        uint64_t tie;                                  // larger is better among equal scores: ~where
+        uint64_t tie;                                  // larger is better among equal scores: ~its Place
     };
     __shared__ __align__(16) Found s_found[kJoined];
     __shared__ uint16_t s_lists[kJoinLists];
@@ -439,9 +459,10 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a,
     }
     if (tid == 0) s_count = s_n_lists = 0;
     __syncthreads();
+    const Place place(a.token_bits);
     // A list's candidate (number `at` of it): its score, -inf where there is none (NaN too),
-    // and its beam and token in one number, which orders ties.
-    const auto score_of = [&](int list, int at, const BeamCandidate& c, double* score, int64_t* where) {
+    // and its place.
+    const auto score_of = [&](int list, int at, const BeamCandidate& c, double* score, uint64_t* where) {
         const int w = static_cast<int>(a.d_splits.div(static_cast<uint32_t>(list)));
         const bool at_end = s_ended[w] != 0;
         const bool first = list == w * a.splits && at == 0;
@@ -449,16 +470,16 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a,
         const double v = at_end ? s_base[w] : s_base[w] + static_cast<double>(c.x);
         const bool is = (at_end ? first : token >= 0) && v > kNone;
         *score = is ? v : kNone;
-        *where = static_cast<int64_t>(w) << 32 | static_cast<uint32_t>(token);
+        *where = place.of(w, at_end ? 0.0f : c.x, token);
     };
-    const auto look = [&](int list, int at, double* score, int64_t* where) {
+    const auto look = [&](int list, int at, double* score, uint64_t* where) {
         BeamCandidate c{0.0f, -1};
         if (at < a.k) c = part[static_cast<int64_t>(list) * a.k + at];
         score_of(list, at, c, score, where);
     };
     const auto rank_of = [&](int list, int n, const BeamCandidate& c) {
         double s;
-        int64_t at;
+        uint64_t at;
         score_of(list, n, c, &s, &at);
         return s > kNone ? score_rank(s) : 0u;
     };
@@ -513,14 +534,14 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a,
         for (int l = tid >> 4; l < n_lists; l += kJoinThreads / 16) {
             for (int at0 = 0; at0 < a.k; at0 += 16) {
                 double s;
-                int64_t at;
+                uint64_t at;
                 look(s_lists[l], at0 + (tid & 15), &s, &at);
                 const uint32_t r = s > kNone ? score_rank(s) : 0u;
                 const bool is = r >= least;
                 if (is) {
                     const int p = atomicAdd(&s_count, 1);
                     if (p < kHalved) s_rank[p] = r;
-                    if (p < kJoined) s_found[p] = Found{score_key(s), ~static_cast<uint64_t>(at)};
+                    if (p < kJoined) s_found[p] = Found{score_key(s), ~at};
                 }
                 if ((__ballot(is) >> (lane & 48) & 0xffffull) != 0xffffull) break;
             }
@@ -554,13 +575,13 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a,
         // lists n * kJoinThreads + tid are the lane's
         for (int i = 0; i < lists_per_lane; ++i) s_at[i * kJoinThreads + tid] = 0;
         double best = kNone;
-        int64_t where = 0;
+        uint64_t where = 0;
         int mine = 0;                                  // which of the lane's lists its best heads
         const auto heads = [&]() {
             best = kNone;
             for (int n = 0; n < lists_per_lane && n * kJoinThreads + tid < lists; ++n) {
                 double s;
-                int64_t at;
+                uint64_t at;
                 look(n * kJoinThreads + tid, s_at[n * kJoinThreads + tid], &s, &at);
                 if (s > best || (s == best && s > kNone && at < where)) {
                     best = s;
@@ -573,18 +594,18 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a,
         __syncthreads();                               // the candidates of the first attempt are read no more
         for (int c = 0; c < a.k; ++c) {
             double top = best;
-            int64_t at = where;
+            uint64_t at = where;
 #pragma unroll
             for (int o = 32; o > 0; o >>= 1) {
                 const double s = __shfl_xor(top, o, 64);
-                const int64_t p = __shfl_xor(at, o, 64);
+                const uint64_t p = __shfl_xor(at, o, 64);
                 if (s > top || (s == top && p < at)) {
                     top = s;
                     at = p;
                 }
             }
             const int to = c * (kJoinThreads / 64) + wave;
-            if (lane == 0) s_found[to] = top > kNone ? Found{score_key(top), ~static_cast<uint64_t>(at)} : Found{0, static_cast<uint64_t>(to)};
+            if (lane == 0) s_found[to] = top > kNone ? Found{score_key(top), ~at} : Found{0, static_cast<uint64_t>(to)};
             if (top > kNone && best == top && where == at) {
                 ++s_at[mine * kJoinThreads + tid];
                 heads();
@@ -593,32 +614,31 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a,
         __syncthreads();
         count = a.k * (kJoinThreads / 64);
     }
-    // a candidate's place is the number of better ones, counted by eight lanes, four at a time
+    // a candidate's rank is the number of better ones, counted by eight lanes, four at a time
     const int padded = (count + 31) & ~31;
     if (tid < padded - count) s_found[count + tid] = Found{0, static_cast<uint64_t>(count + tid)};
     __syncthreads();
     const auto write = [&](int c, const Found& f) {
         const int64_t o = b * a.k + c;
         const bool none = f.key == 0;
-        const uint64_t at = ~f.tie;
         a.out_scores[o] = none ? -__builtin_huge_valf() : static_cast<float>(key_score(f.key));
-        a.parents[o] = none ? -1 : static_cast<int32_t>(at >> 32);
-        a.tokens[o] = none ? -1 : static_cast<int32_t>(at);
+        a.parents[o] = none ? -1 : place.beam(~f.tie);
+        a.tokens[o] = none ? -1 : place.token(~f.tie);
     };
     for (int i0 = 0; i0 < count; i0 += kJoinThreads / 8) {
         const int i = i0 + (tid >> 3);
         const Found f = s_found[min(i, count - 1)];
-        int place = 0;
+        int better = 0;
         for (int j = tid & 7; j < padded; j += 32) {
             Found o[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[e] = s_found[j + 8 * e];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) place += o[e].key > f.key || (o[e].key == f.key && o[e].tie > f.tie) ? 1 : 0;
+            for (int e = 0; e < 4; ++e) better += o[e].key > f.key || (o[e].key == f.key && o[e].tie > f.tie) ? 1 : 0;
         }
 #pragma unroll
-        for (int o = 1; o < 8; o <<= 1) place += __shfl_xor(place, o, 64);
-        if (i < count && (tid & 7) == 0 && place < a.k) write(place, f);
+        for (int o = 1; o < 8; o <<= 1) better += __shfl_xor(better, o, 64);
+        if (i < count && (tid & 7) == 0 && better < a.k) write(better, f);
     }
     for (int c = count + tid; c < a.k; c += kJoinThreads) write(c, Found{0, 0});
 }

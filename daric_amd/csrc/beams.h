@@ -13,6 +13,7 @@ constexpr int kMaxBeams = 64;          // of a request, in a choice
 // Of a row of logits, for one wavefront. MI355X, 4, 8 and 16 KiB: 256 rows of 128000 bf16 33,
 // 27 and 31 us, 4 rows 13.6, 13.7 and 13.6, 35 rows of 50021 fp32 14.1, 13.5 and 14.0.
 constexpr int kSplitBytes = 8192;
+constexpr int64_t kMaxSplits = 32768;  // of a request
 
 // A candidate of a split of a row: its logit and its token (-1: none).
 struct alignas(8) BeamCandidate {
@@ -32,6 +33,7 @@ struct SelectArgs {
     float* part_ms;                // [B * W][splits][2]: maximum, sum of exp(x - maximum)
     int32_t W, k, splits, end_token;
     int32_t B;
+    int32_t token_bits;            // of a token in a candidate's place: 26 for fp32 logits, else 32
     int64_t V;
     FastDiv d_splits, d_beams;     // by splits and by W
 };

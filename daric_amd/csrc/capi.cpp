@@ -2364,7 +2364,7 @@ SelectCall select_call(const daric_tensor* logits, int64_t k) {
     DARIC_CHECK(V <= kMaxTokens, "the vocabulary is too large");
     const int64_t per = kSplitBytes / logits->elem_size;
     const int64_t splits = (V + per - 1) / per;
-    DARIC_CHECK(W * splits <= 32768, "the vocabulary is too large for ", W, " beams");
+    DARIC_CHECK(W * splits <= kMaxSplits, "the vocabulary is too large for ", W, " beams");
     // the join's workgroups of 512 lanes count twice
     DARIC_CHECK(B <= kMaxTiles / 2 && B * W * splits <= kMaxTiles, "too many rows in one select_beams call");
     SelectArgs& a = c.a;
@@ -2376,6 +2376,7 @@ SelectCall select_call(const daric_tensor* logits, int64_t k) {
     a.V = V;
     a.k = static_cast<int32_t>(k);
     a.splits = static_cast<int32_t>(splits);
+    a.token_bits = c.kind == kF32 ? 26 : 32;
     a.d_splits = FastDiv(static_cast<uint32_t>(splits));
     a.d_beams = FastDiv(static_cast<uint32_t>(W));
     return c;

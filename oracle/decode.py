@@ -65,7 +65,7 @@ def append(layer, page_first, bt, k, v, seqs, positions=None, rope=None, k_scale
 
 def select(logits, scores, k, ended=None, end_token=-1):
     """(scores, parents, tokens) [B, k] of the best candidates, in 64 bits, by a sort of
-    all of a request's."""
+    all of a request's: by score, then beam, then logit, then token."""
     x = _f64(logits)
     B, W, V = x.shape
     out = np.full((B, k), -np.inf), np.full((B, k), -1, np.int32), np.full((B, k), -1, np.int32)
@@ -82,7 +82,10 @@ def select(logits, scores, k, ended=None, end_token=-1):
                 s[w] = base + (x[b, w] - lse)
         s[np.isnan(s)] = -np.inf
         flat = s.reshape(-1)
-        best = np.argsort(-flat, kind="stable")[:k]
+        logit = np.where(np.isneginf(flat), 0.0, x[b].reshape(-1))
+        if ended is not None:
+            logit.reshape(W, V)[np.asarray(ended[b], bool)] = 0.0          # not looked at
+        best = np.lexsort((np.arange(W * V), -logit, np.arange(W * V) // V, -flat))[:k]
         for i, c in enumerate(best):
             if flat[c] > -np.inf:
                 out[0][b, i], out[1][b, i], out[2][b, i] = flat[c], c // V, c % V

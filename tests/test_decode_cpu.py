@@ -64,6 +64,17 @@ def test_oracle_selection_is_a_search_over_log_softmax():
     assert odec.select(x, [[0.0, 0.0]], 1)[1].tolist() == [[1]]
 
 
+def test_oracle_selection_of_swallowed_logits():
+    """Where the score leaves nothing of the logits in 64 bits they still order their beam's tokens."""
+    x = torch.tensor([[[0.0, 3.0, -1.0, 3.0], [5.0, 9.0, 7.0, 8.0]]])
+    low = torch.finfo(torch.float32).min
+    for first, second in ((low, low), (-1e18, -1e18), (math.inf, math.inf)):
+        got = odec.select(x, [[first, second]], 7)
+        assert got[1].tolist() == [[0, 0, 0, 0, 1, 1, 1]] and got[2].tolist() == [[1, 3, 0, 2, 1, 3, 2]]
+    got = odec.select(x, [[low, -1.0]], 6)
+    assert got[1].tolist() == [[1, 1, 1, 1, 0, 0]] and got[2].tolist() == [[1, 3, 2, 0, 1, 3]]
+
+
 def test_oracle_reorder_follows_parents():
     layer, pf = make_layer("nhd", 9, 2, 1, 2, torch.float16, torch.Generator().manual_seed(1))
     before = layer.clone()

@@ -417,6 +417,26 @@ def test_select_signed_zeros_and_infinite_scores(dev):
         check_select(cache_ops.select_beams(x.to(dev), s.to(dev), k, ended=ended.to(dev), end_token=7), x, s, k, ended, 7)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("W,V,k", [(4, 50, 3), (4, 50, 40), (3, 9000, 8), (4, 20011, 64), (32, 20000, 40), (64, 70000, 64)])
+def test_select_scores_that_swallow_the_logits(dev, dtype, W, V, k):
+    """Beams masked by the type's lowest value, -1e18 or +inf: in 64 bits all their candidates are
+    alike, and stay in the order of their logits. Few lists and many, joined each way."""
+    low = torch.finfo(torch.float32).min
+    B = 4 if W * V < 10 ** 6 else 1
+    x, _ = select_case(B, W, V, dtype, seed=V + k)
+    x[:, :, ::7] = -0.0
+    x[:, :, 3::7] = 0.0
+    s = torch.full((B, W), low)
+    if B == 4:
+        s[1, 1:] = -1e18
+        s[2, W // 2:] = torch.inf
+        s[3, W - 1] = -2.0
+    for ended in (None, torch.rand(B, W, generator=torch.Generator().manual_seed(1)) < 0.3):
+        got = cache_ops.select_beams(x.to(dev), s.to(dev), k, ended=None if ended is None else ended.to(dev), end_token=V - 1)
+        check_select(got, x, s, k, ended, V - 1)
+
+
 def test_select_ended_beams(dev):
     for W, k in ((4, 8), (1, 3), (32, 64)):
         x, s = select_case(5, W, 3001, torch.bfloat16, W)
