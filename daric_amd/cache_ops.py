@@ -89,10 +89,14 @@ def _on_stream(stream: int, device: torch.device):
 _HERE = nullcontext()
 
 
-def _in_dual_level() -> bool:
-    """Whether tensors may have forward-mode tangents. Where torch does not tell, they may:
-    asking each tensor takes a microsecond."""
-    return getattr(forward_ad, "_current_level", 0) >= 0
+# Whether tensors may have forward-mode tangents. Where torch does not tell, they may:
+# asking each tensor takes a microsecond.
+if hasattr(forward_ad, "_current_level"):
+    def _in_dual_level() -> bool:
+        return forward_ad._current_level >= 0
+else:
+    def _in_dual_level() -> bool:
+        return True
 
 
 _REQUIRES_GRAD = attrgetter("requires_grad")
