@@ -701,7 +701,8 @@ def append_tokens(layer: torch.Tensor, page_first: bool, block_table: torch.Tens
     positions: int64 [T] (None: the token's place, n_ctx + i; after an eviction they
     differ); inv_freq None: nothing is rotated. rotary_dim, is_neox_style,
     attention_scale as in rotate_rows. An fp8 (e4m3) cache takes bf16 or fp16 rows as
-    sat_rtne(x / scale) with its [H] fp32 k_scale / v_scale (None: 1). Tokens in pages
+    sat_rtne(x / scale) with its [H] fp32 k_scale / v_scale (None: 1). MLA rows (v None)
+    whose rotated part stands last: rotate_rows of k[..., -R:] in place, then no inv_freq here. Tokens in pages
     of id 0 are not written, nor is anything of rows of no sequence; no slot may be
     written by two rows of a call. Returns
     q_out (q itself, or a contiguous tensor, made if None), or None without q. No
@@ -765,7 +766,7 @@ def reorder_beams(layers: Sequence[torch.Tensor], page_first: bool, block_table:
     w * stride]. The ids of its full pages become its parent's, and its last, partly
     filled page, which no other list may hold there, takes the rows of the parent's, in
     every layer at once. Up to 32 beams of a request; caches of any type and
-    layout."""
+    layout, no two of which share memory."""
     layers = list(layers)
     if _in_dual_level() or (torch.is_grad_enabled() and any(map(_REQUIRES_GRAD, layers))):
         _no_backward("reorder_beams", *layers)

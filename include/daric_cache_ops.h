@@ -511,7 +511,8 @@ int daric_rotate_rows(const daric_tensor* rows, const daric_tensor* positions, c
  * written by two rows.
  * layer: one paged cache, bfloat16, float16 or e4m3, head_dim from 2 on. k, v: [T, H, D] rows of its type, or
  * bfloat16 or float16 for an e4m3 cache, strides as daric_rotate_rows' rows; v is NULL for
- * a 3-D (MLA) cache, whose rows are k's one head. An e4m3 cache takes the saturating
+ * a 3-D (MLA) cache, whose rows are k's one head; rows whose rotated part stands last are turned
+ * beforehand (daric_rotate_rows of that part, in place) and appended without rope. An e4m3 cache takes the saturating
  * round-to-nearest-even code of the rotated fp32 value / scale[h], the quotient
  * correctly rounded; k_scale, v_scale: NULL (1) or contiguous fp32 [H], for such a cache
  * only. q: NULL, or [T, Hq, D] rows of k's type; q_out: as daric_rotate_rows' out.
@@ -561,9 +562,9 @@ typedef struct daric_beams {
  * no other beam's or request's list may hold it there; full pages may be shared. Rows whose
  * page id, or whose parent's, is 0 or outside [1, num_blocks) are not moved. Which full
  * pages no list names any more is the caller's to find.
- * layers: caches of any type and layout, head_dim from 2 on, none given twice. parents: int32 [n, columns], rows
+ * layers: caches of any type and layout, head_dim from 2 on, no two of which share memory. parents: int32 [n, columns], rows
  * contiguous (daric_select_beams' parents, or their first columns). Up to 32 beams of a
- * request; block lists do not overlap. block_table is written. */
+ * request, half of what daric_select_beams takes: a lane holds a unit of each in registers; block lists do not overlap. block_table is written. */
 int daric_reorder_beams(const daric_tensor* layers, int64_t n_layers, int page_first, daric_tensor* block_table,
                         const daric_tensor* parents, const daric_beams* beams, int64_t n_beams, uint64_t stream);
 

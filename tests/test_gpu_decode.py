@@ -293,6 +293,45 @@ def test_append_on_another_stream_and_twice_at_once(dev):
         (a, b)[i % 2].check(o, (la, lb)[i % 2])
 
 
+def test_append_at_once_each_to_a_cache_of_its_own(dev):
+    """Calls on two streams, each with other rows and another cache: what any of them did not
+    write, or wrote elsewhere, is seen."""
+    steps = [Step([(1, 5 + i)] * 40 if i % 2 == 0 else [(600, i)], seed=10 + i) for i in range(6)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    f = torch.from_numpy(np.asarray(steps[0].rope[0])).to(dev)
+    layers, args = [to_dev(s.layer, dev) for s in steps], []
+    for s, layer in zip(steps, layers):
+        q, k, v = s.parts(s.joint.to(dev))
+        args.append((layer, s.pf, torch.from_numpy(s.bt).to(dev), k, v, s.seqs, f, s.R, True, q))
+    torch.cuda.synchronize()
+    outs = [cache_ops.append_tokens(*x[:-1], q=x[-1], stream=streams[i % 2].cuda_stream) for i, x in enumerate(args)]
+    torch.cuda.synchronize()
+    for s, out, layer in zip(steps, outs, layers):
+        assert not same_bytes(layer, s.layer)
+        s.check(out, layer)
+
+
+def test_append_mla_rows_that_are_rotated_at_their_end(dev):
+    """Rows whose rotated part stands last: turned in place by rotate_rows, then appended as they are."""
+    s = Step([(3, 5), (1, 0), (33, 1)], "mla", torch.bfloat16, rotary=0, d=96, g=2)
+    R, pos = 32, torch.cat([torch.arange(c, c + n) for n, c in ((3, 5), (1, 0), (33, 1))])
+    f = orope.default_inv_freq(R, 10000.0)
+    joint = s.joint.to(dev)
+    k = s.parts(joint)[1]
+    end = k[..., -R:]
+    cache_ops.rotate_rows(end, pos.to(dev), torch.from_numpy(np.asarray(f)).to(dev), R, out=end)
+    want, off = odec.rotate(s.parts(s.joint)[1][..., -R:], pos.numpy(), f, R)
+    close(end, want, off, torch.bfloat16)
+    layer = to_dev(s.layer, dev)
+    cache_ops.append_tokens(layer, s.pf, torch.from_numpy(s.bt).to(dev), k, None, s.seqs)
+    torch.cuda.synchronize()
+    before = s.joint.clone()
+    s.parts(before)[1][..., -R:] = end.cpu()
+    assert same_bytes(joint, before)
+    s.joint = before
+    s.check(None, layer)
+
+
 # ------------------------------------------------------------------ selection
 def select_case(B, W, V, dtype, seed=0, likely=8):
     g = torch.Generator().manual_seed(seed)
