@@ -733,9 +733,12 @@ def select_beams(logits: torch.Tensor, scores: torch.Tensor, k: Optional[int] = 
     (scores [B, k] fp32, parents [B, k] int32, tokens [B, k] int32), best first. A
     candidate's score is scores[b, w] + log_softmax(logits[b, w])[v] (logits: [B, W, V]
     bf16, fp16 or fp32; scores: fp32), compared in 64 bits, ties to the lower beam,
-    then the larger logit, then the lower token. Beams that `ended` (bool [B, W]) offer end_token alone, at
-    their own score. Candidates of score -inf or NaN are not there: score -inf, parent
-    and token -1 fill the places left. No backward pass, as attend_pages."""
+    then the larger logit, then the lower token. Beams that `ended` (bool [B, W]) offer
+    end_token alone, at their own score. Candidates of score -inf or NaN are not there:
+    score -inf, parent and token -1 fill the places left. A beam's log-sum is off by up to
+    2.3e-6 (its sums are fp32): closer candidates of different beams may come in either
+    order. Up to 64 beams of a request; reorder_beams takes 32. No backward pass, as
+    attend_pages."""
     _no_backward("select_beams", logits, scores)
     dev = logits.device
     st = _resolve_stream(stream, dev)

@@ -539,8 +539,10 @@ int daric_append_tokens(const daric_tensor* layer, int page_first, const daric_t
  * [B, W]. out_scores (fp32), parents, tokens (int32): contiguous [B, k], 1 <= k <= 64.
  * workspace: at least the bytes that daric_select_workspace gives, in use until the
  * call's work on `stream` is done. What is written overlaps neither each other nor what is
- * read. Sums of exponentials are fp32 over up to 8192 values, joined in fp64, and scores are
- * compared in fp64; the same call gives the same bits. */
+ * read. Sums of exponentials are fp32 over up to 4096 values (2048 of fp32 logits), joined in
+ * fp64, and scores are compared in fp64: a row's log-sum is off by up to 2.3e-6 (38 2^-24), and
+ * candidates of different beams that are closer than that may come in either order. The same
+ * call gives the same bits. */
 int daric_select_workspace(const daric_tensor* logits, int64_t k, int64_t* bytes);
 int daric_select_beams(const daric_tensor* logits, const daric_tensor* scores, const daric_tensor* ended,
                        int64_t end_token, daric_tensor* out_scores, daric_tensor* parents, daric_tensor* tokens,

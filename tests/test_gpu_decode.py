@@ -412,6 +412,22 @@ def test_select_ties(dev, dtype, V):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("V,spread", [(4096, 0.0), (4096, 8.0), (128000, 2.0), (128000, 0.01), (2 ** 20, 4.0)])
+def test_select_scores_within_the_sums_roundings(dev, dtype, V, spread):
+    """A row's log-sum is off by its splits' alone, which are joined in 64 bits. A split of 4096
+    values (2048 of fp32) is summed in chains of 16 (8) to a lane and 8 more steps of a tree: 24 e at
+    most. A term is off by 2 e of the exponential, e |d| of its argument's rounding and e |d| of the
+    difference d to the maximum itself; weighted by the terms |d| is 5.6 at most (one value at 0, the
+    others at -t: t - 1 where t - 1 = 4095 exp(-t)). In all 38 e, and e of the score for its rounding."""
+    g = torch.Generator().manual_seed(V)
+    x = (spread * torch.randn(2, 2, V, generator=g)).to(dtype)
+    s = torch.tensor([[-1.5, -torch.inf], [-torch.inf, -3.0]])
+    got = cache_ops.select_beams(x.to(dev), s.to(dev), 4)[0].double().cpu().numpy()
+    want = odec.select(x, s.numpy(), 4)[0]
+    assert (np.abs(got - want) <= E * np.abs(want) + 38 * E).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("V", [600, 20000])
 def test_select_best_in_few_lanes(dev, dtype, V):
     """A run of neighbouring likely tokens, more than a wavefront ranks at once."""
