@@ -187,7 +187,7 @@ def packed(t: torch.Tensor) -> bytes:
 class _Views:
     """daric_tensor views of tensors in one call of the library (daric_amd/csrc/pyviews.cpp),
     where torch offers the C function that it needs, else one by one (packed). Eight tensors
-    take 2 us on the host, 9 one by one."""
+    take 1.9 us on the host, 7.6 one by one."""
 
     def __init__(self):
         self.fill = None
@@ -237,7 +237,7 @@ def views(*tensors):
 
 
 def layer_views(layers) -> ctypes.Array:
-    """daric_tensor array of a call's layers: 80 take 11 us on the host."""
+    """daric_tensor array of a call's layers: 80 take 5.6 us on the host."""
     global _views
     if _views is None:
         _views = _Views()

@@ -7,7 +7,7 @@
 // since positions are absolute: at position 10^6 an fp32 product is off by up to
 // 0.03 rad, where in fp64 it is exact to 2^-53 of itself. What remains, at most
 // pi / 4, goes through the power series of sine and cosine in fp32 (to y^9 and
-// y^10: 2^-29 and 2^-33 of a turn off at pi / 4). The rotation is fp32, rounded
+// y^10: sine and cosine off by 2^-29 and 2^-33 at pi / 4). The rotation is fp32, rounded
 // once to the type it is stored in; an e4m3 cache takes the correctly rounded
 // quotient by the head's scale, saturating, as the row merge does.
 //
@@ -19,11 +19,12 @@
 // table is made.
 //
 // Bound by memory where rows are many, by latency (position, block table, angles,
-// then the stores) where they are few. MI355X, bf16: 16384 rows of 40 heads of 128
-// rotated into a new tensor, 336 MB, in 53 us with the rows in the 256 MB cache behind
-// the L2s (6.3 TB/s) and 66 us without (5.1; a copy of 1 GiB by torch runs at 5.1);
-// 16303 rows of 32 + 8 + 8 heads appended, 401 MB, 63 us and 78; one row 4 us; 48 single
-// rows of 64 + 8 + 8 heads into an e4m3 cache 7 us. Vector issue takes 25 of the 53 us.
+// then the stores) where they are few. MI355X, bf16, traced medians: 16384 rows of 40
+// heads of 128 rotated into a new tensor, 336 MB, in 54 us with the rows in the 256 MB
+// cache behind the L2s (6.2 TB/s) and 70 us without (4.8; a copy of 1 GiB by torch runs
+// at 5.15); 16303 rows of 32 + 8 + 8 heads appended, 401 MB, 65 us and 84; one row 5 us;
+// 48 single rows of 64 + 8 + 8 heads into an e4m3 cache 7 us. Vector issue takes 25 of
+// the 54 us.
 // Odd halves cost width: rows of 80 with 20 rotated values go in 4-byte accesses,
 // 77 MB in 32 us.
 #include <hip/hip_runtime.h>

@@ -12,11 +12,11 @@
 // the exponentials' argument (x - max) log2(e) is one product with log2(e) to 48 bits,
 // rounded once, and what follows the splits' fp32 sums is fp64.
 //
-// MI355X, 256 rows of 128000 bf16, 16 candidates of 8 beams: splits 17.5 us, join 5. The
-// splits' loads and maxima alone take 11.3 us (65.5 MB at 5.8 TB/s), the exponentials 1.7
-// more, thresholds, hits and their ranks the rest: vector instructions issue for 10 us of
-// the 17.5 and overlap the loads only in part. One request of four such rows: 5.5 + 4 us,
-// latency.
+// MI355X, traced medians, 256 rows of 128000 bf16, 16 candidates of 8 beams: splits 18.4
+// us, join 6.0. The splits' loads and maxima alone take 11.3 us (65.5 MB at 5.8 TB/s), the
+// exponentials 1.7 more, thresholds, hits and their ranks the rest: vector instructions
+// issue for 10 us of the 18 and overlap the loads only in part. One request of four such
+// rows: 6.1 + 6.1 us, latency.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -34,7 +34,11 @@ constexpr int kSplitThreads = 256;                     // wavefronts of a workgr
 constexpr int kSplitsPerBlock = kSplitThreads / 64;
 constexpr int kListed = 512;                           // candidates that a wavefront ranks
 // Candidates up to which thresholds are taken of one maximum a lane, with one test a step:
-// the looser, the more of the 64 lanes are asked for.
+// the looser, the more of the 64 lanes are asked for. MI355X, splits and join of 32 requests
+// of 8 beams of 128000 bf16, by lanes and by units: 8 candidates 24 and 28 us, 16 25 and 29, 32
+// 28 and 31, 48 38 and 34, 64 140 and 38; two requests of 32 beams 16 17 and 19, 32 20 and
+// 21, 48 28 and 26, 64 77 and 29; 7 of 5 of 50021 fp32 16 12 and 15, 48 17 and 17, 64 72 and 20.
+// They cross between 32 and 48.
 constexpr int kFewCandidates = 16;
 
 // Order of a type's values as unsigned numbers, in the leading bits that they differ
@@ -396,7 +400,7 @@ static_assert(kMaxBeams <= 64 && kMaxSplits * (kSplitBytes / 4) <= 1ll << 26 && 
 // them they may be many: a rank that leaves few is found then bit by bit, and they are taken
 // again from it on. Where they are too many for that (scores alike), each wavefront takes k
 // times the best head of its share of the lists, and those are ranked. Bound by latency: three
-// rounds of loads. MI355X, two requests of 32 beams of 128000 bf16, 64 candidates: 17 us where
+// rounds of loads. MI355X, two requests of 32 beams of 128000 bf16, 64 candidates: 15 us where
 // the scores spread over the beams, 490 where one wavefront took 64 times the best of all heads.
 constexpr int kJoinThreads = 512;
 constexpr int kJoined = kJoinThreads / 64 * kMaxCandidates;
