@@ -6,7 +6,7 @@
 // pass over them: a wavefront takes a split of a row, 8 KiB, into registers, reduces its
 // maximum and its sum of exponentials, and leaves the split's k best logits in order, ties
 // to the lower token. select_join_kernel, a workgroup per request, joins the splits' sums to
-// each beam's lse in fp64 and chooses among the lists by score.
+// each beam's in fp64 and chooses among the lists by score.
 //
 // Scores of different beams differ by more than what the sums err by, almost always: so
 // the exponentials' argument (x - max) log2(e) is one product with log2(e) to 48 bits,
@@ -409,7 +409,11 @@ constexpr int kHalved = 4096;         // candidates of which a few are found so;
 constexpr int kHeadsPerLane = 64;     // of the first wavefront: what is beyond is not asked for the threshold
 __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a, int lists_per_lane, int log2_heads) {
     extern __shared__ uint8_t s_at[];                  // [lists_per_lane][kJoinThreads]: candidates taken from each list
-    __shared__ double s_base[kMaxBeams];               // score - lse of each beam; of one at its end, its score
+    // A candidate's score is (score - log sum exp(x - most)) + (x - most), most the row's largest
+    // logit: logits of any size cancel before a score is added to them, also in rows of nothing
+    // but a mask's -3e38.
+    __shared__ double s_base[kMaxBeams];               // the first term of each beam; of one at its end, its score
+    __shared__ float s_most[kMaxBeams];
     __shared__ uint8_t s_ended[kMaxBeams];
     __shared__ uint32_t s_rank[kHalved];               // of the lists' heads, then of the candidates
     struct Found {
@@ -442,9 +446,9 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a,
         const float score = a.scores[row0 + w];
         const bool at_end = a.ended != nullptr && a.ended[row0 + w] != 0;
         double base = score;
+        float most = -__builtin_huge_valf();
         if (!at_end) {
             const float* ms = a.part_ms + (row0 + w) * a.splits * 2;
-            float most = -__builtin_huge_valf();
             for (int i = tid & 15; i < a.splits; i += 16) most = fmaxf(most, ms[2 * i]);
 #pragma unroll
             for (int o = 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
@@ -454,10 +458,11 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a,
 #pragma unroll
             for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
             // a beam without a score left no sums
-            base = score > -__builtin_huge_valf() ? base - (static_cast<double>(most) + log(sum)) : kNone;
+            base = score > -__builtin_huge_valf() ? base - log(sum) : kNone;
         }
         if ((tid & 15) == 0) {
             s_base[w] = base;
+            s_most[w] = most;
             s_ended[w] = at_end ? 1 : 0;
         }
     }
@@ -471,7 +476,7 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a,
         const bool at_end = s_ended[w] != 0;
         const bool first = list == w * a.splits && at == 0;
         const int token = at_end ? a.end_token : c.token;
-        const double v = at_end ? s_base[w] : s_base[w] + static_cast<double>(c.x);
+        const double v = at_end ? s_base[w] : s_base[w] + (static_cast<double>(c.x) - static_cast<double>(s_most[w]));
         const bool is = (at_end ? first : token >= 0) && v > kNone;
         *score = is ? v : kNone;
         *where = place.of(w, at_end ? 0.0f : c.x, token);

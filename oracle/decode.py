@@ -77,9 +77,8 @@ def select(logits, scores, k, ended=None, end_token=-1):
                 s[w, end_token] = base
                 continue
             with np.errstate(all="ignore"):
-                top = np.max(x[b, w])
-                lse = top + np.log(np.sum(np.exp(x[b, w] - top)))
-                s[w] = base + (x[b, w] - lse)
+                d = x[b, w] - np.max(x[b, w])        # before the sum's logarithm: logits may be huge
+                s[w] = base + (d - np.log(np.sum(np.exp(d))))
         s[np.isnan(s)] = -np.inf
         flat = s.reshape(-1)
         logit = np.where(np.isneginf(flat), 0.0, x[b].reshape(-1))

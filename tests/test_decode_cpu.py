@@ -64,6 +64,15 @@ def test_oracle_selection_is_a_search_over_log_softmax():
     assert odec.select(x, [[0.0, 0.0]], 1)[1].tolist() == [[1]]
 
 
+def test_oracle_selection_of_huge_logits():
+    """Rows of the type's lowest value alone are rows of equal logits, and so are those of 1e30."""
+    for level in (torch.finfo(torch.float32).min, 1e30, torch.finfo(torch.float32).max):
+        x = torch.full((1, 2, 10), level)
+        got = odec.select(x, [[-1.5, -2.0]], 12)
+        assert np.allclose(got[0][0], [-1.5 - math.log(10)] * 10 + [-2.0 - math.log(10)] * 2, rtol=1e-14)
+        assert got[1].tolist() == [[0] * 10 + [1] * 2] and got[2].tolist() == [[*range(10), 0, 1]]
+
+
 def test_oracle_selection_of_swallowed_logits():
     """Where the score leaves nothing of the logits in 64 bits they still order their beam's tokens."""
     x = torch.tensor([[[0.0, 3.0, -1.0, 3.0], [5.0, 9.0, 7.0, 8.0]]])

@@ -473,6 +473,26 @@ def test_select_signed_zeros_and_infinite_scores(dev):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("V", [1, 50, 9000, 50021])
+def test_select_rows_of_huge_logits(dev, dtype, V):
+    """A mask of the type's lowest value that leaves nothing of a row, and logits as large: the beam's
+    score and the number of tokens are what remains."""
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    x, s = select_case(5, 3, V, dtype, seed=V)
+    x[0, 1] = low                                 # beside beams with logits
+    x[1] = low
+    x[2] = high
+    x[3, :, ::3] = high / 4
+    x[3, :, 1::3] = high / 2
+    x[4, 0] = high / 2
+    x[4, 0, V // 2] = high
+    s[1:4] = torch.tensor([-1.5, -2.0, -2.5])
+    s[0, 2] = s[3, 1:] = s[4, 2] = -torch.inf     # no two beams whose candidates may come close
+    for k in (3, 20, 64):
+        check_select(cache_ops.select_beams(x.to(dev), s.to(dev), k), x, s, k)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("W,V,k", [(4, 50, 3), (4, 50, 40), (3, 9000, 8), (4, 20011, 64), (32, 20000, 40), (64, 70000, 64)])
 def test_select_scores_that_swallow_the_logits(dev, dtype, W, V, k):
     """Beams masked by the type's lowest value, -1e18 or +inf: in 64 bits all their candidates are
