@@ -429,6 +429,8 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a,
     const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = tid >> 6;
     const int64_t row0 = b * a.W;
     const double kNone = -__builtin_huge_val();
+    // what is not above it rounds to -inf in the fp32 that scores are given in
+    constexpr double kLeastScore = -0x1.ffffffp+127;
     const int lists = a.W * a.splits;
     const BeamCandidate* const part = a.part + row0 * a.splits * a.k;
     constexpr int kMine = 2;                           // of a lane's samples, read ahead
@@ -477,7 +479,7 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs a,
         const bool first = list == w * a.splits && at == 0;
         const int token = at_end ? a.end_token : c.token;
         const double v = at_end ? s_base[w] : s_base[w] + (static_cast<double>(c.x) - static_cast<double>(s_most[w]));
-        const bool is = (at_end ? first : token >= 0) && v > kNone;
+        const bool is = (at_end ? first : token >= 0) && v > kLeastScore;
         *score = is ? v : kNone;
         *where = place.of(w, at_end ? 0.0f : c.x, token);
     };

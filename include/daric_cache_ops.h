@@ -531,7 +531,7 @@ int daric_append_tokens(const daric_tensor* layer, int page_first, const daric_t
  * is scores[b, w] + logits[b, w, v] - log(sum over the vocabulary of exp(logits[b, w])).
  * Candidates of one score are in the order of w, of a beam's the larger logit comes first
  * (a score of -1e38 or +inf swallows the logits, not their order), then the lower v. A beam whose `ended` is not 0 offers end_token
- * alone, at the score scores[b, w]. Candidates whose score is -inf or NaN are not there
+ * alone, at the score scores[b, w]. Candidates whose score is NaN, or -inf in fp32, are not there
  * (masked logits, beams of score -inf; all of a row that holds +inf or NaN); places
  * that none is left for get score -inf, parent -1 and token -1.
  * logits: [B, W, V] bfloat16, float16 or float32, rows contiguous, other strides free

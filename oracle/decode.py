@@ -13,6 +13,7 @@ from .attend import _f64
 from .select import k_rows_view, v_view
 
 E = 2.0 ** -24
+LEAST = 2.0 ** 103 - 2.0 ** 128      # rounds to -inf in fp32, as all below does
 
 
 def rotate(x, positions, inv_freq, rotary_dim, neox=True, m=1.0):
@@ -86,7 +87,7 @@ def select(logits, scores, k, ended=None, end_token=-1):
             logit.reshape(W, V)[np.asarray(ended[b], bool)] = 0.0          # not looked at
         best = np.lexsort((np.arange(W * V), -logit, np.arange(W * V) // V, -flat))[:k]
         for i, c in enumerate(best):
-            if flat[c] > -np.inf:
+            if flat[c] > LEAST:
                 out[0][b, i], out[1][b, i], out[2][b, i] = flat[c], c // V, c % V
     return out
 

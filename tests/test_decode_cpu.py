@@ -73,6 +73,16 @@ def test_oracle_selection_of_huge_logits():
         assert got[1].tolist() == [[0] * 10 + [1] * 2] and got[2].tolist() == [[*range(10), 0, 1]]
 
 
+def test_oracle_selection_below_the_scores_range():
+    """A candidate whose score is -inf in the fp32 that scores are given in is not there."""
+    low = torch.finfo(torch.float32).min
+    assert np.float32(odec.LEAST) == -np.inf and np.float32(np.nextafter(odec.LEAST, 0)) == low
+    x = torch.tensor([[[0.0, low, low / 2, -1.0]]])
+    got = odec.select(x, [[low / 2]], 4)
+    assert got[2].tolist() == [[0, 3, 2, -1]] and got[1].tolist() == [[0, 0, 0, -1]] and got[0][0, 3] == -np.inf
+    assert (got[0][0, :3].astype(np.float32) > -np.inf).all()
+
+
 def test_oracle_selection_of_swallowed_logits():
     """Where the score leaves nothing of the logits in 64 bits they still order their beam's tokens."""
     x = torch.tensor([[[0.0, 3.0, -1.0, 3.0], [5.0, 9.0, 7.0, 8.0]]])

@@ -492,6 +492,21 @@ def test_select_rows_of_huge_logits(dev, dtype, V):
         check_select(cache_ops.select_beams(x.to(dev), s.to(dev), k), x, s, k)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [50, 9000])
+def test_select_scores_below_their_range(dev, dtype, V):
+    """Masked logits of a masked beam: their sum is -inf in fp32, and no candidate."""
+    low = torch.finfo(torch.float32).min
+    x, s = select_case(3, 2, V, dtype, seed=V)
+    x[:, :, 5:] = torch.finfo(dtype).min
+    s[:, 0] = low
+    s[1, 1], s[2, 1] = low / 2, -torch.inf
+    for k in (4, 30, 64):
+        got = cache_ops.select_beams(x.to(dev), s.to(dev), k)
+        check_select(got, x, s, k)
+        assert ((got[1] < 0) == (got[0] == -torch.inf)).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("W,V,k", [(4, 50, 3), (4, 50, 40), (3, 9000, 8), (4, 20011, 64), (32, 20000, 40), (64, 70000, 64)])
 def test_select_scores_that_swallow_the_logits(dev, dtype, W, V, k):
