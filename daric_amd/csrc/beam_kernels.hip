@@ -12,11 +12,11 @@
 // the exponentials' argument (x - max) log2(e) is one product with log2(e) to 48 bits,
 // rounded once, and what follows the splits' fp32 sums is fp64.
 //
-// MI355X, traced medians, 256 rows of 128000 bf16, 16 candidates of 8 beams: splits 18.4
-// us, join 6.0. The splits' loads and maxima alone take 11.3 us (65.5 MB at 5.8 TB/s), the
+// MI355X, traced medians, 256 rows of 128000 bf16, 16 candidates of 8 beams: splits 18.5
+// us, join 6.2. The splits' loads and maxima alone take 11.3 us (65.5 MB at 5.8 TB/s), the
 // exponentials 1.7 more, thresholds, hits and their ranks the rest: vector instructions
 // issue for 10 us of the 18 and overlap the loads only in part. One request of four such
-// rows: 6.1 + 6.1 us, latency.
+// rows: 6.1 + 5.9 us, latency.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
