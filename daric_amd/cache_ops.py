@@ -702,7 +702,8 @@ def append_tokens(layer: torch.Tensor, page_first: bool, block_table: torch.Tens
     differ); inv_freq None: nothing is rotated. rotary_dim, is_neox_style,
     attention_scale as in rotate_rows. An fp8 (e4m3) cache takes bf16 or fp16 rows as
     sat_rtne(x / scale) with its [H] fp32 k_scale / v_scale (None: 1). MLA rows (v None)
-    whose rotated part stands last: rotate_rows of k[..., -R:] in place, then no inv_freq here. Tokens in pages
+    whose rotated part stands last: rotate_rows of k[..., -R:] in place, then no inv_freq
+    here. Tokens in pages
     of id 0 are not written, nor is anything of rows of no sequence; no slot may be
     written by two rows of a call. Returns
     q_out (q itself, or a contiguous tensor, made if None), or None without q. No

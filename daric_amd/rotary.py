@@ -51,7 +51,7 @@ def _yarn_scale(scaling: dict, factor: float) -> float:
     def g(s):
         return 0.1 * s * math.log(factor) + 1 if factor > 1 else 1.0
 
-    part, whole = _number(scaling, "mscale", 0), _number(scaling, "mscale_all_dim", 0)
+    part, whole = (0 if scaling.get(n) is None else _number(scaling, n) for n in ("mscale", "mscale_all_dim"))
     if part and whole:
         return g(part) / g(whole)
     if (part or whole) and g(part or 1) / g(whole) != g(1):
@@ -72,10 +72,11 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional
       linearly in n / wavelength;
     - "yarn": dims that turn fewer than "beta_slow" (1) times over n positions are
       stretched by "factor", those of more than "beta_fast" (32) stay, between them mixed
-      linearly in the dim, the ends moved out to whole dims unless "truncate" is False; attention_scale is "attention_factor", or g(1), or g(mscale) /
-      g(mscale_all_dim) where both are given, with g(s) = 0.1 s ln(factor) + 1 (1 for
-      factors up to 1). One of them without the other (or 0) is refused unless both readings
-      of it, g(1) and that ratio with g(0) = 1 for the missing one, agree.
+      linearly in the dim, the ends moved out to whole dims unless "truncate" is False;
+      attention_scale is "attention_factor", or g(1), or g(mscale) / g(mscale_all_dim) where
+      both are given, with g(s) = 0.1 s ln(factor) + 1 (1 for factors up to 1). One of them
+      without the other (or 0) is refused unless both readings of it, g(1) and that ratio with
+      g(0) = 1 for the missing one, agree.
 
     Names that none of them knows are refused, and a "rope_theta" that is not `base`.
     """
@@ -117,7 +118,7 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional
                 return R * math.log(n / (2 * math.pi * turns)) / (2 * math.log(base))
 
             lo, hi = dim_of(fast), dim_of(slow)
-            if scaling.get("truncate", True):
+            if scaling.get("truncate") in (None, True):
                 lo, hi = math.floor(lo), math.ceil(hi)
             lo, hi = max(lo, 0), min(hi, R - 1)
             far = ((torch.arange(R // 2, dtype=torch.float64) - lo) / max(hi - lo, 1e-3)).clamp(0, 1)

@@ -511,8 +511,9 @@ int daric_rotate_rows(const daric_tensor* rows, const daric_tensor* positions, c
  * written by two rows.
  * layer: one paged cache, bfloat16, float16 or e4m3, head_dim from 2 on. k, v: [T, H, D] rows of its type, or
  * bfloat16 or float16 for an e4m3 cache, strides as daric_rotate_rows' rows; v is NULL for
- * a 3-D (MLA) cache, whose rows are k's one head; rows whose rotated part stands last are turned
- * beforehand (daric_rotate_rows of that part, in place) and appended without rope. An e4m3 cache takes the saturating
+ * a 3-D (MLA) cache, whose rows are k's one head; rows whose rotated part stands last are
+ * turned beforehand (daric_rotate_rows of that part, in place) and appended without rope.
+ * An e4m3 cache takes the saturating
  * round-to-nearest-even code of the rotated fp32 value / scale[h], the quotient
  * correctly rounded; k_scale, v_scale: NULL (1) or contiguous fp32 [H], for such a cache
  * only. q: NULL, or [T, Hq, D] rows of k's type; q_out: as daric_rotate_rows' out.
@@ -530,8 +531,8 @@ int daric_append_tokens(const daric_tensor* layer, int page_first, const daric_t
 /* For each request the k best candidates (beam w, token v), best first: the score of one
  * is scores[b, w] + logits[b, w, v] - log(sum over the vocabulary of exp(logits[b, w])).
  * Candidates of one score are in the order of w, of a beam's the larger logit comes first
- * (a score of -1e38 or +inf swallows the logits, not their order), then the lower v. A beam whose `ended` is not 0 offers end_token
- * alone, at the score scores[b, w]. Candidates whose score is NaN, or -inf in fp32, are not there
+ * (a score of -1e38 or +inf swallows the logits, not their order), then the lower v. A beam
+ * whose `ended` is not 0 offers end_token alone, at the score scores[b, w]. Candidates whose score is NaN, or -inf in fp32, are not there
  * (masked logits, beams of score -inf; all of a row that holds +inf or NaN); places
  * that none is left for get score -inf, parent -1 and token -1.
  * logits: [B, W, V] bfloat16, float16 or float32, rows contiguous, other strides free
@@ -566,7 +567,8 @@ typedef struct daric_beams {
  * pages no list names any more is the caller's to find.
  * layers: caches of any type and layout, head_dim from 2 on, no two of which share memory. parents: int32 [n, columns], rows
  * contiguous (daric_select_beams' parents, or their first columns). Up to 32 beams of a
- * request, half of what daric_select_beams takes: a lane holds a unit of each in registers; block lists do not overlap. block_table is written. */
+ * request, half of what daric_select_beams takes: a lane holds a unit of each in registers.
+ * Block lists do not overlap. block_table is written. */
 int daric_reorder_beams(const daric_tensor* layers, int64_t n_layers, int page_first, daric_tensor* block_table,
                         const daric_tensor* parents, const daric_beams* beams, int64_t n_beams, uint64_t stream);
 

@@ -165,6 +165,9 @@ def test_yarn_scale_of_two_parts(scale, part, whole, want):
     given = {k: v for k, v in (("mscale", part), ("mscale_all_dim", whole)) if v is not None}
     yarn = {"type": "yarn", "factor": scale, "original_max_position_embeddings": 4096, **given}
     assert np.isclose(rotary.rotary_frequencies(64, 10000.0, yarn)[1], want, rtol=1e-14, atol=0)
+    null = {**{"mscale": None, "mscale_all_dim": None, "truncate": None, "attention_factor": None}, **yarn}      # as left out
+    assert np.isclose(rotary.rotary_frequencies(64, 10000.0, null)[1], want, rtol=1e-14, atol=0)
+    assert torch.equal(rotary.rotary_frequencies(64, 10000.0, null)[0], rotary.rotary_frequencies(64, 10000.0, yarn)[0])
     assert rotary.rotary_frequencies(64, 10000.0, {**yarn, "attention_factor": 1.5})[1] == 1.5
 
 
