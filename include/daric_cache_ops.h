@@ -532,7 +532,8 @@ int daric_append_tokens(const daric_tensor* layer, int page_first, const daric_t
  * is scores[b, w] + logits[b, w, v] - log(sum over the vocabulary of exp(logits[b, w])).
  * Candidates of one score are in the order of w, of a beam's the larger logit comes first
  * (a score of -1e38 or +inf swallows the logits, not their order), then the lower v. A beam
- * whose `ended` is not 0 offers end_token alone, at the score scores[b, w]. Candidates whose score is NaN, or -inf in fp32, are not there
+ * whose `ended` is not 0 offers end_token alone, at the score scores[b, w]. Candidates whose
+ * score is NaN, or -inf in fp32, are not there
  * (masked logits, beams of score -inf; all of a row that holds +inf or NaN); places
  * that none is left for get score -inf, parent -1 and token -1.
  * logits: [B, W, V] bfloat16, float16 or float32, rows contiguous, other strides free
@@ -565,7 +566,8 @@ typedef struct daric_beams {
  * no other beam's or request's list may hold it there; full pages may be shared. Rows whose
  * page id, or whose parent's, is 0 or outside [1, num_blocks) are not moved. Which full
  * pages no list names any more is the caller's to find.
- * layers: caches of any type and layout, head_dim from 2 on, no two of which share memory. parents: int32 [n, columns], rows
+ * layers: caches of any type and layout, head_dim from 2 on, no two of which share memory.
+ * parents: int32 [n, columns], rows
  * contiguous (daric_select_beams' parents, or their first columns). Up to 32 beams of a
  * request, half of what daric_select_beams takes: a lane holds a unit of each in registers.
  * Block lists do not overlap. block_table is written. */
